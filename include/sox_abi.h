@@ -559,6 +559,66 @@ typedef struct sox_lds_probe_args {
     int32_t pad_;
 } sox_lds_probe_args;
 
+/* ---- 8-bit products and the norms around a transformer block (no counterpart in the reference) ---- */
+
+/* Rows to 8 bits (sox_qrows_*): scale[r] = amax / 127, q[r][c] = rint(127 x[r][c] / amax), amax the row's largest
+ * magnitude; columns k .. k16 - 1 (k16 = k rounded up to 16) are written as zeros. q rows are ldq bytes apart,
+ * a multiple of 16. vec: x rows on 16-byte boundaries. */
+typedef struct sox_qrows_args {
+    const void* x;
+    int8_t* q;
+    float* scale;
+    int64_t ldx, ldq;
+    int32_t rows, k;
+    int32_t vec, pad_;
+} sox_qrows_args;
+
+/* Product of 8-bit rows and 8-bit weights (sox_qgemm_*, sox_qfew_*):
+ *   y[r][c] = act(sum_k a[r][k] w[k][c] * xs[r] * ws[c] + bias[c] (+ add[r][c]))
+ * w: blocks of 32 columns x 32 k, one KiB each, block (c / 32) * kb + k / 32; byte (k % 32 / 16 * 32 + c % 32) * 16 +
+ * k % 16 of its block is w[k][c] (zeros past k and the last column). ws and bias are padded with zeros to a multiple
+ * of 256. The sox_qfew_* kernels with floating rows (x) bring them to 8 bits themselves. */
+typedef struct sox_qgemm_args {
+    const int8_t* a;
+    const float* xs;
+    const int8_t* w;
+    const float* ws;
+    const float* bias;
+    const void* add;    /* residual, or null */
+    void* y;
+    const void* zeros;  /* >= 16 zero bytes */
+    const void* x;
+    int64_t lda, ldx, ldr, ldy; /* lda in bytes, the others in elements */
+    int32_t m, n, k, k16;
+    int32_t kb, nb;     /* 32-k blocks of a column block, column blocks */
+    int32_t tiles_n, act;
+    int32_t vec;        /* bit0: y (and residual) rows on 16-byte boundaries, n whole chunks; bit1: x rows too */
+    int32_t pad_;
+} sox_qgemm_args;
+
+/* Norms before and after a transformer block (sox_bnorm_*): for each row
+ *   h = res_scale * residual + act(gate) * (post(x) * scale),  y = pre(h)
+ * post / pre: SOX_NORM_*. pg = post gamma * scale, pb = post beta * scale, g / b: the pre norm's. y in the storage
+ * type, or (q) as 8-bit rows with their scales (as sox_qrows_args). gate row of row r: r / gate_group. */
+typedef struct sox_bnorm_args {
+    const void* x;         /* or null: no branch */
+    const void* residual;  /* or null: 0 */
+    const void* gate;      /* or null: 1 */
+    const float* pg;
+    const float* pb;
+    const float* g;
+    const float* b;
+    void* h;               /* or null */
+    void* y;               /* or null */
+    int8_t* q;             /* or null */
+    float* qs;
+    int64_t ldx, ldr, ldg, ldh, ldy, ldq;
+    int32_t rows, c, gate_group;
+    int32_t post, pre, gate_act;
+    float post_eps, pre_eps, res_scale;
+    int32_t pad_;
+} sox_bnorm_args;
+
 #ifdef __cplusplus
 }
 #endif

@@ -289,6 +289,80 @@ int sox_ctc_argmax(sox_ctc* ctc, sox_session* session, int32_t feature_value, in
 int sox_ctc_argmax_noalloc(sox_ctc* ctc, sox_session* session, int32_t feature_value, int32_t batch, int32_t rows,
                            int32_t* d_indices, float* d_probabilities, int32_t* d_status);
 
+/* ---- 8-bit transformer layers (no counterpart in the reference) ----
+ * A product in 8-bit integers with a scale for each row (token) and each output channel, and the norms around a
+ * transformer block with its gate and residual scale, which can hand the product its 8-bit rows. One object holds a
+ * layer's parameters on the device; calls work on the caller's device memory, enqueue on the caller's stream
+ * (NULL: the device's null stream; sox_session_stream and sox_session_value_ptr for a session's) and return. They
+ * allocate nothing, keep nothing of a call and never wait, so they may be captured into a graph, and calls on one
+ * object may run at once from any threads and on any streams, each with a workspace of its own.
+ *
+ * Matrices are rows of `storage` elements (SOX_STORAGE_*), ld elements from row to row (>= the row's length), any
+ * element alignment (whole 16-byte chunks are faster). rows = 0 does nothing; at most 2^23 rows. Columns past a row's
+ * length and rows past the last are neither read nor written. Memory of another device, memory no GPU can read
+ * and a stream of another device are refused (SOX_E_INVALID), as are outputs that overlap an input or each other,
+ * except where said. An offline backend's objects check calls and then return SOX_E_UNSUPPORTED. */
+
+/* Brought to 8 bits: q[r][k] = rint(127 x[r][k] / amax), scale[r] = amax / 127, amax = max_k |x[r][k]|, ties to even,
+ * the exact rounding for 16-bit and fp32 x. A row of zeros has scale 0. A row that holds a NaN or an infinity has
+ * scale NaN and zeros: all its outputs are NaN, and no other row's. */
+typedef struct sox_qlinear sox_qlinear;
+/* weights row-major [inner][columns] (an ONNX MatMul's B), brought to 8 bits by column as above (finite ones only);
+ * bias [columns] or NULL. inner <= 131071: the 32-bit sums cannot overflow (SOX_E_UNSUPPORTED above). */
+int sox_qlinear_create(sox_backend* backend, const float* weights, const float* bias, int32_t inner, int32_t columns,
+                       sox_qlinear** linear);
+/* From 8-bit weights [inner][columns] and their scales [columns] (an ONNX MatMulInteger's B and its scale). */
+int sox_qlinear_create_int8(sox_backend* backend, const int8_t* weights, const float* scales, const float* bias,
+                            int32_t inner, int32_t columns, sox_qlinear** linear);
+/* After the last call's work has run. */
+void sox_qlinear_destroy(sox_qlinear* linear);
+/* Bytes from row to row that sox_qlinear_run_quantized's rows are best held at (inner rounded up to 64). */
+int sox_qlinear_pitch(sox_qlinear* linear);
+/* Workspace bytes of sox_qlinear_run at this many rows (0: none needed). */
+uint64_t sox_qlinear_workspace(sox_qlinear* linear, int32_t rows);
+/* y[r][c] = act(sum_k q[r][k] w[k][c] * scale[r] * ws[c] + bias[c] (+ residual[r][c])) over floating rows x [rows][inner].
+ * act: enum sox_act; residual [rows][columns] or NULL (may be y itself, same ld). workspace: 16-byte-aligned device
+ * memory, held by this call until its work has run. */
+int sox_qlinear_run(sox_qlinear* linear, void* stream, int32_t storage, const void* x, int64_t ldx, int32_t rows,
+                    const void* residual, int64_t ldr, void* y, int64_t ldy, int32_t act, void* workspace,
+                    uint64_t workspace_bytes);
+/* The same over 8-bit rows and their scales [rows]: rows 16-byte aligned, ldq bytes apart (a multiple of 16, >= inner
+ * rounded up to 16); the bytes from inner to that may hold anything. storage is y's and the residual's. */
+int sox_qlinear_run_quantized(sox_qlinear* linear, void* stream, const int8_t* q, int64_t ldq, const float* scales,
+                              int32_t rows, int32_t storage, const void* residual, int64_t ldr, void* y, int64_t ldy,
+                              int32_t act);
+
+/* h = res_scale * residual + act(gate) * (post(x) * scale),  y = pre(h), each row on its own:
+ *   SOX_NORM_RMS    v / sqrt(mean(v^2) + eps) * gamma
+ *   SOX_NORM_LAYER  (v - mean v) / sqrt(mean((v - mean v)^2) + eps) * gamma + beta
+ * in fp32, rounded once; y is computed from h as summed, not from its rounded copy. */
+enum { SOX_NORM_NONE = 0, SOX_NORM_RMS = 1, SOX_NORM_LAYER = 2 };
+typedef struct sox_block_norm_p {
+    int32_t channels;         /* 1 .. 16384 */
+    int32_t post, pre;        /* SOX_NORM_* */
+    int32_t gate_act;         /* enum sox_act */
+    float post_eps, pre_eps;
+    float res_scale;
+} sox_block_norm_p;
+typedef struct sox_block_norm sox_block_norm;
+/* [channels] each: gammas NULL = ones, betas (SOX_NORM_LAYER) NULL = zeros, scale NULL = ones. */
+int sox_block_norm_create(sox_backend* backend, const sox_block_norm_p* params, const float* post_gamma,
+                          const float* post_beta, const float* scale, const float* pre_gamma, const float* pre_beta,
+                          sox_block_norm** norm);
+void sox_block_norm_destroy(sox_block_norm* norm);
+/* residual, x, h and y are [rows][channels]. x NULL: no branch (h = res_scale * residual); residual NULL: h = the branch
+ * alone; one of them is needed. gate: [gate_rows][channels], gate row g for rows [g, g + 1) * rows / gate_rows
+ * (rows a multiple of gate_rows: 1 = one vector, a row for each sequence, or one for each row); NULL = ones, and then
+ * without gate_act. h or y may be NULL, not both; h or y (one of them) may be x or residual itself (same ld). */
+int sox_block_norm_run(sox_block_norm* norm, void* stream, int32_t storage, int32_t rows, const void* residual, int64_t ldr,
+                       const void* x, int64_t ldx, const void* gate, int64_t ldg, int32_t gate_rows, void* h, int64_t ldh,
+                       void* y, int64_t ldy);
+/* The same with y brought to 8 bits (in fp32) as sox_qlinear_run_quantized takes it: q rows ldq bytes apart, 16-byte
+ * aligned, written up to channels rounded up to 16 (with zeros), and their scales [rows]. */
+int sox_block_norm_run_quantized(sox_block_norm* norm, void* stream, int32_t storage, int32_t rows, const void* residual,
+                                 int64_t ldr, const void* x, int64_t ldx, const void* gate, int64_t ldg, int32_t gate_rows,
+                                 void* h, int64_t ldh, int8_t* q, int64_t ldq, float* scales);
+
 /* ---- image session (VkImageSession, Backends/Vulkan/VkImageSession.cs:7-297) ----
  * Image-to-image inference with the pixel conversions on the device, in the same stream as the model:
  * one upload of the bytes, the dispatches, one download. The model maps [1, 3, H, W] to [1, 3, H, W];

@@ -72,6 +72,18 @@ int sox_module_function(void** fn, void* module, const char* name);
 int sox_launch(void* fn, const uint32_t grid[3], const uint32_t block[3], uint32_t lds_bytes, void* stream,
                const void* kernarg, size_t kernarg_bytes);
 
+/* The same on `device` whatever device the caller's thread is on (restored before the call returns), with the kernel's
+ * one argument struct given by address: the runtime copies it, also into a graph that another library captures on the
+ * stream (hipStreamBeginCapture without sox_graph_begin). */
+int sox_launch_on(int device, void* fn, const uint32_t grid[3], const uint32_t block[3], uint32_t lds_bytes, void* stream,
+                  const void* args);
+/* Makes `device` the calling thread's current device and gives back the one before. */
+int sox_device_swap(int device, int* previous);
+/* The device whose memory ptr is in (pinned host memory: the device it was mapped for), -1 for memory no GPU can read. */
+int sox_pointer_device(const void* ptr, int* device);
+/* The device of a stream (not the null stream, which is the calling thread's current device's). */
+int sox_stream_device(void* stream, int* device);
+
 /* Streams: one per session (the compute queue, VkDevice.cs:92; vkQueueSubmit/WaitForFences, Vk.cs:467-473). */
 int sox_stream_create(void** stream);
 int sox_stream_destroy(void* stream);

@@ -578,3 +578,125 @@ class HipUnitRunner:
         except Exception:
             pass
 
+
+
+def _address(host: Optional[np.ndarray]):
+    return None if host is None else host.ctypes.data
+
+
+def _vector(v, n: int, what: str) -> Optional[np.ndarray]:
+    if v is None:
+        return None
+    v = np.ascontiguousarray(v, dtype=np.float32).reshape(-1)
+    if v.size != n:
+        raise ValueError(f"{what} must hold {n} floats")
+    return v
+
+
+class HipQuantLinear:
+    """A product in 8-bit integers with a scale for each row and each output channel (sox_qlinear_* of
+    include/sox_backend.h): y = act((q . w) * row scale * channel scale + bias (+ residual)).
+
+    `weights` is [inner, columns]: floats, brought to 8 bits by column, or int8 with `scales` [columns]. Matrices are
+    device addresses (a torch tensor's data_ptr(), sox_session_value_ptr) with the elements from row to row; calls
+    enqueue on `stream` (a torch stream's cuda_stream, sox_session_stream; None: the null stream) and return."""
+
+    def __init__(self, backend: HipBackend, weights: np.ndarray, bias: Optional[np.ndarray], inner: int, columns: int,
+                 scales: Optional[np.ndarray] = None):
+        w = np.ascontiguousarray(weights, dtype=np.float32 if scales is None else np.int8)
+        if scales is not None and not np.array_equal(w, weights):
+            raise ValueError("weights with scales must be whole numbers of 8 bits")
+        if w.size != inner * columns:
+            raise ValueError("weights must hold inner x columns values")
+        b, s = _vector(bias, columns, "bias"), _vector(scales, columns, "scales")
+        h = N.c_void_p()
+        if s is None:
+            N.check(N.backend().sox_qlinear_create(backend.h, w.ctypes.data, _address(b), inner, columns, ctypes.byref(h)),
+                    "QuantLinear")
+        else:
+            N.check(N.backend().sox_qlinear_create_int8(backend.h, w.ctypes.data, s.ctypes.data, _address(b), inner,
+                                                        columns, ctypes.byref(h)), "QuantLinear")
+        self.h, self.inner, self.columns = h, inner, columns
+        self.pitch = N.backend().sox_qlinear_pitch(h)
+
+    def workspace(self, rows: int) -> int:
+        """Bytes of workspace that `run` needs at this many rows."""
+        return int(N.backend().sox_qlinear_workspace(self.h, rows))
+
+    def run(self, x: int, rows: int, y: int, storage: str = "f16", ldx: Optional[int] = None, ldy: Optional[int] = None,
+            act: str = "none", residual: Optional[int] = None, ldr: Optional[int] = None, workspace: Optional[int] = None,
+            workspace_bytes: int = 0, stream: Optional[int] = None):
+        """y [rows, columns] from floating rows x [rows, inner]."""
+        N.check(N.backend().sox_qlinear_run(self.h, stream, STORAGE[storage], x, self.inner if ldx is None else ldx, rows,
+                                            residual, self.columns if ldr is None else ldr, y,
+                                            self.columns if ldy is None else ldy, N.ACT[act], workspace, workspace_bytes),
+                "QuantLinear.Run")
+
+    def run_quantized(self, q: int, scales: int, rows: int, y: int, storage: str = "f16", ldq: Optional[int] = None,
+                      ldy: Optional[int] = None, act: str = "none", residual: Optional[int] = None,
+                      ldr: Optional[int] = None, stream: Optional[int] = None):
+        """y [rows, columns] from 8-bit rows (`pitch` bytes apart unless ldq says so) and their scales [rows]."""
+        N.check(N.backend().sox_qlinear_run_quantized(self.h, stream, q, self.pitch if ldq is None else ldq, scales, rows,
+                                                      STORAGE[storage], residual, self.columns if ldr is None else ldr, y,
+                                                      self.columns if ldy is None else ldy, N.ACT[act]),
+                "QuantLinear.RunQuantized")
+
+    def close(self):
+        if self.h:
+            N.backend().sox_qlinear_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class HipBlockNorm:
+    """The norms before and after a transformer block with its gate and residual scale (sox_block_norm_* of
+    include/sox_backend.h): h = res_scale * residual + act(gate) * (post(x) * scale), y = pre(h), y in the storage type
+    or as the 8-bit rows a HipQuantLinear reads. Addresses and streams as there."""
+
+    def __init__(self, backend: HipBackend, channels: int, post: str = "none", pre: str = "layer", post_gamma=None,
+                 post_beta=None, scale=None, pre_gamma=None, pre_beta=None, res_scale: float = 1.0, gate_act: str = "none",
+                 post_eps: float = 1e-5, pre_eps: float = 1e-5):
+        p = N.BlockNormP(channels, N.NORM[post], N.NORM[pre], N.ACT[gate_act], post_eps, pre_eps, res_scale)
+        v = [_vector(a, channels, what) for a, what in ((post_gamma, "post_gamma"), (post_beta, "post_beta"), (scale, "scale"),
+                                                        (pre_gamma, "pre_gamma"), (pre_beta, "pre_beta"))]
+        h = N.c_void_p()
+        N.check(N.backend().sox_block_norm_create(backend.h, ctypes.byref(p), *[_address(a) for a in v], ctypes.byref(h)),
+                "BlockNorm")
+        self.h, self.channels = h, channels
+
+    def run(self, residual: Optional[int], rows: int, storage: str = "f16", ldr: Optional[int] = None,
+            x: Optional[int] = None, ldx: Optional[int] = None, gate: Optional[int] = None, ldg: Optional[int] = None,
+            gate_rows: int = 1, h: Optional[int] = None, ldh: Optional[int] = None, y: Optional[int] = None,
+            ldy: Optional[int] = None, stream: Optional[int] = None):
+        """h and y [rows, channels] (either may be left out) from the residual and the branch x."""
+        c = self.channels
+        N.check(N.backend().sox_block_norm_run(self.h, stream, STORAGE[storage], rows, residual, c if ldr is None else ldr, x,
+                                               c if ldx is None else ldx, gate, c if ldg is None else ldg, gate_rows, h,
+                                               c if ldh is None else ldh, y, c if ldy is None else ldy), "BlockNorm.Run")
+
+    def run_quantized(self, residual: Optional[int], rows: int, q: int, scales: int, storage: str = "f16",
+                      ldr: Optional[int] = None, x: Optional[int] = None, ldx: Optional[int] = None,
+                      gate: Optional[int] = None, ldg: Optional[int] = None, gate_rows: int = 1, h: Optional[int] = None,
+                      ldh: Optional[int] = None, ldq: Optional[int] = None, stream: Optional[int] = None):
+        """h, and y as 8-bit rows q (channels rounded up to 64 bytes apart unless ldq says so) and their scales [rows]."""
+        c = self.channels
+        N.check(N.backend().sox_block_norm_run_quantized(
+            self.h, stream, STORAGE[storage], rows, residual, c if ldr is None else ldr, x, c if ldx is None else ldx, gate,
+            c if ldg is None else ldg, gate_rows, h, c if ldh is None else ldh, q, -(-c // 64) * 64 if ldq is None else ldq,
+            scales), "BlockNorm.RunQuantized")
+
+    def close(self):
+        if self.h:
+            N.backend().sox_block_norm_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

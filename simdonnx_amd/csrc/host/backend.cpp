@@ -4695,3 +4695,464 @@ int sox_unit_runner_wait(sox_unit_runner* r, int32_t wave) {
 }
 
 }  // extern "C"
+
+// ---- 8-bit transformer layers (kernels in qgemm.hip, qlinear.hip, block_norm.hip) ----
+namespace {
+
+const char* const kStorageName[] = {"f32", "f16", "bf16"};  // by SOX_STORAGE_*
+
+// Rows of a caller's device matrix: `rows` rows of `width` bytes, `pitch` bytes apart.
+struct Rows {
+    const char* what;
+    uint64_t at = 0;
+    int64_t rows = 0, width = 0, pitch = 0;
+    bool any() const { return at && rows > 0 && width > 0; }
+    uint64_t end() const { return at + (uint64_t)(rows - 1) * (uint64_t)pitch + (uint64_t)width; }
+    bool same(const Rows& o) const { return at == o.at && (pitch == o.pitch || rows == 1); }
+    bool overlaps(const Rows& o) const {
+        if (!any() || !o.any() || end() <= o.at || o.end() <= at) return false;
+        if (pitch != o.pitch || rows == 1 || o.rows == 1) return true;
+        const int64_t d = (int64_t)((o.at >= at ? o.at - at : (uint64_t)pitch - (at - o.at) % (uint64_t)pitch) % (uint64_t)pitch);
+        return d < width || d + o.width > pitch;  // (side by side in the rows of one buffer: disjoint)
+    }
+};
+
+// What the layers' calls check alike, named for their errors.
+struct LayerCall {
+    sox_backend* be;
+    const char* name;
+    int64_t rows, es = 0;
+
+    [[noreturn]] void bad(const std::string& why) const { fail(SOX_E_INVALID, std::string(name) + ": " + why); }
+    Rows matrix(const char* what, const void* p, int64_t ld, int64_t cols, int64_t elem, int64_t align, bool optional,
+                int64_t nrows) const {
+        Rows r{what};
+        if (!p) {
+            if (!optional) bad(std::string(what) + " is null");
+            return r;
+        }
+        if (ld < cols || ld > ((int64_t)1 << 40)) bad(std::string(what) + ": rows of " + std::to_string(cols) + " elements cannot be " + std::to_string(ld) + " apart");
+        if ((uintptr_t)p % (uint64_t)align || ld * elem % align) bad(std::string(what) + " is not on " + std::to_string(align) + "-byte boundaries");
+        r.at = (uint64_t)(uintptr_t)p;
+        r.rows = nrows;
+        r.width = cols * elem;
+        r.pitch = ld * elem;
+        return r;
+    }
+    Rows matrix(const char* what, const void* p, int64_t ld, int64_t cols, bool optional = false) const {
+        return matrix(what, p, ld, cols, es, es, optional, rows);
+    }
+    // every row on 16-byte boundaries and of whole 16-byte chunks
+    static bool chunked(const Rows& r) { return !r.any() || (r.at % 16 == 0 && r.pitch % 16 == 0 && r.width % 16 == 0); }
+    // rows on 16-byte boundaries, whatever their length
+    static bool on16(const Rows& r) { return r.at % 16 == 0 && r.pitch % 16 == 0; }
+
+    LayerCall(sox_backend* b, const char* n, int32_t nrows, int32_t storage) : be(b), name(n), rows(nrows) {
+        if (nrows < 0) bad("rows");
+        if (nrows > 1 << 23) fail(SOX_E_UNSUPPORTED, std::string(n) + ": more than 2^23 rows");
+        if (storage < SOX_STORAGE_F32 || storage > SOX_STORAGE_BF16) bad("storage");
+        es = storage == SOX_STORAGE_F32 ? 4 : 2;
+    }
+    void act(int32_t a) const {
+        if (a < SOX_ACT_NONE || a > SOX_ACT_SWISH) fail(SOX_E_UNSUPPORTED, std::string(name) + ": activation " + std::to_string(a));
+    }
+    // out may share no byte with the others; those of `inplace` it may be, row for row
+    void apart(const Rows& out, std::initializer_list<const Rows*> others, std::initializer_list<const Rows*> inplace = {}) const {
+        for (const Rows* o : others)
+            if (out.overlaps(*o)) bad(std::string(out.what) + " overlaps " + o->what);
+        for (const Rows* o : inplace)
+            if (out.overlaps(*o) && !out.same(*o)) bad(std::string(out.what) + " overlaps " + o->what + " without being it");
+    }
+    // the last check: everything lives on the backend's device
+    void device(void* stream, std::initializer_list<const Rows*> all) const {
+        be->need_device(name);
+        if (be->lost || sox_device_lost()) fail(SOX_E_LOST, "device lost");
+        int d = be->info.device;
+        if (stream) check(sox_stream_device(stream, &d), name);
+        if (d != be->info.device) bad("the stream is another device's");
+        for (const Rows* r : all) {
+            if (!r->any()) continue;
+            check(sox_pointer_device((const void*)(uintptr_t)r->at, &d), name);
+            if (d != be->info.device) bad(std::string(r->what) + (d < 0 ? " is not in memory the GPU reads" : " is on another device"));
+        }
+    }
+    template <class A> void launch(void* fn, uint32_t gx, uint32_t threads, void* stream, const A& args) const {
+        const uint32_t grid[3] = {gx, 1, 1}, block[3] = {threads, 1, 1};
+        check(sox_launch_on(be->info.device, fn, grid, block, 0, stream, &args), name);
+    }
+};
+
+// Parameters in one device block on the backend's device.
+struct DeviceBlock {
+    void* p = nullptr;
+    ~DeviceBlock() {
+        if (p) sox_free(p);
+    }
+    void upload(sox_backend* be, const void* src, size_t bytes, const char* what) {
+        if (be->offline) return;
+        int before = 0;
+        check(sox_device_swap(be->info.device, &before), what);
+        int rc = sox_malloc(&p, bytes);
+        if (!rc) rc = sox_memcpy_h2d(p, src, bytes, nullptr);
+        if (!rc) rc = sox_stream_sync(nullptr);
+        int ours = 0;
+        const int back = sox_device_swap(before, &ours);
+        check(rc, what);
+        check(back, what);
+    }
+};
+
+}  // namespace
+
+struct sox_qlinear {
+    sox_backend* be = nullptr;
+    int inner = 0, columns = 0, k16 = 0, kb = 0, nb = 0, npad = 0;
+    DeviceBlock mem;  // packed weights, then the scales and the bias (zeros without one), padded to npad columns
+    uint64_t scales_at = 0;
+    void *fn_rows[3][2], *fn_few[3][3], *fn_fewx[3][3];  // by storage
+
+    const int8_t* w() const { return (const int8_t*)mem.p; }
+    const float* ws() const { return (const float*)((const uint8_t*)mem.p + scales_at); }
+    const float* bias() const { return ws() + npad; }
+    int pitch() const { return round_up(inner, 64); }
+    // rows [rows][pitch], then their scales
+    uint64_t work_rows(int64_t rows) const { return (uint64_t)rows * pitch(); }
+    bool fused(int64_t rows) const { return rows <= 16 && inner <= 4096; }
+    uint64_t workspace(int64_t rows) const { return rows <= 0 || fused(rows) ? 0 : work_rows(rows) + (uint64_t)round_up((int)rows, 4) * 4; }
+};
+
+namespace {
+
+// The tilings of the 8-bit ring (qgemm.hip).
+struct QTile {
+    const char* name;
+    int bm, bn, wgs_per_cu, threads;
+};
+const QTile kQTiles[] = {
+    {"256x256_w8k64s3", 256, 256, 1, 512}, {"128x128_w4k64s2", 128, 128, 2, 256}, {"64x64_w4k64s2", 64, 64, 2, 256},
+};
+
+void qlinear_pack(sox_qlinear& L, const int8_t* w, const float* scales, const float* bias) {
+    const size_t wbytes = (size_t)L.nb * L.kb * 1024;
+    L.scales_at = wbytes;
+    std::vector<uint8_t> host(wbytes + (size_t)L.npad * 8, 0);
+    for (int k = 0; k < L.inner; k++) {
+        const int8_t* src = w + (size_t)k * L.columns;
+        const size_t at = (size_t)(k / 32) * 1024 + (size_t)(k % 32 / 16) * 512 + k % 16;
+        for (int cb = 0; cb < L.nb; cb++) {
+            uint8_t* d = host.data() + (size_t)cb * L.kb * 1024 + at;
+            const int cols = std::min(32, L.columns - cb * 32);
+            for (int c = 0; c < cols; c++) d[c * 16] = (uint8_t)src[cb * 32 + c];
+        }
+    }
+    memcpy(host.data() + L.scales_at, scales, (size_t)L.columns * 4);
+    if (bias) memcpy(host.data() + L.scales_at + (size_t)L.npad * 4, bias, (size_t)L.columns * 4);
+    L.mem.upload(L.be, host.data(), host.size(), "QuantLinear weights");
+    for (int s = 0; s < 3; s++) {
+        const std::string st = kStorageName[s];
+        L.fn_rows[s][0] = L.be->fn("sox_qrows_" + st);
+        L.fn_rows[s][1] = L.be->fn("sox_qrows_" + st + "_wide");
+        for (int i = 0; i < 3; i++) {
+            L.fn_few[s][i] = L.be->fn("sox_qfew_" + st + "_r" + std::to_string(1 << i));
+            L.fn_fewx[s][i] = L.be->fn("sox_qfewx_" + st + "_s" + std::to_string(1 << i));
+        }
+    }
+}
+
+std::unique_ptr<sox_qlinear> qlinear_new(sox_backend* be, const void* weights, int32_t inner, int32_t columns, sox_qlinear** out) {
+    if (!be || !weights || !out || inner <= 0 || columns <= 0) fail(SOX_E_INVALID, "QuantLinear: arguments");
+    if (inner > 131071) fail(SOX_E_UNSUPPORTED, "QuantLinear: 32-bit sums over more than 131071 products");
+    if (columns > 1 << 24) fail(SOX_E_UNSUPPORTED, "QuantLinear: more than 2^24 columns");
+    auto L = std::make_unique<sox_qlinear>();
+    L->be = be;
+    L->inner = inner;
+    L->columns = columns;
+    L->k16 = round_up(inner, 16);
+    L->kb = round_up(inner, 128) / 32;
+    L->nb = (columns + 31) / 32;
+    L->npad = round_up(columns, 256);
+    return L;
+}
+
+// The product over 8-bit rows (fused: over floating ones).
+void qlinear_product(const LayerCall& c, sox_qlinear* L, void* stream, sox_qgemm_args& a, int32_t storage, bool fused) {
+    a.w = L->w();
+    a.ws = L->ws();
+    a.bias = L->bias();
+    a.zeros = c.be->dummy;
+    a.m = (int32_t)c.rows;
+    a.n = L->columns;
+    a.k = L->inner;
+    a.k16 = L->k16;
+    a.kb = L->kb;
+    a.nb = L->nb;
+    const int steps = (L->inner + 63) / 64;
+    const uint32_t col_groups = (uint32_t)((L->columns + 15) / 16);
+    if (fused) {
+        const int si = steps <= 16 ? 0 : steps <= 32 ? 1 : 2, waves = (steps + (1 << si) - 1) >> si;
+        c.launch(L->fn_fewx[storage][si], col_groups, (uint32_t)waves * 64, stream, a);
+        return;
+    }
+    if (c.rows <= 64) {
+        const int ri = c.rows <= 16 ? 0 : c.rows <= 32 ? 1 : 2, s = 8 >> ri;
+        c.launch(L->fn_few[storage][ri], col_groups, (uint32_t)std::min(8, (steps + s - 1) / s) * 64, stream, a);
+        return;
+    }
+    const int64_t cus = std::max(1, c.be->info.compute_units);
+    const QTile* pick = &kQTiles[2];
+    for (const QTile& t : kQTiles)
+        if (((c.rows + t.bm - 1) / t.bm) * ((L->columns + t.bn - 1) / t.bn) >= cus) {
+            pick = &t;
+            break;
+        }
+    if (const char* forced = getenv("SIMDONNX_HIP_QGEMM")) {  // any tiling by name (tuning, tests)
+        pick = nullptr;
+        for (const QTile& t : kQTiles)
+            if (!strcmp(t.name, forced)) pick = &t;
+        if (!pick) fail(SOX_E_INVALID, std::string("SIMDONNX_HIP_QGEMM: unknown tiling ") + forced);
+    }
+    a.tiles_n = (L->columns + pick->bn - 1) / pick->bn;
+    const int64_t tiles = ((c.rows + pick->bm - 1) / pick->bm) * a.tiles_n;
+    if (tiles >= (int64_t)1 << 31) fail(SOX_E_UNSUPPORTED, std::string(c.name) + ": too many outputs");
+    c.launch(c.be->fn(std::string("sox_qgemm_") + kStorageName[storage] + "_" + pick->name),
+             (uint32_t)std::min<int64_t>(tiles, cus * pick->wgs_per_cu), (uint32_t)pick->threads, stream, a);
+}
+
+}  // namespace
+
+struct sox_block_norm {
+    sox_backend* be = nullptr;
+    sox_block_norm_p p{};
+    DeviceBlock mem;  // pg, pb, g, b: [channels] each
+};
+
+namespace {
+
+// block_norm.hip's instances: threads of a row, and chunks of 8 columns of a thread
+struct BnormShape {
+    int tpr, ch;
+};
+BnormShape bnorm_shape(int c) {
+    static const BnormShape shapes[] = {{64, 1}, {64, 2}, {256, 1}, {256, 2}, {1024, 1}, {512, 4}};
+    for (const BnormShape& s : shapes)
+        if (s.tpr * s.ch * 8 >= c) return s;
+    unsupported("BlockNorm: channels");
+}
+std::string bnorm_kernel(int32_t storage, int c, bool vec) {
+    const BnormShape s = bnorm_shape(c);  // (a 16-byte chunk of fp32 is half as many columns)
+    return std::string("sox_bnorm_") + kStorageName[storage] + "_t" + std::to_string(s.tpr) + "c" +
+           std::to_string(s.ch * (storage == SOX_STORAGE_F32 ? 2 : 1)) + (vec ? "v" : "s");
+}
+
+void bnorm_run(sox_block_norm* N, const char* name, void* stream, int32_t storage, int32_t rows, const void* residual,
+               int64_t ldr, const void* x, int64_t ldx, const void* gate, int64_t ldg, int32_t gate_rows, void* h, int64_t ldh,
+               void* y, int64_t ldy, int8_t* q, int64_t ldq, float* scales, bool quantized) {
+    if (!N) fail(SOX_E_INVALID, std::string(name) + ": arguments");
+    const LayerCall c(N->be, name, rows, storage);
+    const int C = N->p.channels;
+    if (!residual && !x) c.bad("neither a residual nor a branch");
+    if (gate && !x) c.bad("a gate without a branch");
+    if (gate && (gate_rows <= 0 || rows % gate_rows)) c.bad("gate rows have to divide the rows");
+    if (rows == 0) return;
+    const Rows R = c.matrix("residual", residual, ldr, C, true), X = c.matrix("x", x, ldx, C, true);
+    const Rows G = c.matrix("gate", gate, ldg, C, c.es, c.es, true, gate_rows);
+    const Rows H = c.matrix("h", h, ldh, C, true);
+    Rows Y{"y"}, S{"scales"};
+    if (quantized) {
+        Y = c.matrix("q", q, ldq, round_up(C, 16), 1, 16, false, rows);
+        S = c.matrix("scales", scales, rows, rows, 4, 4, false, 1);
+    } else {
+        Y = c.matrix("y", y, ldy, C, true);
+        if (!Y.any() && !H.any()) c.bad("neither h nor y");
+    }
+    // a row is read whole before it is written, so h or y may be an input's rows; two outputs may not share any
+    c.apart(H, {&G, &Y, &S}, {&R, &X});
+    if (quantized)
+        c.apart(Y, {&R, &X, &G, &S});
+    else
+        c.apart(Y, {&G}, {&R, &X});
+    c.apart(S, {&R, &X, &G});
+    c.device(stream, {&R, &X, &G, &H, &Y, &S});
+    sox_bnorm_args a{};
+    const float* v = (const float*)N->mem.p;
+    a.x = x; a.residual = residual; a.gate = gate; a.h = h; a.y = y; a.q = q; a.qs = scales;
+    a.pg = v; a.pb = v + C; a.g = v + 2 * (size_t)C; a.b = v + 3 * (size_t)C;
+    a.ldx = ldx; a.ldr = ldr; a.ldg = ldg; a.ldh = ldh; a.ldy = ldy; a.ldq = ldq;
+    a.rows = rows; a.c = C; a.gate_group = gate ? rows / gate_rows : 1;
+    a.post = N->p.post; a.pre = N->p.pre; a.gate_act = N->p.gate_act;
+    a.post_eps = N->p.post_eps; a.pre_eps = N->p.pre_eps; a.res_scale = N->p.res_scale;
+    const bool vec = C * c.es % 16 == 0 && c.chunked(R) && c.chunked(X) && c.chunked(G) && c.chunked(H) && (quantized || c.chunked(Y));
+    const int tpr = bnorm_shape(C).tpr, per_block = tpr == 64 ? 4 : 1;
+    // enough workgroups to fill the GPU; past that each walks several rows with its parameters in registers
+    const int64_t blocks = (rows + per_block - 1) / per_block, cap = (int64_t)std::max(1, c.be->info.compute_units) * (tpr > 256 ? 2 : 8);
+    c.launch(c.be->fn(bnorm_kernel(storage, C, vec)), (uint32_t)std::min(blocks, cap), (uint32_t)std::max(tpr, 256), stream, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sox_qlinear_create(sox_backend* be, const float* weights, const float* bias, int32_t inner, int32_t columns, sox_qlinear** out) {
+    return guarded([&] {
+        auto L = qlinear_new(be, weights, inner, columns, out);
+        std::vector<float> amax((size_t)columns, 0.0f), scales((size_t)columns);
+        for (int k = 0; k < inner; k++)
+            for (int c = 0; c < columns; c++) {
+                const float v = fabsf(weights[(size_t)k * columns + c]);
+                if (!std::isfinite(v)) fail(SOX_E_INVALID, "QuantLinear: weights have to be finite");
+                amax[c] = std::max(amax[c], v);
+            }
+        for (int c = 0; c < columns; c++) scales[c] = amax[c] / 127.0f;
+        std::vector<int8_t> w((size_t)inner * columns);
+        for (int k = 0; k < inner; k++)
+            for (int c = 0; c < columns; c++) {
+                const size_t i = (size_t)k * columns + c;
+                w[i] = amax[c] > 0.0f ? (int8_t)std::nearbyint(127.0 * weights[i] / amax[c]) : (int8_t)0;
+            }
+        qlinear_pack(*L, w.data(), scales.data(), bias);
+        *out = L.release();
+    });
+}
+
+int sox_qlinear_create_int8(sox_backend* be, const int8_t* weights, const float* scales, const float* bias, int32_t inner,
+                            int32_t columns, sox_qlinear** out) {
+    return guarded([&] {
+        auto L = qlinear_new(be, weights, inner, columns, out);
+        if (!scales) fail(SOX_E_INVALID, "QuantLinear: arguments");
+        for (int c = 0; c < columns; c++)
+            if (!std::isfinite(scales[c])) fail(SOX_E_INVALID, "QuantLinear: scales have to be finite");
+        qlinear_pack(*L, weights, scales, bias);
+        *out = L.release();
+    });
+}
+
+void sox_qlinear_destroy(sox_qlinear* L) { delete L; }
+
+int sox_qlinear_pitch(sox_qlinear* L) { return L ? L->pitch() : 0; }
+
+uint64_t sox_qlinear_workspace(sox_qlinear* L, int32_t rows) { return L ? L->workspace(rows) : 0; }
+
+int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x, int64_t ldx, int32_t rows, const void* residual,
+                    int64_t ldr, void* y, int64_t ldy, int32_t act, void* workspace, uint64_t workspace_bytes) {
+    return guarded([&] {
+        const char* name = "QuantLinear.Run";
+        if (!L) fail(SOX_E_INVALID, std::string(name) + ": arguments");
+        const LayerCall c(L->be, name, rows, storage);
+        c.act(act);
+        if (rows == 0) return;
+        const Rows X = c.matrix("x", x, ldx, L->inner), R = c.matrix("residual", residual, ldr, L->columns, true);
+        const Rows Y = c.matrix("y", y, ldy, L->columns);
+        const bool fused = L->fused(rows);
+        Rows W{"workspace"};
+        if (!fused) {
+            const uint64_t need = L->workspace(rows);
+            if (!workspace || workspace_bytes < need)
+                c.bad("needs " + std::to_string(need) + " bytes of workspace, has " + std::to_string(workspace ? workspace_bytes : 0));
+            W = c.matrix("workspace", workspace, (int64_t)need, (int64_t)need, 1, 16, false, 1);
+        }
+        c.apart(Y, {&X, &W}, {&R});
+        c.apart(W, {&X, &R});
+        c.device(stream, {&X, &R, &Y, &W});
+        sox_qgemm_args a{};
+        a.x = x;
+        a.ldx = ldx;
+        a.add = residual;
+        a.ldr = ldr;
+        a.y = y;
+        a.ldy = ldy;
+        a.act = act;
+        a.vec = (c.chunked(Y) && c.chunked(R) ? 1 : 0) | (c.on16(X) ? 2 : 0);
+        if (!fused) {
+            sox_qrows_args q{};
+            q.x = x;
+            q.ldx = ldx;
+            q.q = (int8_t*)workspace;
+            q.ldq = L->pitch();
+            q.scale = (float*)((uint8_t*)workspace + L->work_rows(rows));
+            q.rows = rows;
+            q.k = L->inner;
+            q.vec = c.on16(X);
+            const bool wide = (int64_t)L->inner * c.es > 4096;  // past what a wave's registers hold
+            c.launch(L->fn_rows[storage][wide], (uint32_t)(wide ? rows : (rows + 3) / 4), 256, stream, q);
+            a.a = q.q;
+            a.lda = q.ldq;
+            a.xs = q.scale;
+        }
+        qlinear_product(c, L, stream, a, storage, fused);
+    });
+}
+
+int sox_qlinear_run_quantized(sox_qlinear* L, void* stream, const int8_t* q, int64_t ldq, const float* scales, int32_t rows,
+                              int32_t storage, const void* residual, int64_t ldr, void* y, int64_t ldy, int32_t act) {
+    return guarded([&] {
+        const char* name = "QuantLinear.RunQuantized";
+        if (!L) fail(SOX_E_INVALID, std::string(name) + ": arguments");
+        const LayerCall c(L->be, name, rows, storage);
+        c.act(act);
+        if (rows == 0) return;
+        const Rows Q = c.matrix("q", q, ldq, L->k16, 1, 16, false, rows), S = c.matrix("scales", scales, rows, rows, 4, 4, false, 1);
+        const Rows R = c.matrix("residual", residual, ldr, L->columns, true), Y = c.matrix("y", y, ldy, L->columns);
+        c.apart(Y, {&Q, &S}, {&R});
+        c.device(stream, {&Q, &S, &R, &Y});
+        sox_qgemm_args a{};
+        a.a = q;
+        a.lda = ldq;
+        a.xs = scales;
+        a.add = residual;
+        a.ldr = ldr;
+        a.y = y;
+        a.ldy = ldy;
+        a.act = act;
+        a.vec = c.chunked(Y) && c.chunked(R) ? 1 : 0;
+        qlinear_product(c, L, stream, a, storage, false);
+    });
+}
+
+int sox_block_norm_create(sox_backend* be, const sox_block_norm_p* p, const float* post_gamma, const float* post_beta,
+                          const float* scale, const float* pre_gamma, const float* pre_beta, sox_block_norm** out) {
+    return guarded([&] {
+        if (!be || !p || !out || p->channels <= 0) fail(SOX_E_INVALID, "BlockNorm: arguments");
+        if (p->channels > 16384) fail(SOX_E_UNSUPPORTED, "BlockNorm: more than 16384 channels");
+        for (int32_t kind : {p->post, p->pre})
+            if (kind < SOX_NORM_NONE || kind > SOX_NORM_LAYER) fail(SOX_E_INVALID, "BlockNorm: norm kind");
+        if (p->gate_act < SOX_ACT_NONE || p->gate_act > SOX_ACT_SWISH) fail(SOX_E_UNSUPPORTED, "BlockNorm: gate activation");
+        if (!(p->post_eps >= 0.0f) || !(p->pre_eps >= 0.0f) || !std::isfinite(p->res_scale)) fail(SOX_E_INVALID, "BlockNorm: eps / residual scale");
+        auto N = std::make_unique<sox_block_norm>();
+        N->be = be;
+        N->p = *p;
+        const size_t C = (size_t)p->channels;
+        std::vector<float> v(4 * C);
+        for (size_t i = 0; i < C; i++) {  // the branch's scale folded into the post norm
+            const float s = scale ? scale[i] : 1.0f;
+            v[i] = (p->post != SOX_NORM_NONE && post_gamma ? post_gamma[i] : 1.0f) * s;
+            v[C + i] = (p->post == SOX_NORM_LAYER && post_beta ? post_beta[i] : 0.0f) * s;
+            v[2 * C + i] = pre_gamma ? pre_gamma[i] : 1.0f;
+            v[3 * C + i] = p->pre == SOX_NORM_LAYER && pre_beta ? pre_beta[i] : 0.0f;
+        }
+        N->mem.upload(be, v.data(), v.size() * 4, "BlockNorm parameters");
+        for (int32_t s = 0; s < 3; s++)
+            for (bool vec : {false, true}) be->fn(bnorm_kernel(s, p->channels, vec));
+        *out = N.release();
+    });
+}
+
+void sox_block_norm_destroy(sox_block_norm* N) { delete N; }
+
+int sox_block_norm_run(sox_block_norm* N, void* stream, int32_t storage, int32_t rows, const void* residual, int64_t ldr, const void* x,
+                       int64_t ldx, const void* gate, int64_t ldg, int32_t gate_rows, void* h, int64_t ldh, void* y, int64_t ldy) {
+    return guarded([&] {
+        bnorm_run(N, "BlockNorm.Run", stream, storage, rows, residual, ldr, x, ldx, gate, ldg, gate_rows, h, ldh, y, ldy, nullptr, 0,
+                  nullptr, false);
+    });
+}
+
+int sox_block_norm_run_quantized(sox_block_norm* N, void* stream, int32_t storage, int32_t rows, const void* residual, int64_t ldr,
+                                 const void* x, int64_t ldx, const void* gate, int64_t ldg, int32_t gate_rows, void* h, int64_t ldh,
+                                 int8_t* q, int64_t ldq, float* scales) {
+    return guarded([&] {
+        bnorm_run(N, "BlockNorm.RunQuantized", stream, storage, rows, residual, ldr, x, ldx, gate, ldg, gate_rows, h, ldh, nullptr, 0, q,
+                  ldq, scales, true);
+    });
+}
+
+}  // extern "C"

@@ -121,7 +121,10 @@ int sox_module_load(void** module, const void* image, size_t bytes) {
 int sox_module_unload(void* module) { return st(hipModuleUnload((hipModule_t)module)); }
 int sox_module_function(void** fn, void* module, const char* name) {
     hipError_t e = hipModuleGetFunction((hipFunction_t*)fn, (hipModule_t)module, name);
-    if (e == hipErrorNotFound) return SOX_E_NOT_FOUND;
+    if (e == hipErrorNotFound) {
+        (void)hipGetLastError();  // a miss is an answer: the next caller of HIP must not find it as its own error
+        return SOX_E_NOT_FOUND;
+    }
     return st(e);
 }
 
@@ -150,6 +153,44 @@ int sox_launch(void* fn, const uint32_t grid[3], const uint32_t block[3], uint32
                       &size, HIP_LAUNCH_PARAM_END};
     return st(hipModuleLaunchKernel((hipFunction_t)fn, grid[0], grid[1], grid[2], block[0], block[1], block[2],
                                     lds_bytes, (hipStream_t)stream, nullptr, config));
+}
+
+int sox_launch_on(int device, void* fn, const uint32_t grid[3], const uint32_t block[3], uint32_t lds_bytes, void* stream,
+                  const void* args) {
+    if (g_lost.load()) return SOX_E_LOST;
+    if (!fn || grid[0] == 0 || grid[1] == 0 || grid[2] == 0) return SOX_E_INVALID;
+    int current = device;
+    if (int rc = st(hipGetDevice(&current))) return rc;
+    if (current != device)
+        if (int rc = st(hipSetDevice(device))) return rc;
+    void* params[] = {const_cast<void*>(args)};
+    const int rc = st(hipModuleLaunchKernel((hipFunction_t)fn, grid[0], grid[1], grid[2], block[0], block[1], block[2],
+                                            lds_bytes, (hipStream_t)stream, params, nullptr));
+    if (current != device) (void)hipSetDevice(current);
+    return rc;
+}
+int sox_device_swap(int device, int* previous) {
+    if (!previous) return SOX_E_INVALID;
+    if (int rc = st(hipGetDevice(previous))) return rc;
+    return *previous == device ? SOX_OK : st(hipSetDevice(device));
+}
+int sox_pointer_device(const void* ptr, int* device) {
+    if (!ptr || !device) return SOX_E_INVALID;
+    hipPointerAttribute_t a;
+    if (hipPointerGetAttributes(&a, ptr) != hipSuccess) {
+        (void)hipGetLastError();
+        *device = -1;
+        return SOX_OK;
+    }
+    *device = a.type == hipMemoryTypeDevice || a.type == hipMemoryTypeManaged || (a.type == hipMemoryTypeHost && a.devicePointer) ? a.device : -1;
+    return SOX_OK;
+}
+int sox_stream_device(void* stream, int* device) {
+    if (!stream || !device) return SOX_E_INVALID;
+    hipDevice_t d = -1;
+    const int rc = st(hipStreamGetDevice((hipStream_t)stream, &d));
+    *device = d;
+    return rc;
 }
 
 int sox_stream_create(void** stream) { return st(hipStreamCreateWithFlags((hipStream_t*)stream, hipStreamNonBlocking)); }

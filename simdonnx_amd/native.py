@@ -32,6 +32,7 @@ CK = dict(raw=0, f32=1, convwt=2, gemmnk=3, dww=4, convtw=5, f32t=7)
 SLOT_ARENA, SLOT_CONSTS, SLOT_DUMMY, SLOT_SYNC = 0, 1, 2, 3
 PIX = dict(Bgr24=0, Rgb24=1, Bgra32=2, Rgba32=3)  # PixelFormat (Imaging/ImageTensor.cs:8-20)
 RUN_STAGING, RUN_DISPATCHES = 1, 2
+NORM = dict(none=0, rms=1, layer=2)  # SOX_NORM_*
 
 
 class DeviceInfo(ctypes.Structure):
@@ -136,6 +137,11 @@ class UpHeadP(ctypes.Structure):
                 ("has_skip_conv", c_int32), ("skip_conv", ConvP), ("skip_w", c_int32), ("skip_b", c_int32)]
 
 
+class BlockNormP(ctypes.Structure):
+    _fields_ = [("channels", c_int32), ("post", c_int32), ("pre", c_int32), ("gate_act", c_int32), ("post_eps", c_float),
+                ("pre_eps", c_float), ("res_scale", c_float)]
+
+
 class Bind(ctypes.Structure):
     _fields_ = [("slot", c_int32), ("pad_", c_int32), ("offset", c_uint64), ("size", c_uint64)]
 
@@ -165,6 +171,11 @@ THIN_API = {
     "sox_module_function": (c_int32, [ctypes.POINTER(c_void_p), c_void_p, ctypes.c_char_p]),
     "sox_launch": (c_int32, [c_void_p, ctypes.POINTER(c_uint32), ctypes.POINTER(c_uint32), c_uint32, c_void_p,
                              c_void_p, c_size_t]),
+    "sox_launch_on": (c_int32, [c_int32, c_void_p, ctypes.POINTER(c_uint32), ctypes.POINTER(c_uint32), c_uint32,
+                                c_void_p, c_void_p]),
+    "sox_device_swap": (c_int32, [c_int32, ctypes.POINTER(c_int32)]),
+    "sox_pointer_device": (c_int32, [c_void_p, ctypes.POINTER(c_int32)]),
+    "sox_stream_device": (c_int32, [c_void_p, ctypes.POINTER(c_int32)]),
     "sox_stream_create": (c_int32, [ctypes.POINTER(c_void_p)]),
     "sox_stream_destroy": (c_int32, [c_void_p]),
     "sox_stream_sync": (c_int32, [c_void_p]),
@@ -268,6 +279,24 @@ BACKEND_API = {
     "sox_ctc_argmax": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "sox_ctc_argmax_noalloc": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                                          c_void_p]),
+    "sox_qlinear_create": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, ctypes.POINTER(c_void_p)]),
+    "sox_qlinear_create_int8": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
+                                          ctypes.POINTER(c_void_p)]),
+    "sox_qlinear_destroy": (None, [c_void_p]),
+    "sox_qlinear_pitch": (c_int32, [c_void_p]),
+    "sox_qlinear_workspace": (c_uint64, [c_void_p, c_int32]),
+    "sox_qlinear_run": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p,
+                                  c_int64, c_int32, c_void_p, c_uint64]),
+    "sox_qlinear_run_quantized": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_void_p,
+                                            c_int64, c_void_p, c_int64, c_int32]),
+    "sox_block_norm_create": (c_int32, [c_void_p, ctypes.POINTER(BlockNormP), c_void_p, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, ctypes.POINTER(c_void_p)]),
+    "sox_block_norm_destroy": (None, [c_void_p]),
+    "sox_block_norm_run": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64,
+                                     c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_int64]),
+    "sox_block_norm_run_quantized": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p,
+                                               c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_int64,
+                                               c_void_p]),
 }
 
 _thin = None
