@@ -4776,9 +4776,9 @@ struct LayerCall {
             if (d != be->info.device) bad(std::string(r->what) + (d < 0 ? " is not in memory the GPU reads" : " is on another device"));
         }
     }
-    template <class A> void launch(void* fn, uint32_t gx, uint32_t threads, void* stream, const A& args) const {
+    template <class A> void launch(void* fn, uint32_t gx, uint32_t threads, void* stream, const A& args, uint32_t lds = 0) const {
         const uint32_t grid[3] = {gx, 1, 1}, block[3] = {threads, 1, 1};
-        check(sox_launch_on(be->info.device, fn, grid, block, 0, stream, &args), name);
+        check(sox_launch_on(be->info.device, fn, grid, block, lds, stream, &args), name);
     }
 };
 
@@ -4829,7 +4829,9 @@ struct QTile {
     int bm, bn, wgs_per_cu, threads;
 };
 const QTile kQTiles[] = {
-    {"256x256_w8k64s3", 256, 256, 1, 512}, {"128x128_w4k64s2", 128, 128, 2, 256}, {"64x64_w4k64s2", 64, 64, 2, 256},
+    {"256x256_w8k128s2", 256, 256, 1, 512}, {"256x128_w8k128s2", 256, 128, 1, 512}, {"256x192_w8k128s2", 256, 192, 1, 512},
+    {"128x128_w4k128s2", 128, 128, 2, 256}, {"128x192_w4k64s2", 128, 192, 2, 256},  {"128x64_w4k128s2", 128, 64, 3, 256},
+    {"64x128_w4k128s3", 64, 128, 2, 256},   {"64x64_w4k128s4", 64, 64, 2, 256},     {"64x64_w4k64s2", 64, 64, 4, 256},
 };
 
 void qlinear_pack(sox_qlinear& L, const int8_t* w, const float* scales, const float* bias) {
@@ -4899,7 +4901,7 @@ void qlinear_product(const LayerCall& c, sox_qlinear* L, void* stream, sox_qgemm
         return;
     }
     const int64_t cus = std::max(1, c.be->info.compute_units);
-    const QTile* pick = &kQTiles[2];
+    const QTile* pick = &kQTiles[7];
     for (const QTile& t : kQTiles)
         if (((c.rows + t.bm - 1) / t.bm) * ((L->columns + t.bn - 1) / t.bn) >= cus) {
             pick = &t;
@@ -4923,23 +4925,36 @@ void qlinear_product(const LayerCall& c, sox_qlinear* L, void* stream, sox_qgemm
 struct sox_block_norm {
     sox_backend* be = nullptr;
     sox_block_norm_p p{};
-    DeviceBlock mem;  // pg, pb, g, b: [channels] each
+    DeviceBlock mem;  // pg, pb, g, b: [cpad] each
+    int cpad = 0, vectors = 0;
+    bool has[4] = {};  // which of them there are (the others are all ones or all zeros)
+    void* fn[3][2][2];  // storage, many rows, vector
 };
 
 namespace {
 
-// block_norm.hip's instances: threads of a row, and chunks of 8 columns of a thread
+// block_norm.hip's instances: threads of a row, chunks of 8 columns of a thread, and whether the parameters stand in LDS (a
+// wave per row).
 struct BnormShape {
     int tpr, ch;
+    bool lds;
 };
-BnormShape bnorm_shape(int c) {
-    static const BnormShape shapes[] = {{64, 1}, {64, 2}, {256, 1}, {256, 2}, {1024, 1}, {512, 4}};
-    for (const BnormShape& s : shapes)
-        if (s.tpr * s.ch * 8 >= c) return s;
+const BnormShape kBnormShapes[] = {{64, 1, true},   {64, 2, true},   {64, 4, true},    {64, 8, true},
+                                   {256, 1, false}, {256, 2, false}, {1024, 1, false}, {512, 4, false}};
+constexpr int kBnormLds = 4;  // (the first of them; in fp32 the last of these, 4096 columns, is left out)
+
+// The first instance that holds c columns: among the waves per row, or among the others.
+int bnorm_shape(int32_t storage, int c, bool many_rows) {
+    const int waves = storage == SOX_STORAGE_F32 ? kBnormLds - 1 : kBnormLds, count = (int)(sizeof kBnormShapes / sizeof *kBnormShapes);
+    if (many_rows)
+        for (int i = 0; i < waves; i++)
+            if (kBnormShapes[i].tpr * kBnormShapes[i].ch * 8 >= c) return i;
+    for (int i = kBnormLds; i < count; i++)
+        if (kBnormShapes[i].tpr * kBnormShapes[i].ch * 8 >= c) return i;
     unsupported("BlockNorm: channels");
 }
-std::string bnorm_kernel(int32_t storage, int c, bool vec) {
-    const BnormShape s = bnorm_shape(c);  // (a 16-byte chunk of fp32 is half as many columns)
+std::string bnorm_kernel(int32_t storage, int shape, bool vec) {
+    const BnormShape& s = kBnormShapes[shape];  // (a 16-byte chunk of fp32 is half as many columns)
     return std::string("sox_bnorm_") + kStorageName[storage] + "_t" + std::to_string(s.tpr) + "c" +
            std::to_string(s.ch * (storage == SOX_STORAGE_F32 ? 2 : 1)) + (vec ? "v" : "s");
 }
@@ -4974,18 +4989,22 @@ void bnorm_run(sox_block_norm* N, const char* name, void* stream, int32_t storag
     c.apart(S, {&R, &X, &G});
     c.device(stream, {&R, &X, &G, &H, &Y, &S});
     sox_bnorm_args a{};
-    const float* v = (const float*)N->mem.p;
+    auto vec_at = [&](int i) { return N->has[i] ? (const float*)N->mem.p + (size_t)i * N->cpad : nullptr; };
     a.x = x; a.residual = residual; a.gate = gate; a.h = h; a.y = y; a.q = q; a.qs = scales;
-    a.pg = v; a.pb = v + C; a.g = v + 2 * (size_t)C; a.b = v + 3 * (size_t)C;
+    a.pg = vec_at(0); a.pb = vec_at(1); a.g = vec_at(2); a.b = vec_at(3);
     a.ldx = ldx; a.ldr = ldr; a.ldg = ldg; a.ldh = ldh; a.ldy = ldy; a.ldq = ldq;
     a.rows = rows; a.c = C; a.gate_group = gate ? rows / gate_rows : 1;
     a.post = N->p.post; a.pre = N->p.pre; a.gate_act = N->p.gate_act;
     a.post_eps = N->p.post_eps; a.pre_eps = N->p.pre_eps; a.res_scale = N->p.res_scale;
-    const bool vec = C * c.es % 16 == 0 && c.chunked(R) && c.chunked(X) && c.chunked(G) && c.chunked(H) && (quantized || c.chunked(Y));
-    const int tpr = bnorm_shape(C).tpr, per_block = tpr == 64 ? 4 : 1;
-    // enough workgroups to fill the GPU; past that each walks several rows with its parameters in registers
-    const int64_t blocks = (rows + per_block - 1) / per_block, cap = (int64_t)std::max(1, c.be->info.compute_units) * (tpr > 256 ? 2 : 8);
-    c.launch(c.be->fn(bnorm_kernel(storage, C, vec)), (uint32_t)std::min(blocks, cap), (uint32_t)std::max(tpr, 256), stream, a);
+    const bool vec = c.chunked(R) && c.chunked(X) && c.chunked(G) && c.chunked(H) && (quantized ? C * c.es % 16 == 0 : c.chunked(Y));
+    const int64_t cus = std::max(1, c.be->info.compute_units);
+    const bool many = rows >= 4 * cus;
+    const BnormShape& shape = kBnormShapes[bnorm_shape(storage, C, many)];
+    // enough workgroups to fill the GPU; past that each walks several rows with its parameters at hand
+    const int64_t per_block = shape.tpr == 64 ? 4 : 1, blocks = (rows + per_block - 1) / per_block;
+    const int64_t cap = cus * (shape.lds ? 4 : shape.tpr == 256 ? 8 : 2);
+    c.launch(N->fn[storage][many][vec], (uint32_t)std::min(blocks, cap), (uint32_t)std::max(shape.tpr, 256), stream, a,
+             shape.lds ? (uint32_t)(N->vectors * shape.tpr * shape.ch * 8 * 4) : 0);
 }
 
 }  // namespace
@@ -5120,18 +5139,27 @@ int sox_block_norm_create(sox_backend* be, const sox_block_norm_p* p, const floa
         auto N = std::make_unique<sox_block_norm>();
         N->be = be;
         N->p = *p;
-        const size_t C = (size_t)p->channels;
-        std::vector<float> v(4 * C);
+        const size_t C = (size_t)p->channels, CP = (size_t)round_up(p->channels, 8);
+        N->cpad = (int)CP;
+        const bool post = p->post != SOX_NORM_NONE, pre = p->pre != SOX_NORM_NONE;
+        const bool pb = p->post == SOX_NORM_LAYER && post_beta, b = p->pre == SOX_NORM_LAYER && pre_beta;
+        std::vector<float> v(4 * CP);
         for (size_t i = 0; i < C; i++) {  // the branch's scale folded into the post norm
             const float s = scale ? scale[i] : 1.0f;
-            v[i] = (p->post != SOX_NORM_NONE && post_gamma ? post_gamma[i] : 1.0f) * s;
-            v[C + i] = (p->post == SOX_NORM_LAYER && post_beta ? post_beta[i] : 0.0f) * s;
-            v[2 * C + i] = pre_gamma ? pre_gamma[i] : 1.0f;
-            v[3 * C + i] = p->pre == SOX_NORM_LAYER && pre_beta ? pre_beta[i] : 0.0f;
+            v[i] = (post && post_gamma ? post_gamma[i] : 1.0f) * s;
+            v[CP + i] = pb ? post_beta[i] * s : 0.0f;
+            v[2 * CP + i] = pre && pre_gamma ? pre_gamma[i] : 1.0f;
+            v[3 * CP + i] = b ? pre_beta[i] : 0.0f;
+        }
+        const bool has[4] = {scale || (post && post_gamma), pb, pre && pre_gamma, b};
+        for (int i = 0; i < 4; i++) {
+            N->has[i] = has[i];
+            N->vectors += has[i];
         }
         N->mem.upload(be, v.data(), v.size() * 4, "BlockNorm parameters");
         for (int32_t s = 0; s < 3; s++)
-            for (bool vec : {false, true}) be->fn(bnorm_kernel(s, p->channels, vec));
+            for (int many = 0; many < 2; many++)
+                for (int vec = 0; vec < 2; vec++) N->fn[s][many][vec] = be->fn(bnorm_kernel(s, bnorm_shape(s, p->channels, many), vec));
         *out = N.release();
     });
 }

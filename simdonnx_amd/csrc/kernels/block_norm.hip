@@ -5,72 +5,72 @@
 //
 // Bound by memory: x, residual and gate are read once, h and y written once, and a row stays in registers in between.
 // All sums and norms in fp32, a variance as the mean square about the mean (a second sum over the registers, so a large
-// mean costs no digits); y is computed from h as summed in fp32, not from its rounded copy. TPR threads share a row; a
-// workgroup walks its rows with the parameter vectors in registers, since reading up to four fp32 vectors per row again
-// would move as much from L2 as the 16-bit rows do from memory.
+// mean costs no digits); y is computed from h as summed in fp32, not from its rounded copy.
+//
+// Two ways to hold a row, by how many rows there are:
+//  * many rows: a wave per row (64 threads, up to 4096 16-bit columns), no barriers; the parameter vectors, which would
+//    move as much from L2 per row as the row itself moves from memory, stand in LDS for all rows the workgroup walks.
+//  * few rows, or long ones: TPR threads per row, which shortens the one row's chain of loads, sums and stores; the
+//    parameters stay in registers (or, for the longest rows, are read where they are used).
 #include "qrows.h"
 
 enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
+enum { PAR_LDS, PAR_REG, PAR_MEM };  // where the parameter vectors are
 
 // CH chunks of E values per thread; VEC: chunk j of thread t is columns (j TPR + t) E .. + E - 1 as one 16-byte access
 // (rows on 16-byte boundaries, c a multiple of E), else value e of it is column (j E + e) TPR + t on its own
 template <typename T, int TPR, int CH, bool VEC> struct Row {
     static constexpr int E = 16 / sizeof(T), N = CH * E;
-    typedef vec_t<T, E> TV;
-    SOX_DEV int col(int t, int i) { return VEC ? (i / E * TPR + t) * E + i % E : i * TPR + t; }
-    SOX_DEV void load(const T* __restrict__ p, int t, int c, float (&v)[N]) {
-        if constexpr (VEC) {
+    typedef vec_t<T, E> TE;
+    TE v[CH];
+    SOX_DEV int col(int t, int j, int e) { return VEC ? (j * TPR + t) * E + e : (j * E + e) * TPR + t; }
+    __device__ __forceinline__ void load(const T* __restrict__ p, int t, int c) {
 #pragma unroll
-            for (int j = 0; j < CH; j++) {
-                const int k = (j * TPR + t) * E;
-                const TV x = k < c ? *(const TV*)(p + k) : TV{};
+        for (int j = 0; j < CH; j++) {
+            if constexpr (VEC) {
+                v[j] = TE{};
+                if (col(t, j, 0) < c) v[j] = *(const TE*)(p + col(t, j, 0));
+            } else {
 #pragma unroll
-                for (int e = 0; e < E; e++) v[j * E + e] = (float)x[e];
+                for (int e = 0; e < E; e++) v[j][e] = col(t, j, e) < c ? p[col(t, j, e)] : (T)0.0f;
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = col(t, i) < c ? (float)p[col(t, i)] : 0.0f;
         }
     }
-    SOX_DEV void store(T* __restrict__ p, int t, int c, const float (&v)[N]) {
-        if constexpr (VEC) {
+    SOX_DEV void store(T* __restrict__ p, int t, int c, const float (&f)[N]) {
 #pragma unroll
-            for (int j = 0; j < CH; j++) {
-                const int k = (j * TPR + t) * E;
-                TV x;
+        for (int j = 0; j < CH; j++) {
+            if constexpr (VEC) {
+                TE o;
 #pragma unroll
-                for (int e = 0; e < E; e++) x[e] = (T)v[j * E + e];
-                if (k < c) *(TV*)(p + k) = x;
+                for (int e = 0; e < E; e++) o[e] = (T)f[j * E + e];
+                if (col(t, j, 0) < c) *(TE*)(p + col(t, j, 0)) = o;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (col(t, j, e) < c) p[col(t, j, e)] = (T)f[j * E + e];
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                if (col(t, i) < c) p[col(t, i)] = (T)v[i];
         }
     }
-    SOX_DEV void param(const float* __restrict__ p, int t, int c, float (&v)[N]) {
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = col(t, i) < c ? p[col(t, i)] : 0.0f;
-    }
-    // columns c .. round_up(c, 16) - 1 hold zeros (v is 0 there)
-    SOX_DEV void store8(int8_t* __restrict__ p, int t, int c, const float (&v)[N], const RowQuant<half_t>& rq) {
+    // columns c .. round_up(c, 16) - 1 hold zeros (f is 0 there)
+    SOX_DEV void store8(int8_t* __restrict__ p, int t, int c, const float (&f)[N], const RowQuant<half_t>& rq) {
         const int c16 = (c + 15) & ~15;
-        if constexpr (VEC) {
 #pragma unroll
-            for (int j = 0; j < CH; j++) {
-                const int k = (j * TPR + t) * E;
+        for (int j = 0; j < CH; j++) {
+            if constexpr (VEC) {
+                uint32_t w[E / 4];
 #pragma unroll
-                for (int w = 0; w < E / 4; w++) {
-                    uint32_t b = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) b |= (uint32_t)(RowQuant<half_t>::q(v[j * E + 4 * w + e], rq) & 255) << (8 * e);
-                    if (k + 4 * w < c16) *(uint32_t*)(p + k + 4 * w) = b;
+                for (int i = 0; i < E / 4; i++) w[i] = RowQuant<half_t>::q4(&f[j * E + 4 * i], rq);
+                if (col(t, j, 0) < c16) {
+                    if constexpr (E == 8)
+                        *(uint2*)(p + col(t, j, 0)) = make_uint2(w[0], w[1]);
+                    else
+                        *(uint32_t*)(p + col(t, j, 0)) = w[0];
                 }
-            }
-        } else {
+            } else {
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                if (col(t, i) < c16) p[col(t, i)] = (int8_t)RowQuant<half_t>::q(v[i], rq);
+                for (int e = 0; e < E; e++)
+                    if (col(t, j, e) < c16) p[col(t, j, e)] = (int8_t)RowQuant<half_t>::q(f[j * E + e], rq);
+            }
         }
     }
 };
@@ -78,120 +78,181 @@ template <typename T, int TPR, int CH, bool VEC> struct Row {
 // Sum (maximum) over the TPR threads of a row. Each reduction over several waves has an LDS row of its own, two sets
 // in turn per row walked, so one barrier per reduction is enough: a set is written again only after the barriers of
 // the row in between.
-template <int TPR> SOX_DEV float row_sum(float v, float* lds) {
-    v = wave_sum<64>(v);
+template <int TPR, class V, class F> SOX_DEV V row_fold(V v, V* lds, F&& f) {
     if constexpr (TPR > 64) {
         constexpr int W = TPR / 64;
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = 0.0f;
+        v = lds[0];
 #pragma unroll
-        for (int w = 0; w < W; w++) v += lds[w];
+        for (int w = 1; w < W; w++) v = f(v, lds[w]);
     }
     return v;
+}
+template <int TPR> SOX_DEV float row_sum(float v, float* lds) {
+    return row_fold<TPR>(wave_sum(v), lds, [](float a, float b) { return a + b; });
 }
 template <int TPR> SOX_DEV uint32_t row_max(uint32_t v, uint32_t* lds) {
-    v = wave_max<64>(v);
-    if constexpr (TPR > 64) {
-        constexpr int W = TPR / 64;
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0;
-#pragma unroll
-        for (int w = 0; w < W; w++) v = max(v, lds[w]);
-    }
-    return v;
+    return row_fold<TPR>(wave_max(v), lds, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
-// KEEP: the parameter vectors stay in registers for all rows (where they fit; else they come from L2 row by row)
-template <typename T, int TPR, int CH, bool VEC, bool KEEP> SOX_DEV void bnorm_body(const sox_bnorm_args& p) {
+template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_body(const sox_bnorm_args& p) {
     typedef Row<T, TPR, CH, VEC> R;
-    constexpr int N = R::N, BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
+    constexpr int E = R::E, N = R::N, BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR, CAP = TPR * N;
+    static_assert(PAR != PAR_LDS || TPR == 64, "a wave per row");
     __shared__ float lds[2][5][BLOCK / 64];
+    extern __shared__ float par_lds[];  // PAR_LDS: the vectors there are, CAP floats each
     const int t = threadIdx.x % TPR, c = p.c;
     const float inv_c = 1.0f / (float)c;
-    constexpr int NK = KEEP ? N : 1;
-    float pg[NK], pb[NK], g[NK], b[NK];
-    if constexpr (KEEP) {
-        R::param(p.pg, t, c, pg);
-        R::param(p.pb, t, c, pb);
-        R::param(p.g, t, c, g);
-        R::param(p.b, t, c, b);
+
+    // The parameter vectors: k = 0 post gamma * scale, 1 post beta * scale, 2 pre gamma, 3 pre beta (null: 1, 0, 1, 0)
+    const float* const vec[4] = {p.pg, p.pb, p.g, p.b};
+    int slot[4];
+    float kept[PAR == PAR_REG ? 4 : 1][PAR == PAR_REG ? N : 1];
+    auto from_memory = [&](const float* v, int j, float (&o)[E]) __attribute__((always_inline)) {
+        if constexpr (VEC) {
+            const bool in = R::col(t, j, 0) < c;
+#pragma unroll
+            for (int i = 0; i < E / 4; i++) {
+                float4v f = {};
+                if (in) f = *(const float4v*)(v + R::col(t, j, 4 * i));
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[4 * i + e] = f[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = R::col(t, j, e) < c ? v[R::col(t, j, e)] : 0.0f;
+        }
+    };
+    if constexpr (PAR == PAR_REG) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (vec[k])
+#pragma unroll
+                for (int j = 0; j < CH; j++) {
+                    float o[E];
+                    from_memory(vec[k], j, o);
+#pragma unroll
+                    for (int e = 0; e < E; e++) kept[k][j * E + e] = o[e];
+                }
     }
-    // (the empty asm: without it the loads are moved out of the row loop, into registers that are not there)
-    auto fresh = [&](const float* vec) {
-        if constexpr (!KEEP) asm volatile("" : "+s"(vec));
-        return vec;
+    if constexpr (PAR == PAR_LDS) {
+        // VEC: the chunks' first four values of all chunks, then their second four, so 16-byte reads of consecutive lanes
+        // are consecutive
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            slot[k] = n * CAP;
+            if (!vec[k]) continue;
+            n++;
+            for (int i = threadIdx.x; i < CAP; i += BLOCK) {
+                const int at = VEC ? i % E / 4 * (CAP / (E / 4)) + i / E * 4 + i % 4 : i;
+                par_lds[slot[k] + at] = i < c ? vec[k][i] : 0.0f;
+            }
+        }
+        __syncthreads();
+    }
+    // the values of chunk j of vector k
+    auto par = [&](int k, int j, float (&o)[E]) __attribute__((always_inline)) {
+        if constexpr (PAR == PAR_REG) {
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = kept[k][j * E + e];
+        } else if constexpr (PAR == PAR_LDS && VEC) {
+#pragma unroll
+            for (int i = 0; i < E / 4; i++) {
+                const float4v f = *(const float4v*)(par_lds + slot[k] + i * (CAP / (E / 4)) + (j * TPR + t) * 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[4 * i + e] = f[e];
+            }
+        } else if constexpr (PAR == PAR_LDS) {
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = par_lds[slot[k] + R::col(t, j, e)];
+        } else {
+            const float* v = vec[k];
+            asm volatile("" : "+s"(v));  // (read here, not ahead of the rows into registers that are not there)
+            from_memory(v, j, o);
+        }
     };
-    auto at = [&](const float* vec, const float (&kept)[NK], int i) {
-        if constexpr (KEEP) return kept[i];
-        return R::col(t, i) < c ? vec[R::col(t, i)] : 0.0f;
-    };
-    auto norm = [&](float (&v)[N], int kind, float eps, const float* gp, const float (&ga)[NK], const float* bp,
-                    const float (&be)[NK], float* l0, float* l1) __attribute__((always_inline)) {
-        float s = 0.0f;
+    // v (zeros past column c) normed in place; the vectors k and k + 1
+    auto norm = [&](float (&v)[N], int kind, float eps, int k, float* l0, float* l1) __attribute__((always_inline)) {
         if (kind == NORM_LAYER) {
+            float s = 0.0f;
 #pragma unroll
             for (int i = 0; i < N; i++) s += v[i];
             const float mean = row_sum<TPR>(s, l0) * inv_c;
 #pragma unroll
-            for (int i = 0; i < N; i++) v[i] = R::col(t, i) < c ? v[i] - mean : 0.0f;
-            s = 0.0f;
+            for (int i = 0; i < N; i++) v[i] = R::col(t, i / E, i % E) < c ? v[i] - mean : 0.0f;
         }
+        float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; i++) s = __builtin_fmaf(v[i], v[i], s);
         const float r = 1.0f / sqrtf(row_sum<TPR>(s, l1) * inv_c + eps);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            v[i] = __builtin_fmaf(v[i] * r, at(gp, ga, i), at(bp, be, i));
-            if constexpr (!KEEP)
-                if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // a few parameters at a time
-        }
+        for (int i = 0; i < N; i++) v[i] *= r;
+    };
+    // v * gamma (+ beta), the vectors k and k + 1
+    auto affine = [&](float (&v)[N], int k) __attribute__((always_inline)) {
+        if (vec[k])
+#pragma unroll
+            for (int j = 0; j < CH; j++) {
+                float o[E];
+                par(k, j, o);
+#pragma unroll
+                for (int e = 0; e < E; e++) v[j * E + e] *= o[e];
+                if constexpr (PAR == PAR_MEM) __builtin_amdgcn_sched_barrier(0);
+            }
+        if (vec[k + 1])
+#pragma unroll
+            for (int j = 0; j < CH; j++) {
+                float o[E];
+                par(k + 1, j, o);
+#pragma unroll
+                for (int e = 0; e < E; e++) v[j * E + e] += o[e];
+                if constexpr (PAR == PAR_MEM) __builtin_amdgcn_sched_barrier(0);
+            }
     };
     int set = 0;
     for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * RPB, set ^= 1) {
-        float h[N], a[N];
+        R rr, gr;  // all of a row's loads go out together
+        float h[N];
         if (p.x) {
-            R::load((const T*)p.x + row * p.ldx, t, c, a);
-            float ga[KEEP ? N : 1];
-            // all of a row's loads go out together where registers allow
-            if constexpr (KEEP) {
-                if (p.gate) R::load((const T*)p.gate + row / p.gate_group * p.ldg, t, c, ga);
-                if (p.residual) R::load((const T*)p.residual + row * p.ldr, t, c, h);
+            R xr;
+            xr.load((const T*)p.x + row * p.ldx, t, c);
+            if (p.residual) rr.load((const T*)p.residual + row * p.ldr, t, c);
+            if (p.gate) gr.load((const T*)p.gate + row / p.gate_group * p.ldg, t, c);
+#pragma unroll
+            for (int i = 0; i < N; i++) h[i] = (float)xr.v[i / E][i % E];
+            if (p.post != NORM_NONE) norm(h, p.post, p.post_eps, 0, lds[set][0], lds[set][1]);
+            affine(h, 0);
+            if (p.gate) {
+                // (one choice per row, each a straight line)
+                auto gated = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < N; i++) h[i] *= f((float)gr.v[i / E][i % E]);
+                };
+                if (p.gate_act == SOX_ACT_NONE)
+                    gated([](float g) { return g; });
+                else if (p.gate_act == SOX_ACT_RELU)
+                    gated([](float g) { return q_out<float, SOX_ACT_RELU>(g); });
+                else if (p.gate_act == SOX_ACT_GELU)
+                    gated([](float g) { return q_out<float, SOX_ACT_GELU>(g); });
+                else
+                    gated([&](float g) { return q_out<float, Q_ACT_GATES>(g, p.gate_act); });
             }
-            if (p.post != NORM_NONE) {
-                norm(a, p.post, p.post_eps, fresh(p.pg), pg, fresh(p.pb), pb, lds[set][0], lds[set][1]);
-            } else {
-                const float* sc = fresh(p.pg);
+            if (p.residual)
 #pragma unroll
-                for (int i = 0; i < N; i++) a[i] *= at(sc, pg, i);
-            }
-            if constexpr (KEEP) {
-                if (p.gate)
-#pragma unroll
-                    for (int i = 0; i < N; i++) a[i] *= q_act<float>(ga[i], p.gate_act);
-#pragma unroll
-                for (int i = 0; i < N; i++) h[i] = p.residual ? __builtin_fmaf(p.res_scale, h[i], a[i]) : a[i];
-            } else {
-                __builtin_amdgcn_sched_barrier(0);
-                if (p.gate) {
-                    R::load((const T*)p.gate + row / p.gate_group * p.ldg, t, c, h);
-#pragma unroll
-                    for (int i = 0; i < N; i++) a[i] *= q_act<float>(h[i], p.gate_act);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                if (p.residual) R::load((const T*)p.residual + row * p.ldr, t, c, h);
-#pragma unroll
-                for (int i = 0; i < N; i++) h[i] = p.residual ? __builtin_fmaf(p.res_scale, h[i], a[i]) : a[i];
-            }
+                for (int i = 0; i < N; i++) h[i] = __builtin_fmaf(p.res_scale, (float)rr.v[i / E][i % E], h[i]);
         } else {
-            R::load((const T*)p.residual + row * p.ldr, t, c, h);
+            rr.load((const T*)p.residual + row * p.ldr, t, c);
 #pragma unroll
-            for (int i = 0; i < N; i++) h[i] *= p.res_scale;
+            for (int i = 0; i < N; i++) h[i] = p.res_scale * (float)rr.v[i / E][i % E];
         }
         if (p.h) R::store((T*)p.h + row * p.ldh, t, c, h);
         if (!p.y && !p.q) continue;
-        if (p.pre != NORM_NONE) norm(h, p.pre, p.pre_eps, fresh(p.g), g, fresh(p.b), b, lds[set][2], lds[set][3]);
+        if (p.pre != NORM_NONE) {
+            norm(h, p.pre, p.pre_eps, 2, lds[set][2], lds[set][3]);
+            affine(h, 2);
+        }
         if (p.y) R::store((T*)p.y + row * p.ldy, t, c, h);
         if (p.q) {
             uint32_t m = 0;
@@ -204,18 +265,19 @@ template <typename T, int TPR, int CH, bool VEC, bool KEEP> SOX_DEV void bnorm_b
     }
 }
 
-#define SOX_BNORM_V(NAME, T, TPR, CH, SUFFIX, VEC, KEEP)                                                                  \
+#define SOX_BNORM_V(NAME, T, TPR, CH, SUFFIX, VEC, PAR)                                                                    \
     extern "C" __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) sox_bnorm_##NAME##_t##TPR##c##CH##SUFFIX(sox_bnorm_args p) { \
-        bnorm_body<T, TPR, CH, VEC, KEEP>(p);                                                                               \
+        bnorm_body<T, TPR, CH, VEC, PAR>(p);                                                                                \
     }
-#define SOX_BNORM(NAME, T, TPR, CH, KEEP) \
-    SOX_BNORM_V(NAME, T, TPR, CH, v, true, KEEP) SOX_BNORM_V(NAME, T, TPR, CH, s, false, KEEP)
-// threads of a row and chunks of a thread: 16-bit rows of up to 512, 1024, 2048, 4096, 8192, 16384 columns ...
+#define SOX_BNORM(NAME, T, TPR, CH, PAR) SOX_BNORM_V(NAME, T, TPR, CH, v, true, PAR) SOX_BNORM_V(NAME, T, TPR, CH, s, false, PAR)
+// threads of a row and chunks of a thread: a wave per row up to 4096 16-bit columns (2048 fp32) ...
 #define SOX_BNORM_16(NAME, T)                                                                                             \
-    SOX_BNORM(NAME, T, 64, 1, true) SOX_BNORM(NAME, T, 64, 2, true) SOX_BNORM(NAME, T, 256, 1, true)                      \
-    SOX_BNORM(NAME, T, 256, 2, true) SOX_BNORM(NAME, T, 1024, 1, true) SOX_BNORM(NAME, T, 512, 4, false)
+    SOX_BNORM(NAME, T, 64, 1, PAR_LDS) SOX_BNORM(NAME, T, 64, 2, PAR_LDS) SOX_BNORM(NAME, T, 64, 4, PAR_LDS)              \
+    SOX_BNORM(NAME, T, 64, 8, PAR_LDS) SOX_BNORM(NAME, T, 256, 1, PAR_REG) SOX_BNORM(NAME, T, 256, 2, PAR_REG)            \
+    SOX_BNORM(NAME, T, 1024, 1, PAR_REG) SOX_BNORM(NAME, T, 512, 4, PAR_MEM)
 SOX_BNORM_16(f16, half_t)
 SOX_BNORM_16(bf16, bf16_t)
 // ... and the same in fp32, twice the chunks
-SOX_BNORM(f32, float, 64, 2, true) SOX_BNORM(f32, float, 64, 4, true) SOX_BNORM(f32, float, 256, 2, true)
-SOX_BNORM(f32, float, 256, 4, true) SOX_BNORM(f32, float, 1024, 2, true) SOX_BNORM(f32, float, 512, 8, false)
+SOX_BNORM(f32, float, 64, 2, PAR_LDS) SOX_BNORM(f32, float, 64, 4, PAR_LDS) SOX_BNORM(f32, float, 64, 8, PAR_LDS)
+SOX_BNORM(f32, float, 256, 2, PAR_REG) SOX_BNORM(f32, float, 256, 4, PAR_REG) SOX_BNORM(f32, float, 1024, 2, PAR_REG)
+SOX_BNORM(f32, float, 512, 8, PAR_MEM)

@@ -41,53 +41,58 @@ SOX_DEV void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(0xc07f); }
 // LDS chunk swizzle for rows of CPR 16-byte chunks: 16 consecutive rows read at one chunk hit 16 distinct bank groups
 template <int CPR> SOX_DEV int swz(int r) { return (r / (16 / CPR)) % CPR; }
 
-// One 32 x 32 block of scaled sums from a wave's LDS stage to memory. The stage holds 32 rows of 8 16-byte chunks of
-// fp32, chunk c of row r at slot c ^ r / 2 % 8: the writers (a row per lane) and the readers (a row per 4 or 8 lanes)
-// both spread over all banks.
-SOX_DEV int stage_at(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7)) << 4); }
+// A wave's stage for outputs on their way to memory, 2 KiB: a 32 x 32 block of 16-bit values (rows of 4 16-byte chunks, chunk
+// c of row r at slot c ^ r / 4 % 4), or 16 rows of a block of fp32 ones (8 chunks, slot c ^ r / 2). The writers (a row per
+// lane) and the readers (a row per 4 or 8 lanes) both spread over all banks, and the stores are whole row segments.
+constexpr int STG_BYTES = 2048;
+template <typename T> SOX_DEV int stage_at(int r, int c) {
+    return sizeof(T) == 2 ? r * 64 + ((c ^ ((r >> 2) & 3)) << 4) : r * 128 + ((c ^ (r >> 1)) << 4);
+}
 
-template <typename T>
-SOX_DEV void store_block(const sox_qgemm_args& p, const unsigned char* stg, int m0, int n0) {
-    const int lane = threadIdx.x & 63;
-    T* __restrict__ Y = (T*)p.y;
-    const T* __restrict__ R = (const T*)p.add;
-    if (p.vec & 1) {  // uniform: 16-byte row chunks
-        constexpr int E = 16 / sizeof(T), PER = 32 / E;  // elements of a chunk, chunks of a row
-        typedef vec_t<T, E> TE;
+// A block's rows between memory at (m0, n0) and the stage: 16-byte chunks where the rows allow it (uniform), else single
+// elements, a half wave per row, in a loop that is not unrolled (the ragged form should not be most of the code).
+// LOAD: the residual's into the stage (zeros outside), else the stage's to the output.
+template <typename T, bool LOAD>
+SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, bool vec, unsigned char* stg, int m0, int n0, int lane) {
+    constexpr int E = 16 / sizeof(T), PER = 32 / E, ROWS = STG_BYTES / (32 * sizeof(T));  // elements of a chunk, chunks of a row
+    typedef vec_t<T, E> TE;
+    if (vec) {
 #pragma unroll
-        for (int t = 0; t < 32 * PER / 64; t++) {
-            const int idx = t * 64 + lane, r = idx / PER, u = idx % PER;
-            const int m = m0 + r, n = n0 + u * E;
-            const bool in = m < p.m && n < p.n;
-            float v[E];
-#pragma unroll
-            for (int c = 0; c < E / 4; c++) {
-                const float4v f = *(const float4v*)(stg + stage_at(r, u * (E / 4) + c));
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[4 * c + e] = f[e];
+        for (int t = 0; t < ROWS * PER / 64; t++) {
+            const int idx = t * 64 + lane, r = idx / PER, u = idx % PER, m = m0 + r, n = n0 + u * E;
+            TE* s = (TE*)(stg + stage_at<T>(r, u));
+            T* g = base + (int64_t)m * ld + n;
+            if constexpr (LOAD) {
+                TE v = {};
+                if (m < M && n < N) v = *(const TE*)g;
+                *s = v;
+            } else {
+                const TE v = *s;
+                if (m < M && n < N) *(TE*)g = v;
             }
-            if (R) {
-                const TE rv = in ? *(const TE*)(R + (int64_t)m * p.ldr + n) : TE{};
-#pragma unroll
-                for (int e = 0; e < E; e++) v[e] += (float)rv[e];
-            }
-            TE o;
-#pragma unroll
-            for (int e = 0; e < E; e++) o[e] = (T)q_act<T>(v[e], p.act);
-            if (in) *(TE*)(Y + (int64_t)m * p.ldy + n) = o;
         }
     } else {
-#pragma unroll 4
-        for (int t = 0; t < 16; t++) {
-            const int idx = t * 64 + lane, r = idx / 32, c = idx % 32;
-            const int m = m0 + r, n = n0 + c;
-            if (m < p.m && n < p.n) {
-                float v = *(const float*)(stg + stage_at(r, c / 4) + (c % 4) * 4);
-                if (R) v += (float)R[(int64_t)m * p.ldr + n];
-                Y[(int64_t)m * p.ldy + n] = (T)q_act<T>(v, p.act);
+#pragma unroll 1
+        for (int t = 0; t < ROWS / 2; t++) {
+            const int idx = t * 64 + lane, r = idx / 32, c = idx % 32, m = m0 + r, n = n0 + c;
+            T* s = (T*)(stg + stage_at<T>(r, c / E) + c % E * sizeof(T));
+            T* g = base + (int64_t)m * ld + n;
+            if constexpr (LOAD) {
+                T v = (T)0.0f;
+                if (m < M && n < N) v = *g;
+                *s = v;
+            } else {
+                const T v = *s;
+                if (m < M && n < N) *g = v;
             }
         }
     }
+}
+// Lanes read what others wrote to the wave's stage, or overwrite what others have read
+SOX_DEV void stage_turn() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 template <typename T, int BM, int BN, int BK, int WM, int WN, int STAGES, int NW, int GM>
@@ -104,12 +109,12 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
     static_assert(A_IT * 1024 * NW == A_BYTES && B_IT * 1024 * NW == B_BYTES, "DMA split");
     static_assert(BM % 64 == 0 && BN <= 256 && NW >= 2, "scale DMA split");
     static_assert(STAGES >= 2 && (STAGES - 1) * LOADS < 64, "vmcnt range");
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGE_BYTES * STAGES + SC_BYTES * SCB + NW * 4096];
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGE_BYTES * STAGES + SC_BYTES * SCB + NW * STG_BYTES];
     unsigned char* const sc_mem = smem + STAGE_BYTES * STAGES;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, hl = lane >> 5;
-    unsigned char* const stg = sc_mem + SC_BYTES * SCB + wave * 4096;
+    unsigned char* const stg = sc_mem + SC_BYTES * SCB + wave * STG_BYTES;
     const int M = p.m, k16 = p.k16;
     const int tiles_n = p.tiles_n, tiles_m = (M + BM - 1) / BM, ntiles = tiles_m * tiles_n;
     const int wm0 = (wave / WAVES_N) * WM, wn0 = (wave % WAVES_N) * WN;
@@ -191,32 +196,74 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
         static_for<0, TJ * TI>([&](auto ji) { acc[decltype(ji)::value / TI][decltype(ji)::value % TI] = (int16v)0; });
     };
     int m_kt = 0, m_tile = vid, m_seq = 0;  // the tile being multiplied
+    // The tile's outputs, block by block: scaled, joined with the residual and activated in registers, staged and stored.
+    // One copy of this with its choices inside, none of them per element: a choice per element, or a copy per form,
+    // multiplied the code until its instruction fetches took most of a short product's time and registers ran out.
     auto epilogue = [&]() __attribute__((always_inline)) {
         int bm, bn;
         tile_origin(m_tile, bm, bn);
         const unsigned char* sc = sc_mem + (m_seq % SCB) * SC_BYTES;
-        static_for<0, TJ * TI>([&](auto ji) {
+        const bool vec = p.vec & 1;
+        static_for<0, TJ * TI>([&](auto ji) __attribute__((always_inline)) {
             constexpr int j = decltype(ji)::value / TI, i = decltype(ji)::value % TI;
+            constexpr int PARTS = sizeof(T) == 2 ? 1 : 2, ROWS = 32 / PARTS;
+            typedef vec_t<T, 4> T4;
+            const int m0 = bm + wm0 + i * 32, n0 = bn + wn0 + j * 32;
             const float xs = *(const float*)(sc + BN * 8 + (wm0 + i * 32 + l32) * 4);
-            static_for<0, 4>([&](auto qq) {
+            float val[16];
+            static_for<0, 4>([&](auto qq) __attribute__((always_inline)) {
                 constexpr int q = decltype(qq)::value;
                 const int n = wn0 + j * 32 + 8 * q + 4 * hl;
                 const float4v ws = *(const float4v*)(sc + n * 4), bs = *(const float4v*)(sc + BN * 4 + n * 4);
-                float4v v;
-                static_for<0, 4>([&](auto ee) {
-                    constexpr int e = decltype(ee)::value;
-                    v[e] = __builtin_fmaf((float)acc[j][i][4 * q + e] * ws[e], xs, bs[e]);
-                });
-                *(float4v*)(stg + stage_at(l32, 2 * q + hl)) = v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) val[4 * q + e] = __builtin_fmaf((float)acc[j][i][4 * q + e] * ws[e], xs, bs[e]);
             });
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // other lanes' rows are read back
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            store_block<T>(p, stg, bm + wm0 + i * 32, bn + wn0 + j * 32);
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // the next block overwrites the stage
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            __builtin_amdgcn_sched_barrier(0);
+            // the lane's four of the stage: 16-bit rows 64 bytes, fp32 ones 128 (and half of them at a time)
+            auto at = [&](int q) __attribute__((always_inline)) {
+                return sizeof(T) == 2 ? (T4*)(stg + stage_at<T>(l32, q) + hl * 8) : (T4*)(stg + stage_at<T>(l32 % ROWS, 2 * q + hl));
+            };
+            if (p.add) {
+#pragma unroll
+                for (int half = 0; half < PARTS; half++) {
+                    move_rows<T, true>((T*)p.add, p.ldr, M, p.n, vec, stg, m0 + half * ROWS, n0, lane);
+                    stage_turn();
+                    if (PARTS == 1 || l32 / ROWS == half) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const T4 r = *at(q);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) val[4 * q + e] += (float)r[e];
+                        }
+                    }
+                    stage_turn();
+                }
+            }
+            if (p.act == SOX_ACT_GELU) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) val[e] = q_out<T, SOX_ACT_GELU>(val[e]);
+            } else if (p.act == SOX_ACT_RELU) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) val[e] = q_out<T, SOX_ACT_RELU>(val[e]);
+            } else if (p.act != SOX_ACT_NONE) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) val[e] = q_out<T, Q_ACT_GATES>(val[e], p.act);
+            }
+#pragma unroll
+            for (int half = 0; half < PARTS; half++) {
+                if (PARTS == 1 || l32 / ROWS == half) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        T4 h;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) h[e] = (T)val[4 * q + e];
+                        *at(q) = h;
+                    }
+                }
+                stage_turn();
+                move_rows<T, false>((T*)p.y, p.ldy, M, p.n, vec, stg, m0 + half * ROWS, n0, lane);
+                stage_turn();
+            }
+            __builtin_amdgcn_sched_barrier(0);  // one block at a time: bounded register pressure
         });
         m_tile += G;
         m_seq++;
@@ -276,13 +323,19 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
     }
 }
 
-#define SOX_QGEMM(TILE, BM, BN, BK, WM, WN, ST, NW, OCC, GM)                                                     \
-    extern "C" __global__ void __launch_bounds__(64 * NW, OCC) sox_qgemm_f16_##TILE(sox_qgemm_args p) {        \
-        qgemm_body<half_t, BM, BN, BK, WM, WN, ST, NW, GM>(p);                                                 \
-    }                                                                                                          \
-    extern "C" __global__ void __launch_bounds__(64 * NW, OCC) sox_qgemm_bf16_##TILE(sox_qgemm_args p) {       \
-        qgemm_body<bf16_t, BM, BN, BK, WM, WN, ST, NW, GM>(p);                                                 \
-    }                                                                                                          \
-    extern "C" __global__ void __launch_bounds__(64 * NW, OCC) sox_qgemm_f32_##TILE(sox_qgemm_args p) {        \
-        qgemm_body<float, BM, BN, BK, WM, WN, ST, NW, GM>(p);                                                  \
+// One kernel per storage type and tiling, named BMxBN tile, wNW waves, kBK bytes of K per slice, sSTAGES; WM x WN of a tile
+// to a wave, OCC waves per SIMD, GM M-tiles to a group.
+#define SOX_QGEMM(NAME, T, TILE, BM, BN, BK, WM, WN, ST, NW, OCC, GM)                                       \
+    extern "C" __global__ void __launch_bounds__(64 * NW, OCC) sox_qgemm_##NAME##_##TILE(sox_qgemm_args p) { \
+        qgemm_body<T, BM, BN, BK, WM, WN, ST, NW, GM>(p);                                                   \
     }
+#define SOX_QGEMM_TILES(NAME, T)                                             \
+    SOX_QGEMM(NAME, T, 256x256_w8k128s2, 256, 256, 128, 128, 64, 2, 8, 2, 4) \
+    SOX_QGEMM(NAME, T, 256x128_w8k128s2, 256, 128, 128, 64, 64, 2, 8, 2, 4) \
+    SOX_QGEMM(NAME, T, 256x192_w8k128s2, 256, 192, 128, 64, 96, 2, 8, 2, 4) \
+    SOX_QGEMM(NAME, T, 128x128_w4k128s2, 128, 128, 128, 64, 64, 2, 4, 2, 4) \
+    SOX_QGEMM(NAME, T, 128x192_w4k64s2, 128, 192, 64, 64, 96, 2, 4, 2, 4)   \
+    SOX_QGEMM(NAME, T, 128x64_w4k128s2, 128, 64, 128, 64, 32, 2, 4, 3, 4)   \
+    SOX_QGEMM(NAME, T, 64x128_w4k128s3, 64, 128, 128, 32, 64, 3, 4, 2, 4)   \
+    SOX_QGEMM(NAME, T, 64x64_w4k128s4, 64, 64, 128, 32, 32, 4, 4, 2, 4)     \
+    SOX_QGEMM(NAME, T, 64x64_w4k64s2, 64, 64, 64, 32, 32, 2, 4, 4, 4)

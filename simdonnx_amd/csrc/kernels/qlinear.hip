@@ -19,10 +19,6 @@ template <typename T, int E> SOX_DEV void load_values(const T* __restrict__ row,
     }
 }
 
-SOX_DEV uint32_t pack4(int a, int b, int c, int d) {
-    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
-}
-
 // ---- rows to 8 bits ----
 // TPR threads per row (a wave, or the workgroup for long rows). A thread keeps its first CH chunks of 16 bytes in
 // registers between the maximum and the rounding; what is past them (rows of more than CH * TPR * 16 bytes) is read
@@ -52,7 +48,7 @@ template <typename T, int TPR> SOX_DEV void qrows_body(const sox_qrows_args& p) 
 #pragma unroll
         for (int e = 0; e < E; e++) m = max(m, abs_bits(u[e]));
     }
-    m = wave_max<64>(m);
+    m = wave_max(m);
     if constexpr (TPR == 256) {
         if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = m;
         __syncthreads();
@@ -63,8 +59,7 @@ template <typename T, int TPR> SOX_DEV void qrows_body(const sox_qrows_args& p) 
     auto put = [&](int c, const float (&u)[E]) {
         uint32_t w[E / 4];
 #pragma unroll
-        for (int i = 0; i < E / 4; i++)
-            w[i] = pack4(Q::q(u[4 * i], rq), Q::q(u[4 * i + 1], rq), Q::q(u[4 * i + 2], rq), Q::q(u[4 * i + 3], rq));
+        for (int i = 0; i < E / 4; i++) w[i] = Q::q4(&u[4 * i], rq);
         if constexpr (E == 8)
             *(uint2*)(q + c * 8) = make_uint2(w[0], w[1]);
         else
@@ -139,8 +134,7 @@ template <typename T, bool FUSED, int S, int RB> SOX_DEV void qfew_body(const so
             for (int s = 0; s < S; s++)
 #pragma unroll
                 for (int c = 0; c < 4; c++)
-                    xf[s][0][c] = (int)pack4(Q::q(v[s][4 * c], rq), Q::q(v[s][4 * c + 1], rq), Q::q(v[s][4 * c + 2], rq),
-                                             Q::q(v[s][4 * c + 3], rq));
+                    xf[s][0][c] = (int)Q::q4(&v[s][4 * c], rq);
         } else {
 #pragma unroll
             for (int b = 0; b < RB; b++) {
@@ -167,7 +161,7 @@ template <typename T, bool FUSED, int S, int RB> SOX_DEV void qfew_body(const so
         for (int w = 0; w < waves; w++) sum += red[w][b][c * 17 + r];
         float v = __builtin_fmaf((float)sum * p.ws[n], FUSED ? xscale[r] : p.xs[row], p.bias[n]);
         if (p.add) v += (float)((const T*)p.add)[row * p.ldr + n];
-        ((T*)p.y)[row * p.ldy + n] = (T)q_act<T>(v, p.act);
+        ((T*)p.y)[row * p.ldy + n] = (T)q_out<T, Q_ACT_ANY>(v, p.act);
     }
 }
 

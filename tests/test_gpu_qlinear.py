@@ -14,7 +14,7 @@ from tests.layers import Matrix, linear64, quantize, rounded
 
 pytestmark = pytest.mark.gpu
 
-TILES = ["256x256_w8k64s3", "128x128_w4k64s2", "64x64_w4k64s2"]
+TILES = ["256x256_w8k128s2", "256x192_w8k128s2", "128x128_w4k128s2", "64x128_w4k128s3", "64x64_w4k128s4"]
 
 
 def weights8(seed, k, n):
@@ -93,7 +93,7 @@ def test_tiles(hip, monkeypatch, tile, storage, rows, k, n, pad, skip):
 def test_many_tiles_per_workgroup(hip, monkeypatch, tile):
     """More tiles than workgroups, with one slice of K each: a workgroup's slices run several tiles ahead."""
     monkeypatch.setenv("SIMDONNX_HIP_QGEMM", tile)
-    rows, n = {"256x256_w8k64s3": (12000, 3300), "128x128_w4k64s2": (9000, 2500), "64x64_w4k64s2": (4200, 2200)}[tile]
+    rows, n = {"256": (12000, 3300), "128": (9000, 2500), "64x": (4200, 2200)}[tile[:3].rstrip("x") if tile[0] != "6" else "64x"]
     print(f"[gpu] qlinear {tile} {rows} x 40 -> {n}", flush=True)
     both_ways(hip, 2100, rows, 40, n, "bf16")
 
