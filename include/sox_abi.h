@@ -592,16 +592,15 @@ typedef struct sox_qgemm_args {
     int32_t m, n, k, k16;
     int32_t kb, nb;     /* 32-k blocks of a column block, column blocks */
     int32_t tiles_n, act;
-    int32_t vec;        /* bit0: y (and residual) rows on 16-byte boundaries, n whole chunks; bit1: x rows too */
+    int32_t vec;        /* bit0: y (and residual) rows on 16-byte boundaries; bit1: x rows too */
     int32_t pad_;
 } sox_qgemm_args;
 
 /* Norms before and after a transformer block (sox_bnorm_*): for each row
  *   h = res_scale * residual + act(gate) * (post(x) * scale),  y = pre(h)
  * post / pre: SOX_NORM_*. pg = post gamma * scale, pb = post beta * scale, g / b: the
- * pre norm's (null: ones, zeros), 16-byte aligned. The instances with a wave per row (t64) take dynamic LDS: the vectors there
- * are x columns they hold x 4 bytes. y in the storage
- * type, or (q) as 8-bit rows with their scales (as sox_qrows_args). gate row of row r: r / gate_group. */
+ * pre norm's (null: ones, zeros), 16-byte aligned. The instances with at most 64 threads per row take dynamic LDS: the
+ * vectors there are x columns they hold x 4 bytes. y in the storage type, or (q) as 8-bit rows with their scales (as sox_qrows_args). gate row of row r: r / gate_group. */
 typedef struct sox_bnorm_args {
     const void* x;         /* or null: no branch */
     const void* residual;  /* or null: 0 */

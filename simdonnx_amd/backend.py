@@ -618,6 +618,7 @@ class HipQuantLinear:
                                                         columns, ctypes.byref(h)), "QuantLinear")
         self.h, self.inner, self.columns = h, inner, columns
         self.pitch = N.backend().sox_qlinear_pitch(h)
+        self._run, self._run_quantized = N.backend().sox_qlinear_run, N.backend().sox_qlinear_run_quantized
 
     def workspace(self, rows: int) -> int:
         """Bytes of workspace that `run` needs at this many rows."""
@@ -627,19 +628,21 @@ class HipQuantLinear:
             act: str = "none", residual: Optional[int] = None, ldr: Optional[int] = None, workspace: Optional[int] = None,
             workspace_bytes: int = 0, stream: Optional[int] = None):
         """y [rows, columns] from floating rows x [rows, inner]."""
-        N.check(N.backend().sox_qlinear_run(self.h, stream, STORAGE[storage], x, self.inner if ldx is None else ldx, rows,
-                                            residual, self.columns if ldr is None else ldr, y,
-                                            self.columns if ldy is None else ldy, N.ACT[act], workspace, workspace_bytes),
-                "QuantLinear.Run")
+        rc = self._run(self.h, stream, STORAGE[storage], x, self.inner if ldx is None else ldx, rows, residual,
+                       self.columns if ldr is None else ldr, y, self.columns if ldy is None else ldy, N.ACT[act], workspace,
+                       workspace_bytes)
+        if rc:
+            N.check(rc, "QuantLinear.Run")
 
     def run_quantized(self, q: int, scales: int, rows: int, y: int, storage: str = "f16", ldq: Optional[int] = None,
                       ldy: Optional[int] = None, act: str = "none", residual: Optional[int] = None,
                       ldr: Optional[int] = None, stream: Optional[int] = None):
         """y [rows, columns] from 8-bit rows (`pitch` bytes apart unless ldq says so) and their scales [rows]."""
-        N.check(N.backend().sox_qlinear_run_quantized(self.h, stream, q, self.pitch if ldq is None else ldq, scales, rows,
-                                                      STORAGE[storage], residual, self.columns if ldr is None else ldr, y,
-                                                      self.columns if ldy is None else ldy, N.ACT[act]),
-                "QuantLinear.RunQuantized")
+        rc = self._run_quantized(self.h, stream, q, self.pitch if ldq is None else ldq, scales, rows, STORAGE[storage],
+                                 residual, self.columns if ldr is None else ldr, y, self.columns if ldy is None else ldy,
+                                 N.ACT[act])
+        if rc:
+            N.check(rc, "QuantLinear.RunQuantized")
 
     def close(self):
         if self.h:
@@ -668,6 +671,7 @@ class HipBlockNorm:
         N.check(N.backend().sox_block_norm_create(backend.h, ctypes.byref(p), *[_address(a) for a in v], ctypes.byref(h)),
                 "BlockNorm")
         self.h, self.channels = h, channels
+        self._run, self._run_quantized = N.backend().sox_block_norm_run, N.backend().sox_block_norm_run_quantized
 
     def run(self, residual: Optional[int], rows: int, storage: str = "f16", ldr: Optional[int] = None,
             x: Optional[int] = None, ldx: Optional[int] = None, gate: Optional[int] = None, ldg: Optional[int] = None,
@@ -675,9 +679,10 @@ class HipBlockNorm:
             ldy: Optional[int] = None, stream: Optional[int] = None):
         """h and y [rows, channels] (either may be left out) from the residual and the branch x."""
         c = self.channels
-        N.check(N.backend().sox_block_norm_run(self.h, stream, STORAGE[storage], rows, residual, c if ldr is None else ldr, x,
-                                               c if ldx is None else ldx, gate, c if ldg is None else ldg, gate_rows, h,
-                                               c if ldh is None else ldh, y, c if ldy is None else ldy), "BlockNorm.Run")
+        rc = self._run(self.h, stream, STORAGE[storage], rows, residual, c if ldr is None else ldr, x, c if ldx is None else ldx,
+                       gate, c if ldg is None else ldg, gate_rows, h, c if ldh is None else ldh, y, c if ldy is None else ldy)
+        if rc:
+            N.check(rc, "BlockNorm.Run")
 
     def run_quantized(self, residual: Optional[int], rows: int, q: int, scales: int, storage: str = "f16",
                       ldr: Optional[int] = None, x: Optional[int] = None, ldx: Optional[int] = None,
@@ -685,10 +690,11 @@ class HipBlockNorm:
                       ldh: Optional[int] = None, ldq: Optional[int] = None, stream: Optional[int] = None):
         """h, and y as 8-bit rows q (channels rounded up to 64 bytes apart unless ldq says so) and their scales [rows]."""
         c = self.channels
-        N.check(N.backend().sox_block_norm_run_quantized(
-            self.h, stream, STORAGE[storage], rows, residual, c if ldr is None else ldr, x, c if ldx is None else ldx, gate,
-            c if ldg is None else ldg, gate_rows, h, c if ldh is None else ldh, q, -(-c // 64) * 64 if ldq is None else ldq,
-            scales), "BlockNorm.RunQuantized")
+        rc = self._run_quantized(self.h, stream, STORAGE[storage], rows, residual, c if ldr is None else ldr, x,
+                                 c if ldx is None else ldx, gate, c if ldg is None else ldg, gate_rows, h,
+                                 c if ldh is None else ldh, q, -(-c // 64) * 64 if ldq is None else ldq, scales)
+        if rc:
+            N.check(rc, "BlockNorm.RunQuantized")
 
     def close(self):
         if self.h:

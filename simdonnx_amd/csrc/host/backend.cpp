@@ -4742,10 +4742,8 @@ struct LayerCall {
     Rows matrix(const char* what, const void* p, int64_t ld, int64_t cols, bool optional = false) const {
         return matrix(what, p, ld, cols, es, es, optional, rows);
     }
-    // every row on 16-byte boundaries and of whole 16-byte chunks
-    static bool chunked(const Rows& r) { return !r.any() || (r.at % 16 == 0 && r.pitch % 16 == 0 && r.width % 16 == 0); }
-    // rows on 16-byte boundaries, whatever their length
-    static bool on16(const Rows& r) { return r.at % 16 == 0 && r.pitch % 16 == 0; }
+    // every row on 16-byte boundaries
+    static bool on16(const Rows& r) { return !r.any() || (r.at % 16 == 0 && (r.pitch % 16 == 0 || r.rows == 1)); }
 
     LayerCall(sox_backend* b, const char* n, int32_t nrows, int32_t storage) : be(b), name(n), rows(nrows) {
         if (nrows < 0) bad("rows");
@@ -4809,7 +4807,7 @@ struct sox_qlinear {
     int inner = 0, columns = 0, k16 = 0, kb = 0, nb = 0, npad = 0;
     DeviceBlock mem;  // packed weights, then the scales and the bias (zeros without one), padded to npad columns
     uint64_t scales_at = 0;
-    void *fn_rows[3][2], *fn_few[3][3], *fn_fewx[3][3];  // by storage
+    void *fn_rows[3][2], *fn_few[3][3], *fn_fewx[3][3], *fn_panel[3][4];  // by storage
 
     const int8_t* w() const { return (const int8_t*)mem.p; }
     const float* ws() const { return (const float*)((const uint8_t*)mem.p + scales_at); }
@@ -4817,7 +4815,15 @@ struct sox_qlinear {
     int pitch() const { return round_up(inner, 64); }
     // rows [rows][pitch], then their scales
     uint64_t work_rows(int64_t rows) const { return (uint64_t)rows * pitch(); }
-    bool fused(int64_t rows) const { return rows <= 16 && inner <= 4096; }
+    // floating rows in one launch: few of them, or not so many that repeating their rounding for every 128 columns costs
+    // more than a launch of its own
+    bool few(int64_t rows) const { return rows <= 16 && inner <= 4096; }
+    bool panel(int64_t rows) const {
+        if (getenv("SOX_PANEL")) return inner<=1024 && atoi(getenv("SOX_PANEL"));
+        if (getenv("SIMDONNX_HIP_QGEMM")) return false;  // (a forced tiling; tests of the ring)
+        return inner <= 1024 && ((rows + 31) / 32) * ((columns + 127) / 128) <= 512;
+    }
+    bool fused(int64_t rows) const { return few(rows) || panel(rows); }
     uint64_t workspace(int64_t rows) const { return rows <= 0 || fused(rows) ? 0 : work_rows(rows) + (uint64_t)round_up((int)rows, 4) * 4; }
 };
 
@@ -4854,6 +4860,7 @@ void qlinear_pack(sox_qlinear& L, const int8_t* w, const float* scales, const fl
         const std::string st = kStorageName[s];
         L.fn_rows[s][0] = L.be->fn("sox_qrows_" + st);
         L.fn_rows[s][1] = L.be->fn("sox_qrows_" + st + "_wide");
+        for (int i = 0; i < 4; i++) L.fn_panel[s][i] = L.be->fn("sox_qpanel_" + st + "_c" + std::to_string(i + 1));
         for (int i = 0; i < 3; i++) {
             L.fn_few[s][i] = L.be->fn("sox_qfew_" + st + "_r" + std::to_string(1 << i));
             L.fn_fewx[s][i] = L.be->fn("sox_qfewx_" + st + "_s" + std::to_string(1 << i));
@@ -4890,9 +4897,16 @@ void qlinear_product(const LayerCall& c, sox_qlinear* L, void* stream, sox_qgemm
     a.nb = L->nb;
     const int steps = (L->inner + 63) / 64;
     const uint32_t col_groups = (uint32_t)((L->columns + 15) / 16);
+    if (fused && !L->few(c.rows)) {
+        const uint32_t grid[3] = {(uint32_t)((L->columns + 127) / 128), (uint32_t)((c.rows + 31) / 32), 1}, block[3] = {512, 1, 1};
+        const uint32_t lds = (uint32_t)((L->inner + 31) / 32) * 1024;
+        check(sox_launch_on(c.be->info.device, L->fn_panel[storage][(L->inner - 1) / 256], grid, block, lds, stream, &a), c.name);
+        return;
+    }
     if (fused) {
-        const int si = steps <= 16 ? 0 : steps <= 32 ? 1 : 2, waves = (steps + (1 << si) - 1) >> si;
-        c.launch(L->fn_fewx[storage][si], col_groups, (uint32_t)waves * 64, stream, a);
+        const int segs = (L->inner + 1023) / 1024, waves = (int)std::min<int64_t>(16, std::max<int64_t>(steps, c.rows * segs));
+        const int si = steps <= waves ? 0 : steps <= 2 * waves ? 1 : 2;
+        c.launch(L->fn_fewx[storage][si], col_groups, (uint32_t)waves * 64, stream, a, (uint32_t)(c.rows * (round_up(L->inner, 256) + 16)));
         return;
     }
     if (c.rows <= 64) {
@@ -4903,7 +4917,7 @@ void qlinear_product(const LayerCall& c, sox_qlinear* L, void* stream, sox_qgemm
     const int64_t cus = std::max(1, c.be->info.compute_units);
     const QTile* pick = &kQTiles[7];
     for (const QTile& t : kQTiles)
-        if (((c.rows + t.bm - 1) / t.bm) * ((L->columns + t.bn - 1) / t.bn) >= cus) {
+        if (((c.rows + t.bm - 1) / t.bm) * ((L->columns + t.bn - 1) / t.bn) >= cus && !(storage == 0 && t.bn * t.bm == 65536)) {
             pick = &t;
             break;
         }
@@ -4933,24 +4947,19 @@ struct sox_block_norm {
 
 namespace {
 
-// block_norm.hip's instances: threads of a row, chunks of 8 columns of a thread, and whether the parameters stand in LDS (a
-// wave per row).
+// block_norm.hip's instances: threads of a row, chunks of 8 columns of a thread, workgroups per CU at most; `many`: for many
+// rows, with the parameters in LDS.
 struct BnormShape {
-    int tpr, ch;
-    bool lds;
+    int tpr, ch, per_cu;
+    bool many;
 };
-const BnormShape kBnormShapes[] = {{64, 1, true},   {64, 2, true},   {64, 4, true},    {64, 8, true},
-                                   {256, 1, false}, {256, 2, false}, {1024, 1, false}, {512, 4, false}};
-constexpr int kBnormLds = 4;  // (the first of them; in fp32 the last of these, 4096 columns, is left out)
+const BnormShape kBnormShapes[] = {{32, 1, 4, true},   {64, 1, 4, true},   {64, 2, 4, true},  {256, 1, 4, false},
+                                   {256, 2, 2, false}, {512, 2, 2, false}, {512, 4, 1, false}};
 
-// The first instance that holds c columns: among the waves per row, or among the others.
-int bnorm_shape(int32_t storage, int c, bool many_rows) {
-    const int waves = storage == SOX_STORAGE_F32 ? kBnormLds - 1 : kBnormLds, count = (int)(sizeof kBnormShapes / sizeof *kBnormShapes);
-    if (many_rows)
-        for (int i = 0; i < waves; i++)
-            if (kBnormShapes[i].tpr * kBnormShapes[i].ch * 8 >= c) return i;
-    for (int i = kBnormLds; i < count; i++)
-        if (kBnormShapes[i].tpr * kBnormShapes[i].ch * 8 >= c) return i;
+// The first instance that holds c columns; those for many rows only where there are many.
+int bnorm_shape(int c, bool many) {
+    for (int i = 0; i < (int)(sizeof kBnormShapes / sizeof *kBnormShapes); i++)
+        if (kBnormShapes[i].tpr * kBnormShapes[i].ch * 8 >= c && (many || !kBnormShapes[i].many)) return i;
     unsupported("BlockNorm: channels");
 }
 std::string bnorm_kernel(int32_t storage, int shape, bool vec) {
@@ -4996,15 +5005,14 @@ void bnorm_run(sox_block_norm* N, const char* name, void* stream, int32_t storag
     a.rows = rows; a.c = C; a.gate_group = gate ? rows / gate_rows : 1;
     a.post = N->p.post; a.pre = N->p.pre; a.gate_act = N->p.gate_act;
     a.post_eps = N->p.post_eps; a.pre_eps = N->p.pre_eps; a.res_scale = N->p.res_scale;
-    const bool vec = c.chunked(R) && c.chunked(X) && c.chunked(G) && c.chunked(H) && (quantized ? C * c.es % 16 == 0 : c.chunked(Y));
+    const bool vec = c.on16(R) && c.on16(X) && c.on16(G) && c.on16(H) && (quantized || c.on16(Y));
     const int64_t cus = std::max(1, c.be->info.compute_units);
-    const bool many = rows >= 4 * cus;
-    const BnormShape& shape = kBnormShapes[bnorm_shape(storage, C, many)];
-    // enough workgroups to fill the GPU; past that each walks several rows with its parameters at hand
-    const int64_t per_block = shape.tpr == 64 ? 4 : 1, blocks = (rows + per_block - 1) / per_block;
-    const int64_t cap = cus * (shape.lds ? 4 : shape.tpr == 256 ? 8 : 2);
-    c.launch(N->fn[storage][many][vec], (uint32_t)std::min(blocks, cap), (uint32_t)std::max(shape.tpr, 256), stream, a,
-             shape.lds ? (uint32_t)(N->vectors * shape.tpr * shape.ch * 8 * 4) : 0);
+    const bool many = rows >= 4 * cus;  // a wave on every SIMD
+    const BnormShape& shape = kBnormShapes[bnorm_shape(C, many)];
+    const int threads = std::max(shape.tpr, 256), per_block = threads / shape.tpr;
+    const int64_t blocks = std::min<int64_t>((rows + per_block - 1) / per_block, cus * shape.per_cu);
+    c.launch(N->fn[storage][many][vec], (uint32_t)blocks, (uint32_t)threads, stream, a,
+             shape.many ? (uint32_t)(N->vectors * shape.tpr * shape.ch * 8 * 4) : 0);
 }
 
 }  // namespace
@@ -5080,7 +5088,7 @@ int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x
         a.y = y;
         a.ldy = ldy;
         a.act = act;
-        a.vec = (c.chunked(Y) && c.chunked(R) ? 1 : 0) | (c.on16(X) ? 2 : 0);
+        a.vec = (c.on16(Y) && c.on16(R) ? 1 : 0) | (c.on16(X) ? 2 : 0);
         if (!fused) {
             sox_qrows_args q{};
             q.x = x;
@@ -5122,7 +5130,7 @@ int sox_qlinear_run_quantized(sox_qlinear* L, void* stream, const int8_t* q, int
         a.y = y;
         a.ldy = ldy;
         a.act = act;
-        a.vec = c.chunked(Y) && c.chunked(R) ? 1 : 0;
+        a.vec = c.on16(Y) && c.on16(R) ? 1 : 0;
         qlinear_product(c, L, stream, a, storage, false);
     });
 }
@@ -5159,7 +5167,7 @@ int sox_block_norm_create(sox_backend* be, const sox_block_norm_p* p, const floa
         N->mem.upload(be, v.data(), v.size() * 4, "BlockNorm parameters");
         for (int32_t s = 0; s < 3; s++)
             for (int many = 0; many < 2; many++)
-                for (int vec = 0; vec < 2; vec++) N->fn[s][many][vec] = be->fn(bnorm_kernel(s, bnorm_shape(s, p->channels, many), vec));
+                for (int vec = 0; vec < 2; vec++) N->fn[s][many][vec] = be->fn(bnorm_kernel(s, bnorm_shape(p->channels, many), vec));
         *out = N.release();
     });
 }

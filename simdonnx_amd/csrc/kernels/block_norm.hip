@@ -7,18 +7,20 @@
 // All sums and norms in fp32, a variance as the mean square about the mean (a second sum over the registers, so a large
 // mean costs no digits); y is computed from h as summed in fp32, not from its rounded copy.
 //
-// Two ways to hold a row, by how many rows there are:
-//  * many rows: a wave per row (64 threads, up to 4096 16-bit columns), no barriers; the parameter vectors, which would
-//    move as much from L2 per row as the row itself moves from memory, stand in LDS for all rows the workgroup walks.
-//  * few rows, or long ones: TPR threads per row, which shortens the one row's chain of loads, sums and stores; the
+// How a row is held, by how many rows there are and how long:
+//  * many rows of up to 1024 columns: a wave per row (half a wave up to 256), no barriers; the parameter vectors, which
+//    would move as much from L2 per row as the row itself moves from memory, stand in LDS for all rows the workgroup walks.
+//  * few rows, or longer ones: TPR threads per row, which shortens the one row's chain of loads, sums and stores; the
 //    parameters stay in registers (or, for the longest rows, are read where they are used).
+// A workgroup walks rows a whole grid apart; the grid is held to what the rows' streams run best with: 16384 x 4096 bf16 in
+// 93 us (5.8 TB/s) on 2 workgroups per CU, 122 with one row each, and 135 to 300 with a wave per row.
 #include "qrows.h"
 
 enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
 enum { PAR_LDS, PAR_REG, PAR_MEM };  // where the parameter vectors are
 
 // CH chunks of E values per thread; VEC: chunk j of thread t is columns (j TPR + t) E .. + E - 1 as one 16-byte access
-// (rows on 16-byte boundaries, c a multiple of E), else value e of it is column (j E + e) TPR + t on its own
+// (rows on 16-byte boundaries), else value e of it is column (j E + e) TPR + t on its own
 template <typename T, int TPR, int CH, bool VEC> struct Row {
     static constexpr int E = 16 / sizeof(T), N = CH * E;
     typedef vec_t<T, E> TE;
@@ -28,8 +30,15 @@ template <typename T, int TPR, int CH, bool VEC> struct Row {
 #pragma unroll
         for (int j = 0; j < CH; j++) {
             if constexpr (VEC) {
+                const int k = col(t, j, 0);
                 v[j] = TE{};
-                if (col(t, j, 0) < c) v[j] = *(const TE*)(p + col(t, j, 0));
+                if (k + E <= c) {
+                    v[j] = *(const TE*)(p + k);
+                } else if (k < c) {  // the row's end inside a chunk
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        if (k + e < c) v[j][e] = p[k + e];
+                }
             } else {
 #pragma unroll
                 for (int e = 0; e < E; e++) v[j][e] = col(t, j, e) < c ? p[col(t, j, e)] : (T)0.0f;
@@ -43,7 +52,14 @@ template <typename T, int TPR, int CH, bool VEC> struct Row {
                 TE o;
 #pragma unroll
                 for (int e = 0; e < E; e++) o[e] = (T)f[j * E + e];
-                if (col(t, j, 0) < c) *(TE*)(p + col(t, j, 0)) = o;
+                const int k = col(t, j, 0);
+                if (k + E <= c) {
+                    *(TE*)(p + k) = o;
+                } else if (k < c) {
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        if (k + e < c) p[k + e] = o[e];
+                }
             } else {
 #pragma unroll
                 for (int e = 0; e < E; e++)
@@ -59,7 +75,10 @@ template <typename T, int TPR, int CH, bool VEC> struct Row {
             if constexpr (VEC) {
                 uint32_t w[E / 4];
 #pragma unroll
-                for (int i = 0; i < E / 4; i++) w[i] = RowQuant<half_t>::q4(&f[j * E + 4 * i], rq);
+                for (int i = 0; i < E / 4; i++) {
+                    const float* g = &f[j * E + 4 * i];
+                    w[i] = RowQuant<half_t>::q4(g[0], g[1], g[2], g[3], rq);
+                }
                 if (col(t, j, 0) < c16) {
                     if constexpr (E == 8)
                         *(uint2*)(p + col(t, j, 0)) = make_uint2(w[0], w[1]);
@@ -69,7 +88,7 @@ template <typename T, int TPR, int CH, bool VEC> struct Row {
             } else {
 #pragma unroll
                 for (int e = 0; e < E; e++)
-                    if (col(t, j, e) < c16) p[col(t, j, e)] = (int8_t)RowQuant<half_t>::q(f[j * E + e], rq);
+                    if (col(t, j, e) < c16) p[col(t, j, e)] = RowQuant<half_t>::q(f[j * E + e], rq);
             }
         }
     }
@@ -90,16 +109,16 @@ template <int TPR, class V, class F> SOX_DEV V row_fold(V v, V* lds, F&& f) {
     return v;
 }
 template <int TPR> SOX_DEV float row_sum(float v, float* lds) {
-    return row_fold<TPR>(wave_sum(v), lds, [](float a, float b) { return a + b; });
+    return row_fold<TPR>(wave_sum<TPR == 32 ? 32 : 64>(v), lds, [](float a, float b) { return a + b; });
 }
 template <int TPR> SOX_DEV uint32_t row_max(uint32_t v, uint32_t* lds) {
-    return row_fold<TPR>(wave_max(v), lds, [](uint32_t a, uint32_t b) { return max(a, b); });
+    return row_fold<TPR>(wave_max<TPR == 32 ? 32 : 64>(v), lds, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
 template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_body(const sox_bnorm_args& p) {
     typedef Row<T, TPR, CH, VEC> R;
     constexpr int E = R::E, N = R::N, BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR, CAP = TPR * N;
-    static_assert(PAR != PAR_LDS || TPR == 64, "a wave per row");
+    static_assert((PAR == PAR_LDS) == (TPR <= 64), "a wave or half of one per row");
     __shared__ float lds[2][5][BLOCK / 64];
     extern __shared__ float par_lds[];  // PAR_LDS: the vectors there are, CAP floats each
     const int t = threadIdx.x % TPR, c = p.c;
@@ -270,14 +289,15 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
         bnorm_body<T, TPR, CH, VEC, PAR>(p);                                                                                \
     }
 #define SOX_BNORM(NAME, T, TPR, CH, PAR) SOX_BNORM_V(NAME, T, TPR, CH, v, true, PAR) SOX_BNORM_V(NAME, T, TPR, CH, s, false, PAR)
-// threads of a row and chunks of a thread: a wave per row up to 4096 16-bit columns (2048 fp32) ...
+// threads of a row and chunks of a thread: 16-bit rows of up to 256, 512, 1024 columns for many rows, and of up to 2048, 4096,
+// 8192, 16384 for few or long ones ...
 #define SOX_BNORM_16(NAME, T)                                                                                             \
-    SOX_BNORM(NAME, T, 64, 1, PAR_LDS) SOX_BNORM(NAME, T, 64, 2, PAR_LDS) SOX_BNORM(NAME, T, 64, 4, PAR_LDS)              \
-    SOX_BNORM(NAME, T, 64, 8, PAR_LDS) SOX_BNORM(NAME, T, 256, 1, PAR_REG) SOX_BNORM(NAME, T, 256, 2, PAR_REG)            \
-    SOX_BNORM(NAME, T, 1024, 1, PAR_REG) SOX_BNORM(NAME, T, 512, 4, PAR_MEM)
+    SOX_BNORM(NAME, T, 32, 1, PAR_LDS) SOX_BNORM(NAME, T, 64, 1, PAR_LDS) SOX_BNORM(NAME, T, 64, 2, PAR_LDS)              \
+    SOX_BNORM(NAME, T, 256, 1, PAR_REG) SOX_BNORM(NAME, T, 256, 2, PAR_REG) SOX_BNORM(NAME, T, 512, 2, PAR_REG)           \
+    SOX_BNORM(NAME, T, 512, 4, PAR_MEM)
 SOX_BNORM_16(f16, half_t)
 SOX_BNORM_16(bf16, bf16_t)
 // ... and the same in fp32, twice the chunks
-SOX_BNORM(f32, float, 64, 2, PAR_LDS) SOX_BNORM(f32, float, 64, 4, PAR_LDS) SOX_BNORM(f32, float, 64, 8, PAR_LDS)
-SOX_BNORM(f32, float, 256, 2, PAR_REG) SOX_BNORM(f32, float, 256, 4, PAR_REG) SOX_BNORM(f32, float, 1024, 2, PAR_REG)
+SOX_BNORM(f32, float, 32, 2, PAR_LDS) SOX_BNORM(f32, float, 64, 2, PAR_LDS) SOX_BNORM(f32, float, 64, 4, PAR_LDS)
+SOX_BNORM(f32, float, 256, 2, PAR_REG) SOX_BNORM(f32, float, 256, 4, PAR_REG) SOX_BNORM(f32, float, 512, 4, PAR_REG)
 SOX_BNORM(f32, float, 512, 8, PAR_MEM)

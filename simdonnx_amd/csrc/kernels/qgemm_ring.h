@@ -49,8 +49,8 @@ template <typename T> SOX_DEV int stage_at(int r, int c) {
     return sizeof(T) == 2 ? r * 64 + ((c ^ ((r >> 2) & 3)) << 4) : r * 128 + ((c ^ (r >> 1)) << 4);
 }
 
-// A block's rows between memory at (m0, n0) and the stage: 16-byte chunks where the rows allow it (uniform), else single
-// elements, a half wave per row, in a loop that is not unrolled (the ragged form should not be most of the code).
+// A block's rows between memory at (m0, n0) and the stage: 16-byte chunks where the rows stand on 16-byte boundaries (uniform;
+// single elements in the chunk that a row ends in), else single elements, a half wave per row, in a loop that is not unrolled (the ragged form should not be most of the code).
 // LOAD: the residual's into the stage (zeros outside), else the stage's to the output.
 template <typename T, bool LOAD>
 SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, bool vec, unsigned char* stg, int m0, int n0, int lane) {
@@ -64,11 +64,21 @@ SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, bool vec,
             T* g = base + (int64_t)m * ld + n;
             if constexpr (LOAD) {
                 TE v = {};
-                if (m < M && n < N) v = *(const TE*)g;
+                if (m < M && n + E <= N) {
+                    v = *(const TE*)g;
+                }
                 *s = v;
+                if (m < M && n < N && n + E > N)
+#pragma unroll 1
+                    for (int e = 0; e < N - n; e++) ((T*)s)[e] = g[e];
             } else {
                 const TE v = *s;
-                if (m < M && n < N) *(TE*)g = v;
+                if (m < M && n + E <= N) {
+                    *(TE*)g = v;
+                } else if (m < M && n < N) {
+#pragma unroll 1
+                    for (int e = 0; e < N - n; e++) g[e] = ((const T*)s)[e];
+                }
             }
         }
     } else {
@@ -93,6 +103,71 @@ SOX_DEV void stage_turn() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A 32 x 32 block's outputs from its sums (lane l: row l % 32, columns 8 q + 4 (l / 32) + e in element 4 q + e): scaled, joined
+// with the residual and activated in registers, staged and stored. One copy of this with its choices inside, none of
+// them per element: a choice per element, or a copy per form, multiplied the ring's code until its instruction fetches
+// took most of a short product's time and registers ran out. ws, bias: the block's 32 columns.
+template <typename T>
+SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs, const float* ws, const float* bias,
+                          unsigned char* stg, int m0, int n0, int lane) {
+    constexpr int PARTS = sizeof(T) == 2 ? 1 : 2, ROWS = 32 / PARTS;
+    typedef vec_t<T, 4> T4;
+    const int l32 = lane & 31, hl = lane >> 5;
+    const bool vec = p.vec & 1;
+    float val[16];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const float4v w4 = *(const float4v*)(ws + 8 * q + 4 * hl), b4 = *(const float4v*)(bias + 8 * q + 4 * hl);
+#pragma unroll
+        for (int e = 0; e < 4; e++) val[4 * q + e] = __builtin_fmaf((float)sums[4 * q + e] * w4[e], xs, b4[e]);
+    }
+    // the lane's four of the stage: 16-bit rows 64 bytes, fp32 ones 128 (and half of them at a time)
+    auto at = [&](int q) __attribute__((always_inline)) {
+        return sizeof(T) == 2 ? (T4*)(stg + stage_at<T>(l32, q) + hl * 8) : (T4*)(stg + stage_at<T>(l32 % ROWS, 2 * q + hl));
+    };
+    if (p.add) {
+#pragma unroll
+        for (int half = 0; half < PARTS; half++) {
+            move_rows<T, true>((T*)p.add, p.ldr, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
+            stage_turn();
+            if (PARTS == 1 || l32 / ROWS == half) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const T4 r = *at(q);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) val[4 * q + e] += (float)r[e];
+                }
+            }
+            stage_turn();
+        }
+    }
+    if (p.act == SOX_ACT_GELU) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) val[e] = q_out<T, SOX_ACT_GELU>(val[e]);
+    } else if (p.act == SOX_ACT_RELU) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) val[e] = q_out<T, SOX_ACT_RELU>(val[e]);
+    } else if (p.act != SOX_ACT_NONE) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) val[e] = q_out<T, Q_ACT_GATES>(val[e], p.act);
+    }
+#pragma unroll
+    for (int half = 0; half < PARTS; half++) {
+        if (PARTS == 1 || l32 / ROWS == half) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                T4 h;
+#pragma unroll
+                for (int e = 0; e < 4; e++) h[e] = (T)val[4 * q + e];
+                *at(q) = h;
+            }
+        }
+        stage_turn();
+        move_rows<T, false>((T*)p.y, p.ldy, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
+        stage_turn();
+    }
 }
 
 template <typename T, int BM, int BN, int BK, int WM, int WN, int STAGES, int NW, int GM>
@@ -196,73 +271,15 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
         static_for<0, TJ * TI>([&](auto ji) { acc[decltype(ji)::value / TI][decltype(ji)::value % TI] = (int16v)0; });
     };
     int m_kt = 0, m_tile = vid, m_seq = 0;  // the tile being multiplied
-    // The tile's outputs, block by block: scaled, joined with the residual and activated in registers, staged and stored.
-    // One copy of this with its choices inside, none of them per element: a choice per element, or a copy per form,
-    // multiplied the code until its instruction fetches took most of a short product's time and registers ran out.
     auto epilogue = [&]() __attribute__((always_inline)) {
         int bm, bn;
         tile_origin(m_tile, bm, bn);
         const unsigned char* sc = sc_mem + (m_seq % SCB) * SC_BYTES;
-        const bool vec = p.vec & 1;
         static_for<0, TJ * TI>([&](auto ji) __attribute__((always_inline)) {
             constexpr int j = decltype(ji)::value / TI, i = decltype(ji)::value % TI;
-            constexpr int PARTS = sizeof(T) == 2 ? 1 : 2, ROWS = 32 / PARTS;
-            typedef vec_t<T, 4> T4;
-            const int m0 = bm + wm0 + i * 32, n0 = bn + wn0 + j * 32;
+            const float* ws = (const float*)sc + wn0 + j * 32;
             const float xs = *(const float*)(sc + BN * 8 + (wm0 + i * 32 + l32) * 4);
-            float val[16];
-            static_for<0, 4>([&](auto qq) __attribute__((always_inline)) {
-                constexpr int q = decltype(qq)::value;
-                const int n = wn0 + j * 32 + 8 * q + 4 * hl;
-                const float4v ws = *(const float4v*)(sc + n * 4), bs = *(const float4v*)(sc + BN * 4 + n * 4);
-#pragma unroll
-                for (int e = 0; e < 4; e++) val[4 * q + e] = __builtin_fmaf((float)acc[j][i][4 * q + e] * ws[e], xs, bs[e]);
-            });
-            // the lane's four of the stage: 16-bit rows 64 bytes, fp32 ones 128 (and half of them at a time)
-            auto at = [&](int q) __attribute__((always_inline)) {
-                return sizeof(T) == 2 ? (T4*)(stg + stage_at<T>(l32, q) + hl * 8) : (T4*)(stg + stage_at<T>(l32 % ROWS, 2 * q + hl));
-            };
-            if (p.add) {
-#pragma unroll
-                for (int half = 0; half < PARTS; half++) {
-                    move_rows<T, true>((T*)p.add, p.ldr, M, p.n, vec, stg, m0 + half * ROWS, n0, lane);
-                    stage_turn();
-                    if (PARTS == 1 || l32 / ROWS == half) {
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const T4 r = *at(q);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) val[4 * q + e] += (float)r[e];
-                        }
-                    }
-                    stage_turn();
-                }
-            }
-            if (p.act == SOX_ACT_GELU) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) val[e] = q_out<T, SOX_ACT_GELU>(val[e]);
-            } else if (p.act == SOX_ACT_RELU) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) val[e] = q_out<T, SOX_ACT_RELU>(val[e]);
-            } else if (p.act != SOX_ACT_NONE) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) val[e] = q_out<T, Q_ACT_GATES>(val[e], p.act);
-            }
-#pragma unroll
-            for (int half = 0; half < PARTS; half++) {
-                if (PARTS == 1 || l32 / ROWS == half) {
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        T4 h;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) h[e] = (T)val[4 * q + e];
-                        *at(q) = h;
-                    }
-                }
-                stage_turn();
-                move_rows<T, false>((T*)p.y, p.ldy, M, p.n, vec, stg, m0 + half * ROWS, n0, lane);
-                stage_turn();
-            }
+            finish_block<T>(p, acc[j][i], xs, ws, ws + BN, stg, bm + wm0 + i * 32, bn + wn0 + j * 32, lane);
             __builtin_amdgcn_sched_barrier(0);  // one block at a time: bounded register pressure
         });
         m_tile += G;
@@ -330,7 +347,6 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
         qgemm_body<T, BM, BN, BK, WM, WN, ST, NW, GM>(p);                                                   \
     }
 #define SOX_QGEMM_TILES(NAME, T)                                             \
-    SOX_QGEMM(NAME, T, 256x256_w8k128s2, 256, 256, 128, 128, 64, 2, 8, 2, 4) \
     SOX_QGEMM(NAME, T, 256x128_w8k128s2, 256, 128, 128, 64, 64, 2, 8, 2, 4) \
     SOX_QGEMM(NAME, T, 256x192_w8k128s2, 256, 192, 128, 64, 96, 2, 8, 2, 4) \
     SOX_QGEMM(NAME, T, 128x128_w4k128s2, 128, 128, 128, 64, 64, 2, 4, 2, 4) \

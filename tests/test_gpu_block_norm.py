@@ -215,7 +215,7 @@ def test_transformer_mlp_in_8_bits(hip):
         mk = lambda cols, st=storage, r=rows: Matrix(None, st, r, cols, stream=stream)  # noqa: E731
         H1, F1, F2, H2, Z = mk(c), mk(hidden), mk(c), mk(c), mk(3 * c)
         Q1, Q2, S1, S2 = mk(n1.channels, "i8"), mk(c, "i8"), mk(rows, "f32", 1), mk(rows, "f32", 1)
-        W = Matrix(None, "i8", 1, fc2.workspace(rows), stream=stream)
+        W = Matrix(None, "i8", 1, max(1, fc2.workspace(rows)), stream=stream)
 
         def block():
             n1.run_quantized(residual, rows, Q1.ptr, S1.ptr, storage, x=attn.ptr, h=H1.ptr, ldq=Q1.ld, stream=stream)

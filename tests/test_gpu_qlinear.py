@@ -84,6 +84,8 @@ def test_few_rows(hip, storage, rows, k, n):
     ("f32", 513, 65, 259, 0, 0), ("f32", 128, 129, 256, 4, 1), ("bf16", 1000, 16, 96, 0, 0)])
 def test_tiles(hip, monkeypatch, tile, storage, rows, k, n, pad, skip):
     """Every tiling, also where the choice would not take it: one slice of K and many, partial tiles on both sides."""
+    if storage == "f32" and tile[:7] == "256x256":
+        tile = "256x192_w8k128s2"  # (fp32 outputs have no 256x256 tiling)
     monkeypatch.setenv("SIMDONNX_HIP_QGEMM", tile)
     print(f"[gpu] qlinear {tile} {storage} {rows} x {k} -> {n}", flush=True)
     both_ways(hip, 2000 + k, rows, k, n, storage, act="none", res=pad > 0, pad=pad, skip=skip)
@@ -166,7 +168,7 @@ def test_halves_round_to_even(hip):
         x[:, 63] = amax / 2
         x = rounded(x, storage)
         q, scale = quantize(x)
-        X, Y, W = Matrix(x, storage), Matrix(None, "f32", 200, k), Matrix(None, "i8", 1, lin.workspace(200))
+        X, Y, W = Matrix(x, storage), Matrix(None, "f32", 200, k), Matrix(None, "i8", 1, max(1, lin.workspace(200)))
         for rows, first in ((200, 0), (16, 3)):  # the row kernel, and the fused one
             print(f"[gpu] qlinear halves {storage} {rows}", flush=True)
             if storage == "f32":
@@ -212,7 +214,7 @@ def test_weights_by_column(hip):
     q, scale = quantize(x)
     want, tol = linear64(q, scale, wq.T, ws, None, None, "none", "bf16")
     lin = HipQuantLinear(hip, w, None, k, n)
-    X, Y, W = Matrix(x, "bf16"), Matrix(None, "bf16", rows, n), Matrix(None, "i8", 1, lin.workspace(rows))
+    X, Y, W = Matrix(x, "bf16"), Matrix(None, "bf16", rows, n), Matrix(None, "i8", 1, max(1, lin.workspace(rows)))
     print("[gpu] qlinear float weights", flush=True)
     lin.run(X.ptr, rows, Y.ptr, "bf16", workspace=W.ptr, workspace_bytes=lin.workspace(rows))
     check(Y.read(), want, tol)
@@ -230,7 +232,7 @@ def test_columns_of_one_buffer(hip):
     want, tol = linear64(q, scale, w, ws, None, None, "none", "f16")
     both = np.concatenate([x, np.zeros((rows, n), np.float32)], axis=1)
     lin = HipQuantLinear(hip, w, None, k, n, scales=ws)
-    B, W = Matrix(both, "f16"), Matrix(None, "i8", 1, lin.workspace(rows))
+    B, W = Matrix(both, "f16"), Matrix(None, "i8", 1, max(1, lin.workspace(rows)))
     print("[gpu] qlinear one buffer", flush=True)
     lin.run(B.ptr, rows, B.ptr + 2 * k, "f16", ldx=k + n, ldy=k + n, workspace=W.ptr, workspace_bytes=lin.workspace(rows))
     got = B.read()
@@ -292,7 +294,7 @@ def test_allocates_nothing(hip):
     w, ws = weights8(11, k, n)
     lin = HipQuantLinear(hip, w, None, k, n, scales=ws)
     X, Y = Matrix(rows_of(11, rows, k, "f16"), "f16"), Matrix(None, "f16", rows, n)
-    W = Matrix(None, "i8", 1, lin.workspace(rows))
+    W = Matrix(None, "i8", 1, max(1, lin.workspace(rows)))
     before = N.thin().sox_alloc_count()
     lin.run(X.ptr, rows, Y.ptr, "f16", workspace=W.ptr, workspace_bytes=lin.workspace(rows))
     lin.run(X.ptr, 0, Y.ptr, "f16")
@@ -309,7 +311,7 @@ def test_memory_of_the_host_is_refused(hip, monkeypatch):
     w, ws = weights8(12, k, n)
     lin = HipQuantLinear(hip, w, None, k, n, scales=ws)
     X, Y = Matrix(rows_of(12, rows, k, "f16"), "f16"), Matrix(None, "f16", rows, n)
-    W = Matrix(None, "i8", 1, lin.workspace(rows))
+    W = Matrix(None, "i8", 1, 1024)
     host = np.zeros(rows * k * 2, np.uint8)
     given = dict(workspace=W.ptr, workspace_bytes=lin.workspace(rows))
     with pytest.raises(SoxError, match="x is not in memory the GPU reads"):

@@ -8,6 +8,7 @@ from simdonnx_amd.backend import HipBackend, HipBlockNorm, HipQuantLinear
 from simdonnx_amd.native import NotSupportedError, SoxError
 
 K, C = 70, 36  # inner, columns
+ROWS = 20000  # enough for the rows to be brought to 8 bits in a workspace
 BASE = 1 << 20  # addresses that nothing reads
 
 
@@ -48,7 +49,7 @@ def at(i):
 
 
 def run_args(**more):
-    return dict(x=at(0), rows=100, y=at(1), workspace=at(2), workspace_bytes=1 << 20) | more
+    return dict(x=at(0), rows=ROWS, y=at(1), workspace=at(2), workspace_bytes=1 << 22) | more
 
 
 def test_linear_checks(linear):
@@ -57,7 +58,7 @@ def test_linear_checks(linear):
     in_order(run, **run_args(ldx=K + 3, ldy=C + 5, residual=at(3), ldr=C + 1, storage="bf16", act="gelu"))
     in_order(run, **run_args(residual=at(1)))  # in place
     in_order(run, **run_args(rows=16, workspace=None, workspace_bytes=0))
-    assert linear.workspace(16) == 0 and linear.workspace(100) > 100 * K
+    assert linear.workspace(16) == linear.workspace(1000) == 0 and linear.workspace(ROWS) > ROWS * K
     linear.run(at(0), 0, at(1))  # no rows: nothing to do, nothing asked
     refused("x is null", run, **run_args(x=None))
     refused("y is null", run, **run_args(y=None))
@@ -72,7 +73,7 @@ def test_linear_checks(linear):
     refused("bytes of workspace, has 0", run, **run_args(workspace=None))
     refused("bytes of workspace, has 100", run, **run_args(workspace_bytes=100))
     refused("workspace is not on 16-byte", run, **run_args(workspace=at(2) + 8))
-    refused("y overlaps x", run, **run_args(y=at(0) + 100 * K * 2 - 2))
+    refused("y overlaps x", run, **run_args(y=at(0) + ROWS * K * 2 - 2))
     refused("y overlaps workspace", run, **run_args(y=at(2) + 64))
     refused("workspace overlaps x", run, **run_args(workspace=at(0) + 16))
     refused("y overlaps residual without being it", run, **run_args(residual=at(1) + 2 * C))
@@ -94,7 +95,7 @@ def test_side_by_side_in_one_buffer(linear):
     refused("y overlaps x", linear.run, **run_args(ldx=ld, ldy=ld, y=at(0) + 2 * K - 2))
     refused("y overlaps x", linear.run, **run_args(ldx=ld, ldy=ld, y=at(0) + 2 * K + 2))
     refused("y overlaps x", linear.run, **run_args(ldx=ld, ldy=ld + 2, y=at(0) + 2 * K))
-    in_order(linear.run, **run_args(ldx=ld, ldy=ld, y=at(0) + 2 * ld * 100 + 2 * K))
+    in_order(linear.run, **run_args(ldx=ld, ldy=ld, y=at(0) + 2 * ld * ROWS + 2 * K))
 
 
 def test_linear_quantized_checks(linear):
