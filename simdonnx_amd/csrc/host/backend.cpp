@@ -4774,8 +4774,9 @@ struct LayerCall {
             if (d != be->info.device) bad(std::string(r->what) + (d < 0 ? " is not in memory the GPU reads" : " is on another device"));
         }
     }
-    template <class A> void launch(void* fn, uint32_t gx, uint32_t threads, void* stream, const A& args, uint32_t lds = 0) const {
-        const uint32_t grid[3] = {gx, 1, 1}, block[3] = {threads, 1, 1};
+    template <class A>
+    void launch(void* fn, uint32_t gx, uint32_t gy, uint32_t threads, void* stream, const A& args, uint32_t lds = 0) const {
+        const uint32_t grid[3] = {gx, gy, 1}, block[3] = {threads, 1, 1};
         check(sox_launch_on(be->info.device, fn, grid, block, lds, stream, &args), name);
     }
 };
@@ -4807,37 +4808,93 @@ struct sox_qlinear {
     int inner = 0, columns = 0, k16 = 0, kb = 0, nb = 0, npad = 0;
     DeviceBlock mem;  // packed weights, then the scales and the bias (zeros without one), padded to npad columns
     uint64_t scales_at = 0;
-    void *fn_rows[3][2], *fn_few[3][3], *fn_fewx[3][3], *fn_panel[3][4];  // by storage
+    // by storage: rows to 8 bits (short, long), few 8-bit rows (16, 32, 64), few floating rows (1, 2, 4 steps a wave), panels
+    // (256 .. 1024 of K), ring tilings
+    void *fn_rows[3][2], *fn_few[3][3], *fn_fewx[3][3], *fn_panel[3][4], *fn_ring[3][8];
 
     const int8_t* w() const { return (const int8_t*)mem.p; }
     const float* ws() const { return (const float*)((const uint8_t*)mem.p + scales_at); }
     const float* bias() const { return ws() + npad; }
     int pitch() const { return round_up(inner, 64); }
-    // rows [rows][pitch], then their scales
-    uint64_t work_rows(int64_t rows) const { return (uint64_t)rows * pitch(); }
-    // floating rows in one launch: few of them, or not so many that repeating their rounding for every 128 columns costs
-    // more than a launch of its own
-    bool few(int64_t rows) const { return rows <= 16 && inner <= 4096; }
-    bool panel(int64_t rows) const {
-        if (getenv("SOX_PANEL")) return inner<=1024 && atoi(getenv("SOX_PANEL"));
-        if (getenv("SIMDONNX_HIP_QGEMM")) return false;  // (a forced tiling; tests of the ring)
-        return inner <= 1024 && ((rows + 31) / 32) * ((columns + 127) / 128) <= 512;
-    }
-    bool fused(int64_t rows) const { return few(rows) || panel(rows); }
-    uint64_t workspace(int64_t rows) const { return rows <= 0 || fused(rows) ? 0 : work_rows(rows) + (uint64_t)round_up((int)rows, 4) * 4; }
 };
 
 namespace {
 
-// The tilings of the 8-bit ring (qgemm.hip).
+// The tilings of the 8-bit ring (qgemm.hip), with the terms of their estimated time in us (QPlan::ring_us).
 struct QTile {
     const char* name;
     int bm, bn, wgs_per_cu, threads;
+    float lat, thr, base, tile, out;
 };
 const QTile kQTiles[] = {
-    {"256x256_w8k128s2", 256, 256, 1, 512}, {"256x128_w8k128s2", 256, 128, 1, 512}, {"256x192_w8k128s2", 256, 192, 1, 512},
-    {"128x128_w4k128s2", 128, 128, 2, 256}, {"128x192_w4k64s2", 128, 192, 2, 256},  {"128x64_w4k128s2", 128, 64, 3, 256},
-    {"64x128_w4k128s3", 64, 128, 2, 256},   {"64x64_w4k128s4", 64, 64, 2, 256},     {"64x64_w4k64s2", 64, 64, 4, 256},
+    {"256x256_w8k128s2", 256, 256, 1, 512, 0.79f, 1.13f, 0.0f, 7.4f, 0.48f},
+    {"256x192_w8k128s2", 256, 192, 1, 512, 0.79f, 0.97f, 1.2f, 5.5f, 0.40f},
+    {"256x128_w8k128s2", 256, 128, 1, 512, 0.83f, 0.84f, 2.6f, 2.9f, 0.35f},
+    {"128x128_w4k128s2", 128, 128, 2, 256, 0.59f, 0.45f, 3.5f, 1.5f, 0.35f},
+    {"64x64_w4k128s4", 64, 64, 2, 256, 0.32f, 0.22f, 3.8f, 0.1f, 0.51f},
+};
+constexpr int kQTileCount = (int)(sizeof kQTiles / sizeof *kQTiles);
+
+// How a product of m rows runs. Every way gives the same bits (whole numbers), so the choice is by time alone, each
+// estimate a fit to measurements on one MI355X:
+//   FEWX   up to 16 floating rows of up to 4096 values, one launch           1 x 768 -> 768: 3.9 us
+//   PANEL  floating rows of up to 1024 values, one launch that rounds them   786 x 768 -> 760: 7.3 us; rounded by a launch
+//          once per 128 columns                                              of its own 9.4. 8192 x 768 -> 2304: 51, 35
+//   FEW    up to 64 8-bit rows, weights straight to registers                64 x 4096 -> 4096: 10.8 us, ring 13.5;
+//                                                                            64 x 1024 -> 8192: 6.9, ring 6.0
+//   RING   8-bit rows on the ring of the tiling with the smallest estimate. Over 75 random products the pick is 2% above
+//          the fastest tiling on average, at most 31%
+// FEW and RING take floating rows behind a launch that brings them to 8 bits in the workspace.
+struct QPlan {
+    enum Way { FEWX, PANEL, FEW, RING } way = RING;
+    const QTile* tile = nullptr;
+
+    // A CU's tiles, each with an epilogue; K slices of 128, bound by their latency with few tiles and by the CU's matrix cores
+    // and loads with many; the outputs' stores.
+    static float ring_us(const QTile& t, double m, double n, double k, double cus) {
+        const float q = (float)ceil(ceil(m / t.bm) * ceil(n / t.bn) / cus), nk = (float)ceil(k / 128);
+        return t.base + q * t.tile + nk * std::max(t.lat, q * t.thr) + t.out * (float)(m * n * 1e-6);
+    }
+    static float few_us(double m, double n, double k) {
+        return (float)(2.6 + 0.03 * m + k * (2e-4 + 2.4e-5 * m) * std::max(1.0, n / 8192));
+    }
+    static float panel_us(double m, double n, double k, int es, double cus) {
+        return (float)(3.0 + ceil(ceil(m / 32) * ceil(n / 128) / cus) * (0.6 + 0.0027 * k * (es == 4 ? 2 : 1)));
+    }
+    // a launch (3 us, and one more of the host's time) and the rows in and out
+    static float rows_us(double m, double k, int es) { return (float)(4.0 + m * k * (es + 1) / 4.5e6); }
+
+    QPlan(const sox_qlinear& L, int64_t m, int32_t storage, bool floating) {
+        const int es = storage == SOX_STORAGE_F32 ? 4 : 2;
+        const double cus = std::max(1, L.be->info.compute_units), n = L.columns, k = L.inner;
+        if (floating && m <= 16 && L.inner <= 4096) {
+            way = FEWX;
+            return;
+        }
+        const char* forced = getenv("SIMDONNX_HIP_QGEMM");  // any tiling by name (tuning, tests)
+        float best = 0.0f;
+        for (const QTile& t : kQTiles) {
+            if (forced && strcmp(t.name, forced)) continue;
+            // (the largest tile has no registers for rows that end inside a chunk, nor an fp32 instance)
+            if (t.bm * t.bn == 256 * 256 && (es == 4 || L.columns % 8)) continue;
+            const float us = ring_us(t, (double)m, n, k, cus);
+            if (!tile || us < best) {
+                tile = &t;
+                best = us;
+            }
+        }
+        if (!tile) fail(SOX_E_INVALID, std::string("SIMDONNX_HIP_QGEMM: no tiling ") + forced + " for this product");
+        if (forced) return;
+        if (m <= 64 && few_us((double)m, n, k) < best) {
+            way = FEW;
+            best = few_us((double)m, n, k);
+        }
+        if (floating && L.inner <= 1024 && panel_us((double)m, n, k, es, cus) < rows_us((double)m, k, es) + best) way = PANEL;
+    }
+    bool rounds_itself() const { return way == FEWX || way == PANEL; }
+    // workspace: rows [m][pitch], then their scales
+    static uint64_t rows_bytes(const sox_qlinear& L, int64_t m) { return (uint64_t)m * L.pitch(); }
+    static uint64_t bytes(const sox_qlinear& L, int64_t m) { return rows_bytes(L, m) + (uint64_t)round_up((int)m, 4) * 4; }
 };
 
 void qlinear_pack(sox_qlinear& L, const int8_t* w, const float* scales, const float* bias) {
@@ -4860,6 +4917,11 @@ void qlinear_pack(sox_qlinear& L, const int8_t* w, const float* scales, const fl
         const std::string st = kStorageName[s];
         L.fn_rows[s][0] = L.be->fn("sox_qrows_" + st);
         L.fn_rows[s][1] = L.be->fn("sox_qrows_" + st + "_wide");
+        for (int i = 0; i < kQTileCount; i++) {
+            L.fn_ring[s][i] = nullptr;
+            if (s != SOX_STORAGE_F32 || kQTiles[i].bm * kQTiles[i].bn < 256 * 256)
+                L.fn_ring[s][i] = L.be->fn("sox_qgemm_" + st + "_" + kQTiles[i].name);
+        }
         for (int i = 0; i < 4; i++) L.fn_panel[s][i] = L.be->fn("sox_qpanel_" + st + "_c" + std::to_string(i + 1));
         for (int i = 0; i < 3; i++) {
             L.fn_few[s][i] = L.be->fn("sox_qfew_" + st + "_r" + std::to_string(1 << i));
@@ -4883,8 +4945,8 @@ std::unique_ptr<sox_qlinear> qlinear_new(sox_backend* be, const void* weights, i
     return L;
 }
 
-// The product over 8-bit rows (fused: over floating ones).
-void qlinear_product(const LayerCall& c, sox_qlinear* L, void* stream, sox_qgemm_args& a, int32_t storage, bool fused) {
+// The product, over 8-bit rows (a.a, a.xs) or where the plan rounds them itself over floating ones (a.x).
+void qlinear_product(const LayerCall& c, sox_qlinear* L, const QPlan& plan, void* stream, sox_qgemm_args& a, int32_t storage) {
     a.w = L->w();
     a.ws = L->ws();
     a.bias = L->bias();
@@ -4896,42 +4958,35 @@ void qlinear_product(const LayerCall& c, sox_qlinear* L, void* stream, sox_qgemm
     a.kb = L->kb;
     a.nb = L->nb;
     const int steps = (L->inner + 63) / 64;
-    const uint32_t col_groups = (uint32_t)((L->columns + 15) / 16);
-    if (fused && !L->few(c.rows)) {
-        const uint32_t grid[3] = {(uint32_t)((L->columns + 127) / 128), (uint32_t)((c.rows + 31) / 32), 1}, block[3] = {512, 1, 1};
-        const uint32_t lds = (uint32_t)((L->inner + 31) / 32) * 1024;
-        check(sox_launch_on(c.be->info.device, L->fn_panel[storage][(L->inner - 1) / 256], grid, block, lds, stream, &a), c.name);
-        return;
-    }
-    if (fused) {
+    const uint32_t groups = (uint32_t)((L->columns + 15) / 16);
+    switch (plan.way) {
+    case QPlan::FEWX: {
         const int segs = (L->inner + 1023) / 1024, waves = (int)std::min<int64_t>(16, std::max<int64_t>(steps, c.rows * segs));
         const int si = steps <= waves ? 0 : steps <= 2 * waves ? 1 : 2;
-        c.launch(L->fn_fewx[storage][si], col_groups, (uint32_t)waves * 64, stream, a, (uint32_t)(c.rows * (round_up(L->inner, 256) + 16)));
-        return;
+        c.launch(L->fn_fewx[storage][si], groups, 1, (uint32_t)waves * 64, stream, a,
+                 (uint32_t)(c.rows * (round_up(L->inner, 256) + 16)));
+        break;
     }
-    if (c.rows <= 64) {
+    case QPlan::PANEL:
+        c.launch(L->fn_panel[storage][(L->inner - 1) / 256], (uint32_t)((L->columns + 127) / 128), (uint32_t)((c.rows + 31) / 32), 512,
+                 stream, a, (uint32_t)((L->inner + 31) / 32) * 1024);
+        break;
+    case QPlan::FEW: {
         const int ri = c.rows <= 16 ? 0 : c.rows <= 32 ? 1 : 2, s = 8 >> ri;
-        c.launch(L->fn_few[storage][ri], col_groups, (uint32_t)std::min(8, (steps + s - 1) / s) * 64, stream, a);
-        return;
+        c.launch(L->fn_few[storage][ri], groups, 1, (uint32_t)std::min(8, (steps + s - 1) / s) * 64, stream, a);
+        break;
     }
-    const int64_t cus = std::max(1, c.be->info.compute_units);
-    const QTile* pick = &kQTiles[7];
-    for (const QTile& t : kQTiles)
-        if (((c.rows + t.bm - 1) / t.bm) * ((L->columns + t.bn - 1) / t.bn) >= cus && !(storage == 0 && t.bn * t.bm == 65536)) {
-            pick = &t;
-            break;
-        }
-    if (const char* forced = getenv("SIMDONNX_HIP_QGEMM")) {  // any tiling by name (tuning, tests)
-        pick = nullptr;
-        for (const QTile& t : kQTiles)
-            if (!strcmp(t.name, forced)) pick = &t;
-        if (!pick) fail(SOX_E_INVALID, std::string("SIMDONNX_HIP_QGEMM: unknown tiling ") + forced);
+    case QPlan::RING: {
+        const QTile& t = *plan.tile;
+        a.tiles_n = (L->columns + t.bn - 1) / t.bn;
+        const int64_t tiles = ((c.rows + t.bm - 1) / t.bm) * a.tiles_n;
+        if (tiles >= (int64_t)1 << 24) fail(SOX_E_UNSUPPORTED, std::string(c.name) + ": too many outputs");
+        c.launch(L->fn_ring[storage][&t - kQTiles],
+                 (uint32_t)std::min<int64_t>(tiles, (int64_t)std::max(1, c.be->info.compute_units) * t.wgs_per_cu), 1,
+                 (uint32_t)t.threads, stream, a);
+        break;
     }
-    a.tiles_n = (L->columns + pick->bn - 1) / pick->bn;
-    const int64_t tiles = ((c.rows + pick->bm - 1) / pick->bm) * a.tiles_n;
-    if (tiles >= (int64_t)1 << 31) fail(SOX_E_UNSUPPORTED, std::string(c.name) + ": too many outputs");
-    c.launch(c.be->fn(std::string("sox_qgemm_") + kStorageName[storage] + "_" + pick->name),
-             (uint32_t)std::min<int64_t>(tiles, cus * pick->wgs_per_cu), (uint32_t)pick->threads, stream, a);
+    }
 }
 
 }  // namespace
@@ -5011,7 +5066,7 @@ void bnorm_run(sox_block_norm* N, const char* name, void* stream, int32_t storag
     const BnormShape& shape = kBnormShapes[bnorm_shape(C, many)];
     const int threads = std::max(shape.tpr, 256), per_block = threads / shape.tpr;
     const int64_t blocks = std::min<int64_t>((rows + per_block - 1) / per_block, cus * shape.per_cu);
-    c.launch(N->fn[storage][many][vec], (uint32_t)blocks, (uint32_t)threads, stream, a,
+    c.launch(N->fn[storage][many][vec], (uint32_t)blocks, 1, (uint32_t)threads, stream, a,
              shape.many ? (uint32_t)(N->vectors * shape.tpr * shape.ch * 8 * 4) : 0);
 }
 
@@ -5057,7 +5112,17 @@ void sox_qlinear_destroy(sox_qlinear* L) { delete L; }
 
 int sox_qlinear_pitch(sox_qlinear* L) { return L ? L->pitch() : 0; }
 
-uint64_t sox_qlinear_workspace(sox_qlinear* L, int32_t rows) { return L ? L->workspace(rows) : 0; }
+uint64_t sox_qlinear_workspace(sox_qlinear* L, int32_t rows) {
+    if (!L || rows <= 0 || rows > 1 << 23) return 0;
+    uint64_t need = 0;  // for every storage type
+    for (int32_t s = 0; s < 3; s++) {
+        const int rc = guarded([&] {
+            if (!QPlan(*L, rows, s, true).rounds_itself()) need = QPlan::bytes(*L, rows);
+        });
+        if (rc) return QPlan::bytes(*L, rows);
+    }
+    return need;
+}
 
 int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x, int64_t ldx, int32_t rows, const void* residual,
                     int64_t ldr, void* y, int64_t ldy, int32_t act, void* workspace, uint64_t workspace_bytes) {
@@ -5069,10 +5134,10 @@ int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x
         if (rows == 0) return;
         const Rows X = c.matrix("x", x, ldx, L->inner), R = c.matrix("residual", residual, ldr, L->columns, true);
         const Rows Y = c.matrix("y", y, ldy, L->columns);
-        const bool fused = L->fused(rows);
+        const QPlan plan(*L, rows, storage, true);
         Rows W{"workspace"};
-        if (!fused) {
-            const uint64_t need = L->workspace(rows);
+        if (!plan.rounds_itself()) {
+            const uint64_t need = QPlan::bytes(*L, rows);
             if (!workspace || workspace_bytes < need)
                 c.bad("needs " + std::to_string(need) + " bytes of workspace, has " + std::to_string(workspace ? workspace_bytes : 0));
             W = c.matrix("workspace", workspace, (int64_t)need, (int64_t)need, 1, 16, false, 1);
@@ -5089,23 +5154,23 @@ int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x
         a.ldy = ldy;
         a.act = act;
         a.vec = (c.on16(Y) && c.on16(R) ? 1 : 0) | (c.on16(X) ? 2 : 0);
-        if (!fused) {
+        if (!plan.rounds_itself()) {
             sox_qrows_args q{};
             q.x = x;
             q.ldx = ldx;
             q.q = (int8_t*)workspace;
             q.ldq = L->pitch();
-            q.scale = (float*)((uint8_t*)workspace + L->work_rows(rows));
+            q.scale = (float*)((uint8_t*)workspace + QPlan::rows_bytes(*L, rows));
             q.rows = rows;
             q.k = L->inner;
             q.vec = c.on16(X);
             const bool wide = (int64_t)L->inner * c.es > 4096;  // past what a wave's registers hold
-            c.launch(L->fn_rows[storage][wide], (uint32_t)(wide ? rows : (rows + 3) / 4), 256, stream, q);
+            c.launch(L->fn_rows[storage][wide], (uint32_t)(wide ? rows : (rows + 3) / 4), 1, 256, stream, q);
             a.a = q.q;
             a.lda = q.ldq;
             a.xs = q.scale;
         }
-        qlinear_product(c, L, stream, a, storage, fused);
+        qlinear_product(c, L, plan, stream, a, storage);
     });
 }
 
@@ -5131,7 +5196,7 @@ int sox_qlinear_run_quantized(sox_qlinear* L, void* stream, const int8_t* q, int
         a.ldy = ldy;
         a.act = act;
         a.vec = c.on16(Y) && c.on16(R) ? 1 : 0;
-        qlinear_product(c, L, stream, a, storage, false);
+        qlinear_product(c, L, QPlan(*L, rows, storage, false), stream, a, storage);
     });
 }
 

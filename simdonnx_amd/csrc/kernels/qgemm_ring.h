@@ -52,7 +52,8 @@ template <typename T> SOX_DEV int stage_at(int r, int c) {
 // A block's rows between memory at (m0, n0) and the stage: 16-byte chunks where the rows stand on 16-byte boundaries (uniform;
 // single elements in the chunk that a row ends in), else single elements, a half wave per row, in a loop that is not unrolled (the ragged form should not be most of the code).
 // LOAD: the residual's into the stage (zeros outside), else the stage's to the output.
-template <typename T, bool LOAD>
+// PART: a row may end inside a chunk.
+template <typename T, bool LOAD, bool PART>
 SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, bool vec, unsigned char* stg, int m0, int n0, int lane) {
     constexpr int E = 16 / sizeof(T), PER = 32 / E, ROWS = STG_BYTES / (32 * sizeof(T));  // elements of a chunk, chunks of a row
     typedef vec_t<T, E> TE;
@@ -68,14 +69,14 @@ SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, bool vec,
                     v = *(const TE*)g;
                 }
                 *s = v;
-                if (m < M && n < N && n + E > N)
+                if (PART && m < M && n < N && n + E > N)
 #pragma unroll 1
                     for (int e = 0; e < N - n; e++) ((T*)s)[e] = g[e];
             } else {
                 const TE v = *s;
                 if (m < M && n + E <= N) {
-                    *(TE*)g = v;
-                } else if (m < M && n < N) {
+                    __builtin_nontemporal_store(v, (TE*)g);  // (not read again here: A and W lines stay in L2)
+                } else if (PART && m < M && n < N) {
 #pragma unroll 1
                     for (int e = 0; e < N - n; e++) g[e] = ((const T*)s)[e];
                 }
@@ -109,7 +110,7 @@ SOX_DEV void stage_turn() {
 // with the residual and activated in registers, staged and stored. One copy of this with its choices inside, none of
 // them per element: a choice per element, or a copy per form, multiplied the ring's code until its instruction fetches
 // took most of a short product's time and registers ran out. ws, bias: the block's 32 columns.
-template <typename T>
+template <typename T, bool PART = true>
 SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs, const float* ws, const float* bias,
                           unsigned char* stg, int m0, int n0, int lane) {
     constexpr int PARTS = sizeof(T) == 2 ? 1 : 2, ROWS = 32 / PARTS;
@@ -130,7 +131,7 @@ SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs,
     if (p.add) {
 #pragma unroll
         for (int half = 0; half < PARTS; half++) {
-            move_rows<T, true>((T*)p.add, p.ldr, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
+            move_rows<T, true, PART>((T*)p.add, p.ldr, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
             stage_turn();
             if (PARTS == 1 || l32 / ROWS == half) {
 #pragma unroll
@@ -165,12 +166,12 @@ SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs,
             }
         }
         stage_turn();
-        move_rows<T, false>((T*)p.y, p.ldy, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
+        move_rows<T, false, PART>((T*)p.y, p.ldy, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
         stage_turn();
     }
 }
 
-template <typename T, int BM, int BN, int BK, int WM, int WN, int STAGES, int NW, int GM>
+template <typename T, int BM, int BN, int BK, int WM, int WN, int STAGES, int NW, int GM, bool PART>
 __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
     constexpr int CPR = BK / 16, KS = BK / 32;
     constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
@@ -215,45 +216,48 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
     auto a_chunk = [&](int i) __attribute__((always_inline)) {
         return (((wave * A_IT + i) * 1024 + lane * 16) % BK / 16) ^ swz<CPR>(a_row(i));
     };
+    // Ring slice gs = (place in this workgroup's tile list) * nk + k-slice; slices are started in order. Past the last tile
+    // they re-read its rows into a stage that nobody reads again, so that every slice has its loads, one count covers
+    // them all and the k-steps stay one basic block.
     const int8_t* a_src[A_IT];
-    int i_kt = 0, i_tile = vid, i_seq = 0, i_bn = 0;  // the slice being issued: its k-slice, tile and the tile's column
-    auto issue = [&](int gs) __attribute__((always_inline)) {
+    int i_kt = nk - 1, i_tile = vid - G, i_seq = -1, i_bn = 0;  // the slice being issued: its k-slice, tile and the tile's column
+    auto start_slice = [&](int gs) __attribute__((always_inline)) {
+        if (++i_kt < nk) return;
+        i_kt = 0;
+        i_tile += G;
+        if (gs >= total) return;
+        i_seq++;
+        int bm;
+        tile_origin(i_tile, bm, i_bn);
+#pragma unroll
+        for (int i = 0; i < A_IT; i++) a_src[i] = p.a + (int64_t)min(bm + a_row(i), M - 1) * p.lda + a_chunk(i) * 16;
+        unsigned char* sc = sc_mem + (i_seq % SCB) * SC_BYTES;
+        // (ws and bias are padded to whole tiles of at most 256 columns)
+        if (wave == 0 && lane < BN / 4) __builtin_amdgcn_global_load_lds(p.ws + i_bn + lane * 4, LDS_PTR(sc), 16, 0, 0);
+        if (wave == 1 && lane < BN / 4)
+            __builtin_amdgcn_global_load_lds(p.bias + i_bn + lane * 4, LDS_PTR(sc + BN * 4), 16, 0, 0);
+#pragma unroll
+        for (int i = 0; i < BM / 64; i++)
+            if (wave == i % NW)
+                __builtin_amdgcn_global_load_lds(p.xs + min(bm + i * 64 + lane, M - 1), LDS_PTR(sc + BN * 8 + i * 256), 4, 0, 0);
+    };
+    // load x of the slice started last
+    auto fire = [&](int gs, auto xx) __attribute__((always_inline)) {
+        constexpr int x = decltype(xx)::value;
         unsigned char* st = smem + (gs % STAGES) * STAGE_BYTES;
-        if (i_kt == 0) {
-            int bm;
-            tile_origin(i_tile, bm, i_bn);
-#pragma unroll
-            for (int i = 0; i < A_IT; i++) a_src[i] = p.a + (int64_t)min(bm + a_row(i), M - 1) * p.lda + a_chunk(i) * 16;
-            unsigned char* sc = sc_mem + (i_seq % SCB) * SC_BYTES;
-            // (ws and bias are padded to whole tiles of at most 256 columns)
-            if (wave == 0 && lane < BN / 4) __builtin_amdgcn_global_load_lds(p.ws + i_bn + lane * 4, LDS_PTR(sc), 16, 0, 0);
-            if (wave == 1 && lane < BN / 4)
-                __builtin_amdgcn_global_load_lds(p.bias + i_bn + lane * 4, LDS_PTR(sc + BN * 4), 16, 0, 0);
-#pragma unroll
-            for (int i = 0; i < BM / 64; i++)
-                if (wave == i % NW)
-                    __builtin_amdgcn_global_load_lds(p.xs + min(bm + i * 64 + lane, M - 1), LDS_PTR(sc + BN * 8 + i * 256), 4, 0, 0);
-        }
-        const int k0 = i_kt * BK;
-        const bool tail = k0 + BK > k16;  // uniform
-#pragma unroll
-        for (int i = 0; i < A_IT; i++) {
-            const int8_t* src = a_src[i] + k0;
-            if (tail) src = k0 + a_chunk(i) * 16 < k16 ? src : (const int8_t*)p.zeros;
-            __builtin_amdgcn_global_load_lds(src, LDS_PTR(st + (wave * A_IT + i) * 1024), 16, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < B_IT; i++) {
-            const int b = wave * B_IT + i, cb = min(i_bn / 32 + b / KS, p.nb - 1);
+        if constexpr (x < A_IT) {
+            const int k = i_kt * BK;
+            const int8_t* src = k + a_chunk(x) * 16 < k16 ? a_src[x] + k : (const int8_t*)p.zeros;
+            __builtin_amdgcn_global_load_lds(src, LDS_PTR(st + (wave * A_IT + x) * 1024), 16, 0, 0);
+        } else {
+            const int b = wave * B_IT + x - A_IT, cb = min(i_bn / 32 + b / KS, p.nb - 1);
             const int8_t* src = p.w + ((int64_t)cb * p.kb + i_kt * KS + b % KS) * 1024 + lane * 16;
             __builtin_amdgcn_global_load_lds(src, LDS_PTR(st + A_BYTES + b * 1024), 16, 0, 0);
         }
-        if (++i_kt == nk) {
-            i_kt = 0;
-            i_tile += G;
-            i_seq++;
-        }
     };
+    // A slice's loads go out in two parts, behind the slice barrier and a k-step later, one after each MFMA: a wave that
+    // issues them stalls while the CU's 64 bytes a cycle drain, and MFMAs queued between keep the matrix cores busy.
+    constexpr int PART0 = (LOADS + 1) / 2;
 
     // fragments: k-step s of a lane covers chunk 2 s + l / 32 of row l % 32 of each block
     const int a_off = (wm0 + l32) * BK + ((hl ^ swz<CPR>(l32)) << 4);  // step s: bits 5.. flipped by s (swz repeats per 32 rows)
@@ -279,7 +283,7 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
             constexpr int j = decltype(ji)::value / TI, i = decltype(ji)::value % TI;
             const float* ws = (const float*)sc + wn0 + j * 32;
             const float xs = *(const float*)(sc + BN * 8 + (wm0 + i * 32 + l32) * 4);
-            finish_block<T>(p, acc[j][i], xs, ws, ws + BN, stg, bm + wm0 + i * 32, bn + wn0 + j * 32, lane);
+            finish_block<T, PART>(p, acc[j][i], xs, ws, ws + BN, stg, bm + wm0 + i * 32, bn + wn0 + j * 32, lane);
             __builtin_amdgcn_sched_barrier(0);  // one block at a time: bounded register pressure
         });
         m_tile += G;
@@ -287,14 +291,13 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
     };
 
 #pragma unroll
-    for (int s = 0; s < STAGES; s++)
-        if (s < total) issue(s);
-    // waits until this wave's loads of the slice after gs have landed. A slice carries LOADS loads or, where it starts a
-    // tile, more, so that many newer ones at least may stay in flight for each newer slice; the last slices wait for all
-    if (total >= STAGES)
-        wait_vmcnt<(STAGES - 1) * LOADS>();
-    else
-        wait_vmcnt<0>();
+    for (int s = 0; s < STAGES; s++) {
+        start_slice(s);
+        static_for<0, LOADS>([&](auto xx) { fire(s, xx); });
+    }
+    // slice 0. (Loads complete in order; a slice carries LOADS loads or, where it starts a tile, more, so at least that many
+    // may stay in flight for each newer slice.)
+    wait_vmcnt<(STAGES - 1) * LOADS>();
     __builtin_amdgcn_s_barrier();
     clear();
     read_step(0, 0, fa0, fb0);
@@ -305,17 +308,19 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
             int4v(&cb)[TJ] = (s & 1) ? fb1 : fb0;
             int4v(&na)[TI] = (s & 1) ? fa0 : fa1;
             int4v(&nb)[TJ] = (s & 1) ? fb0 : fb1;
+            constexpr int DM = s == KS - 1 ? PART0 : s == 0 ? LOADS - PART0 : 0;  // loads issued in this k-step
             if constexpr (s == KS - 1) {
-                // slice gs + 1 landed and every read of slice gs done; after the barrier both hold for all waves
-                if (gs + STAGES < total)
-                    wait_vmcnt<(STAGES - 2) * LOADS>();
-                else
-                    wait_vmcnt<0>();
+                // slice gs + 1 landed and every read of slice gs done; after the barrier both hold for all waves, and the
+                // stage of slice gs takes slice gs + STAGES
+                wait_vmcnt<(STAGES - 2) * LOADS>();
                 wait_lgkmcnt0();
                 __builtin_amdgcn_s_barrier();
-                if (gs + STAGES < total) issue(gs + STAGES);
+                start_slice(gs + STAGES);
+                static_for<0, PART0>([&](auto xx) { fire(gs + STAGES, xx); });
                 read_step(gs + 1, 0, na, nb);  // (past the last slice: a stage whose content is not used)
             } else {
+                if constexpr (s == 0)
+                    if (gs > 0) static_for<PART0, LOADS>([&](auto xx) { fire(gs - 1 + STAGES, xx); });
                 read_step(gs, s + 1, na, nb);
             }
             static_for<0, TJ * TI>([&](auto ji) {
@@ -323,11 +328,13 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
                 acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(cb[j], ca[i], acc[j][i], 0, 0, 0);
             });
             constexpr int RD = TI + TJ, MF = TI * TJ;
-            static_for<0, (RD < MF ? RD : MF)>([&](auto) {
+            static_for<0, MF>([&](auto ii) {
+                constexpr int i = decltype(ii)::value;
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                if constexpr (i < DM) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+                if constexpr (i < RD) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             });
-            if constexpr (MF > RD) __builtin_amdgcn_sched_group_barrier(0x008, MF - RD, 0);
+            if constexpr (DM > MF) __builtin_amdgcn_sched_group_barrier(0x010, DM - MF, 0);
             if constexpr (RD > MF) __builtin_amdgcn_sched_group_barrier(0x100, RD - MF, 0);
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -338,20 +345,17 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
             clear();
         }
     }
+    wait_vmcnt<0>();  // the slices past the end land before the workgroup's LDS is given back
 }
 
 // One kernel per storage type and tiling, named BMxBN tile, wNW waves, kBK bytes of K per slice, sSTAGES; WM x WN of a tile
 // to a wave, OCC waves per SIMD, GM M-tiles to a group.
-#define SOX_QGEMM(NAME, T, TILE, BM, BN, BK, WM, WN, ST, NW, OCC, GM)                                       \
+#define SOX_QGEMM(NAME, T, TILE, BM, BN, BK, WM, WN, ST, NW, OCC, GM, PART)                                       \
     extern "C" __global__ void __launch_bounds__(64 * NW, OCC) sox_qgemm_##NAME##_##TILE(sox_qgemm_args p) { \
-        qgemm_body<T, BM, BN, BK, WM, WN, ST, NW, GM>(p);                                                   \
+        qgemm_body<T, BM, BN, BK, WM, WN, ST, NW, GM, PART>(p);                                                   \
     }
-#define SOX_QGEMM_TILES(NAME, T)                                             \
-    SOX_QGEMM(NAME, T, 256x128_w8k128s2, 256, 128, 128, 64, 64, 2, 8, 2, 4) \
-    SOX_QGEMM(NAME, T, 256x192_w8k128s2, 256, 192, 128, 64, 96, 2, 8, 2, 4) \
-    SOX_QGEMM(NAME, T, 128x128_w4k128s2, 128, 128, 128, 64, 64, 2, 4, 2, 4) \
-    SOX_QGEMM(NAME, T, 128x192_w4k64s2, 128, 192, 64, 64, 96, 2, 4, 2, 4)   \
-    SOX_QGEMM(NAME, T, 128x64_w4k128s2, 128, 64, 128, 64, 32, 2, 4, 3, 4)   \
-    SOX_QGEMM(NAME, T, 64x128_w4k128s3, 64, 128, 128, 32, 64, 3, 4, 2, 4)   \
-    SOX_QGEMM(NAME, T, 64x64_w4k128s4, 64, 64, 128, 32, 32, 4, 4, 2, 4)     \
-    SOX_QGEMM(NAME, T, 64x64_w4k64s2, 64, 64, 64, 32, 32, 2, 4, 4, 4)
+#define SOX_QGEMM_TILES(NAME, T)                                                   \
+    SOX_QGEMM(NAME, T, 256x192_w8k128s2, 256, 192, 128, 64, 96, 2, 8, 2, 4, true) \
+    SOX_QGEMM(NAME, T, 256x128_w8k128s2, 256, 128, 128, 64, 64, 2, 8, 2, 4, true) \
+    SOX_QGEMM(NAME, T, 128x128_w4k128s2, 128, 128, 128, 64, 64, 2, 4, 2, 4, true) \
+    SOX_QGEMM(NAME, T, 64x64_w4k128s4, 64, 64, 128, 32, 32, 4, 4, 2, 4, true)

@@ -14,7 +14,7 @@ from tests.layers import Matrix, linear64, quantize, rounded
 
 pytestmark = pytest.mark.gpu
 
-TILES = ["256x256_w8k128s2", "256x192_w8k128s2", "128x128_w4k128s2", "64x128_w4k128s3", "64x64_w4k128s4"]
+TILES = ["256x256_w8k128s2", "256x192_w8k128s2", "256x128_w8k128s2", "128x128_w4k128s2", "64x64_w4k128s4"]
 
 
 def weights8(seed, k, n):
@@ -84,8 +84,8 @@ def test_few_rows(hip, storage, rows, k, n):
     ("f32", 513, 65, 259, 0, 0), ("f32", 128, 129, 256, 4, 1), ("bf16", 1000, 16, 96, 0, 0)])
 def test_tiles(hip, monkeypatch, tile, storage, rows, k, n, pad, skip):
     """Every tiling, also where the choice would not take it: one slice of K and many, partial tiles on both sides."""
-    if storage == "f32" and tile[:7] == "256x256":
-        tile = "256x192_w8k128s2"  # (fp32 outputs have no 256x256 tiling)
+    if tile[:7] == "256x256" and (storage == "f32" or n % 8):
+        pytest.skip("the largest tiling takes 16-bit outputs of whole 16-byte chunks")
     monkeypatch.setenv("SIMDONNX_HIP_QGEMM", tile)
     print(f"[gpu] qlinear {tile} {storage} {rows} x {k} -> {n}", flush=True)
     both_ways(hip, 2000 + k, rows, k, n, storage, act="none", res=pad > 0, pad=pad, skip=skip)
@@ -95,7 +95,7 @@ def test_tiles(hip, monkeypatch, tile, storage, rows, k, n, pad, skip):
 def test_many_tiles_per_workgroup(hip, monkeypatch, tile):
     """More tiles than workgroups, with one slice of K each: a workgroup's slices run several tiles ahead."""
     monkeypatch.setenv("SIMDONNX_HIP_QGEMM", tile)
-    rows, n = {"256": (12000, 3300), "128": (9000, 2500), "64x": (4200, 2200)}[tile[:3].rstrip("x") if tile[0] != "6" else "64x"]
+    rows, n = {"256": (12000, 3304), "128": (9000, 2500), "64x": (4200, 2200)}[tile[:3].rstrip("x") if tile[0] != "6" else "64x"]
     print(f"[gpu] qlinear {tile} {rows} x 40 -> {n}", flush=True)
     both_ways(hip, 2100, rows, 40, n, "bf16")
 
@@ -319,7 +319,7 @@ def test_memory_of_the_host_is_refused(hip, monkeypatch):
     with pytest.raises(SoxError, match="y is not in memory the GPU reads"):
         lin.run(X.ptr, rows - 1, host.ctypes.data // 16 * 16 + 16, "f16", **given)
     monkeypatch.setenv("SIMDONNX_HIP_QGEMM", "1x1")
-    with pytest.raises(SoxError, match="unknown tiling 1x1"):
+    with pytest.raises(SoxError, match="no tiling 1x1"):
         lin.run_quantized(X.ptr, W.ptr, rows, Y.ptr, "f16", ldq=64)
     Y.read()
     for m in (X, Y, W):

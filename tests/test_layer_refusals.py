@@ -7,8 +7,8 @@ from simdonnx_amd import native as N
 from simdonnx_amd.backend import HipBackend, HipBlockNorm, HipQuantLinear
 from simdonnx_amd.native import NotSupportedError, SoxError
 
-K, C = 70, 36  # inner, columns
-ROWS = 20000  # enough for the rows to be brought to 8 bits in a workspace
+K, C = 1100, 36  # inner, columns
+ROWS = 2000  # (brought to 8 bits in a workspace)
 BASE = 1 << 20  # addresses that nothing reads
 
 
@@ -58,13 +58,13 @@ def test_linear_checks(linear):
     in_order(run, **run_args(ldx=K + 3, ldy=C + 5, residual=at(3), ldr=C + 1, storage="bf16", act="gelu"))
     in_order(run, **run_args(residual=at(1)))  # in place
     in_order(run, **run_args(rows=16, workspace=None, workspace_bytes=0))
-    assert linear.workspace(16) == linear.workspace(1000) == 0 and linear.workspace(ROWS) > ROWS * K
+    assert linear.workspace(0) == linear.workspace(16) == 0 and linear.workspace(ROWS) > ROWS * K
     linear.run(at(0), 0, at(1))  # no rows: nothing to do, nothing asked
     refused("x is null", run, **run_args(x=None))
     refused("y is null", run, **run_args(y=None))
     refused("rows", run, **run_args(rows=-1))
     refused("2\\^23 rows", run, **run_args(rows=(1 << 23) + 1))
-    refused("x: rows of 70 elements cannot be 69 apart", run, **run_args(ldx=K - 1))
+    refused("x: rows of 1100 elements cannot be 1099 apart", run, **run_args(ldx=K - 1))
     refused("y: rows of 36", run, **run_args(ldy=C - 1))
     refused("y: rows of 36", run, **run_args(ldy=1 << 50))
     refused("residual: rows of 36", run, **run_args(residual=at(3), ldr=0))
@@ -102,14 +102,14 @@ def test_linear_quantized_checks(linear):
     run = linear.run_quantized
     ok = dict(q=at(0), scales=at(1), rows=50, y=at(2))
     in_order(run, **ok)
-    in_order(run, **ok | dict(ldq=80))
-    assert linear.pitch == 128
+    in_order(run, **ok | dict(ldq=1104))
+    assert linear.pitch == 1152
     linear.run_quantized(at(0), at(1), 0, at(2))
     refused("q is null", run, **ok | dict(q=None))
     refused("scales is null", run, **ok | dict(scales=None))
     refused("q is not on 16-byte", run, **ok | dict(q=at(0) + 8))
-    refused("q is not on 16-byte", run, **ok | dict(ldq=88))
-    refused("q: rows of 80", run, **ok | dict(ldq=64))
+    refused("q is not on 16-byte", run, **ok | dict(ldq=1112))
+    refused("q: rows of 1104", run, **ok | dict(ldq=1088))
     refused("scales is not on 4-byte", run, **ok | dict(scales=at(1) + 2))
     refused("y overlaps q", run, **ok | dict(y=at(0) + 128))
     refused("y overlaps scales", run, **ok | dict(y=at(1) + 196))
