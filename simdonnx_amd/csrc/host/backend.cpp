@@ -4808,9 +4808,9 @@ struct sox_qlinear {
     int inner = 0, columns = 0, k16 = 0, kb = 0, nb = 0, npad = 0;
     DeviceBlock mem;  // packed weights, then the scales and the bias (zeros without one), padded to npad columns
     uint64_t scales_at = 0;
-    // by storage: rows to 8 bits (short, long), few 8-bit rows (16, 32, 64), few floating rows (1, 2, 4 steps a wave), panels
+    // by storage: rows to 8 bits (32, 64, 256 threads a row), few 8-bit rows (16, 32, 64), few floating rows (1, 2, 4 steps a wave), panels
     // (256 .. 1024 of K), ring tilings
-    void *fn_rows[3][2], *fn_few[3][3], *fn_fewx[3][3], *fn_panel[3][4], *fn_ring[3][8];
+    void *fn_rows[3][3], *fn_few[3][3], *fn_fewx[3][3], *fn_panel[3][4], *fn_ring[3][8];
 
     const int8_t* w() const { return (const int8_t*)mem.p; }
     const float* ws() const { return (const float*)((const uint8_t*)mem.p + scales_at); }
@@ -4833,6 +4833,7 @@ const QTile kQTiles[] = {
     {"128x128_w4k128s2", 128, 128, 2, 256, 0.59f, 0.45f, 3.5f, 1.5f, 0.35f},
     {"64x64_w4k128s4", 64, 64, 2, 256, 0.32f, 0.22f, 3.8f, 0.1f, 0.51f},
 };
+const int kRowThreads[] = {32, 64, 256};  // of a row brought to 8 bits, each with four 16-byte chunks in registers
 constexpr int kQTileCount = (int)(sizeof kQTiles / sizeof *kQTiles);
 
 // How a product of m rows runs. Every way gives the same bits (whole numbers), so the choice is by time alone, each
@@ -4915,8 +4916,7 @@ void qlinear_pack(sox_qlinear& L, const int8_t* w, const float* scales, const fl
     L.mem.upload(L.be, host.data(), host.size(), "QuantLinear weights");
     for (int s = 0; s < 3; s++) {
         const std::string st = kStorageName[s];
-        L.fn_rows[s][0] = L.be->fn("sox_qrows_" + st);
-        L.fn_rows[s][1] = L.be->fn("sox_qrows_" + st + "_wide");
+        for (int i = 0; i < 3; i++) L.fn_rows[s][i] = L.be->fn("sox_qrows_" + st + "_t" + std::to_string(kRowThreads[i]));
         for (int i = 0; i < kQTileCount; i++) {
             L.fn_ring[s][i] = nullptr;
             if (s != SOX_STORAGE_F32 || kQTiles[i].bm * kQTiles[i].bn < 256 * 256)
@@ -5164,8 +5164,9 @@ int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x
             q.rows = rows;
             q.k = L->inner;
             q.vec = c.on16(X);
-            const bool wide = (int64_t)L->inner * c.es > 4096;  // past what a wave's registers hold
-            c.launch(L->fn_rows[storage][wide], (uint32_t)(wide ? rows : (rows + 3) / 4), 1, 256, stream, q);
+            const int64_t bytes = (int64_t)L->inner * c.es;
+            const int ti = bytes <= 32 * 64 ? 0 : bytes <= 64 * 64 ? 1 : 2, per_block = 256 / kRowThreads[ti];
+            c.launch(L->fn_rows[storage][ti], (uint32_t)((rows + per_block - 1) / per_block), 1, 256, stream, q);
             a.a = q.q;
             a.lda = q.ldq;
             a.xs = q.scale;

@@ -2,7 +2,7 @@
 #include "qgemm_ring.h"
 
 // ---- rows to 8 bits ----
-// TPR threads per row (a wave, or the workgroup for long rows). A thread keeps its first CH chunks of 16 bytes in
+// TPR threads per row (half a wave, a wave, or the workgroup for long rows). A thread keeps its first CH chunks of 16 bytes in
 // registers between the maximum and the rounding; what is past them (rows of more than CH * TPR * 16 bytes) is read
 // again, from L2. One read of x and one write of q: bound by memory.
 template <typename T, int TPR> SOX_DEV void qrows_body(const sox_qrows_args& p) {
@@ -12,7 +12,7 @@ template <typename T, int TPR> SOX_DEV void qrows_body(const sox_qrows_args& p) 
     __shared__ uint32_t wmax[4];
     const int t = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR;
-    if (row >= p.rows) return;  // (whole waves; with the workgroup per row the grid has no such row)
+    if (TPR < 256 && row >= p.rows) return;  // (with the workgroup per row the grid has no such row)
     const T* x = (const T*)p.x + row * p.ldx;
     int8_t* q = p.q + row * p.ldq;
     const int chunks = ((p.k + 15) / 16 * 16) / E;
@@ -29,7 +29,7 @@ template <typename T, int TPR> SOX_DEV void qrows_body(const sox_qrows_args& p) 
         u.load(x, c * E, p.k, p.vec);
         top.add(u);
     }
-    uint32_t m = wave_max(top.lane());
+    uint32_t m = wave_max<TPR == 32 ? 32 : 64>(top.lane());
     if constexpr (TPR == 256) {
         if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = m;
         __syncthreads();
@@ -53,9 +53,9 @@ template <typename T, int TPR> SOX_DEV void qrows_body(const sox_qrows_args& p) 
     if (t == 0) p.scale[row] = rq.scale;
 }
 
-#define SOX_QROWS(NAME, T)                                                                                               \
-    extern "C" __global__ void __launch_bounds__(256) sox_qrows_##NAME(sox_qrows_args p) { qrows_body<T, 64>(p); }      \
-    extern "C" __global__ void __launch_bounds__(256) sox_qrows_##NAME##_wide(sox_qrows_args p) { qrows_body<T, 256>(p); }
+#define SOX_QROWS_T(NAME, T, TPR) \
+    extern "C" __global__ void __launch_bounds__(256) sox_qrows_##NAME##_t##TPR(sox_qrows_args p) { qrows_body<T, TPR>(p); }
+#define SOX_QROWS(NAME, T) SOX_QROWS_T(NAME, T, 32) SOX_QROWS_T(NAME, T, 64) SOX_QROWS_T(NAME, T, 256)
 SOX_QROWS(f16, half_t)
 SOX_QROWS(bf16, bf16_t)
 SOX_QROWS(f32, float)
@@ -199,9 +199,6 @@ SOX_QFEW_ALL(f32, float)
 // LDS, block kb of 32 k: slot (k % 32 / 16 * 32 + row) ^ (k / 16 % 16) of 16 bytes, so the writers (a lane per 16 k of a row)
 // spread over the banks, and a fragment read stays a permutation of one KiB.
 constexpr int QP_ROWS = 32;
-#ifndef TS
-#define TS(i)
-#endif
 template <typename T, int CH> SOX_DEV void qpanel_body(const sox_qgemm_args& p) {
     typedef RowQuant<T> Q;
     extern __shared__ __attribute__((aligned(1024))) unsigned char panel[];  // [kb][1 KiB]
@@ -214,7 +211,6 @@ template <typename T, int CH> SOX_DEV void qpanel_body(const sox_qgemm_args& p) 
     const int m0 = blockIdx.y * QP_ROWS;
     const bool live = cb < p.nb;  // (uniform per wave)
     const int8_t* w = p.w + (int64_t)min(cb, p.nb - 1) * p.kb * 1024 + lane * 16;
-    TS(0);
     int4v wf[4 * CH];  // the wave's weights, all of them (K <= 256 CH)
 #pragma unroll
     for (int i = 0; i < 4 * CH; i++) wf[i] = k0 + i < k1 ? *(const int4v*)(w + (int64_t)(k0 + i) * 1024) : (int4v)0;
@@ -227,8 +223,7 @@ template <typename T, int CH> SOX_DEV void qpanel_body(const sox_qgemm_args& p) 
         AbsMax<T> top;
 #pragma unroll
         for (int c = 0; c < CH; c++) top.add(v[c]);
-        TS(1);
-        const Q rq = Q::make(AbsMax<T>::row_bits(row16_max(top.lane())));
+            const Q rq = Q::make(AbsMax<T>::row_bits(row16_max(top.lane())));
         if (i16 == 0) xscale[row] = rq.scale;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
@@ -238,9 +233,7 @@ template <typename T, int CH> SOX_DEV void qpanel_body(const sox_qgemm_args& p) 
                     int4v{(int)Q::q4(v[c], 0, rq), (int)Q::q4(v[c], 4, rq), (int)Q::q4(v[c], 8, rq), (int)Q::q4(v[c], 12, rq)};
         }
     }
-    TS(2);
     __syncthreads();
-    TS(3);
     int16v acc = (int16v)0;
 #pragma unroll
     for (int i = 0; i < 4 * CH; i++) {
@@ -248,12 +241,10 @@ template <typename T, int CH> SOX_DEV void qpanel_body(const sox_qgemm_args& p) 
         const int4v xf = *(const int4v*)(panel + kb * 1024 + ((lane ^ ((2 * kb + lane / 32) % 16)) << 4));
         acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[i], xf, acc, 0, 0, 0);
     }
-    TS(4);
     if (wave >= 4)
 #pragma unroll
         for (int q = 0; q < 4; q++) half_sums[wave - 4][q][lane] = int4v{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
     __syncthreads();
-    TS(5);
     if (wave >= 4 || !live) return;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
@@ -262,7 +253,6 @@ template <typename T, int CH> SOX_DEV void qpanel_body(const sox_qgemm_args& p) 
         for (int e = 0; e < 4; e++) acc[4 * q + e] += o[e];
     }
     finish_block<T>(p, acc, xscale[lane & 31], p.ws + cb * 32, p.bias + cb * 32, stage[wave], m0, cb * 32, lane);
-    TS(6);
 }
 
 #define SOX_QPANEL(NAME, T, CH)                                                                                              \
