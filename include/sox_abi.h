@@ -592,7 +592,7 @@ typedef struct sox_qgemm_args {
     int32_t m, n, k, k16;
     int32_t kb, nb;     /* 32-k blocks of a column block, column blocks */
     int32_t tiles_n, act;
-    int32_t vec;        /* bit0: y (and residual) rows on 16-byte boundaries; bit1: x rows too */
+    int32_t vec;        /* bit0: y (and residual) rows on 16-byte boundaries; bit1: x rows too; bit2: y rows on 128-byte lines */
     int32_t pad_;
 } sox_qgemm_args;
 

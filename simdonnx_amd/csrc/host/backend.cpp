@@ -4742,8 +4742,8 @@ struct LayerCall {
     Rows matrix(const char* what, const void* p, int64_t ld, int64_t cols, bool optional = false) const {
         return matrix(what, p, ld, cols, es, es, optional, rows);
     }
-    // every row on 16-byte boundaries
-    static bool on16(const Rows& r) { return !r.any() || (r.at % 16 == 0 && (r.pitch % 16 == 0 || r.rows == 1)); }
+    // every row on boundaries of 16 bytes, or `to`
+    static bool on(const Rows& r, uint64_t to = 16) { return !r.any() || (r.at % to == 0 && (r.pitch % (int64_t)to == 0 || r.rows == 1)); }
 
     LayerCall(sox_backend* b, const char* n, int32_t nrows, int32_t storage) : be(b), name(n), rows(nrows) {
         if (nrows < 0) bad("rows");
@@ -4827,11 +4827,11 @@ struct QTile {
     float lat, thr, base, tile, out;
 };
 const QTile kQTiles[] = {
-    {"256x256_w8k128s2", 256, 256, 1, 512, 0.79f, 1.13f, 0.0f, 7.4f, 0.48f},
-    {"256x192_w8k128s2", 256, 192, 1, 512, 0.79f, 0.97f, 1.2f, 5.5f, 0.40f},
-    {"256x128_w8k128s2", 256, 128, 1, 512, 0.83f, 0.84f, 2.6f, 2.9f, 0.35f},
-    {"128x128_w4k128s2", 128, 128, 2, 256, 0.59f, 0.45f, 3.5f, 1.5f, 0.35f},
-    {"64x64_w4k128s4", 64, 64, 2, 256, 0.32f, 0.22f, 3.8f, 0.1f, 0.51f},
+    {"256x256_w8k128s2", 256, 256, 1, 512, 0.35f, 1.15f, 3.3f, 3.8f, 0.51f},
+    {"256x192_w8k128s2", 256, 192, 1, 512, 0.43f, 0.99f, 2.7f, 3.9f, 0.43f},
+    {"256x128_w8k128s2", 256, 128, 1, 512, 0.84f, 0.85f, 4.0f, 1.2f, 0.43f},
+    {"128x128_w4k128s2", 128, 128, 2, 256, 0.59f, 0.465f, 4.45f, 0.4f, 0.44f},
+    {"64x64_w4k128s4", 64, 64, 2, 256, 0.31f, 0.22f, 3.5f, 0.2f, 0.57f},
 };
 const int kRowThreads[] = {32, 64, 256};  // of a row brought to 8 bits, each with four 16-byte chunks in registers
 constexpr int kQTileCount = (int)(sizeof kQTiles / sizeof *kQTiles);
@@ -4843,8 +4843,8 @@ constexpr int kQTileCount = (int)(sizeof kQTiles / sizeof *kQTiles);
 //          once per 128 columns                                              of its own 9.4. 8192 x 768 -> 2304: 51, 35
 //   FEW    up to 64 8-bit rows, weights straight to registers                64 x 4096 -> 4096: 10.8 us, ring 13.5;
 //                                                                            64 x 1024 -> 8192: 6.9, ring 6.0
-//   RING   8-bit rows on the ring of the tiling with the smallest estimate. Over 75 random products the pick is 2% above
-//          the fastest tiling on average, at most 31%
+//   RING   8-bit rows on the ring of the tiling with the smallest estimate. Over 170 random products the pick is 1.4% above
+//          the fastest tiling on average, at most 21%
 // FEW and RING take floating rows behind a launch that brings them to 8 bits in the workspace.
 struct QPlan {
     enum Way { FEWX, PANEL, FEW, RING } way = RING;
@@ -5060,7 +5060,7 @@ void bnorm_run(sox_block_norm* N, const char* name, void* stream, int32_t storag
     a.rows = rows; a.c = C; a.gate_group = gate ? rows / gate_rows : 1;
     a.post = N->p.post; a.pre = N->p.pre; a.gate_act = N->p.gate_act;
     a.post_eps = N->p.post_eps; a.pre_eps = N->p.pre_eps; a.res_scale = N->p.res_scale;
-    const bool vec = c.on16(R) && c.on16(X) && c.on16(G) && c.on16(H) && (quantized || c.on16(Y));
+    const bool vec = c.on(R) && c.on(X) && c.on(G) && c.on(H) && (quantized || c.on(Y));
     const int64_t cus = std::max(1, c.be->info.compute_units);
     const bool many = rows >= 4 * cus;  // a wave on every SIMD
     const BnormShape& shape = kBnormShapes[bnorm_shape(C, many)];
@@ -5153,7 +5153,7 @@ int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x
         a.y = y;
         a.ldy = ldy;
         a.act = act;
-        a.vec = (c.on16(Y) && c.on16(R) ? 1 : 0) | (c.on16(X) ? 2 : 0);
+        a.vec = (c.on(Y) && c.on(R) ? 1 : 0) | (c.on(X) ? 2 : 0) | (c.on(Y, 128) ? 4 : 0);
         if (!plan.rounds_itself()) {
             sox_qrows_args q{};
             q.x = x;
@@ -5163,7 +5163,7 @@ int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x
             q.scale = (float*)((uint8_t*)workspace + QPlan::rows_bytes(*L, rows));
             q.rows = rows;
             q.k = L->inner;
-            q.vec = c.on16(X);
+            q.vec = c.on(X);
             const int64_t bytes = (int64_t)L->inner * c.es;
             const int ti = bytes <= 32 * 64 ? 0 : bytes <= 64 * 64 ? 1 : 2, per_block = 256 / kRowThreads[ti];
             c.launch(L->fn_rows[storage][ti], (uint32_t)((rows + per_block - 1) / per_block), 1, 256, stream, q);
@@ -5196,7 +5196,7 @@ int sox_qlinear_run_quantized(sox_qlinear* L, void* stream, const int8_t* q, int
         a.y = y;
         a.ldy = ldy;
         a.act = act;
-        a.vec = c.on16(Y) && c.on16(R) ? 1 : 0;
+        a.vec = (c.on(Y) && c.on(R) ? 1 : 0) | (c.on(Y, 128) ? 4 : 0);
         qlinear_product(c, L, QPlan(*L, rows, storage, false), stream, a, storage);
     });
 }

@@ -51,13 +51,16 @@ template <typename T> SOX_DEV int stage_at(int r, int c) {
 
 // A block's rows between memory at (m0, n0) and the stage: 16-byte chunks where the rows stand on 16-byte boundaries (uniform;
 // single elements in the chunk that a row ends in), else single elements, a half wave per row, in a loop that is not unrolled (the ragged form should not be most of the code).
+// Outputs whose rows stand on 128-byte lines pass L2 by (vec bit 2), which leaves it to the A and W lines that are read
+// again: 8192 x 768 -> 2304 29.4 -> 28.2 us. Other rows' lines are written in parts by different stores, and in parts
+// they would reach memory: 2954 x 320 -> 3112 took 19.8 us so, 13.3 through L2.
 // LOAD: the residual's into the stage (zeros outside), else the stage's to the output.
 // PART: a row may end inside a chunk.
 template <typename T, bool LOAD, bool PART>
-SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, bool vec, unsigned char* stg, int m0, int n0, int lane) {
+SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, int vec, unsigned char* stg, int m0, int n0, int lane) {
     constexpr int E = 16 / sizeof(T), PER = 32 / E, ROWS = STG_BYTES / (32 * sizeof(T));  // elements of a chunk, chunks of a row
     typedef vec_t<T, E> TE;
-    if (vec) {
+    if (vec & 1) {
 #pragma unroll
         for (int t = 0; t < ROWS * PER / 64; t++) {
             const int idx = t * 64 + lane, r = idx / PER, u = idx % PER, m = m0 + r, n = n0 + u * E;
@@ -75,7 +78,10 @@ SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, bool vec,
             } else {
                 const TE v = *s;
                 if (m < M && n + E <= N) {
-                    __builtin_nontemporal_store(v, (TE*)g);  // (not read again here: A and W lines stay in L2)
+                    if (vec & 4)
+                        __builtin_nontemporal_store(v, (TE*)g);
+                    else
+                        *(TE*)g = v;
                 } else if (PART && m < M && n < N) {
 #pragma unroll 1
                     for (int e = 0; e < N - n; e++) g[e] = ((const T*)s)[e];
@@ -116,7 +122,7 @@ SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs,
     constexpr int PARTS = sizeof(T) == 2 ? 1 : 2, ROWS = 32 / PARTS;
     typedef vec_t<T, 4> T4;
     const int l32 = lane & 31, hl = lane >> 5;
-    const bool vec = p.vec & 1;
+    const int vec = p.vec;
     float val[16];
 #pragma unroll
     for (int q = 0; q < 4; q++) {
