@@ -577,7 +577,7 @@ typedef struct sox_qrows_args {
  *   y[r][c] = act(sum_k a[r][k] w[k][c] * xs[r] * ws[c] + bias[c] (+ add[r][c]))
  * w: blocks of 32 columns x 32 k, one KiB each, block (c / 32) * kb + k / 32; byte (k % 32 / 16 * 32 + c % 32) * 16 +
  * k % 16 of its block is w[k][c] (zeros past k and the last column). ws and bias are padded with zeros to a multiple
- * of 256. The sox_qfew_* kernels with floating rows (x) bring them to 8 bits themselves. */
+ * of 256 and 256 more. The sox_qfew_* kernels with floating rows (x) bring them to 8 bits themselves. */
 typedef struct sox_qgemm_args {
     const int8_t* a;
     const float* xs;

@@ -4731,7 +4731,7 @@ struct LayerCall {
             if (!optional) bad(std::string(what) + " is null");
             return r;
         }
-        if (ld < cols || ld > ((int64_t)1 << 40)) bad(std::string(what) + ": rows of " + std::to_string(cols) + " elements cannot be " + std::to_string(ld) + " apart");
+        if (ld < cols || ld > ((int64_t)1 << 60) / std::max<int64_t>(nrows, 1) / elem) bad(std::string(what) + ": rows of " + std::to_string(cols) + " elements cannot be " + std::to_string(ld) + " apart");
         if ((uintptr_t)p % (uint64_t)align || ld * elem % align) bad(std::string(what) + " is not on " + std::to_string(align) + "-byte boundaries");
         r.at = (uint64_t)(uintptr_t)p;
         r.rows = nrows;
@@ -4770,8 +4770,10 @@ struct LayerCall {
         if (d != be->info.device) bad("the stream is another device's");
         for (const Rows* r : all) {
             if (!r->any()) continue;
-            check(sox_pointer_device((const void*)(uintptr_t)r->at, &d), name);
-            if (d != be->info.device) bad(std::string(r->what) + (d < 0 ? " is not in memory the GPU reads" : " is on another device"));
+            for (uint64_t at : {r->at, r->end() - 1}) {  // its first and its last byte
+                check(sox_pointer_device((const void*)(uintptr_t)at, &d), name);
+                if (d != be->info.device) bad(std::string(r->what) + (d < 0 ? " is not in memory the GPU reads" : " is on another device"));
+            }
         }
     }
     template <class A>
@@ -4941,7 +4943,7 @@ std::unique_ptr<sox_qlinear> qlinear_new(sox_backend* be, const void* weights, i
     L->k16 = round_up(inner, 16);
     L->kb = round_up(inner, 128) / 32;
     L->nb = (columns + 31) / 32;
-    L->npad = round_up(columns, 256);
+    L->npad = round_up(columns, 256) + 256;  // (a last tile of 192 columns may start inside the last 256)
     return L;
 }
 

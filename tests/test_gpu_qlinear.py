@@ -2,6 +2,10 @@
 whole numbers and 64 bits. Tolerances are the steps' roundings (tests/layers.py); what the 8-bit rounding itself does
 is exact on both sides."""
 import ctypes
+import os
+import subprocess
+import sys
+import threading
 
 import numpy as np
 import pytest
@@ -10,7 +14,7 @@ from simdonnx_amd import native as N
 from simdonnx_amd import synth
 from simdonnx_amd.backend import HipQuantLinear
 from simdonnx_amd.native import SoxError
-from tests.layers import Matrix, linear64, quantize, rounded
+from tests.layers import Matrix, from_bits, linear64, quantize, rounded, to_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -71,7 +75,7 @@ def both_ways(hip, seed, rows, k, n, storage, act="none", bias=True, res=False, 
 
 
 @pytest.mark.parametrize("storage", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("rows,k,n", [(1, 1, 1), (1, 768, 768), (2, 16, 15), (3, 65, 33), (7, 4096, 80), (16, 1000, 17), (16, 4097, 40),
+@pytest.mark.parametrize("rows,k,n", [(1, 1, 1), (1, 768, 768), (2, 16, 15), (3, 65, 33), (7, 4096, 80), (16, 1000, 17), (16, 4097, 40), (16, 4096, 24),
                                       (17, 577, 301), (33, 129, 64), (64, 320, 100), (1, 9000, 31)])
 def test_few_rows(hip, storage, rows, k, n):
     print(f"[gpu] qlinear {storage} {rows} x {k} -> {n}", flush=True)
@@ -325,3 +329,146 @@ def test_memory_of_the_host_is_refused(hip, monkeypatch):
     for m in (X, Y, W):
         m.free()
     lin.close()
+
+
+def rows_apart(data, storage, pitch):
+    """The rows of a matrix `pitch` bytes apart in an allocation that nothing else of is written or read: (address, read)."""
+    bits = to_bits(data, storage)
+    p = N.c_void_p()
+    N.check(N.thin().sox_malloc(ctypes.byref(p), (len(bits) - 1) * pitch + bits[0].nbytes), "sox_malloc")
+    for i, row in enumerate(bits):
+        row = np.ascontiguousarray(row)
+        N.check(N.thin().sox_memcpy_h2d(p.value + i * pitch, row.ctypes.data, row.nbytes, None), "h2d")
+    N.check(N.thin().sox_stream_sync(None), "sync")
+
+    def read():
+        got = np.empty_like(bits)
+        for i in range(len(got)):
+            N.check(N.thin().sox_memcpy_d2h(got[i].ctypes.data, p.value + i * pitch, got[i].nbytes, None), "d2h")
+        N.check(N.thin().sox_stream_sync(None), "sync")
+        return from_bits(got, storage)
+    return p, read
+
+
+@pytest.mark.parametrize("rows,k", [(70, 1100), (40, 96), (12, 200)])
+def test_rows_far_apart(hip, rows, k):
+    """Offsets past 32 bits, in elements and in bytes, of the input, the 8-bit rows, the residual and the output."""
+    n, pitch, st = 40, 1 << 28, "bf16"
+    w, ws = weights8(13, k, n)
+    x, r = rows_of(13, rows, k, st), rounded(synth.normal(13, 6, (rows, n), 1.0), st)
+    q, scale = quantize(x)
+    want, tol = linear64(q, scale, w, ws, None, r, "none", st)
+    lin = HipQuantLinear(hip, w, None, k, n, scales=ws)
+    (X, _), (Y, read), (R, _) = rows_apart(x, st, pitch), rows_apart(np.zeros((rows, n), np.float32), st, pitch), rows_apart(r, st, pitch)
+    W = Matrix(None, "i8", 1, max(1, lin.workspace(rows)))
+    print(f"[gpu] qlinear rows far apart {rows} x {k}", flush=True)
+    lin.run(X.value, rows, Y.value, st, ldx=pitch // 2, ldy=pitch // 2, residual=R.value, ldr=pitch // 2, workspace=W.ptr,
+            workspace_bytes=lin.workspace(rows))
+    got = read()
+    check(got, want, tol)
+    q8 = np.zeros((rows, -(-k // 16) * 16), np.float32)
+    q8[:, :k] = q
+    S = Matrix(scale.astype(np.float32)[None], "f32")
+    N.check(N.thin().sox_free(X), "free")
+    p = N.c_void_p()
+    N.check(N.thin().sox_malloc(ctypes.byref(p), (rows - 1) * pitch + q8.shape[1]), "sox_malloc")
+    for i, row in enumerate(q8.astype(np.int8)):
+        N.check(N.thin().sox_memcpy_h2d(p.value + i * pitch, row.ctypes.data, row.nbytes, None), "h2d")
+    N.check(N.thin().sox_stream_sync(None), "sync")
+    lin.run_quantized(p.value, S.ptr, rows, Y.value, st, ldq=pitch, ldy=pitch // 2, residual=R.value, ldr=pitch // 2)
+    assert np.array_equal(read(), got)
+    for m in (p, Y, R):
+        N.thin().sox_free(m)
+    for m in (W, S):
+        m.free()
+    lin.close()
+
+
+def test_calls_from_threads(hip):
+    """One layer called from four threads at once, each on a stream and with a workspace of its own."""
+    k, n, rows, times = 1200, 136, 90, 20
+    w, ws = weights8(14, k, n)
+    lin = HipQuantLinear(hip, w, None, k, n, scales=ws)
+    T = N.thin()
+    sides, errors = [], []
+    for i in range(4):
+        st = N.c_void_p()
+        N.check(T.sox_stream_create(ctypes.byref(st)), "stream")
+        x = rows_of(30 + i, rows, k, "f16")
+        X, Y = Matrix(x, "f16"), Matrix(None, "f16", rows, n)
+        W = Matrix(None, "i8", 1, lin.workspace(rows))
+        q, scale = quantize(x)
+        sides.append((st, X, Y, W, linear64(q, scale, w, ws, None, None, "none", "f16")))
+
+    def work(st, X, Y, W, want):
+        try:
+            for _ in range(times):
+                lin.run(X.ptr, rows, Y.ptr, "f16", workspace=W.ptr, workspace_bytes=lin.workspace(rows), stream=st)
+            N.check(T.sox_stream_sync(st), "sync")
+        except Exception as e:  # noqa: BLE001 (reported by the test's own thread)
+            errors.append(e)
+    print("[gpu] qlinear from threads", flush=True)
+    threads = [threading.Thread(target=work, args=s) for s in sides]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for st, X, Y, W, want in sides:
+        check(Y.read(), *want)
+        T.sox_stream_destroy(st)
+        for m in (X, Y, W):
+            m.free()
+    lin.close()
+
+
+TORCH = """
+import sys
+import torch  # before the backend's libraries: both then share one HIP runtime
+sys.path.insert(0, {root!r})
+import numpy as np
+from simdonnx_amd.backend import HipBackend, HipBlockNorm, HipQuantLinear
+hip = HipBackend.default()
+torch.manual_seed(1)
+k, n = 320, 200
+lin = HipQuantLinear(hip, torch.randint(-127, 128, (k, n)).numpy(), None, k, n, scales=np.full(n, 1e-3, np.float32))
+norm = HipBlockNorm(hip, k, post="rms", pre="layer")
+assert torch.zeros(3, device="cuda").add(1).sum().item() == 3  # no error of the backend's is left for torch to find
+for rows in (5, 300):
+    x, r = (torch.randn(rows, k, device="cuda", dtype=torch.float16) for _ in range(2))
+    h, y = torch.zeros_like(x), torch.zeros(rows, n, device="cuda", dtype=torch.float16)
+    q, s = torch.zeros(rows, lin.pitch, device="cuda", dtype=torch.int8), torch.zeros(rows, device="cuda")
+
+    def step():
+        st = torch.cuda.current_stream().cuda_stream
+        norm.run_quantized(r.data_ptr(), rows, q.data_ptr(), s.data_ptr(), x=x.data_ptr(), h=h.data_ptr(), stream=st)
+        lin.run_quantized(q.data_ptr(), s.data_ptr(), rows, y.data_ptr(), stream=st)
+    print("[gpu] torch capture", rows, flush=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        step()
+    for rep in range(3):
+        x.normal_()
+        step()
+        torch.cuda.synchronize()
+        want = [t.clone() for t in (h, y, q, s)]
+        for t in (h, y, q, s):
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, (h, y, q, s))), rep
+        assert y.abs().max().item() > 0
+print("torch ok", flush=True)
+"""
+
+
+def test_beside_torch():
+    """torch's tensors and streams in, and a graph that torch captures: in a process that loads torch first."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-u", "-c", TORCH.format(root=root)], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "torch ok" in r.stdout, r.stdout + r.stderr[-3000:]
