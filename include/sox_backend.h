@@ -363,6 +363,23 @@ int sox_block_norm_run_quantized(sox_block_norm* norm, void* stream, int32_t sto
                                  int64_t ldr, const void* x, int64_t ldx, const void* gate, int64_t ldg, int32_t gate_rows,
                                  void* h, int64_t ldh, int8_t* q, int64_t ldq, float* scales);
 
+/* Both as nodes of a plan, SOX_OP_EXT nodes named "QuantLinear" and "BlockNorm" (a consumer's registration of the name
+ * wins). Values are rows over their last dimension, stored in the order of their shape. A BlockNorm whose y only
+ * QuantLinears read, as x, hands them 8-bit rows (channels a multiple of 16; SIMDONNX_HIP_NO_QUANT_NORM leaves y in
+ * storage elements, rounded again by each reader). */
+typedef struct sox_quant_linear_p { /* in: x, weights (const [inner][columns]), bias (const) if any, residual if any; out: y */
+    int32_t act, has_bias, has_residual;
+} sox_quant_linear_p;
+/* operands of a BlockNorm node: which values its in and out list, in this order. The vectors are consts [channels]. */
+enum {
+    SOX_BN_RESIDUAL = 1, SOX_BN_X = 2, SOX_BN_GATE = 4, SOX_BN_POST_GAMMA = 8, SOX_BN_POST_BETA = 16, SOX_BN_SCALE = 32,
+    SOX_BN_PRE_GAMMA = 64, SOX_BN_PRE_BETA = 128, SOX_BN_H = 256, SOX_BN_Y = 512
+};
+typedef struct sox_block_norm_node_p {
+    sox_block_norm_p norm;
+    uint32_t operands;               /* SOX_BN_* */
+} sox_block_norm_node_p;
+
 /* ---- image session (VkImageSession, Backends/Vulkan/VkImageSession.cs:7-297) ----
  * Image-to-image inference with the pixel conversions on the device, in the same stream as the model:
  * one upload of the bytes, the dispatches, one download. The model maps [1, 3, H, W] to [1, 3, H, W];

@@ -272,6 +272,293 @@ sox_backend* g_default = nullptr;
 }  // namespace
 
 // ================================================================================================
+// 8-bit transformer layers: how they run (the objects at the end of this file and the plan nodes share it)
+// ================================================================================================
+namespace {
+
+int round_up(int k, int to) { return (k + to - 1) / to * to; }
+
+const char* const kStorageName[] = {"f32", "f16", "bf16"};  // by SOX_STORAGE_*
+
+// The tilings of the 8-bit ring (qgemm.hip), with the terms of their estimated time in us (QPlan::ring_us).
+struct QTile {
+    const char* name;
+    int bm, bn, wgs_per_cu, threads;
+    float lat, thr, base, tile, out;
+};
+const QTile kQTiles[] = {
+    {"256x256_w8k128s2", 256, 256, 1, 512, 0.35f, 1.15f, 3.3f, 3.8f, 0.51f},
+    {"256x192_w8k128s2", 256, 192, 1, 512, 0.43f, 0.99f, 2.7f, 3.9f, 0.43f},
+    {"256x128_w8k128s2", 256, 128, 1, 512, 0.84f, 0.85f, 4.0f, 1.2f, 0.43f},
+    {"128x128_w4k128s2", 128, 128, 2, 256, 0.59f, 0.465f, 4.45f, 0.4f, 0.44f},
+    {"64x64_w4k128s4", 64, 64, 2, 256, 0.31f, 0.22f, 3.5f, 0.2f, 0.57f},
+};
+const int kRowThreads[] = {32, 64, 256};  // of a row brought to 8 bits, each with four 16-byte chunks in registers
+constexpr int kQTileCount = (int)(sizeof kQTiles / sizeof *kQTiles);
+
+// How a product of m rows runs. Every way gives the same bits (whole numbers), so the choice is by time alone, each
+// estimate a fit to measurements on one MI355X:
+//   FEWX   up to 16 floating rows of up to 4096 values, one launch           1 x 768 -> 768: 3.9 us
+//   PANEL  floating rows of up to 1024 values, one launch that rounds them   786 x 768 -> 760: 7.3 us; rounded by a launch
+//          once per 128 columns                                              of its own 9.4. 8192 x 768 -> 2304: 51, 35
+//   FEW    up to 64 8-bit rows, weights straight to registers                64 x 4096 -> 4096: 10.8 us, ring 13.5;
+//                                                                            64 x 1024 -> 8192: 6.9, ring 6.0
+//   RING   8-bit rows on the ring of the tiling with the smallest estimate. Over 170 random products the pick is 1.4% above
+//          the fastest tiling on average, at most 21%
+// FEW and RING take floating rows behind a launch that brings them to 8 bits in the workspace.
+struct QPlan {
+    enum Way { FEWX, PANEL, FEW, RING } way = RING;
+    const QTile* tile = nullptr;
+
+    // A CU's tiles, each with an epilogue; K slices of 128, bound by their latency with few tiles and by the CU's matrix cores
+    // and loads with many; the outputs' stores.
+    static float ring_us(const QTile& t, double m, double n, double k, double cus) {
+        const float q = (float)ceil(ceil(m / t.bm) * ceil(n / t.bn) / cus), nk = (float)ceil(k / 128);
+        return t.base + q * t.tile + nk * std::max(t.lat, q * t.thr) + t.out * (float)(m * n * 1e-6);
+    }
+    static float few_us(double m, double n, double k) {
+        return (float)(2.6 + 0.03 * m + k * (2e-4 + 2.4e-5 * m) * std::max(1.0, n / 8192));
+    }
+    static float panel_us(double m, double n, double k, int es, double cus) {
+        return (float)(3.0 + ceil(ceil(m / 32) * ceil(n / 128) / cus) * (0.6 + 0.0027 * k * (es == 4 ? 2 : 1)));
+    }
+    // a launch (3 us, and one more of the host's time) and the rows in and out
+    static float rows_us(double m, double k, int es) { return (float)(4.0 + m * k * (es + 1) / 4.5e6); }
+
+    QPlan(int inner, int columns, int compute_units, int64_t m, int32_t storage, bool floating) {
+        const int es = storage == SOX_STORAGE_F32 ? 4 : 2;
+        const double cus = std::max(1, compute_units), n = columns, k = inner;
+        if (floating && m <= 16 && inner <= 4096) {
+            way = FEWX;
+            return;
+        }
+        const char* forced = getenv("SIMDONNX_HIP_QGEMM");  // any tiling by name (tuning, tests)
+        float best = 0.0f;
+        for (const QTile& t : kQTiles) {
+            if (forced && strcmp(t.name, forced)) continue;
+            // (the largest tile has no registers for rows that end inside a chunk, nor an fp32 instance)
+            if (t.bm * t.bn == 256 * 256 && (es == 4 || columns % 8)) continue;
+            const float us = ring_us(t, (double)m, n, k, cus);
+            if (!tile || us < best) {
+                tile = &t;
+                best = us;
+            }
+        }
+        if (!tile) fail(SOX_E_INVALID, std::string("SIMDONNX_HIP_QGEMM: no tiling ") + forced + " for this product");
+        if (forced) return;
+        if (m <= 64 && few_us((double)m, n, k) < best) {
+            way = FEW;
+            best = few_us((double)m, n, k);
+        }
+        if (floating && inner <= 1024 && panel_us((double)m, n, k, es, cus) < rows_us((double)m, k, es) + best) way = PANEL;
+    }
+    bool rounds_itself() const { return way == FEWX || way == PANEL; }
+    // workspace: rows [m][pitch], then their scales
+    static int pitch(int inner) { return round_up(inner, 64); }
+    static uint64_t rows_bytes(int inner, int64_t m) { return (uint64_t)m * pitch(inner); }
+    static uint64_t bytes(int inner, int64_t m) { return rows_bytes(inner, m) + (uint64_t)round_up((int)m, 4) * 4; }
+};
+
+// A launch of the 8-bit layers: the kernel by its place among its kind's instances, and the grid.
+struct QLaunch {
+    enum Kind { ROWS = QPlan::RING + 1, KINDS };
+    int kind = 0, index = 0;  // kind: QPlan::Way, or ROWS
+    uint32_t gx = 1, gy = 1, threads = 256, lds = 0;
+    int tiles_n = 0;
+
+    static int instances(int kind) {
+        static const int n[KINDS] = {3, 4, 3, kQTileCount, 3};
+        return n[kind];
+    }
+    // "" for an instance that the storage type does not have
+    static std::string kernel(int kind, int index, int32_t storage) {
+        const std::string st = kStorageName[storage];
+        switch (kind) {
+        case QPlan::FEWX: return "sox_qfewx_" + st + "_s" + std::to_string(1 << index);    // steps of a wave
+        case QPlan::PANEL: return "sox_qpanel_" + st + "_c" + std::to_string(index + 1);   // K / 256
+        case QPlan::FEW: return "sox_qfew_" + st + "_r" + std::to_string(1 << index);      // rows / 16
+        case ROWS: return "sox_qrows_" + st + "_t" + std::to_string(kRowThreads[index]);
+        default:
+            if (storage == SOX_STORAGE_F32 && kQTiles[index].bm * kQTiles[index].bn == 256 * 256) return "";
+            return "sox_qgemm_" + st + "_" + kQTiles[index].name;
+        }
+    }
+    // rows of `inner` elements of es bytes to 8 bits
+    static QLaunch rows(int inner, int64_t m, int es) {
+        const int64_t bytes = (int64_t)inner * es;
+        QLaunch l;
+        l.kind = ROWS;
+        l.index = bytes <= 32 * 64 ? 0 : bytes <= 64 * 64 ? 1 : 2;
+        const int per_block = 256 / kRowThreads[l.index];
+        l.gx = (uint32_t)((m + per_block - 1) / per_block);
+        return l;
+    }
+    static QLaunch product(const QPlan& plan, int inner, int columns, int64_t m, int compute_units) {
+        QLaunch l;
+        l.kind = plan.way;
+        const int steps = (inner + 63) / 64;
+        l.gx = (uint32_t)((columns + 15) / 16);
+        switch (plan.way) {
+        case QPlan::FEWX: {
+            const int segs = (inner + 1023) / 1024, waves = (int)std::min<int64_t>(16, std::max<int64_t>(steps, m * segs));
+            l.index = steps <= waves ? 0 : steps <= 2 * waves ? 1 : 2;
+            l.threads = (uint32_t)waves * 64;
+            l.lds = (uint32_t)(m * (round_up(inner, 256) + 16));
+            break;
+        }
+        case QPlan::PANEL:
+            l.index = (inner - 1) / 256;
+            l.gx = (uint32_t)((columns + 127) / 128);
+            l.gy = (uint32_t)((m + 31) / 32);
+            l.threads = 512;
+            l.lds = (uint32_t)((inner + 31) / 32) * 1024;
+            break;
+        case QPlan::FEW:
+            l.index = m <= 16 ? 0 : m <= 32 ? 1 : 2;
+            l.threads = (uint32_t)std::min(8, (steps + (8 >> l.index) - 1) / (8 >> l.index)) * 64;
+            break;
+        case QPlan::RING: {
+            const QTile& t = *plan.tile;
+            l.index = (int)(&t - kQTiles);
+            l.tiles_n = (columns + t.bn - 1) / t.bn;
+            const int64_t tiles = ((m + t.bm - 1) / t.bm) * l.tiles_n;
+            if (tiles >= (int64_t)1 << 24) unsupported("8-bit product: too many outputs");
+            l.gx = (uint32_t)std::min<int64_t>(tiles, (int64_t)std::max(1, compute_units) * t.wgs_per_cu);
+            l.threads = (uint32_t)t.threads;
+            break;
+        }
+        }
+        return l;
+    }
+};
+
+// 8-bit weights as the kernels read them: packed blocks (sox_qgemm_args), then the scales and the bias (zeros without one).
+struct Packed8 {
+    int kb = 0, nb = 0, npad = 0;
+    uint64_t scales_at = 0, bias_at = 0;
+    std::vector<uint8_t> bytes;
+
+    static void check_sizes(int inner, int columns) {
+        if (inner <= 0 || columns <= 0) fail(SOX_E_INVALID, "QuantLinear: arguments");
+        if (inner > 131071) unsupported("QuantLinear: 32-bit sums over more than 131071 products");
+        if (columns > 1 << 24) unsupported("QuantLinear: more than 2^24 columns");
+    }
+    static int padded(int columns) { return round_up(columns, 256) + 256; }  // (a last tile of 192 columns may start inside the last 256)
+    Packed8(int inner, int columns) {
+        kb = round_up(inner, 128) / 32;
+        nb = (columns + 31) / 32;
+        npad = padded(columns);
+        scales_at = (uint64_t)nb * kb * 1024;
+        bias_at = scales_at + (uint64_t)npad * 4;
+    }
+    uint64_t size() const { return bias_at + (uint64_t)npad * 4; }
+    Packed8(int inner, int columns, const int8_t* w, const float* scales, const float* bias) : Packed8(inner, columns) {
+        bytes.assign(size(), 0);
+        for (int c = 0; c < columns; c++)
+            if (!std::isfinite(scales[c])) fail(SOX_E_INVALID, "QuantLinear: scales have to be finite");
+        for (int k = 0; k < inner; k++) {
+            const int8_t* src = w + (size_t)k * columns;
+            const size_t at = (size_t)(k / 32) * 1024 + (size_t)(k % 32 / 16) * 512 + k % 16;
+            for (int cb = 0; cb < nb; cb++) {
+                uint8_t* d = bytes.data() + (size_t)cb * kb * 1024 + at;
+                const int cols = std::min(32, columns - cb * 32);
+                for (int c = 0; c < cols; c++) d[c * 16] = (uint8_t)src[cb * 32 + c];
+            }
+        }
+        memcpy(bytes.data() + scales_at, scales, (size_t)columns * 4);
+        if (bias) memcpy(bytes.data() + bias_at, bias, (size_t)columns * 4);
+    }
+};
+// Floating weights [inner][columns] to 8 bits by column
+void quantize_columns(const float* weights, int inner, int columns, std::vector<int8_t>& w, std::vector<float>& scales) {
+    std::vector<float> amax((size_t)columns, 0.0f);
+    for (int k = 0; k < inner; k++)
+        for (int c = 0; c < columns; c++) {
+            const float v = fabsf(weights[(size_t)k * columns + c]);
+            if (!std::isfinite(v)) fail(SOX_E_INVALID, "QuantLinear: weights have to be finite");
+            amax[c] = std::max(amax[c], v);
+        }
+    scales.resize(columns);
+    for (int c = 0; c < columns; c++) scales[c] = amax[c] / 127.0f;
+    w.resize((size_t)inner * columns);
+    for (int k = 0; k < inner; k++)
+        for (int c = 0; c < columns; c++) {
+            const size_t i = (size_t)k * columns + c;
+            w[i] = amax[c] > 0.0f ? (int8_t)std::nearbyint(127.0 * weights[i] / amax[c]) : (int8_t)0;
+        }
+}
+
+// block_norm.hip's instances: threads of a row, chunks of 8 columns of a thread, workgroups per CU at most; `many`: for many
+// rows, with the parameters in LDS.
+struct BnormShape {
+    int tpr, ch, per_cu;
+    bool many;
+};
+const BnormShape kBnormShapes[] = {{32, 1, 4, true},   {64, 1, 4, true},   {64, 2, 4, true},  {256, 1, 4, false},
+                                   {256, 2, 2, false}, {512, 2, 2, false}, {512, 4, 1, false}};
+
+// The first instance that holds c columns; those for many rows only where there are many.
+int bnorm_shape(int c, bool many) {
+    for (int i = 0; i < (int)(sizeof kBnormShapes / sizeof *kBnormShapes); i++)
+        if (kBnormShapes[i].tpr * kBnormShapes[i].ch * 8 >= c && (many || !kBnormShapes[i].many)) return i;
+    unsupported("BlockNorm: channels");
+}
+bool bnorm_many(int64_t rows, int compute_units) { return rows >= 4 * (int64_t)std::max(1, compute_units); }  // a wave on every SIMD
+std::string bnorm_kernel(int32_t storage, int shape, bool vec) {
+    const BnormShape& s = kBnormShapes[shape];  // (a 16-byte chunk of fp32 is half as many columns)
+    return std::string("sox_bnorm_") + kStorageName[storage] + "_t" + std::to_string(s.tpr) + "c" +
+           std::to_string(s.ch * (storage == SOX_STORAGE_F32 ? 2 : 1)) + (vec ? "v" : "s");
+}
+
+struct BnormLaunch {
+    int shape;
+    uint32_t blocks, threads, lds;
+    BnormLaunch(int c, int64_t rows, int vectors, int compute_units) {
+        const int64_t cus = std::max(1, compute_units);
+        shape = bnorm_shape(c, bnorm_many(rows, compute_units));
+        const BnormShape& s = kBnormShapes[shape];
+        threads = (uint32_t)std::max(s.tpr, 256);
+        const int per_block = (int)threads / s.tpr;
+        blocks = (uint32_t)std::min<int64_t>((rows + per_block - 1) / per_block, cus * s.per_cu);
+        lds = s.many ? (uint32_t)(vectors * s.tpr * s.ch * 8 * 4) : 0;
+    }
+};
+// The parameter vectors as the kernel reads them, [cpad] each: post gamma * scale, post beta * scale, pre gamma, pre beta.
+struct BnormVectors {
+    int cpad = 0, count = 0;
+    bool has[4] = {};  // the others are all ones or all zeros
+    std::vector<float> v;
+    BnormVectors(const sox_block_norm_p& p, const float* post_gamma, const float* post_beta, const float* scale, const float* pre_gamma,
+                 const float* pre_beta) {
+        if (p.channels <= 0) fail(SOX_E_INVALID, "BlockNorm: arguments");
+        if (p.channels > 16384) unsupported("BlockNorm: more than 16384 channels");
+        for (int32_t kind : {p.post, p.pre})
+            if (kind < SOX_NORM_NONE || kind > SOX_NORM_LAYER) fail(SOX_E_INVALID, "BlockNorm: norm kind");
+        if (p.gate_act < SOX_ACT_NONE || p.gate_act > SOX_ACT_SWISH) unsupported("BlockNorm: gate activation");
+        if (!(p.post_eps >= 0.0f) || !(p.pre_eps >= 0.0f) || !std::isfinite(p.res_scale)) fail(SOX_E_INVALID, "BlockNorm: eps / residual scale");
+        const size_t C = (size_t)p.channels, CP = (size_t)round_up(p.channels, 8);
+        cpad = (int)CP;
+        const bool post = p.post != SOX_NORM_NONE, pre = p.pre != SOX_NORM_NONE;
+        const bool pb = p.post == SOX_NORM_LAYER && post_beta, b = p.pre == SOX_NORM_LAYER && pre_beta;
+        v.assign(4 * CP, 0.0f);
+        for (size_t i = 0; i < C; i++) {
+            const float s = scale ? scale[i] : 1.0f;
+            v[i] = (post && post_gamma ? post_gamma[i] : 1.0f) * s;
+            v[CP + i] = pb ? post_beta[i] * s : 0.0f;
+            v[2 * CP + i] = pre && pre_gamma ? pre_gamma[i] : 1.0f;
+            v[3 * CP + i] = b ? pre_beta[i] : 0.0f;
+        }
+        const bool there[4] = {scale || (post && post_gamma), pb, pre && pre_gamma, b};
+        for (int i = 0; i < 4; i++) {
+            has[i] = there[i];
+            count += there[i];
+        }
+    }
+};
+
+}  // namespace
+
+// ================================================================================================
 // Graph model
 // ================================================================================================
 struct Patch {
@@ -331,6 +618,9 @@ struct sox_graph {
     // first ConvT (2x2 s2, run as a Gemm) -> the one-channel 2x2 s2 ConvT that alone reads its output:
     // both run as one kernel at the first one's place (plan_convt_chain)
     std::map<int, int> convt_chain;
+    std::map<int, int> bnorm_vectors;  // BlockNorm node -> const value of its BnormVectors
+    // values only QuantLinears read, as x: their buffer holds 8-bit rows [rows][channels], then the rows' scales
+    std::set<int> q8rows;
     uint64_t scratch_off = 0, scratch_bytes = 0, tail_bytes = 0;
     int refs = 1;
 
@@ -372,9 +662,10 @@ enum { CK_FRAG32 = 10 };
 // conv weights over channels padded with zeros to a multiple of 8 or 4 (16-byte chunks of 16-bit or fp32):
 // [OC][tap * ICp + ic], ICp = ceil(IC / pad) pad
 enum { CK_CONVWT_P8 = 11, CK_CONVWT_P4 = 12 };
+enum { CK_Q8 = 13 };        // weights [K][N] brought to 8 bits by column: Packed8 (its bias zeros)
+enum { CK_Q8_BIAS = 14 };   // fp32 [Packed8::padded(N)]
 
 int pad8(int k) { return (k + 7) & ~7; }
-int round_up(int k, int to) { return (k + to - 1) / to * to; }
 
 // Element count of a const in a packing (Extensions.cs:144-159; K rows padded to 8 for 16-byte loads).
 int64_t packed_elems(const PlanValue& v, int kind) {
@@ -387,6 +678,8 @@ int64_t packed_elems(const PlanValue& v, int kind) {
         case CK_GEMMNK_T: return (int64_t)s[0] * pad8(s[1]);
         case CK_CONVT_NK: return (int64_t)s[1] * s[2] * s[3] * pad8(s[0]);
         case CK_FRAG32: return (int64_t)s[0] * s[1];
+        case CK_Q8: return (int64_t)Packed8(s[0], s[1]).size();  // (bytes)
+        case CK_Q8_BIAS: return Packed8::padded((int)v.count());
         // plain consts: padded with zeros to a multiple of 4 floats, so a float4 read of a bias
         // group that straddles the end stays inside the const
         default: return std::max<int64_t>((v.count() + 3) & ~3ll, 4);
@@ -461,6 +754,90 @@ void pack_const(const PlanValue& v, int kind, float* d) {
         }
         default: memcpy(d, src, sizeof(float) * v.floats.size());
     }
+}
+
+// The nodes of the 8-bit layers: their values by role (-1: not there), checked.
+bool rows_value(const sox_graph& g, int v, int64_t count, int cols) {  // `count` elements in rows of cols, stored in that order
+    const PlanValue& pv = g.V(v);
+    return v >= 0 && !pv.shape.empty() && pv.phys() == pv.shape && pv.shape.back() == cols && pv.count() == count;
+}
+struct QuantLinearNode {
+    sox_quant_linear_p p;
+    int x, w, bias = -1, residual = -1, y, inner, columns;
+    int64_t rows;
+    QuantLinearNode(const sox_graph& g, const PlanNode& n) : p(n.p<sox_quant_linear_p>()) {
+        auto bad = [](const char* why) { fail(SOX_E_INVALID, std::string("QuantLinear: ") + why); };
+        size_t at = 2;
+        if (n.in.size() != at + !!p.has_bias + !!p.has_residual || n.out.size() != 1) bad("operands");
+        x = n.in[0];
+        w = n.in[1];
+        if (p.has_bias) bias = n.in[at++];
+        if (p.has_residual) residual = n.in[at++];
+        y = n.out[0];
+        const PlanValue& wv = g.V(w);
+        if (!wv.is_const || wv.shape.size() != 2 || (int64_t)wv.floats.size() != wv.count()) bad("weights are not a const [inner, columns]");
+        inner = wv.shape[0];
+        columns = wv.shape[1];
+        Packed8::check_sizes(inner, columns);
+        rows = g.V(x).count() / inner;
+        if (rows <= 0 || !rows_value(g, x, rows * inner, inner)) bad("x is not rows of the weights' inner size");
+        if (g.V(y).buf < 0 || !rows_value(g, y, rows * columns, columns)) bad("y is not rows of the weights' columns");
+        if (residual >= 0 && !rows_value(g, residual, rows * columns, columns)) bad("the residual is not shaped as y");
+        if (bias >= 0 && (!g.V(bias).is_const || g.V(bias).count() != columns || (int64_t)g.V(bias).floats.size() != columns)) bad("bias is not a const [columns]");
+        if (p.act < SOX_ACT_NONE || p.act > SOX_ACT_SWISH) unsupported("QuantLinear: activation");
+        if (rows > 1 << 23) unsupported("QuantLinear: more than 2^23 rows");
+    }
+};
+struct BlockNormNode {
+    sox_block_norm_node_p p;
+    int residual = -1, x = -1, gate = -1, vec[5] = {-1, -1, -1, -1, -1}, h = -1, y = -1;  // vec: post gamma, post beta, scale, pre gamma, pre beta
+    int channels, gate_rows = 0;
+    int64_t rows;
+    BlockNormNode(const sox_graph& g, const PlanNode& n) : p(n.p<sox_block_norm_node_p>()) {
+        auto bad = [](const char* why) { fail(SOX_E_INVALID, std::string("BlockNorm: ") + why); };
+        size_t in = 0, out = 0;
+        int* const ins[] = {&residual, &x, &gate, vec, vec + 1, vec + 2, vec + 3, vec + 4};
+        for (int i = 0; i < 8; i++)
+            if (p.operands >> i & 1) {
+                if (in == n.in.size()) bad("operands");
+                *ins[i] = n.in[in++];
+            }
+        int* const outs[] = {&h, &y};
+        for (int i = 0; i < 2; i++)
+            if (p.operands >> (8 + i) & 1) {
+                if (out == n.out.size()) bad("operands");
+                *outs[i] = n.out[out++];
+            }
+        if (in != n.in.size() || out != n.out.size() || p.operands >> 10) bad("operands");
+        if (residual < 0 && x < 0) bad("neither a residual nor a branch");
+        if (gate >= 0 && x < 0) bad("a gate without a branch");
+        if (h < 0 && y < 0) bad("neither h nor y");
+        channels = p.norm.channels;
+        if (channels <= 0) bad("channels");
+        const int64_t count = g.V(x >= 0 ? x : residual).count();
+        rows = count / channels;
+        if (rows <= 0) bad("rows");
+        if (rows > 1 << 23) unsupported("BlockNorm: more than 2^23 rows");
+        for (int v : {residual, x, h, y})
+            if (v >= 0 && !rows_value(g, v, count, channels)) bad("values are not rows of the channels");
+        for (int v : {h, y})
+            if (v >= 0 && g.V(v).buf < 0) bad("an output is a const");
+        if (gate >= 0) {
+            gate_rows = (int)std::min<int64_t>(g.V(gate).count() / channels, rows + 1);
+            if (gate_rows <= 0 || !rows_value(g, gate, (int64_t)gate_rows * channels, channels) || rows % gate_rows)
+                bad("gate rows have to divide the rows");
+        }
+        for (int v : vec)
+            if (v >= 0 && (!g.V(v).is_const || g.V(v).count() != channels || (int64_t)g.V(v).floats.size() != channels)) bad("a vector is not a const [channels]");
+    }
+    BnormVectors vectors(const sox_graph& g) const {
+        auto at = [&](int i) { return vec[i] < 0 ? nullptr : g.V(vec[i]).floats.data(); };
+        return BnormVectors(p.norm, at(0), at(1), at(2), at(3), at(4));
+    }
+};
+bool builtin_node(const sox_graph& g, int ni, const char* name) {
+    const PlanNode& n = g.plan.nodes[ni];
+    return n.op == SOX_OP_EXT && n.ext == name && !g.folded.count(ni) && !g.be->exts.count(n.ext);
 }
 
 // fp16 ConvTranspose (stride == kernel) with ic % 8 == 0 runs as a GEMM over the input pixels on the
@@ -2163,8 +2540,116 @@ struct Emitter {
             (uint32_t)((nn + 63) / 64), (uint32_t)((m + 63) / 64), (uint32_t)batch, 256, 0, "matmul");
     }
 
+    // ---- 8-bit transformer layers ----
+    int32_t storage() const { return g.bf16 ? SOX_STORAGE_BF16 : g.f16 ? SOX_STORAGE_F16 : SOX_STORAGE_F32; }
+    // rows of `width` elements, one behind the other, all on boundaries of `to` bytes (-1: not there)
+    bool rows_on(int v, int width, int to = 16) { return v < 0 || (bind(v).offset % (uint64_t)to == 0 && width * g.es % to == 0); }
+    static sox_bind part(sox_bind b, uint64_t at, uint64_t size) { return sox_bind{b.slot, 0, b.offset + at, size}; }
+
+    void quant_linear(int ni, const PlanNode& n) {
+        const QuantLinearNode q(g, n);
+        const bool rounded = g.q8rows.count(q.x) > 0;
+        const int cus = g.be->info.compute_units, es = g.es;
+        const QPlan plan(q.inner, q.columns, cus, q.rows, storage(), !rounded);
+        const Packed8 w(q.inner, q.columns);
+        const sox_bind wb = bind(q.w, CK_Q8);
+        sox_qgemm_args a{};
+        std::vector<std::pair<size_t, sox_bind>> ptrs = {
+            {offsetof(sox_qgemm_args, w), part(wb, 0, w.scales_at)},
+            {offsetof(sox_qgemm_args, ws), part(wb, w.scales_at, (uint64_t)w.npad * 4)},
+            {offsetof(sox_qgemm_args, bias), q.bias >= 0 ? bind(q.bias, CK_Q8_BIAS) : part(wb, w.bias_at, (uint64_t)w.npad * 4)},
+            {offsetof(sox_qgemm_args, zeros), none()},
+            {offsetof(sox_qgemm_args, y), bind(q.y)}};
+        if (q.residual >= 0) ptrs.push_back({offsetof(sox_qgemm_args, add), bind(q.residual)});
+        const uint64_t scales = (uint64_t)q.rows * 4;
+        if (rounded) {
+            const uint64_t bytes = (uint64_t)q.rows * q.inner;
+            a.lda = q.inner;
+            ptrs.push_back({offsetof(sox_qgemm_args, a), part(bind(q.x), 0, bytes)});
+            ptrs.push_back({offsetof(sox_qgemm_args, xs), part(bind(q.x), bytes, scales)});
+        } else if (plan.rounds_itself()) {
+            ptrs.push_back({offsetof(sox_qgemm_args, x), bind(q.x)});
+        } else {
+            const sox_bind ws = scratch(QPlan::bytes(q.inner, q.rows));
+            const uint64_t bytes = QPlan::rows_bytes(q.inner, q.rows);
+            sox_qrows_args r{};
+            r.ldx = q.inner;
+            r.ldq = QPlan::pitch(q.inner);
+            r.rows = (int32_t)q.rows;
+            r.k = q.inner;
+            r.vec = rows_on(q.x, q.inner);
+            const QLaunch l = QLaunch::rows(q.inner, q.rows, es);
+            add(ni, QLaunch::kernel(l.kind, l.index, storage()), r,
+                {{offsetof(sox_qrows_args, x), bind(q.x)}, {offsetof(sox_qrows_args, q), part(ws, 0, bytes)},
+                 {offsetof(sox_qrows_args, scale), part(ws, bytes, scales)}},
+                l.gx, l.gy, 1, l.threads, l.lds, "quant_rows");
+            a.lda = r.ldq;
+            ptrs.push_back({offsetof(sox_qgemm_args, a), part(ws, 0, bytes)});
+            ptrs.push_back({offsetof(sox_qgemm_args, xs), part(ws, bytes, scales)});
+        }
+        const QLaunch l = QLaunch::product(plan, q.inner, q.columns, q.rows, cus);
+        a.ldx = q.inner;
+        a.ldr = a.ldy = q.columns;
+        a.act = q.p.act;
+        a.vec = (rows_on(q.y, q.columns) && rows_on(q.residual, q.columns) ? 1 : 0) | (rows_on(q.x, q.inner) ? 2 : 0) |
+                (rows_on(q.y, q.columns, 128) ? 4 : 0);
+        a.m = (int32_t)q.rows;
+        a.n = q.columns;
+        a.k = q.inner;
+        a.k16 = round_up(q.inner, 16);
+        a.kb = w.kb;
+        a.nb = w.nb;
+        a.tiles_n = l.tiles_n;
+        add(ni, QLaunch::kernel(l.kind, l.index, storage()), a, ptrs, l.gx, l.gy, 1, l.threads, l.lds, "quant_linear");
+    }
+
+    void block_norm(int ni, const PlanNode& n) {
+        const BlockNormNode b(g, n);
+        const BnormVectors vectors = b.vectors(g);
+        const sox_bind vb = bind(g.bnorm_vectors.at(ni), SOX_CK_F32);
+        const bool rounded = g.q8rows.count(b.y) > 0;
+        const int C = b.channels;
+        sox_bnorm_args a{};
+        std::vector<std::pair<size_t, sox_bind>> ptrs;
+        const size_t fields[4] = {offsetof(sox_bnorm_args, pg), offsetof(sox_bnorm_args, pb), offsetof(sox_bnorm_args, g), offsetof(sox_bnorm_args, b)};
+        for (int i = 0; i < 4; i++)
+            if (vectors.has[i]) ptrs.push_back({fields[i], part(vb, (uint64_t)i * vectors.cpad * 4, (uint64_t)vectors.cpad * 4)});
+        const std::pair<size_t, int> values[4] = {{offsetof(sox_bnorm_args, residual), b.residual}, {offsetof(sox_bnorm_args, x), b.x},
+                                                  {offsetof(sox_bnorm_args, gate), b.gate}, {offsetof(sox_bnorm_args, h), b.h}};
+        for (auto& v : values)
+            if (v.second >= 0) ptrs.push_back({v.first, bind(v.second)});
+        if (rounded) {
+            const uint64_t bytes = (uint64_t)b.rows * C;
+            ptrs.push_back({offsetof(sox_bnorm_args, q), part(bind(b.y), 0, bytes)});
+            ptrs.push_back({offsetof(sox_bnorm_args, qs), part(bind(b.y), bytes, (uint64_t)b.rows * 4)});
+        } else if (b.y >= 0) {
+            ptrs.push_back({offsetof(sox_bnorm_args, y), bind(b.y)});
+        }
+        a.ldx = a.ldr = a.ldg = a.ldh = a.ldy = a.ldq = C;
+        a.rows = (int32_t)b.rows;
+        a.c = C;
+        a.gate_group = b.gate >= 0 ? (int32_t)(b.rows / b.gate_rows) : 1;
+        a.post = b.p.norm.post;
+        a.pre = b.p.norm.pre;
+        a.gate_act = b.p.norm.gate_act;
+        a.post_eps = b.p.norm.post_eps;
+        a.pre_eps = b.p.norm.pre_eps;
+        a.res_scale = b.p.norm.res_scale;
+        const bool vec = rows_on(b.residual, C) && rows_on(b.x, C) && rows_on(b.gate, C) && rows_on(b.h, C) && rows_on(b.y, C);
+        const BnormLaunch l(C, b.rows, vectors.count, g.be->info.compute_units);
+        add(ni, bnorm_kernel(storage(), l.shape, vec), a, ptrs, l.blocks, 1, 1, l.threads, l.lds, "block_norm");
+    }
+
     // ---- built-in extension ops (Engine/Fusions/*.cs EmitVulkan twins) ----
     bool builtin_ext(int ni, const PlanNode& n) {
+        if (n.ext == "QuantLinear") {
+            quant_linear(ni, n);
+            return true;
+        }
+        if (n.ext == "BlockNorm") {
+            block_norm(ni, n);
+            return true;
+        }
         if (n.ext == "SafeDiv") {  // SafeDivOp.cs:26-33
             const auto& p = n.p<sox_safediv_p>();
             const int64_t cnt = g.V(n.out[0]).count();
@@ -3107,6 +3592,50 @@ bool conv_pads_channels(const sox_graph& g, const PlanNode& n) {
     return pads_rows(g, (int64_t)xs[0] * a.ih * a.iw, ic, oc, taps);
 }
 
+// The nodes of the 8-bit layers. A BlockNorm's parameters become one const. An output that the plan put over an operand gets
+// a buffer of its own (workgroups write it while others still read). A BlockNorm whose y only QuantLinears read hands
+// them 8-bit rows, rounded once and from fp32, in y's own buffer: channels bytes a row and 4 for its scale fit where
+// 2 * channels were (8192 rows of 1024: the rounding launch of each product, 8 us, falls away).
+void plan_layers8(sox_graph& g) {
+    auto& P = g.plan;
+    auto apart = [&](int out, std::initializer_list<int> others) {
+        for (int v : others) {
+            if (out < 0 || v < 0 || P.values[v].buf < 0 || P.values[v].buf == P.values[out].buf) continue;
+            const auto a = value_range(P, out), b = value_range(P, v);
+            if (a.first < b.second && b.first < a.second) relocate_value(P, out);
+        }
+        for (int v : others)
+            if (out >= 0 && v >= 0 && P.values[v].buf >= 0 && P.values[v].buf == P.values[out].buf) fail(SOX_E_INVALID, "QuantLinear / BlockNorm: an output in an operand's buffer");
+    };
+    for (int ni = 0; ni < (int)P.nodes.size(); ni++) {
+        if (builtin_node(g, ni, "QuantLinear")) {
+            const QuantLinearNode q(g, P.nodes[ni]);
+            apart(q.y, {q.x, q.residual});
+        }
+        if (!builtin_node(g, ni, "BlockNorm")) continue;
+        const BlockNormNode b(g, P.nodes[ni]);
+        apart(b.h, {b.residual, b.x, b.gate, b.y});
+        apart(b.y, {b.residual, b.x, b.gate, b.h});
+        const BnormVectors vectors = b.vectors(g);
+        PlanValue v;
+        v.name = "BlockNorm vectors";
+        v.is_const = true;
+        v.shape = {4, vectors.cpad};
+        v.floats = vectors.v;
+        P.values.push_back(std::move(v));
+        g.bnorm_vectors[ni] = (int)P.values.size() - 1;
+        if (b.y < 0 || b.channels % 16 || getenv("SIMDONNX_HIP_NO_QUANT_NORM")) continue;
+        int shared = 0, reads = 0;
+        for (const PlanValue& o : P.values) shared += o.buf == P.values[b.y].buf;
+        for (int k = 0; k < (int)P.nodes.size(); k++)
+            if (builtin_node(g, k, "QuantLinear")) {
+                const QuantLinearNode q(g, P.nodes[k]);
+                reads += q.x == b.y && q.residual != b.y;
+            }
+        if (shared == 1 && reads > 0 && buffer_reads(g, b.y, -1) == reads) g.q8rows.insert(b.y);
+    }
+}
+
 // Const kinds each node's dispatches bind (the per-consumer packing, VkGraph.cs:81-143).
 void collect_consts(sox_graph& g, std::vector<std::pair<int, int>>& need) {
     auto want = [&](int v, int k) {
@@ -3191,6 +3720,16 @@ void collect_consts(sox_graph& g, std::vector<std::pair<int, int>>& need) {
                             want(p.skip_w, SOX_CK_RAW);
                             want(p.skip_b, SOX_CK_F32);
                         }
+                    } else if (n.ext == "QuantLinear") {
+                        const QuantLinearNode q(g, n);
+                        want(q.x, SOX_CK_RAW);
+                        want(q.w, CK_Q8);
+                        want(q.bias, CK_Q8_BIAS);
+                        want(q.residual, SOX_CK_RAW);
+                    } else if (n.ext == "BlockNorm") {
+                        const BlockNormNode b(g, n);
+                        for (int v : {b.residual, b.x, b.gate}) want(v, SOX_CK_RAW);
+                        want(g.bnorm_vectors.at(ni), SOX_CK_F32);
                     } else {
                         for (int v : n.in) want(v, SOX_CK_RAW);
                     }
@@ -3219,7 +3758,7 @@ void upload_consts(sox_graph& g) {
         int64_t n = packed_elems(v, need[i].second);
         total = (total + 63) & ~63ull;
         offs[i] = total;
-        bytes[i] = (uint64_t)n * (g.elem_fp32(need[i].second) ? 4 : 2);
+        bytes[i] = (uint64_t)n * (need[i].second == CK_Q8 ? 1 : g.elem_fp32(need[i].second) || need[i].second == CK_Q8_BIAS ? 4 : 2);
         total += bytes[i];
         g.const_off[need[i]] = {offs[i], bytes[i]};
     }
@@ -3229,9 +3768,17 @@ void upload_consts(sox_graph& g) {
     for (size_t i = 0; i < need.size(); i++) {
         const PlanValue& v = g.V(need[i].first);
         int64_t n = packed_elems(v, need[i].second);
+        if (need[i].second == CK_Q8) {
+            std::vector<int8_t> w;
+            std::vector<float> scales;
+            quantize_columns(v.floats.data(), v.shape[0], v.shape[1], w, scales);
+            const Packed8 packed(v.shape[0], v.shape[1], w.data(), scales.data(), nullptr);
+            memcpy(host.data() + offs[i], packed.bytes.data(), packed.bytes.size());
+            continue;
+        }
         tmp.assign((size_t)n, 0.0f);
         pack_const(v, need[i].second, tmp.data());
-        if (g.elem_fp32(need[i].second)) {
+        if (g.elem_fp32(need[i].second) || need[i].second == CK_Q8_BIAS) {
             memcpy(host.data() + offs[i], tmp.data(), (size_t)n * 4);
         } else {
             uint16_t* d = reinterpret_cast<uint16_t*>(host.data() + offs[i]);
@@ -3713,6 +4260,7 @@ int sox_graph_create(sox_backend* backend, const sox_plan* plan, int32_t f16, so
         plan_upsample_concat(*g);
         plan_upsample_add(*g);
         plan_se_fold_space(*g);
+        plan_layers8(*g);
         // activations occupy [0, arena_floats*es); scratch follows, 256-byte aligned (VkGraph.cs:145)
         g->scratch_off = ((uint64_t)g->plan.arena_floats * g->es + 255) & ~255ull;
         for (const PlanValue& v : g->plan.values)
@@ -4699,8 +5247,6 @@ int sox_unit_runner_wait(sox_unit_runner* r, int32_t wave) {
 // ---- 8-bit transformer layers (kernels in qgemm.hip, qlinear.hip, block_norm.hip) ----
 namespace {
 
-const char* const kStorageName[] = {"f32", "f16", "bf16"};  // by SOX_STORAGE_*
-
 // Rows of a caller's device matrix: `rows` rows of `width` bytes, `pitch` bytes apart.
 struct Rows {
     const char* what;
@@ -4807,188 +5353,52 @@ struct DeviceBlock {
 
 struct sox_qlinear {
     sox_backend* be = nullptr;
-    int inner = 0, columns = 0, k16 = 0, kb = 0, nb = 0, npad = 0;
-    DeviceBlock mem;  // packed weights, then the scales and the bias (zeros without one), padded to npad columns
+    int inner = 0, columns = 0, kb = 0, nb = 0, npad = 0;
+    DeviceBlock mem;  // Packed8
     uint64_t scales_at = 0;
-    // by storage: rows to 8 bits (32, 64, 256 threads a row), few 8-bit rows (16, 32, 64), few floating rows (1, 2, 4 steps a wave), panels
-    // (256 .. 1024 of K), ring tilings
-    void *fn_rows[3][3], *fn_few[3][3], *fn_fewx[3][3], *fn_panel[3][4], *fn_ring[3][8];
+    std::vector<void*> fns[QLaunch::KINDS][3];  // by storage
 
-    const int8_t* w() const { return (const int8_t*)mem.p; }
-    const float* ws() const { return (const float*)((const uint8_t*)mem.p + scales_at); }
-    const float* bias() const { return ws() + npad; }
-    int pitch() const { return round_up(inner, 64); }
+    void* fn(const QLaunch& l, int32_t storage) const { return fns[l.kind][storage][l.index]; }
+    QPlan plan(int64_t m, int32_t storage, bool floating) const { return QPlan(inner, columns, be->info.compute_units, m, storage, floating); }
 };
 
 namespace {
 
-// The tilings of the 8-bit ring (qgemm.hip), with the terms of their estimated time in us (QPlan::ring_us).
-struct QTile {
-    const char* name;
-    int bm, bn, wgs_per_cu, threads;
-    float lat, thr, base, tile, out;
-};
-const QTile kQTiles[] = {
-    {"256x256_w8k128s2", 256, 256, 1, 512, 0.35f, 1.15f, 3.3f, 3.8f, 0.51f},
-    {"256x192_w8k128s2", 256, 192, 1, 512, 0.43f, 0.99f, 2.7f, 3.9f, 0.43f},
-    {"256x128_w8k128s2", 256, 128, 1, 512, 0.84f, 0.85f, 4.0f, 1.2f, 0.43f},
-    {"128x128_w4k128s2", 128, 128, 2, 256, 0.59f, 0.465f, 4.45f, 0.4f, 0.44f},
-    {"64x64_w4k128s4", 64, 64, 2, 256, 0.31f, 0.22f, 3.5f, 0.2f, 0.57f},
-};
-const int kRowThreads[] = {32, 64, 256};  // of a row brought to 8 bits, each with four 16-byte chunks in registers
-constexpr int kQTileCount = (int)(sizeof kQTiles / sizeof *kQTiles);
-
-// How a product of m rows runs. Every way gives the same bits (whole numbers), so the choice is by time alone, each
-// estimate a fit to measurements on one MI355X:
-//   FEWX   up to 16 floating rows of up to 4096 values, one launch           1 x 768 -> 768: 3.9 us
-//   PANEL  floating rows of up to 1024 values, one launch that rounds them   786 x 768 -> 760: 7.3 us; rounded by a launch
-//          once per 128 columns                                              of its own 9.4. 8192 x 768 -> 2304: 51, 35
-//   FEW    up to 64 8-bit rows, weights straight to registers                64 x 4096 -> 4096: 10.8 us, ring 13.5;
-//                                                                            64 x 1024 -> 8192: 6.9, ring 6.0
-//   RING   8-bit rows on the ring of the tiling with the smallest estimate. Over 170 random products the pick is 1.4% above
-//          the fastest tiling on average, at most 21%
-// FEW and RING take floating rows behind a launch that brings them to 8 bits in the workspace.
-struct QPlan {
-    enum Way { FEWX, PANEL, FEW, RING } way = RING;
-    const QTile* tile = nullptr;
-
-    // A CU's tiles, each with an epilogue; K slices of 128, bound by their latency with few tiles and by the CU's matrix cores
-    // and loads with many; the outputs' stores.
-    static float ring_us(const QTile& t, double m, double n, double k, double cus) {
-        const float q = (float)ceil(ceil(m / t.bm) * ceil(n / t.bn) / cus), nk = (float)ceil(k / 128);
-        return t.base + q * t.tile + nk * std::max(t.lat, q * t.thr) + t.out * (float)(m * n * 1e-6);
-    }
-    static float few_us(double m, double n, double k) {
-        return (float)(2.6 + 0.03 * m + k * (2e-4 + 2.4e-5 * m) * std::max(1.0, n / 8192));
-    }
-    static float panel_us(double m, double n, double k, int es, double cus) {
-        return (float)(3.0 + ceil(ceil(m / 32) * ceil(n / 128) / cus) * (0.6 + 0.0027 * k * (es == 4 ? 2 : 1)));
-    }
-    // a launch (3 us, and one more of the host's time) and the rows in and out
-    static float rows_us(double m, double k, int es) { return (float)(4.0 + m * k * (es + 1) / 4.5e6); }
-
-    QPlan(const sox_qlinear& L, int64_t m, int32_t storage, bool floating) {
-        const int es = storage == SOX_STORAGE_F32 ? 4 : 2;
-        const double cus = std::max(1, L.be->info.compute_units), n = L.columns, k = L.inner;
-        if (floating && m <= 16 && L.inner <= 4096) {
-            way = FEWX;
-            return;
-        }
-        const char* forced = getenv("SIMDONNX_HIP_QGEMM");  // any tiling by name (tuning, tests)
-        float best = 0.0f;
-        for (const QTile& t : kQTiles) {
-            if (forced && strcmp(t.name, forced)) continue;
-            // (the largest tile has no registers for rows that end inside a chunk, nor an fp32 instance)
-            if (t.bm * t.bn == 256 * 256 && (es == 4 || L.columns % 8)) continue;
-            const float us = ring_us(t, (double)m, n, k, cus);
-            if (!tile || us < best) {
-                tile = &t;
-                best = us;
-            }
-        }
-        if (!tile) fail(SOX_E_INVALID, std::string("SIMDONNX_HIP_QGEMM: no tiling ") + forced + " for this product");
-        if (forced) return;
-        if (m <= 64 && few_us((double)m, n, k) < best) {
-            way = FEW;
-            best = few_us((double)m, n, k);
-        }
-        if (floating && L.inner <= 1024 && panel_us((double)m, n, k, es, cus) < rows_us((double)m, k, es) + best) way = PANEL;
-    }
-    bool rounds_itself() const { return way == FEWX || way == PANEL; }
-    // workspace: rows [m][pitch], then their scales
-    static uint64_t rows_bytes(const sox_qlinear& L, int64_t m) { return (uint64_t)m * L.pitch(); }
-    static uint64_t bytes(const sox_qlinear& L, int64_t m) { return rows_bytes(L, m) + (uint64_t)round_up((int)m, 4) * 4; }
-};
-
-void qlinear_pack(sox_qlinear& L, const int8_t* w, const float* scales, const float* bias) {
-    const size_t wbytes = (size_t)L.nb * L.kb * 1024;
-    L.scales_at = wbytes;
-    std::vector<uint8_t> host(wbytes + (size_t)L.npad * 8, 0);
-    for (int k = 0; k < L.inner; k++) {
-        const int8_t* src = w + (size_t)k * L.columns;
-        const size_t at = (size_t)(k / 32) * 1024 + (size_t)(k % 32 / 16) * 512 + k % 16;
-        for (int cb = 0; cb < L.nb; cb++) {
-            uint8_t* d = host.data() + (size_t)cb * L.kb * 1024 + at;
-            const int cols = std::min(32, L.columns - cb * 32);
-            for (int c = 0; c < cols; c++) d[c * 16] = (uint8_t)src[cb * 32 + c];
-        }
-    }
-    memcpy(host.data() + L.scales_at, scales, (size_t)L.columns * 4);
-    if (bias) memcpy(host.data() + L.scales_at + (size_t)L.npad * 4, bias, (size_t)L.columns * 4);
-    L.mem.upload(L.be, host.data(), host.size(), "QuantLinear weights");
-    for (int s = 0; s < 3; s++) {
-        const std::string st = kStorageName[s];
-        for (int i = 0; i < 3; i++) L.fn_rows[s][i] = L.be->fn("sox_qrows_" + st + "_t" + std::to_string(kRowThreads[i]));
-        for (int i = 0; i < kQTileCount; i++) {
-            L.fn_ring[s][i] = nullptr;
-            if (s != SOX_STORAGE_F32 || kQTiles[i].bm * kQTiles[i].bn < 256 * 256)
-                L.fn_ring[s][i] = L.be->fn("sox_qgemm_" + st + "_" + kQTiles[i].name);
-        }
-        for (int i = 0; i < 4; i++) L.fn_panel[s][i] = L.be->fn("sox_qpanel_" + st + "_c" + std::to_string(i + 1));
-        for (int i = 0; i < 3; i++) {
-            L.fn_few[s][i] = L.be->fn("sox_qfew_" + st + "_r" + std::to_string(1 << i));
-            L.fn_fewx[s][i] = L.be->fn("sox_qfewx_" + st + "_s" + std::to_string(1 << i));
-        }
-    }
-}
-
-std::unique_ptr<sox_qlinear> qlinear_new(sox_backend* be, const void* weights, int32_t inner, int32_t columns, sox_qlinear** out) {
-    if (!be || !weights || !out || inner <= 0 || columns <= 0) fail(SOX_E_INVALID, "QuantLinear: arguments");
-    if (inner > 131071) fail(SOX_E_UNSUPPORTED, "QuantLinear: 32-bit sums over more than 131071 products");
-    if (columns > 1 << 24) fail(SOX_E_UNSUPPORTED, "QuantLinear: more than 2^24 columns");
+std::unique_ptr<sox_qlinear> qlinear_new(sox_backend* be, int inner, int columns, const int8_t* w, const float* scales, const float* bias) {
     auto L = std::make_unique<sox_qlinear>();
+    const Packed8 packed(inner, columns, w, scales, bias);
     L->be = be;
     L->inner = inner;
     L->columns = columns;
-    L->k16 = round_up(inner, 16);
-    L->kb = round_up(inner, 128) / 32;
-    L->nb = (columns + 31) / 32;
-    L->npad = round_up(columns, 256) + 256;  // (a last tile of 192 columns may start inside the last 256)
+    L->kb = packed.kb;
+    L->nb = packed.nb;
+    L->npad = packed.npad;
+    L->scales_at = packed.scales_at;
+    L->mem.upload(be, packed.bytes.data(), packed.bytes.size(), "QuantLinear weights");
+    for (int kind = 0; kind < QLaunch::KINDS; kind++)
+        for (int32_t st = 0; st < 3; st++)
+            for (int i = 0; i < QLaunch::instances(kind); i++) {
+                const std::string kernel = QLaunch::kernel(kind, i, st);
+                L->fns[kind][st].push_back(kernel.empty() ? nullptr : be->fn(kernel));
+            }
     return L;
 }
 
 // The product, over 8-bit rows (a.a, a.xs) or where the plan rounds them itself over floating ones (a.x).
 void qlinear_product(const LayerCall& c, sox_qlinear* L, const QPlan& plan, void* stream, sox_qgemm_args& a, int32_t storage) {
-    a.w = L->w();
-    a.ws = L->ws();
-    a.bias = L->bias();
+    const QLaunch l = QLaunch::product(plan, L->inner, L->columns, c.rows, c.be->info.compute_units);
+    a.w = (const int8_t*)L->mem.p;
+    a.ws = (const float*)((const uint8_t*)L->mem.p + L->scales_at);
+    a.bias = a.ws + L->npad;
     a.zeros = c.be->dummy;
     a.m = (int32_t)c.rows;
     a.n = L->columns;
     a.k = L->inner;
-    a.k16 = L->k16;
+    a.k16 = round_up(L->inner, 16);
     a.kb = L->kb;
     a.nb = L->nb;
-    const int steps = (L->inner + 63) / 64;
-    const uint32_t groups = (uint32_t)((L->columns + 15) / 16);
-    switch (plan.way) {
-    case QPlan::FEWX: {
-        const int segs = (L->inner + 1023) / 1024, waves = (int)std::min<int64_t>(16, std::max<int64_t>(steps, c.rows * segs));
-        const int si = steps <= waves ? 0 : steps <= 2 * waves ? 1 : 2;
-        c.launch(L->fn_fewx[storage][si], groups, 1, (uint32_t)waves * 64, stream, a,
-                 (uint32_t)(c.rows * (round_up(L->inner, 256) + 16)));
-        break;
-    }
-    case QPlan::PANEL:
-        c.launch(L->fn_panel[storage][(L->inner - 1) / 256], (uint32_t)((L->columns + 127) / 128), (uint32_t)((c.rows + 31) / 32), 512,
-                 stream, a, (uint32_t)((L->inner + 31) / 32) * 1024);
-        break;
-    case QPlan::FEW: {
-        const int ri = c.rows <= 16 ? 0 : c.rows <= 32 ? 1 : 2, s = 8 >> ri;
-        c.launch(L->fn_few[storage][ri], groups, 1, (uint32_t)std::min(8, (steps + s - 1) / s) * 64, stream, a);
-        break;
-    }
-    case QPlan::RING: {
-        const QTile& t = *plan.tile;
-        a.tiles_n = (L->columns + t.bn - 1) / t.bn;
-        const int64_t tiles = ((c.rows + t.bm - 1) / t.bm) * a.tiles_n;
-        if (tiles >= (int64_t)1 << 24) fail(SOX_E_UNSUPPORTED, std::string(c.name) + ": too many outputs");
-        c.launch(L->fn_ring[storage][&t - kQTiles],
-                 (uint32_t)std::min<int64_t>(tiles, (int64_t)std::max(1, c.be->info.compute_units) * t.wgs_per_cu), 1,
-                 (uint32_t)t.threads, stream, a);
-        break;
-    }
-    }
+    a.tiles_n = l.tiles_n;
+    c.launch(L->fn(l, storage), l.gx, l.gy, l.threads, stream, a, l.lds);
 }
 
 }  // namespace
@@ -4996,34 +5406,13 @@ void qlinear_product(const LayerCall& c, sox_qlinear* L, const QPlan& plan, void
 struct sox_block_norm {
     sox_backend* be = nullptr;
     sox_block_norm_p p{};
-    DeviceBlock mem;  // pg, pb, g, b: [cpad] each
+    DeviceBlock mem;  // BnormVectors
     int cpad = 0, vectors = 0;
-    bool has[4] = {};  // which of them there are (the others are all ones or all zeros)
+    bool has[4] = {};
     void* fn[3][2][2];  // storage, many rows, vector
 };
 
 namespace {
-
-// block_norm.hip's instances: threads of a row, chunks of 8 columns of a thread, workgroups per CU at most; `many`: for many
-// rows, with the parameters in LDS.
-struct BnormShape {
-    int tpr, ch, per_cu;
-    bool many;
-};
-const BnormShape kBnormShapes[] = {{32, 1, 4, true},   {64, 1, 4, true},   {64, 2, 4, true},  {256, 1, 4, false},
-                                   {256, 2, 2, false}, {512, 2, 2, false}, {512, 4, 1, false}};
-
-// The first instance that holds c columns; those for many rows only where there are many.
-int bnorm_shape(int c, bool many) {
-    for (int i = 0; i < (int)(sizeof kBnormShapes / sizeof *kBnormShapes); i++)
-        if (kBnormShapes[i].tpr * kBnormShapes[i].ch * 8 >= c && (many || !kBnormShapes[i].many)) return i;
-    unsupported("BlockNorm: channels");
-}
-std::string bnorm_kernel(int32_t storage, int shape, bool vec) {
-    const BnormShape& s = kBnormShapes[shape];  // (a 16-byte chunk of fp32 is half as many columns)
-    return std::string("sox_bnorm_") + kStorageName[storage] + "_t" + std::to_string(s.tpr) + "c" +
-           std::to_string(s.ch * (storage == SOX_STORAGE_F32 ? 2 : 1)) + (vec ? "v" : "s");
-}
 
 void bnorm_run(sox_block_norm* N, const char* name, void* stream, int32_t storage, int32_t rows, const void* residual,
                int64_t ldr, const void* x, int64_t ldx, const void* gate, int64_t ldg, int32_t gate_rows, void* h, int64_t ldh,
@@ -5063,13 +5452,8 @@ void bnorm_run(sox_block_norm* N, const char* name, void* stream, int32_t storag
     a.post = N->p.post; a.pre = N->p.pre; a.gate_act = N->p.gate_act;
     a.post_eps = N->p.post_eps; a.pre_eps = N->p.pre_eps; a.res_scale = N->p.res_scale;
     const bool vec = c.on(R) && c.on(X) && c.on(G) && c.on(H) && (quantized || c.on(Y));
-    const int64_t cus = std::max(1, c.be->info.compute_units);
-    const bool many = rows >= 4 * cus;  // a wave on every SIMD
-    const BnormShape& shape = kBnormShapes[bnorm_shape(C, many)];
-    const int threads = std::max(shape.tpr, 256), per_block = threads / shape.tpr;
-    const int64_t blocks = std::min<int64_t>((rows + per_block - 1) / per_block, cus * shape.per_cu);
-    c.launch(N->fn[storage][many][vec], (uint32_t)blocks, 1, (uint32_t)threads, stream, a,
-             shape.many ? (uint32_t)(N->vectors * shape.tpr * shape.ch * 8 * 4) : 0);
+    const BnormLaunch l(C, rows, N->vectors, c.be->info.compute_units);
+    c.launch(N->fn[storage][bnorm_many(rows, c.be->info.compute_units)][vec], l.blocks, 1, l.threads, stream, a, l.lds);
 }
 
 }  // namespace
@@ -5078,50 +5462,36 @@ extern "C" {
 
 int sox_qlinear_create(sox_backend* be, const float* weights, const float* bias, int32_t inner, int32_t columns, sox_qlinear** out) {
     return guarded([&] {
-        auto L = qlinear_new(be, weights, inner, columns, out);
-        std::vector<float> amax((size_t)columns, 0.0f), scales((size_t)columns);
-        for (int k = 0; k < inner; k++)
-            for (int c = 0; c < columns; c++) {
-                const float v = fabsf(weights[(size_t)k * columns + c]);
-                if (!std::isfinite(v)) fail(SOX_E_INVALID, "QuantLinear: weights have to be finite");
-                amax[c] = std::max(amax[c], v);
-            }
-        for (int c = 0; c < columns; c++) scales[c] = amax[c] / 127.0f;
-        std::vector<int8_t> w((size_t)inner * columns);
-        for (int k = 0; k < inner; k++)
-            for (int c = 0; c < columns; c++) {
-                const size_t i = (size_t)k * columns + c;
-                w[i] = amax[c] > 0.0f ? (int8_t)std::nearbyint(127.0 * weights[i] / amax[c]) : (int8_t)0;
-            }
-        qlinear_pack(*L, w.data(), scales.data(), bias);
-        *out = L.release();
+        if (!be || !weights || !out) fail(SOX_E_INVALID, "QuantLinear: arguments");
+        Packed8::check_sizes(inner, columns);
+        std::vector<int8_t> w;
+        std::vector<float> scales;
+        quantize_columns(weights, inner, columns, w, scales);
+        *out = qlinear_new(be, inner, columns, w.data(), scales.data(), bias).release();
     });
 }
 
 int sox_qlinear_create_int8(sox_backend* be, const int8_t* weights, const float* scales, const float* bias, int32_t inner,
                             int32_t columns, sox_qlinear** out) {
     return guarded([&] {
-        auto L = qlinear_new(be, weights, inner, columns, out);
-        if (!scales) fail(SOX_E_INVALID, "QuantLinear: arguments");
-        for (int c = 0; c < columns; c++)
-            if (!std::isfinite(scales[c])) fail(SOX_E_INVALID, "QuantLinear: scales have to be finite");
-        qlinear_pack(*L, weights, scales, bias);
-        *out = L.release();
+        if (!be || !weights || !scales || !out) fail(SOX_E_INVALID, "QuantLinear: arguments");
+        Packed8::check_sizes(inner, columns);
+        *out = qlinear_new(be, inner, columns, weights, scales, bias).release();
     });
 }
 
 void sox_qlinear_destroy(sox_qlinear* L) { delete L; }
 
-int sox_qlinear_pitch(sox_qlinear* L) { return L ? L->pitch() : 0; }
+int sox_qlinear_pitch(sox_qlinear* L) { return L ? QPlan::pitch(L->inner) : 0; }
 
 uint64_t sox_qlinear_workspace(sox_qlinear* L, int32_t rows) {
     if (!L || rows <= 0 || rows > 1 << 23) return 0;
     uint64_t need = 0;  // for every storage type
     for (int32_t s = 0; s < 3; s++) {
         const int rc = guarded([&] {
-            if (!QPlan(*L, rows, s, true).rounds_itself()) need = QPlan::bytes(*L, rows);
+            if (!L->plan(rows, s, true).rounds_itself()) need = QPlan::bytes(L->inner, rows);
         });
-        if (rc) return QPlan::bytes(*L, rows);
+        if (rc) return QPlan::bytes(L->inner, rows);
     }
     return need;
 }
@@ -5136,10 +5506,10 @@ int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x
         if (rows == 0) return;
         const Rows X = c.matrix("x", x, ldx, L->inner), R = c.matrix("residual", residual, ldr, L->columns, true);
         const Rows Y = c.matrix("y", y, ldy, L->columns);
-        const QPlan plan(*L, rows, storage, true);
+        const QPlan plan = L->plan(rows, storage, true);
         Rows W{"workspace"};
         if (!plan.rounds_itself()) {
-            const uint64_t need = QPlan::bytes(*L, rows);
+            const uint64_t need = QPlan::bytes(L->inner, rows);
             if (!workspace || workspace_bytes < need)
                 c.bad("needs " + std::to_string(need) + " bytes of workspace, has " + std::to_string(workspace ? workspace_bytes : 0));
             W = c.matrix("workspace", workspace, (int64_t)need, (int64_t)need, 1, 16, false, 1);
@@ -5161,14 +5531,13 @@ int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x
             q.x = x;
             q.ldx = ldx;
             q.q = (int8_t*)workspace;
-            q.ldq = L->pitch();
-            q.scale = (float*)((uint8_t*)workspace + QPlan::rows_bytes(*L, rows));
+            q.ldq = QPlan::pitch(L->inner);
+            q.scale = (float*)((uint8_t*)workspace + QPlan::rows_bytes(L->inner, rows));
             q.rows = rows;
             q.k = L->inner;
             q.vec = c.on(X);
-            const int64_t bytes = (int64_t)L->inner * c.es;
-            const int ti = bytes <= 32 * 64 ? 0 : bytes <= 64 * 64 ? 1 : 2, per_block = 256 / kRowThreads[ti];
-            c.launch(L->fn_rows[storage][ti], (uint32_t)((rows + per_block - 1) / per_block), 1, 256, stream, q);
+            const QLaunch l = QLaunch::rows(L->inner, rows, (int)c.es);
+            c.launch(L->fn(l, storage), l.gx, 1, l.threads, stream, q);
             a.a = q.q;
             a.lda = q.ldq;
             a.xs = q.scale;
@@ -5185,7 +5554,7 @@ int sox_qlinear_run_quantized(sox_qlinear* L, void* stream, const int8_t* q, int
         const LayerCall c(L->be, name, rows, storage);
         c.act(act);
         if (rows == 0) return;
-        const Rows Q = c.matrix("q", q, ldq, L->k16, 1, 16, false, rows), S = c.matrix("scales", scales, rows, rows, 4, 4, false, 1);
+        const Rows Q = c.matrix("q", q, ldq, round_up(L->inner, 16), 1, 16, false, rows), S = c.matrix("scales", scales, rows, rows, 4, 4, false, 1);
         const Rows R = c.matrix("residual", residual, ldr, L->columns, true), Y = c.matrix("y", y, ldy, L->columns);
         c.apart(Y, {&Q, &S}, {&R});
         c.device(stream, {&Q, &S, &R, &Y});
@@ -5199,40 +5568,22 @@ int sox_qlinear_run_quantized(sox_qlinear* L, void* stream, const int8_t* q, int
         a.ldy = ldy;
         a.act = act;
         a.vec = (c.on(Y) && c.on(R) ? 1 : 0) | (c.on(Y, 128) ? 4 : 0);
-        qlinear_product(c, L, QPlan(*L, rows, storage, false), stream, a, storage);
+        qlinear_product(c, L, L->plan(rows, storage, false), stream, a, storage);
     });
 }
 
 int sox_block_norm_create(sox_backend* be, const sox_block_norm_p* p, const float* post_gamma, const float* post_beta,
                           const float* scale, const float* pre_gamma, const float* pre_beta, sox_block_norm** out) {
     return guarded([&] {
-        if (!be || !p || !out || p->channels <= 0) fail(SOX_E_INVALID, "BlockNorm: arguments");
-        if (p->channels > 16384) fail(SOX_E_UNSUPPORTED, "BlockNorm: more than 16384 channels");
-        for (int32_t kind : {p->post, p->pre})
-            if (kind < SOX_NORM_NONE || kind > SOX_NORM_LAYER) fail(SOX_E_INVALID, "BlockNorm: norm kind");
-        if (p->gate_act < SOX_ACT_NONE || p->gate_act > SOX_ACT_SWISH) fail(SOX_E_UNSUPPORTED, "BlockNorm: gate activation");
-        if (!(p->post_eps >= 0.0f) || !(p->pre_eps >= 0.0f) || !std::isfinite(p->res_scale)) fail(SOX_E_INVALID, "BlockNorm: eps / residual scale");
+        if (!be || !p || !out) fail(SOX_E_INVALID, "BlockNorm: arguments");
+        const BnormVectors vectors(*p, post_gamma, post_beta, scale, pre_gamma, pre_beta);
         auto N = std::make_unique<sox_block_norm>();
         N->be = be;
         N->p = *p;
-        const size_t C = (size_t)p->channels, CP = (size_t)round_up(p->channels, 8);
-        N->cpad = (int)CP;
-        const bool post = p->post != SOX_NORM_NONE, pre = p->pre != SOX_NORM_NONE;
-        const bool pb = p->post == SOX_NORM_LAYER && post_beta, b = p->pre == SOX_NORM_LAYER && pre_beta;
-        std::vector<float> v(4 * CP);
-        for (size_t i = 0; i < C; i++) {  // the branch's scale folded into the post norm
-            const float s = scale ? scale[i] : 1.0f;
-            v[i] = (post && post_gamma ? post_gamma[i] : 1.0f) * s;
-            v[CP + i] = pb ? post_beta[i] * s : 0.0f;
-            v[2 * CP + i] = pre && pre_gamma ? pre_gamma[i] : 1.0f;
-            v[3 * CP + i] = b ? pre_beta[i] : 0.0f;
-        }
-        const bool has[4] = {scale || (post && post_gamma), pb, pre && pre_gamma, b};
-        for (int i = 0; i < 4; i++) {
-            N->has[i] = has[i];
-            N->vectors += has[i];
-        }
-        N->mem.upload(be, v.data(), v.size() * 4, "BlockNorm parameters");
+        N->cpad = vectors.cpad;
+        N->vectors = vectors.count;
+        memcpy(N->has, vectors.has, sizeof N->has);
+        N->mem.upload(be, vectors.v.data(), vectors.v.size() * 4, "BlockNorm parameters");
         for (int32_t s = 0; s < 3; s++)
             for (int many = 0; many < 2; many++)
                 for (int vec = 0; vec < 2; vec++) N->fn[s][many][vec] = be->fn(bnorm_kernel(s, bnorm_shape(p->channels, many), vec));

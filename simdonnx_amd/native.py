@@ -142,6 +142,14 @@ class BlockNormP(ctypes.Structure):
                 ("pre_eps", c_float), ("res_scale", c_float)]
 
 
+class QuantLinearP(ctypes.Structure):
+    _fields_ = [("act", c_int32), ("has_bias", c_int32), ("has_residual", c_int32)]
+
+
+class BlockNormNodeP(ctypes.Structure):
+    _fields_ = [("norm", BlockNormP), ("operands", c_uint32)]
+
+
 class Bind(ctypes.Structure):
     _fields_ = [("slot", c_int32), ("pad_", c_int32), ("offset", c_uint64), ("size", c_uint64)]
 

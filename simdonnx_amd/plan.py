@@ -671,6 +671,32 @@ class PlanBuilder:
         self._node("Ext", ins, [y], bytes(p), name or "uphead", ext="UpHead")
         return y
 
+    # ---- 8-bit transformer layers (HipQuantLinear and HipBlockNorm as nodes) ----
+    def quant_linear(self, x, w, b=None, *, residual=None, act="none", name=""):
+        """act(x . w + b + residual) with the rows of x and the columns of w [K, N] brought to 8 bits."""
+        wv = w if isinstance(w, int) else self.const(w, name + ".w")
+        bv = b if b is None or isinstance(b, int) else self.const(b, name + ".b")
+        ins = [v for v in (x, wv, bv, residual) if v is not None]
+        y = self.activation(tuple(self.values[x].shape[:-1]) + (self.values[wv].shape[1],), None, name or "quant_linear")
+        p = N.QuantLinearP(ACT[act], int(b is not None), int(residual is not None))
+        return self._node("Ext", ins, [y], bytes(p), name or "quant_linear", ext="QuantLinear")
+
+    def block_norm(self, residual=None, x=None, gate=None, *, post="none", pre="layer", post_gamma=None, post_beta=None,
+                   scale=None, pre_gamma=None, pre_beta=None, res_scale=1.0, gate_act="none", post_eps=1e-5, pre_eps=1e-5,
+                   h=True, y=True, name=""):
+        """h = res_scale * residual + act(gate) * (post(x) * scale), y = pre(h) over the last dimension: (h, y), None for
+        one that is not asked for. A gate row holds for as many consecutive rows as rows / gate rows."""
+        shape = self.values[x if x is not None else residual].shape
+        vecs = [v if v is None or isinstance(v, int) else self.const(v, f"{name}.{i}")
+                for i, v in enumerate((post_gamma, post_beta, scale, pre_gamma, pre_beta))]
+        ins = [residual, x, gate] + vecs
+        out = [self.activation(shape, None, f"{name or 'block_norm'}.{k}") if want else None for k, want in (("h", h), ("y", y))]
+        norm = N.BlockNormP(shape[-1], N.NORM[post], N.NORM[pre], ACT[gate_act], post_eps, pre_eps, res_scale)
+        p = N.BlockNormNodeP(norm, sum(1 << i for i, v in enumerate(ins + out) if v is not None))
+        self._node("Ext", [v for v in ins if v is not None], [v for v in out if v is not None], bytes(p), name or "block_norm",
+                   ext="BlockNorm")
+        return tuple(out)
+
     def ext(self, name, ins, out_shape, params: bytes = b"", layout=None, node_name=""):
         """ExecOp.Ext node of a consumer-registered operator."""
         y = self.activation(out_shape, layout, node_name or name)
