@@ -287,11 +287,11 @@ struct QTile {
     float lat, thr, base, tile, out;
 };
 const QTile kQTiles[] = {
-    {"256x256_w8k128s2", 256, 256, 1, 512, 0.35f, 1.15f, 3.3f, 3.8f, 0.51f},
-    {"256x192_w8k128s2", 256, 192, 1, 512, 0.43f, 0.99f, 2.7f, 3.9f, 0.43f},
-    {"256x128_w8k128s2", 256, 128, 1, 512, 0.84f, 0.85f, 4.0f, 1.2f, 0.43f},
-    {"128x128_w4k128s2", 128, 128, 2, 256, 0.59f, 0.465f, 4.45f, 0.4f, 0.44f},
-    {"64x64_w4k128s4", 64, 64, 2, 256, 0.31f, 0.22f, 3.5f, 0.2f, 0.57f},
+    {"256x256_w8k128s2", 256, 256, 1, 512, 0.92f, 1.15f, 2.9f, 4.2f, 0.46f},
+    {"256x192_w8k128s2", 256, 192, 1, 512, 0.96f, 0.98f, 2.4f, 4.1f, 0.38f},
+    {"256x128_w8k128s2", 256, 128, 1, 512, 0.85f, 0.85f, 3.6f, 1.6f, 0.37f},
+    {"128x128_w4k128s2", 128, 128, 2, 256, 0.59f, 0.46f, 4.35f, 0.43f, 0.39f},
+    {"64x64_w4k128s4", 64, 64, 2, 256, 0.31f, 0.22f, 3.45f, 0.24f, 0.48f},
 };
 const int kRowThreads[] = {32, 64, 256};  // of a row brought to 8 bits, each with four 16-byte chunks in registers
 constexpr int kQTileCount = (int)(sizeof kQTiles / sizeof *kQTiles);
@@ -303,8 +303,8 @@ constexpr int kQTileCount = (int)(sizeof kQTiles / sizeof *kQTiles);
 //          once per 128 columns                                              of its own 9.4. 8192 x 768 -> 2304: 51, 35
 //   FEW    up to 64 8-bit rows, weights straight to registers                64 x 4096 -> 4096: 10.8 us, ring 13.5;
 //                                                                            64 x 1024 -> 8192: 6.9, ring 6.0
-//   RING   8-bit rows on the ring of the tiling with the smallest estimate. Over 170 random products the pick is 1.4% above
-//          the fastest tiling on average, at most 21%
+//   RING   8-bit rows on the ring of the tiling with the smallest estimate. Over 170 random products the pick is 1.3% above
+//          the fastest tiling on average, at most 18%
 // FEW and RING take floating rows behind a launch that brings them to 8 bits in the workspace.
 struct QPlan {
     enum Way { FEWX, PANEL, FEW, RING } way = RING;
@@ -367,7 +367,7 @@ struct QLaunch {
     int tiles_n = 0;
 
     static int instances(int kind) {
-        static const int n[KINDS] = {3, 4, 3, kQTileCount, 3};
+        static const int n[KINDS] = {3, 4, 3, 2 * kQTileCount, 3};
         return n[kind];
     }
     // "" for an instance that the storage type does not have
@@ -379,8 +379,8 @@ struct QLaunch {
         case QPlan::FEW: return "sox_qfew_" + st + "_r" + std::to_string(1 << index);      // rows / 16
         case ROWS: return "sox_qrows_" + st + "_t" + std::to_string(kRowThreads[index]);
         default:
-            if (storage == SOX_STORAGE_F32 && kQTiles[index].bm * kQTiles[index].bn == 256 * 256) return "";
-            return "sox_qgemm_" + st + "_" + kQTiles[index].name;
+            if (storage == SOX_STORAGE_F32 && kQTiles[index / 2].bm * kQTiles[index / 2].bn == 256 * 256) return "";
+            return "sox_qgemm_" + st + "_" + kQTiles[index / 2].name + (index % 2 ? "_l" : "");  // (outputs on lines)
         }
     }
     // rows of `inner` elements of es bytes to 8 bits
@@ -393,7 +393,8 @@ struct QLaunch {
         l.gx = (uint32_t)((m + per_block - 1) / per_block);
         return l;
     }
-    static QLaunch product(const QPlan& plan, int inner, int columns, int64_t m, int compute_units) {
+    // vec: sox_qgemm_args.vec
+    static QLaunch product(const QPlan& plan, int inner, int columns, int64_t m, int vec, int compute_units) {
         QLaunch l;
         l.kind = plan.way;
         const int steps = (inner + 63) / 64;
@@ -419,7 +420,7 @@ struct QLaunch {
             break;
         case QPlan::RING: {
             const QTile& t = *plan.tile;
-            l.index = (int)(&t - kQTiles);
+            l.index = 2 * (int)(&t - kQTiles) + ((vec & 5) == 5 && columns % 8 == 0);
             l.tiles_n = (columns + t.bn - 1) / t.bn;
             const int64_t tiles = ((m + t.bm - 1) / t.bm) * l.tiles_n;
             if (tiles >= (int64_t)1 << 24) unsupported("8-bit product: too many outputs");
@@ -2587,12 +2588,12 @@ struct Emitter {
             ptrs.push_back({offsetof(sox_qgemm_args, a), part(ws, 0, bytes)});
             ptrs.push_back({offsetof(sox_qgemm_args, xs), part(ws, bytes, scales)});
         }
-        const QLaunch l = QLaunch::product(plan, q.inner, q.columns, q.rows, cus);
         a.ldx = q.inner;
         a.ldr = a.ldy = q.columns;
         a.act = q.p.act;
         a.vec = (rows_on(q.y, q.columns) && rows_on(q.residual, q.columns) ? 1 : 0) | (rows_on(q.x, q.inner) ? 2 : 0) |
                 (rows_on(q.y, q.columns, 128) ? 4 : 0);
+        const QLaunch l = QLaunch::product(plan, q.inner, q.columns, q.rows, a.vec, cus);
         a.m = (int32_t)q.rows;
         a.n = q.columns;
         a.k = q.inner;
@@ -3595,7 +3596,7 @@ bool conv_pads_channels(const sox_graph& g, const PlanNode& n) {
 // The nodes of the 8-bit layers. A BlockNorm's parameters become one const. An output that the plan put over an operand gets
 // a buffer of its own (workgroups write it while others still read). A BlockNorm whose y only QuantLinears read hands
 // them 8-bit rows, rounded once and from fp32, in y's own buffer: channels bytes a row and 4 for its scale fit where
-// 2 * channels were (8192 rows of 1024: the rounding launch of each product, 8 us, falls away).
+// 2 * channels were. Saves each product its rounding launch: 10 us of 62 at 8192 x 1024 -> 4096 in fp16.
 void plan_layers8(sox_graph& g) {
     auto& P = g.plan;
     auto apart = [&](int out, std::initializer_list<int> others) {
@@ -5386,7 +5387,7 @@ std::unique_ptr<sox_qlinear> qlinear_new(sox_backend* be, int inner, int columns
 
 // The product, over 8-bit rows (a.a, a.xs) or where the plan rounds them itself over floating ones (a.x).
 void qlinear_product(const LayerCall& c, sox_qlinear* L, const QPlan& plan, void* stream, sox_qgemm_args& a, int32_t storage) {
-    const QLaunch l = QLaunch::product(plan, L->inner, L->columns, c.rows, c.be->info.compute_units);
+    const QLaunch l = QLaunch::product(plan, L->inner, L->columns, c.rows, a.vec, c.be->info.compute_units);
     a.w = (const int8_t*)L->mem.p;
     a.ws = (const float*)((const uint8_t*)L->mem.p + L->scales_at);
     a.bias = a.ws + L->npad;

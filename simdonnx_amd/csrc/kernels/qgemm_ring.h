@@ -17,8 +17,15 @@
 //  * The tile's scales and bias ride into LDS with its first slice.
 //  * Persistent: each workgroup walks its tiles as one ring, the next tile's slices load during the epilogue.
 //    Workgroups are numbered XCD-major, so the tiles in flight on one XCD share rows and columns in its L2.
-//  * Epilogue per 32 x 32 block through 4 KiB of LDS per wave: scaled fp32 values in, rows out, so residual loads
-//    and output stores are whole row segments and one code path serves every storage type.
+//  * Epilogue per 32 x 32 block: scaled and activated in registers, turned into rows through 2 KiB of LDS per wave, so
+//    residual loads and output stores are whole row segments.
+//
+// Tiles by size (the host's estimates choose): 256 x 256 with its 8 waves holds a wave's 128 x 64 outputs in registers and
+// reads 1 byte of LDS for 128 multiply-adds; 256 x 192 for shapes that fill the CUs' rounds better (8192 x 768 -> 2304: 27 us,
+// 1.5 rounds; 256 x 128 33); down to 64 x 64, four slices deep, where there are few tiles and a slice's latency counts.
+// Bound: with long K by the matrix cores, 4096 x 4096 -> 8192 in 126 us (2.18e15 operations a second; a large library product of
+// 8-bit integers reaches 2.1e15 on the same card). With K = 4096 a 256 x 256 tile takes 52 us, 43 of them without its DMA and 35
+// without its MFMAs, the epilogue 4 us. With short K by the prologue (2 us), the epilogue and the outputs' stores.
 #pragma once
 #include "qrows.h"
 
@@ -49,18 +56,24 @@ template <typename T> SOX_DEV int stage_at(int r, int c) {
     return sizeof(T) == 2 ? r * 64 + ((c ^ ((r >> 2) & 3)) << 4) : r * 128 + ((c ^ (r >> 1)) << 4);
 }
 
+// What a kernel knows of the rows of its outputs and residual:
+//   Q_LINES  rows of y on 128-byte lines, of the residual on 16-byte boundaries, whole 16-byte chunks in both. The stores pass
+//            L2 by, which leaves it to the A and W lines that are read again: 4096 x 4096 -> 8192 124 us, 133 with stores
+//            through L2, 128 with the choice made in the kernel
+//   Q_CHUNKS whole chunks where the rows stand on 16-byte boundaries. Their stores go through L2: a line that different stores
+//            write in parts would reach memory in parts, 2954 x 320 -> 3112 19.8 us so and 13.3 through L2
+//   Q_PART   any
+enum { Q_LINES, Q_CHUNKS, Q_PART };
+
 // A block's rows between memory at (m0, n0) and the stage: 16-byte chunks where the rows stand on 16-byte boundaries (uniform;
-// single elements in the chunk that a row ends in), else single elements, a half wave per row, in a loop that is not unrolled (the ragged form should not be most of the code).
-// Outputs whose rows stand on 128-byte lines pass L2 by (vec bit 2), which leaves it to the A and W lines that are read
-// again: 8192 x 768 -> 2304 29.4 -> 28.2 us. Other rows' lines are written in parts by different stores, and in parts
-// they would reach memory: 2954 x 320 -> 3112 took 19.8 us so, 13.3 through L2.
+// single elements in the chunk that a row ends in), else single elements, a half wave per row, in a loop that is not
+// unrolled (the ragged form should not be most of the code).
 // LOAD: the residual's into the stage (zeros outside), else the stage's to the output.
-// PART: a row may end inside a chunk.
-template <typename T, bool LOAD, bool PART>
-SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, int vec, unsigned char* stg, int m0, int n0, int lane) {
+template <typename T, bool LOAD, int FORM>
+SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, bool vec, unsigned char* stg, int m0, int n0, int lane) {
     constexpr int E = 16 / sizeof(T), PER = 32 / E, ROWS = STG_BYTES / (32 * sizeof(T));  // elements of a chunk, chunks of a row
     typedef vec_t<T, E> TE;
-    if (vec & 1) {
+    if (FORM == Q_LINES || vec) {
 #pragma unroll
         for (int t = 0; t < ROWS * PER / 64; t++) {
             const int idx = t * 64 + lane, r = idx / PER, u = idx % PER, m = m0 + r, n = n0 + u * E;
@@ -72,17 +85,17 @@ SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, int vec, 
                     v = *(const TE*)g;
                 }
                 *s = v;
-                if (PART && m < M && n < N && n + E > N)
+                if (FORM == Q_PART && m < M && n < N && n + E > N)
 #pragma unroll 1
                     for (int e = 0; e < N - n; e++) ((T*)s)[e] = g[e];
             } else {
                 const TE v = *s;
                 if (m < M && n + E <= N) {
-                    if (vec & 4)
+                    if constexpr (FORM == Q_LINES)
                         __builtin_nontemporal_store(v, (TE*)g);
                     else
                         *(TE*)g = v;
-                } else if (PART && m < M && n < N) {
+                } else if (FORM == Q_PART && m < M && n < N) {
 #pragma unroll 1
                     for (int e = 0; e < N - n; e++) g[e] = ((const T*)s)[e];
                 }
@@ -116,13 +129,13 @@ SOX_DEV void stage_turn() {
 // with the residual and activated in registers, staged and stored. One copy of this with its choices inside, none of
 // them per element: a choice per element, or a copy per form, multiplied the ring's code until its instruction fetches
 // took most of a short product's time and registers ran out. ws, bias: the block's 32 columns.
-template <typename T, bool PART = true>
+template <typename T, int FORM = Q_PART>
 SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs, const float* ws, const float* bias,
                           unsigned char* stg, int m0, int n0, int lane) {
     constexpr int PARTS = sizeof(T) == 2 ? 1 : 2, ROWS = 32 / PARTS;
     typedef vec_t<T, 4> T4;
     const int l32 = lane & 31, hl = lane >> 5;
-    const int vec = p.vec;
+    const bool vec = p.vec & 1;
     float val[16];
 #pragma unroll
     for (int q = 0; q < 4; q++) {
@@ -137,7 +150,7 @@ SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs,
     if (p.add) {
 #pragma unroll
         for (int half = 0; half < PARTS; half++) {
-            move_rows<T, true, PART>((T*)p.add, p.ldr, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
+            move_rows<T, true, FORM>((T*)p.add, p.ldr, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
             stage_turn();
             if (PARTS == 1 || l32 / ROWS == half) {
 #pragma unroll
@@ -172,12 +185,12 @@ SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs,
             }
         }
         stage_turn();
-        move_rows<T, false, PART>((T*)p.y, p.ldy, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
+        move_rows<T, false, FORM>((T*)p.y, p.ldy, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
         stage_turn();
     }
 }
 
-template <typename T, int BM, int BN, int BK, int WM, int WN, int STAGES, int NW, int GM, bool PART>
+template <typename T, int BM, int BN, int BK, int WM, int WN, int STAGES, int NW, int GM, int FORM>
 __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
     constexpr int CPR = BK / 16, KS = BK / 32;
     constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
@@ -289,7 +302,7 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
             constexpr int j = decltype(ji)::value / TI, i = decltype(ji)::value % TI;
             const float* ws = (const float*)sc + wn0 + j * 32;
             const float xs = *(const float*)(sc + BN * 8 + (wm0 + i * 32 + l32) * 4);
-            finish_block<T, PART>(p, acc[j][i], xs, ws, ws + BN, stg, bm + wm0 + i * 32, bn + wn0 + j * 32, lane);
+            finish_block<T, FORM>(p, acc[j][i], xs, ws, ws + BN, stg, bm + wm0 + i * 32, bn + wn0 + j * 32, lane);
             __builtin_amdgcn_sched_barrier(0);  // one block at a time: bounded register pressure
         });
         m_tile += G;
@@ -354,14 +367,17 @@ __device__ __forceinline__ void qgemm_body(const sox_qgemm_args& p) {
     wait_vmcnt<0>();  // the slices past the end land before the workgroup's LDS is given back
 }
 
-// One kernel per storage type and tiling, named BMxBN tile, wNW waves, kBK bytes of K per slice, sSTAGES; WM x WN of a tile
-// to a wave, OCC waves per SIMD, GM M-tiles to a group.
-#define SOX_QGEMM(NAME, T, TILE, BM, BN, BK, WM, WN, ST, NW, OCC, GM, PART)                                       \
+// Two kernels per storage type and tiling, for outputs on lines (_l) and others, named BMxBN tile, wNW waves, kBK bytes of K per
+// slice, sSTAGES; WM x WN of a tile to a wave, OCC waves per SIMD, GM M-tiles to a group.
+#define SOX_QGEMM_FORM(NAME, T, TILE, BM, BN, BK, WM, WN, ST, NW, OCC, GM, FORM)                                  \
     extern "C" __global__ void __launch_bounds__(64 * NW, OCC) sox_qgemm_##NAME##_##TILE(sox_qgemm_args p) { \
-        qgemm_body<T, BM, BN, BK, WM, WN, ST, NW, GM, PART>(p);                                                   \
+        qgemm_body<T, BM, BN, BK, WM, WN, ST, NW, GM, FORM>(p);                                                   \
     }
-#define SOX_QGEMM_TILES(NAME, T)                                                   \
-    SOX_QGEMM(NAME, T, 256x192_w8k128s2, 256, 192, 128, 64, 96, 2, 8, 2, 4, true) \
-    SOX_QGEMM(NAME, T, 256x128_w8k128s2, 256, 128, 128, 64, 64, 2, 8, 2, 4, true) \
-    SOX_QGEMM(NAME, T, 128x128_w4k128s2, 128, 128, 128, 64, 64, 2, 4, 2, 4, true) \
-    SOX_QGEMM(NAME, T, 64x64_w4k128s4, 64, 64, 128, 32, 32, 4, 4, 2, 4, true)
+#define SOX_QGEMM(NAME, T, TILE, BM, BN, BK, WM, WN, ST, NW, OCC, GM, FORM)                           \
+    SOX_QGEMM_FORM(NAME, T, TILE, BM, BN, BK, WM, WN, ST, NW, OCC, GM, FORM)                          \
+    SOX_QGEMM_FORM(NAME, T, TILE##_l, BM, BN, BK, WM, WN, ST, NW, OCC, GM, Q_LINES)
+#define SOX_QGEMM_TILES(NAME, T)                                                     \
+    SOX_QGEMM(NAME, T, 256x192_w8k128s2, 256, 192, 128, 64, 96, 2, 8, 2, 4, Q_PART) \
+    SOX_QGEMM(NAME, T, 256x128_w8k128s2, 256, 128, 128, 64, 64, 2, 8, 2, 4, Q_PART) \
+    SOX_QGEMM(NAME, T, 128x128_w4k128s2, 128, 128, 128, 64, 64, 2, 4, 2, 4, Q_PART) \
+    SOX_QGEMM(NAME, T, 64x64_w4k128s4, 64, 64, 128, 32, 32, 4, 4, 2, 4, Q_PART)

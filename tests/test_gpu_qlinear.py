@@ -96,6 +96,42 @@ def test_tiles(hip, monkeypatch, tile, storage, rows, k, n, pad, skip):
 
 
 @pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("storage", ["f16", "bf16", "f32"])
+def test_outputs_on_lines_and_off(hip, monkeypatch, tile, storage):
+    """Output rows on 128-byte lines (a kernel of their own), on 16-byte boundaries only, and on neither, a residual on less
+    than they are: the same bits each time."""
+    if storage == "f32" and tile.startswith("256x256"):
+        pytest.skip("16-bit outputs only")
+    monkeypatch.setenv("SIMDONNX_HIP_QGEMM", tile)
+    rows, k, n, line = 300, 200, 328, 384
+    w, ws = weights8(3, k, n)
+    x = rows_of(4, rows, k, storage)
+    r = rounded(synth.normal(5, 5, (rows, n), 1.0), storage)
+    q, scale = quantize(x)
+    want, tol = linear64(q, scale, w, ws, None, r, "swish", storage)
+    lin = HipQuantLinear(hip, w, None, k, n, scales=ws)
+    q8 = np.zeros((rows, lin.pitch), np.int8)
+    q8[:, :k] = q
+    Q, S = Matrix(q8, "i8"), Matrix(scale.astype(np.float32)[None], "f32")
+    chunk = 16 // (4 if storage == "f32" else 2)
+    outs = []
+    for (ld, skip), (ldr, skipr) in (((line, 0), (line, 0)), ((line, 0), (n, chunk)), ((line, 0), (n + 1, 0)),
+                                     ((n, 0), (line, 0)), ((line, chunk), (line, 0)), ((line, 1), (line, 0)), ((n + 3, 0), (n, 1))):
+        print(f"[gpu] {tile} {storage} y {ld} {skip} residual {ldr} {skipr}", flush=True)
+        Y, R = Matrix(None, storage, rows, n, ld=ld, skip=skip), Matrix(r, storage, ld=ldr, skip=skipr)
+        lin.run_quantized(Q.ptr, S.ptr, rows, Y.ptr, storage, ldq=Q.ld, ldy=ld, act="swish", residual=R.ptr, ldr=ldr)
+        outs.append(Y.read())
+        Y.free()
+        R.free()
+    check(outs[0], want, tol)
+    for o in outs[1:]:
+        assert np.array_equal(o, outs[0], equal_nan=True)
+    Q.free()
+    S.free()
+    lin.close()
+
+
+@pytest.mark.parametrize("tile", TILES)
 def test_many_tiles_per_workgroup(hip, monkeypatch, tile):
     """More tiles than workgroups, with one slice of K each: a workgroup's slices run several tiles ahead."""
     monkeypatch.setenv("SIMDONNX_HIP_QGEMM", tile)
