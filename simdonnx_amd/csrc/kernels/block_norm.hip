@@ -13,7 +13,8 @@
 //  * few rows, or longer ones: TPR threads per row, which shortens the one row's chain of loads, sums and stores; the
 //    parameters stay in registers (or, for the longest rows, are read where they are used).
 // A workgroup walks rows a whole grid apart; the grid is held to what the rows' streams run best with: 16384 x 4096 bf16 in
-// 93 us (5.8 TB/s) on 2 workgroups per CU, 122 with one row each, and 135 to 300 with a wave per row.
+// 95 us (5.7 TB/s) on 2 workgroups per CU, 122 with one row each, and 135 to 300 with a wave per row. Registers decide how
+// many waves there are: 8192 x 768 with a gate 13.8 us (100 registers, 4 waves on a SIMD), 17.5 when it took 144.
 #include "qrows.h"
 
 enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
@@ -26,6 +27,8 @@ template <typename T, int TPR, int CH, bool VEC> struct Row {
     typedef vec_t<T, E> TE;
     TE v[CH];
     SOX_DEV int col(int t, int j, int e) { return VEC ? (j * TPR + t) * E + e : (j * E + e) * TPR + t; }
+    // value e of chunk j is inside the row (a compare with a constant: the columns themselves would be held in registers)
+    SOX_DEV bool in(int t, int j, int e, int c) { return VEC ? e < c - col(t, j, 0) : (j * E + e) * TPR < c - t; }
     __device__ __forceinline__ void load(const T* __restrict__ p, int t, int c) {
 #pragma unroll
         for (int j = 0; j < CH; j++) {
@@ -37,11 +40,11 @@ template <typename T, int TPR, int CH, bool VEC> struct Row {
                 } else if (k < c) {  // the row's end inside a chunk
 #pragma unroll
                     for (int e = 0; e < E; e++)
-                        if (k + e < c) v[j][e] = p[k + e];
+                        if (in(t, j, e, c)) v[j][e] = p[k + e];
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < E; e++) v[j][e] = col(t, j, e) < c ? p[col(t, j, e)] : (T)0.0f;
+                for (int e = 0; e < E; e++) v[j][e] = in(t, j, e, c) ? p[col(t, j, e)] : (T)0.0f;
             }
         }
     }
@@ -58,12 +61,12 @@ template <typename T, int TPR, int CH, bool VEC> struct Row {
                 } else if (k < c) {
 #pragma unroll
                     for (int e = 0; e < E; e++)
-                        if (k + e < c) p[k + e] = o[e];
+                        if (in(t, j, e, c)) p[k + e] = o[e];
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < E; e++)
-                    if (col(t, j, e) < c) p[col(t, j, e)] = (T)f[j * E + e];
+                    if (in(t, j, e, c)) p[col(t, j, e)] = (T)f[j * E + e];
             }
         }
     }
@@ -88,7 +91,7 @@ template <typename T, int TPR, int CH, bool VEC> struct Row {
             } else {
 #pragma unroll
                 for (int e = 0; e < E; e++)
-                    if (col(t, j, e) < c16) p[col(t, j, e)] = RowQuant<half_t>::q(f[j * E + e], rq);
+                    if (in(t, j, e, c16)) p[col(t, j, e)] = RowQuant<half_t>::q(f[j * E + e], rq);
             }
         }
     }
@@ -140,7 +143,7 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < E; e++) o[e] = R::col(t, j, e) < c ? v[R::col(t, j, e)] : 0.0f;
+            for (int e = 0; e < E; e++) o[e] = R::in(t, j, e, c) ? v[R::col(t, j, e)] : 0.0f;
         }
     };
     if constexpr (PAR == PAR_REG) {
@@ -200,7 +203,7 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
             for (int i = 0; i < N; i++) s += v[i];
             const float mean = row_sum<TPR>(s, l0) * inv_c;
 #pragma unroll
-            for (int i = 0; i < N; i++) v[i] = R::col(t, i / E, i % E) < c ? v[i] - mean : 0.0f;
+            for (int i = 0; i < N; i++) v[i] = R::in(t, i / E, i % E, c) ? v[i] - mean : 0.0f;
         }
         float s = 0.0f;
 #pragma unroll
@@ -231,14 +234,16 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
             }
     };
     int set = 0;
-    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * RPB, set ^= 1) {
+    // (a wave's row is one number: its addresses stay in scalar registers)
+    const int sub = TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : threadIdx.x / TPR;
+    for (int64_t row = (int64_t)blockIdx.x * RPB + sub; row < p.rows; row += (int64_t)gridDim.x * RPB, set ^= 1) {
         R rr, gr;  // all of a row's loads go out together
         float h[N];
         if (p.x) {
             R xr;
             xr.load((const T*)p.x + row * p.ldx, t, c);
             if (p.residual) rr.load((const T*)p.residual + row * p.ldr, t, c);
-            if (p.gate) gr.load((const T*)p.gate + row / p.gate_group * p.ldg, t, c);
+            if (p.gate) gr.load((const T*)p.gate + (int64_t)((uint32_t)row / (uint32_t)p.gate_group) * p.ldg, t, c);
 #pragma unroll
             for (int i = 0; i < N; i++) h[i] = (float)xr.v[i / E][i % E];
             if (p.post != NORM_NONE) norm(h, p.post, p.post_eps, 0, lds[set][0], lds[set][1]);
@@ -285,19 +290,19 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
 }
 
 #define SOX_BNORM_V(NAME, T, TPR, CH, SUFFIX, VEC, PAR)                                                                    \
-    extern "C" __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) sox_bnorm_##NAME##_t##TPR##c##CH##SUFFIX(sox_bnorm_args p) { \
+    extern "C" __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 256 ? 4 : 1) sox_bnorm_##NAME##_t##TPR##c##CH##SUFFIX(sox_bnorm_args p) { \
         bnorm_body<T, TPR, CH, VEC, PAR>(p);                                                                                \
     }
 #define SOX_BNORM(NAME, T, TPR, CH, PAR) SOX_BNORM_V(NAME, T, TPR, CH, v, true, PAR) SOX_BNORM_V(NAME, T, TPR, CH, s, false, PAR)
-// threads of a row and chunks of a thread: 16-bit rows of up to 256, 512, 1024 columns for many rows, and of up to 2048, 4096,
-// 8192, 16384 for few or long ones ...
+// threads of a row and chunks of a thread: 16-bit rows of up to 256, 512, 1024 columns for many rows, and of up to 2048, 2560,
+// 4096, 8192, 16384 for few or long ones ...
 #define SOX_BNORM_16(NAME, T)                                                                                             \
     SOX_BNORM(NAME, T, 32, 1, PAR_LDS) SOX_BNORM(NAME, T, 64, 1, PAR_LDS) SOX_BNORM(NAME, T, 64, 2, PAR_LDS)              \
-    SOX_BNORM(NAME, T, 256, 1, PAR_REG) SOX_BNORM(NAME, T, 256, 2, PAR_REG) SOX_BNORM(NAME, T, 512, 2, PAR_REG)           \
+    SOX_BNORM(NAME, T, 256, 1, PAR_REG) SOX_BNORM(NAME, T, 320, 1, PAR_REG) SOX_BNORM(NAME, T, 256, 2, PAR_REG) SOX_BNORM(NAME, T, 512, 2, PAR_REG)           \
     SOX_BNORM(NAME, T, 512, 4, PAR_MEM)
 SOX_BNORM_16(f16, half_t)
 SOX_BNORM_16(bf16, bf16_t)
 // ... and the same in fp32, twice the chunks
 SOX_BNORM(f32, float, 32, 2, PAR_LDS) SOX_BNORM(f32, float, 64, 2, PAR_LDS) SOX_BNORM(f32, float, 64, 4, PAR_LDS)
-SOX_BNORM(f32, float, 256, 2, PAR_REG) SOX_BNORM(f32, float, 256, 4, PAR_REG) SOX_BNORM(f32, float, 512, 4, PAR_REG)
+SOX_BNORM(f32, float, 256, 2, PAR_REG) SOX_BNORM(f32, float, 320, 2, PAR_REG) SOX_BNORM(f32, float, 256, 4, PAR_REG) SOX_BNORM(f32, float, 512, 4, PAR_REG)
 SOX_BNORM(f32, float, 512, 8, PAR_MEM)

@@ -87,7 +87,8 @@ KINDS = [("none", "rms"), ("rms", "rms"), ("layer", "layer"), ("none", "layer"),
 @pytest.mark.parametrize("storage", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("rows,c,pad,skip", [(1, 1, 0, 0), (1, 768, 0, 0), (3, 8, 0, 0), (5, 192, 8, 0), (9, 513, 0, 1), (4, 1024, 0, 0),
                                              (6, 1111, 5, 0), (3, 2048, 0, 0), (5, 2056, 16, 0), (2, 4096, 0, 0), (3, 4099, 0, 0),
-                                             (2, 8192, 0, 0), (3, 8200, 0, 0), (2, 16384, 0, 0), (2, 16383, 0, 3)])
+                                             (2, 8192, 0, 0), (3, 8200, 0, 0), (2, 16384, 0, 0), (2, 16383, 0, 3),
+                                             (3, 2304, 0, 0), (4, 2559, 3, 1), (2, 2560, 0, 0), (3, 2561, 7, 0), (3, 2568, 0, 0)])
 def test_sizes(hip, storage, rows, c, pad, skip):
     """Every instance at both ends of its range, vector and scalar."""
     print(f"[gpu] block norm {storage} {rows} x {c}", flush=True)
@@ -114,6 +115,14 @@ def test_more_rows_than_workgroups(hip):
     for rows, c in ((9000, 64), (2500, 1100), (1300, 4104), (700, 8200)):
         print(f"[gpu] block norm {rows} x {c}", flush=True)
         run_case(hip, 60, rows, c, "bf16", params(9, c, "layer", "layer"), gate_rows=rows // 10)
+
+
+@pytest.mark.parametrize("rows,c,pad", [(13001, 192, 0), (13001, 190, 3), (7003, 512, 0), (7003, 391, 0), (5002, 768, 8), (5002, 1023, 0),
+                                        (1207, 2304, 0), (1207, 2450, 1), (1100, 1536, 0)])
+def test_rows_past_one_round(hip, rows, c, pad):
+    """More rows than a launch holds at once, and not a multiple of a workgroup's."""
+    print(f"[gpu] block norm {rows} x {c} + {pad}", flush=True)
+    run_case(hip, rows, rows, c, "f16", params(c, c, "rms", "layer", gate_act="sigmoid"), gate_rows=1, pad=pad)
 
 
 def test_large_means(hip):
