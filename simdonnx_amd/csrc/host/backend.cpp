@@ -491,14 +491,14 @@ void quantize_columns(const float* weights, int inner, int columns, std::vector<
 
 // block_norm.hip's instances: threads of a row, chunks of 8 columns of a thread, workgroups per CU at most; `many`: for many
 // rows, with the parameters in LDS. The workgroups are what a CU holds at once of an instance (one more of 256 threads a row
-// waits for a second round: 16384 x 1536 60.8 us with 5, 45.5 with 4) or what its rows' streams run best with. Rows of
-// 2049 .. 2560 columns leave most of 256 threads' second chunk empty: 16384 x 2560 108 us so, 75 with 320 threads.
+// waits for a second round: 16384 x 1536 60.8 us with 5, 45.5 with 4) or what its rows' streams run best with. Rows that
+// leave much of 256 threads' second chunk empty go to 128 threads with three: 30000 x 2304 132 us, 201 so, 180 with 320 threads.
 struct BnormShape {
     int tpr, ch, per_cu;
     bool many;
 };
 const BnormShape kBnormShapes[] = {{32, 1, 6, true},   {64, 1, 6, true},   {64, 2, 4, true},   {256, 1, 4, false},
-                                   {320, 1, 2, false}, {256, 2, 2, false}, {512, 2, 2, false}, {512, 4, 1, false}};
+                                   {128, 3, 4, false}, {256, 2, 2, false}, {512, 2, 2, false}, {512, 4, 1, false}};
 
 // The first instance that holds c columns; those for many rows only where there are many.
 int bnorm_shape(int c, bool many) {
@@ -520,7 +520,7 @@ struct BnormLaunch {
         const int64_t cus = std::max(1, compute_units);
         shape = bnorm_shape(c, bnorm_many(rows, compute_units));
         const BnormShape& s = kBnormShapes[shape];
-        threads = (uint32_t)std::max(s.tpr, 256);
+        threads = (uint32_t)(s.tpr <= 64 ? 256 : s.tpr);
         const int per_block = (int)threads / s.tpr;
         blocks = (uint32_t)std::min<int64_t>((rows + per_block - 1) / per_block, cus * s.per_cu);
         lds = s.many ? (uint32_t)(vectors * s.tpr * s.ch * 8 * 4) : 0;
