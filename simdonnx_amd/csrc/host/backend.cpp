@@ -350,7 +350,7 @@ struct QPlan {
             way = FEW;
             best = few_us((double)m, n, k);
         }
-        if (floating && inner <= 1024 && panel_us((double)m, n, k, es, cus) < rows_us((double)m, k, es) + best) way = PANEL;
+        if (floating && inner <= 1024 && m <= 1 << 20 && panel_us((double)m, n, k, es, cus) < rows_us((double)m, k, es) + best) way = PANEL;
     }
     bool rounds_itself() const { return way == FEWX || way == PANEL; }
     // workspace: rows [m][pitch], then their scales
@@ -3966,6 +3966,7 @@ struct sox_session {
         current();
         const PlanValue& pv = g->V(v);
         if (pv.buf < 0) fail(SOX_E_INVALID, "value is not an activation");
+        if (g->q8rows.count(v)) fail(SOX_E_INVALID, "value holds 8-bit rows for the products that read it");
         return (uint8_t*)arena + (uint64_t)g->plan.buf_offset[pv.buf] * g->es;
     }
 

@@ -226,7 +226,7 @@ template <typename T, int CH> SOX_DEV void qpanel_body(const sox_qgemm_args& p) 
         AbsMax<T> top;
 #pragma unroll
         for (int c = 0; c < CH; c++) top.add(v[c]);
-            const Q rq = Q::make(AbsMax<T>::row_bits(row16_max(top.lane())));
+        const Q rq = Q::make(AbsMax<T>::row_bits(row16_max(top.lane())));
         if (i16 == 0) xscale[row] = rq.scale;
 #pragma unroll
         for (int c = 0; c < CH; c++) {

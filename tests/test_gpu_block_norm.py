@@ -176,7 +176,7 @@ def test_rows_that_are_not_finite(hip):
     norm.close()
 
 
-@pytest.mark.parametrize("rows,c", [(40, 192), (5, 3000)])
+@pytest.mark.parametrize("rows,c", [(40, 192), (5, 3000), (700, 4200)])
 def test_in_place(hip, rows, c):
     """The residual stream updated where it stands, and the branch's buffer taking y."""
     x, r = values(100, 1, rows, c, "bf16"), values(100, 2, rows, c, "bf16")

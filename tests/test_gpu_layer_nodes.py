@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 from simdonnx_amd.backend import HipBlockNorm, HipInferenceSession, HipQuantLinear, HipUnitRunner
+from simdonnx_amd.native import SoxError
 from simdonnx_amd.plan import PlanBuilder
 from tests.layers import Matrix, linear64, quantize, rounded
 
@@ -109,6 +110,31 @@ def test_block(hip, b, t, c, f, storage, handed, monkeypatch):
             s.set_input(gate, 1)
             got = s.run().reshape(x.shape)
             assert np.array_equal(got, block.by_calls(hip, x, gate, storage, handed))
+
+
+def test_handed_rows_are_not_read_as_elements(hip, monkeypatch):
+    """A session gives out a norm's y, but not where it holds 8-bit rows."""
+    def session():
+        pb = PlanBuilder()
+        x = pb.input((20, 64))
+        h, y = pb.block_norm(residual=x, pre="none")
+        z = pb.quant_linear(y, np.eye(64, dtype=np.float32), residual=h)
+        return HipInferenceSession(hip.graph(pb.build(z), True)), h, y
+
+    x = rounded(rng(1).normal(size=(20, 64)), "f16")
+    for kept in (False, True):
+        if kept:
+            monkeypatch.setenv("SIMDONNX_HIP_NO_QUANT_NORM", "1")
+        s, h, y = session()
+        with s:
+            s.set_input(x, 0)
+            s.run()
+            assert np.array_equal(s.read_value(h).reshape(x.shape), x)
+            if kept:
+                assert np.array_equal(s.read_value(y).reshape(x.shape), x)
+            else:
+                with pytest.raises(SoxError, match="8-bit rows"):
+                    s.read_value(y)
 
 
 def test_odd_block(hip):
