@@ -563,14 +563,13 @@ typedef struct sox_lds_probe_args {
 
 /* Rows to 8 bits (sox_qrows_*): scale[r] = amax / 127, q[r][c] = rint(127 x[r][c] / amax), amax the row's largest
  * magnitude; columns k .. k16 - 1 (k16 = k rounded up to 16) are written as zeros. q rows are ldq bytes apart,
- * a multiple of 16. vec: x rows on 16-byte boundaries. */
+ * a multiple of 16. */
 typedef struct sox_qrows_args {
     const void* x;
     int8_t* q;
     float* scale;
     int64_t ldx, ldq;
     int32_t rows, k;
-    int32_t vec, pad_;
 } sox_qrows_args;
 
 /* Product of 8-bit rows and 8-bit weights (sox_qgemm_*, sox_qfew_*):
@@ -592,8 +591,6 @@ typedef struct sox_qgemm_args {
     int32_t m, n, k, k16;
     int32_t kb, nb;     /* 32-k blocks of a column block, column blocks */
     int32_t tiles_n, act;
-    int32_t vec;        /* bit0: y (and residual) rows on 16-byte boundaries; bit1: x rows too; bit2: y rows on 128-byte lines */
-    int32_t pad_;
 } sox_qgemm_args;
 
 /* Norms before and after a transformer block (sox_bnorm_*): for each row

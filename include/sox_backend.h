@@ -298,7 +298,7 @@ int sox_ctc_argmax_noalloc(sox_ctc* ctc, sox_session* session, int32_t feature_v
  * object may run at once from any threads and on any streams, each with a workspace of its own.
  *
  * Matrices are rows of `storage` elements (SOX_STORAGE_*), ld elements from row to row (>= the row's length), any
- * element alignment (whole 16-byte chunks are faster). rows = 0 does nothing; at most 2^23 rows. Columns past a row's
+ * element alignment (a product's y on 128-byte lines is faster). rows = 0 does nothing; at most 2^23 rows. Columns past a row's
  * length and rows past the last are neither read nor written. Memory of another device, memory no GPU can read
  * and a stream of another device are refused (SOX_E_INVALID), as are outputs that overlap an input or each other,
  * except where said. An offline backend's objects check calls and then return SOX_E_UNSUPPORTED. */

@@ -393,8 +393,8 @@ struct QLaunch {
         l.gx = (uint32_t)((m + per_block - 1) / per_block);
         return l;
     }
-    // vec: sox_qgemm_args.vec
-    static QLaunch product(const QPlan& plan, int inner, int columns, int64_t m, int vec, int compute_units) {
+    // lines: y's rows stand on 128-byte lines
+    static QLaunch product(const QPlan& plan, int inner, int columns, int64_t m, bool lines, int compute_units) {
         QLaunch l;
         l.kind = plan.way;
         const int steps = (inner + 63) / 64;
@@ -420,7 +420,7 @@ struct QLaunch {
             break;
         case QPlan::RING: {
             const QTile& t = *plan.tile;
-            l.index = 2 * (int)(&t - kQTiles) + ((vec & 5) == 5 && columns % 8 == 0);
+            l.index = 2 * (int)(&t - kQTiles) + (lines && columns % 8 == 0);
             l.tiles_n = (columns + t.bn - 1) / t.bn;
             const int64_t tiles = ((m + t.bm - 1) / t.bm) * l.tiles_n;
             if (tiles >= (int64_t)1 << 24) unsupported("8-bit product: too many outputs");
@@ -507,10 +507,10 @@ int bnorm_shape(int c, bool many) {
     unsupported("BlockNorm: channels");
 }
 bool bnorm_many(int64_t rows, int compute_units) { return rows >= 4 * (int64_t)std::max(1, compute_units); }  // a wave on every SIMD
-std::string bnorm_kernel(int32_t storage, int shape, bool vec) {
+std::string bnorm_kernel(int32_t storage, int shape) {
     const BnormShape& s = kBnormShapes[shape];  // (a 16-byte chunk of fp32 is half as many columns)
     return std::string("sox_bnorm_") + kStorageName[storage] + "_t" + std::to_string(s.tpr) + "c" +
-           std::to_string(s.ch * (storage == SOX_STORAGE_F32 ? 2 : 1)) + (vec ? "v" : "s");
+           std::to_string(s.ch * (storage == SOX_STORAGE_F32 ? 2 : 1));
 }
 
 struct BnormLaunch {
@@ -2545,8 +2545,6 @@ struct Emitter {
 
     // ---- 8-bit transformer layers ----
     int32_t storage() const { return g.bf16 ? SOX_STORAGE_BF16 : g.f16 ? SOX_STORAGE_F16 : SOX_STORAGE_F32; }
-    // rows of `width` elements, one behind the other, all on boundaries of `to` bytes (-1: not there)
-    bool rows_on(int v, int width, int to = 16) { return v < 0 || (bind(v).offset % (uint64_t)to == 0 && width * g.es % to == 0); }
     static sox_bind part(sox_bind b, uint64_t at, uint64_t size) { return sox_bind{b.slot, 0, b.offset + at, size}; }
 
     void quant_linear(int ni, const PlanNode& n) {
@@ -2580,7 +2578,6 @@ struct Emitter {
             r.ldq = QPlan::pitch(q.inner);
             r.rows = (int32_t)q.rows;
             r.k = q.inner;
-            r.vec = rows_on(q.x, q.inner);
             const QLaunch l = QLaunch::rows(q.inner, q.rows, es);
             add(ni, QLaunch::kernel(l.kind, l.index, storage()), r,
                 {{offsetof(sox_qrows_args, x), bind(q.x)}, {offsetof(sox_qrows_args, q), part(ws, 0, bytes)},
@@ -2593,9 +2590,8 @@ struct Emitter {
         a.ldx = q.inner;
         a.ldr = a.ldy = q.columns;
         a.act = q.p.act;
-        a.vec = (rows_on(q.y, q.columns) && rows_on(q.residual, q.columns) ? 1 : 0) | (rows_on(q.x, q.inner) ? 2 : 0) |
-                (rows_on(q.y, q.columns, 128) ? 4 : 0);
-        const QLaunch l = QLaunch::product(plan, q.inner, q.columns, q.rows, a.vec, cus);
+        const bool lines = bind(q.y).offset % 128 == 0 && q.columns * es % 128 == 0;
+        const QLaunch l = QLaunch::product(plan, q.inner, q.columns, q.rows, lines, cus);
         a.m = (int32_t)q.rows;
         a.n = q.columns;
         a.k = q.inner;
@@ -2638,9 +2634,8 @@ struct Emitter {
         a.post_eps = b.p.norm.post_eps;
         a.pre_eps = b.p.norm.pre_eps;
         a.res_scale = b.p.norm.res_scale;
-        const bool vec = rows_on(b.residual, C) && rows_on(b.x, C) && rows_on(b.gate, C) && rows_on(b.h, C) && rows_on(b.y, C);
         const BnormLaunch l(C, b.rows, vectors.count, g.be->info.compute_units);
-        add(ni, bnorm_kernel(storage(), l.shape, vec), a, ptrs, l.blocks, 1, 1, l.threads, l.lds, "block_norm");
+        add(ni, bnorm_kernel(storage(), l.shape), a, ptrs, l.blocks, 1, 1, l.threads, l.lds, "block_norm");
     }
 
     // ---- built-in extension ops (Engine/Fusions/*.cs EmitVulkan twins) ----
@@ -5292,8 +5287,8 @@ struct LayerCall {
     Rows matrix(const char* what, const void* p, int64_t ld, int64_t cols, bool optional = false) const {
         return matrix(what, p, ld, cols, es, es, optional, rows);
     }
-    // every row on boundaries of 16 bytes, or `to`
-    static bool on(const Rows& r, uint64_t to = 16) { return !r.any() || (r.at % to == 0 && (r.pitch % (int64_t)to == 0 || r.rows == 1)); }
+    // every row on a line of 128 bytes
+    static bool lines(const Rows& r) { return r.at % 128 == 0 && (r.pitch % 128 == 0 || r.rows == 1); }
 
     LayerCall(sox_backend* b, const char* n, int32_t nrows, int32_t storage) : be(b), name(n), rows(nrows) {
         if (nrows < 0) bad("rows");
@@ -5389,8 +5384,8 @@ std::unique_ptr<sox_qlinear> qlinear_new(sox_backend* be, int inner, int columns
 }
 
 // The product, over 8-bit rows (a.a, a.xs) or where the plan rounds them itself over floating ones (a.x).
-void qlinear_product(const LayerCall& c, sox_qlinear* L, const QPlan& plan, void* stream, sox_qgemm_args& a, int32_t storage) {
-    const QLaunch l = QLaunch::product(plan, L->inner, L->columns, c.rows, a.vec, c.be->info.compute_units);
+void qlinear_product(const LayerCall& c, sox_qlinear* L, const QPlan& plan, void* stream, sox_qgemm_args& a, int32_t storage, bool lines) {
+    const QLaunch l = QLaunch::product(plan, L->inner, L->columns, c.rows, lines, c.be->info.compute_units);
     a.w = (const int8_t*)L->mem.p;
     a.ws = (const float*)((const uint8_t*)L->mem.p + L->scales_at);
     a.bias = a.ws + L->npad;
@@ -5413,7 +5408,7 @@ struct sox_block_norm {
     DeviceBlock mem;  // BnormVectors
     int cpad = 0, vectors = 0;
     bool has[4] = {};
-    void* fn[3][2][2];  // storage, many rows, vector
+    void* fn[3][2];  // storage, many rows
 };
 
 namespace {
@@ -5455,9 +5450,8 @@ void bnorm_run(sox_block_norm* N, const char* name, void* stream, int32_t storag
     a.rows = rows; a.c = C; a.gate_group = gate ? rows / gate_rows : 1;
     a.post = N->p.post; a.pre = N->p.pre; a.gate_act = N->p.gate_act;
     a.post_eps = N->p.post_eps; a.pre_eps = N->p.pre_eps; a.res_scale = N->p.res_scale;
-    const bool vec = c.on(R) && c.on(X) && c.on(G) && c.on(H) && (quantized || c.on(Y));
     const BnormLaunch l(C, rows, N->vectors, c.be->info.compute_units);
-    c.launch(N->fn[storage][bnorm_many(rows, c.be->info.compute_units)][vec], l.blocks, 1, l.threads, stream, a, l.lds);
+    c.launch(N->fn[storage][bnorm_many(rows, c.be->info.compute_units)], l.blocks, 1, l.threads, stream, a, l.lds);
 }
 
 }  // namespace
@@ -5529,7 +5523,6 @@ int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x
         a.y = y;
         a.ldy = ldy;
         a.act = act;
-        a.vec = (c.on(Y) && c.on(R) ? 1 : 0) | (c.on(X) ? 2 : 0) | (c.on(Y, 128) ? 4 : 0);
         if (!plan.rounds_itself()) {
             sox_qrows_args q{};
             q.x = x;
@@ -5539,14 +5532,13 @@ int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x
             q.scale = (float*)((uint8_t*)workspace + QPlan::rows_bytes(L->inner, rows));
             q.rows = rows;
             q.k = L->inner;
-            q.vec = c.on(X);
             const QLaunch l = QLaunch::rows(L->inner, rows, (int)c.es);
             c.launch(L->fn(l, storage), l.gx, 1, l.threads, stream, q);
             a.a = q.q;
             a.lda = q.ldq;
             a.xs = q.scale;
         }
-        qlinear_product(c, L, plan, stream, a, storage);
+        qlinear_product(c, L, plan, stream, a, storage, c.lines(Y));
     });
 }
 
@@ -5571,8 +5563,7 @@ int sox_qlinear_run_quantized(sox_qlinear* L, void* stream, const int8_t* q, int
         a.y = y;
         a.ldy = ldy;
         a.act = act;
-        a.vec = (c.on(Y) && c.on(R) ? 1 : 0) | (c.on(Y, 128) ? 4 : 0);
-        qlinear_product(c, L, L->plan(rows, storage, false), stream, a, storage);
+        qlinear_product(c, L, L->plan(rows, storage, false), stream, a, storage, c.lines(Y));
     });
 }
 
@@ -5590,7 +5581,7 @@ int sox_block_norm_create(sox_backend* be, const sox_block_norm_p* p, const floa
         N->mem.upload(be, vectors.v.data(), vectors.v.size() * 4, "BlockNorm parameters");
         for (int32_t s = 0; s < 3; s++)
             for (int many = 0; many < 2; many++)
-                for (int vec = 0; vec < 2; vec++) N->fn[s][many][vec] = be->fn(bnorm_kernel(s, bnorm_shape(p->channels, many), vec));
+                N->fn[s][many] = be->fn(bnorm_kernel(s, bnorm_shape(p->channels, many)));
         *out = N.release();
     });
 }

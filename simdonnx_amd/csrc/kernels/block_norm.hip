@@ -20,53 +20,42 @@
 enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
 enum { PAR_LDS, PAR_REG, PAR_MEM };  // where the parameter vectors are
 
-// CH chunks of E values per thread; VEC: chunk j of thread t is columns (j TPR + t) E .. + E - 1 as one 16-byte access
-// (rows on 16-byte boundaries), else value e of it is column (j E + e) TPR + t on its own
-template <typename T, int TPR, int CH, bool VEC> struct Row {
+// CH chunks of E values per thread: chunk j of thread t is columns (j TPR + t) E .. + E - 1 as one 16-byte access
+template <typename T, int TPR, int CH> struct Row {
     static constexpr int E = 16 / sizeof(T), N = CH * E;
-    typedef vec_t<T, E> TE;
+    typedef typename Chunk16<T>::V TE;
+    typedef typename Chunk16<T>::At At;
     TE v[CH];
-    SOX_DEV int col(int t, int j, int e) { return VEC ? (j * TPR + t) * E + e : (j * E + e) * TPR + t; }
+    SOX_DEV int col(int t, int j) { return (j * TPR + t) * E; }
     // value e of chunk j is inside the row (a compare with a constant: the columns themselves would be held in registers)
-    SOX_DEV bool in(int t, int j, int e, int c) { return VEC ? e < c - col(t, j, 0) : (j * E + e) * TPR < c - t; }
+    SOX_DEV bool in(int t, int j, int e, int c) { return e < c - col(t, j); }
     __device__ __forceinline__ void load(const T* __restrict__ p, int t, int c) {
 #pragma unroll
         for (int j = 0; j < CH; j++) {
-            if constexpr (VEC) {
-                const int k = col(t, j, 0);
-                v[j] = TE{};
-                if (k + E <= c) {
-                    v[j] = *(const TE*)(p + k);
-                } else if (k < c) {  // the row's end inside a chunk
+            const int k = col(t, j);
+            v[j] = TE{};
+            if (k + E <= c) {
+                v[j] = *(const At*)(p + k);
+            } else if (k < c) {  // the row's end inside a chunk
 #pragma unroll
-                    for (int e = 0; e < E; e++)
-                        if (in(t, j, e, c)) v[j][e] = p[k + e];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e++) v[j][e] = in(t, j, e, c) ? p[col(t, j, e)] : (T)0.0f;
+                for (int e = 0; e < E; e++)
+                    if (in(t, j, e, c)) v[j][e] = p[k + e];
             }
         }
     }
     SOX_DEV void store(T* __restrict__ p, int t, int c, const float (&f)[N]) {
 #pragma unroll
         for (int j = 0; j < CH; j++) {
-            if constexpr (VEC) {
-                TE o;
+            TE o;
 #pragma unroll
-                for (int e = 0; e < E; e++) o[e] = (T)f[j * E + e];
-                const int k = col(t, j, 0);
-                if (k + E <= c) {
-                    *(TE*)(p + k) = o;
-                } else if (k < c) {
-#pragma unroll
-                    for (int e = 0; e < E; e++)
-                        if (in(t, j, e, c)) p[k + e] = o[e];
-                }
-            } else {
+            for (int e = 0; e < E; e++) o[e] = (T)f[j * E + e];
+            const int k = col(t, j);
+            if (k + E <= c) {
+                *(At*)(p + k) = o;
+            } else if (k < c) {
 #pragma unroll
                 for (int e = 0; e < E; e++)
-                    if (in(t, j, e, c)) p[col(t, j, e)] = (T)f[j * E + e];
+                    if (in(t, j, e, c)) p[k + e] = o[e];
             }
         }
     }
@@ -75,23 +64,17 @@ template <typename T, int TPR, int CH, bool VEC> struct Row {
         const int c16 = (c + 15) & ~15;
 #pragma unroll
         for (int j = 0; j < CH; j++) {
-            if constexpr (VEC) {
-                uint32_t w[E / 4];
+            uint32_t w[E / 4];
 #pragma unroll
-                for (int i = 0; i < E / 4; i++) {
-                    const float* g = &f[j * E + 4 * i];
-                    w[i] = RowQuant<half_t>::q4(g[0], g[1], g[2], g[3], rq);
-                }
-                if (col(t, j, 0) < c16) {
-                    if constexpr (E == 8)
-                        *(uint2*)(p + col(t, j, 0)) = make_uint2(w[0], w[1]);
-                    else
-                        *(uint32_t*)(p + col(t, j, 0)) = w[0];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (in(t, j, e, c16)) p[col(t, j, e)] = RowQuant<half_t>::q(f[j * E + e], rq);
+            for (int i = 0; i < E / 4; i++) {
+                const float* g = &f[j * E + 4 * i];
+                w[i] = RowQuant<half_t>::q4(g[0], g[1], g[2], g[3], rq);
+            }
+            if (col(t, j) < c16) {
+                if constexpr (E == 8)
+                    *(uint2*)(p + col(t, j)) = make_uint2(w[0], w[1]);
+                else
+                    *(uint32_t*)(p + col(t, j)) = w[0];
             }
         }
     }
@@ -118,8 +101,8 @@ template <int TPR> SOX_DEV uint32_t row_max(uint32_t v, uint32_t* lds) {
     return row_fold<TPR>(wave_max<TPR == 32 ? 32 : 64>(v), lds, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
-template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_body(const sox_bnorm_args& p) {
-    typedef Row<T, TPR, CH, VEC> R;
+template <typename T, int TPR, int CH, int PAR> SOX_DEV void bnorm_body(const sox_bnorm_args& p) {
+    typedef Row<T, TPR, CH> R;
     constexpr int E = R::E, N = R::N, BLOCK = TPR <= 64 ? 256 : TPR, RPB = BLOCK / TPR, CAP = TPR * N;
     static_assert((PAR == PAR_LDS) == (TPR <= 64), "a wave or half of one per row");
     __shared__ float lds[2][5][BLOCK / 64];
@@ -132,18 +115,13 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
     int slot[4];
     float kept[PAR == PAR_REG ? 4 : 1][PAR == PAR_REG ? N : 1];
     auto from_memory = [&](const float* v, int j, float (&o)[E]) __attribute__((always_inline)) {
-        if constexpr (VEC) {
-            const bool in = R::col(t, j, 0) < c;
+        const bool in = R::col(t, j) < c;
 #pragma unroll
-            for (int i = 0; i < E / 4; i++) {
-                float4v f = {};
-                if (in) f = *(const float4v*)(v + R::col(t, j, 4 * i));
+        for (int i = 0; i < E / 4; i++) {
+            float4v f = {};
+            if (in) f = *(const float4v*)(v + R::col(t, j) + 4 * i);
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[4 * i + e] = f[e];
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; e++) o[e] = R::in(t, j, e, c) ? v[R::col(t, j, e)] : 0.0f;
+            for (int e = 0; e < 4; e++) o[4 * i + e] = f[e];
         }
     };
     if constexpr (PAR == PAR_REG) {
@@ -159,8 +137,8 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
                 }
     }
     if constexpr (PAR == PAR_LDS) {
-        // VEC: the chunks' first four values of all chunks, then their second four, so 16-byte reads of consecutive lanes
-        // are consecutive
+        // The chunks' first four values of all chunks, then their second four, so 16-byte reads of consecutive lanes are
+        // consecutive
         int n = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -168,7 +146,7 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
             if (!vec[k]) continue;
             n++;
             for (int i = threadIdx.x; i < CAP; i += BLOCK) {
-                const int at = VEC ? i % E / 4 * (CAP / (E / 4)) + i / E * 4 + i % 4 : i;
+                const int at = i % E / 4 * (CAP / (E / 4)) + i / E * 4 + i % 4;
                 par_lds[slot[k] + at] = i < c ? vec[k][i] : 0.0f;
             }
         }
@@ -179,16 +157,13 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
         if constexpr (PAR == PAR_REG) {
 #pragma unroll
             for (int e = 0; e < E; e++) o[e] = kept[k][j * E + e];
-        } else if constexpr (PAR == PAR_LDS && VEC) {
+        } else if constexpr (PAR == PAR_LDS) {
 #pragma unroll
             for (int i = 0; i < E / 4; i++) {
                 const float4v f = *(const float4v*)(par_lds + slot[k] + i * (CAP / (E / 4)) + (j * TPR + t) * 4);
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[4 * i + e] = f[e];
             }
-        } else if constexpr (PAR == PAR_LDS) {
-#pragma unroll
-            for (int e = 0; e < E; e++) o[e] = par_lds[slot[k] + R::col(t, j, e)];
         } else {
             const float* v = vec[k];
             asm volatile("" : "+s"(v));  // (read here, not ahead of the rows into registers that are not there)
@@ -240,7 +215,7 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
     // Where a workgroup fills a CU (512 threads a row), the next row's values come while the row before is worked on; smaller
     // ones have each other's loads for that, and fewer registers: 4096 x 8192 bf16 55 us, 64 without; 40000 x 192 19.4, 14.8
     // without.
-    constexpr bool AHEAD = TPR == 512 && PAR == PAR_REG && VEC;
+    constexpr bool AHEAD = TPR == 512 && PAR == PAR_REG;
     struct Rows {
         R x, r, g;
     };
@@ -323,11 +298,11 @@ template <typename T, int TPR, int CH, bool VEC, int PAR> SOX_DEV void bnorm_bod
     }
 }
 
-#define SOX_BNORM_V(NAME, T, TPR, CH, SUFFIX, VEC, PAR)                                                                    \
-    extern "C" __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR <= 64 ? 4 : TPR == 128 ? 2 : 1) sox_bnorm_##NAME##_t##TPR##c##CH##SUFFIX(sox_bnorm_args p) { \
-        bnorm_body<T, TPR, CH, VEC, PAR>(p);                                                                                \
+#define SOX_BNORM(NAME, T, TPR, CH, PAR)                                                                                   \
+    extern "C" __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR <= 64 ? 4 : TPR == 128 ? 2 : 1)                \
+        sox_bnorm_##NAME##_t##TPR##c##CH(sox_bnorm_args p) {                                                               \
+        bnorm_body<T, TPR, CH, PAR>(p);                                                                                    \
     }
-#define SOX_BNORM(NAME, T, TPR, CH, PAR) SOX_BNORM_V(NAME, T, TPR, CH, v, true, PAR) SOX_BNORM_V(NAME, T, TPR, CH, s, false, PAR)
 // threads of a row and chunks of a thread: 16-bit rows of up to 256, 512, 1024 columns for many rows, and of up to 2048, one
 // and a half times that, 4096, 8192, 16384 for few or long ones ...
 #define SOX_BNORM_16(NAME, T)                                                                                             \

@@ -56,64 +56,46 @@ template <typename T> SOX_DEV int stage_at(int r, int c) {
     return sizeof(T) == 2 ? r * 64 + ((c ^ ((r >> 2) & 3)) << 4) : r * 128 + ((c ^ (r >> 1)) << 4);
 }
 
-// What a kernel knows of the rows of its outputs and residual:
-//   Q_LINES  rows of y on 128-byte lines, of the residual on 16-byte boundaries, whole 16-byte chunks in both. The stores pass
-//            L2 by, which leaves it to the A and W lines that are read again: 4096 x 4096 -> 8192 124 us, 133 with stores
-//            through L2, 128 with the choice made in the kernel
-//   Q_CHUNKS whole chunks where the rows stand on 16-byte boundaries. Their stores go through L2: a line that different stores
-//            write in parts would reach memory in parts, 2954 x 320 -> 3112 19.8 us so and 13.3 through L2
+// What a kernel knows of its outputs' rows:
+//   Q_LINES  they stand on 128-byte lines and hold whole 16-byte chunks. Their stores pass L2 by, which leaves it to the A and W
+//            lines that are read again: 4096 x 4096 -> 8192 124 us, 133 with stores through L2, 128 with the choice made in
+//            the kernel
+//   Q_CHUNKS they hold whole chunks. Their stores go through L2: a line that different stores write in parts would reach memory
+//            in parts, 2954 x 320 -> 3112 19.8 us so and 13.3 through L2
 //   Q_PART   any
 enum { Q_LINES, Q_CHUNKS, Q_PART };
 
-// A block's rows between memory at (m0, n0) and the stage: 16-byte chunks where the rows stand on 16-byte boundaries (uniform;
-// single elements in the chunk that a row ends in), else single elements, a half wave per row, in a loop that is not
-// unrolled (the ragged form should not be most of the code).
+// A block's rows between memory at (m0, n0) and the stage, 16 bytes at a time, single elements in the chunk that a row ends in.
 // LOAD: the residual's into the stage (zeros outside), else the stage's to the output.
 template <typename T, bool LOAD, int FORM>
-SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, bool vec, unsigned char* stg, int m0, int n0, int lane) {
+SOX_DEV void move_rows(T* __restrict__ base, int64_t ld, int M, int N, unsigned char* stg, int m0, int n0, int lane) {
     constexpr int E = 16 / sizeof(T), PER = 32 / E, ROWS = STG_BYTES / (32 * sizeof(T));  // elements of a chunk, chunks of a row
-    typedef vec_t<T, E> TE;
-    if (FORM == Q_LINES || vec) {
+    typedef typename Chunk16<T>::V TE;
+    typedef typename Chunk16<T>::At At;
 #pragma unroll
-        for (int t = 0; t < ROWS * PER / 64; t++) {
-            const int idx = t * 64 + lane, r = idx / PER, u = idx % PER, m = m0 + r, n = n0 + u * E;
-            TE* s = (TE*)(stg + stage_at<T>(r, u));
-            T* g = base + (int64_t)m * ld + n;
-            if constexpr (LOAD) {
-                TE v = {};
-                if (m < M && n + E <= N) {
-                    v = *(const TE*)g;
-                }
-                *s = v;
-                if (FORM == Q_PART && m < M && n < N && n + E > N)
-#pragma unroll 1
-                    for (int e = 0; e < N - n; e++) ((T*)s)[e] = g[e];
-            } else {
-                const TE v = *s;
-                if (m < M && n + E <= N) {
-                    if constexpr (FORM == Q_LINES)
-                        __builtin_nontemporal_store(v, (TE*)g);
-                    else
-                        *(TE*)g = v;
-                } else if (FORM == Q_PART && m < M && n < N) {
-#pragma unroll 1
-                    for (int e = 0; e < N - n; e++) g[e] = ((const T*)s)[e];
-                }
+    for (int t = 0; t < ROWS * PER / 64; t++) {
+        const int idx = t * 64 + lane, r = idx / PER, u = idx % PER, m = m0 + r, n = n0 + u * E;
+        TE* s = (TE*)(stg + stage_at<T>(r, u));
+        T* g = base + (int64_t)m * ld + n;
+        if constexpr (LOAD) {
+            TE v = {};
+            if (m < M && n + E <= N) {
+                v = *(const At*)g;
             }
-        }
-    } else {
+            *s = v;
+            if (FORM == Q_PART && m < M && n < N && n + E > N)
 #pragma unroll 1
-        for (int t = 0; t < ROWS / 2; t++) {
-            const int idx = t * 64 + lane, r = idx / 32, c = idx % 32, m = m0 + r, n = n0 + c;
-            T* s = (T*)(stg + stage_at<T>(r, c / E) + c % E * sizeof(T));
-            T* g = base + (int64_t)m * ld + n;
-            if constexpr (LOAD) {
-                T v = (T)0.0f;
-                if (m < M && n < N) v = *g;
-                *s = v;
-            } else {
-                const T v = *s;
-                if (m < M && n < N) *g = v;
+                for (int e = 0; e < N - n; e++) ((T*)s)[e] = g[e];
+        } else {
+            const TE v = *s;
+            if (m < M && n + E <= N) {
+                if constexpr (FORM == Q_LINES)
+                    __builtin_nontemporal_store(v, (TE*)g);
+                else
+                    *(At*)g = v;
+            } else if (FORM == Q_PART && m < M && n < N) {
+#pragma unroll 1
+                for (int e = 0; e < N - n; e++) g[e] = ((const T*)s)[e];
             }
         }
     }
@@ -135,7 +117,6 @@ SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs,
     constexpr int PARTS = sizeof(T) == 2 ? 1 : 2, ROWS = 32 / PARTS;
     typedef vec_t<T, 4> T4;
     const int l32 = lane & 31, hl = lane >> 5;
-    const bool vec = p.vec & 1;
     float val[16];
 #pragma unroll
     for (int q = 0; q < 4; q++) {
@@ -150,7 +131,7 @@ SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs,
     if (p.add) {
 #pragma unroll
         for (int half = 0; half < PARTS; half++) {
-            move_rows<T, true, FORM>((T*)p.add, p.ldr, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
+            move_rows<T, true, FORM>((T*)p.add, p.ldr, p.m, p.n, stg, m0 + half * ROWS, n0, lane);
             stage_turn();
             if (PARTS == 1 || l32 / ROWS == half) {
 #pragma unroll
@@ -185,7 +166,7 @@ SOX_DEV void finish_block(const sox_qgemm_args& p, const int16v& sums, float xs,
             }
         }
         stage_turn();
-        move_rows<T, false, FORM>((T*)p.y, p.ldy, p.m, p.n, vec, stg, m0 + half * ROWS, n0, lane);
+        move_rows<T, false, FORM>((T*)p.y, p.ldy, p.m, p.n, stg, m0 + half * ROWS, n0, lane);
         stage_turn();
     }
 }

@@ -21,13 +21,13 @@ template <typename T, int TPR> SOX_DEV void qrows_body(const sox_qrows_args& p) 
     AbsMax<T> top;
 #pragma unroll
     for (int j = 0; j < CH; j++)
-        if (t + j * TPR < chunks) v[j].load(x, (t + j * TPR) * E, p.k, p.vec);
+        if (t + j * TPR < chunks) v[j].load(x, (t + j * TPR) * E, p.k);
 #pragma unroll
     for (int j = 0; j < CH; j++)
         if (t + j * TPR < chunks) top.add(v[j]);
     for (int c = t + CH * TPR; c < chunks; c += TPR) {
         Chunk u;
-        u.load(x, c * E, p.k, p.vec);
+        u.load(x, c * E, p.k);
         top.add(u);
     }
     uint32_t m = wave_max<TPR == 32 ? 32 : 64>(top.lane());
@@ -48,7 +48,7 @@ template <typename T, int TPR> SOX_DEV void qrows_body(const sox_qrows_args& p) 
         if (t + j * TPR < chunks) put(t + j * TPR, v[j]);
     for (int c = t + CH * TPR; c < chunks; c += TPR) {
         Chunk u;
-        u.load(x, c * E, p.k, p.vec);
+        u.load(x, c * E, p.k);
         put(c, u);
     }
     if (t == 0) p.scale[row] = rq.scale;
@@ -144,7 +144,7 @@ template <typename T, int S> SOX_DEV void qfewx_body(const sox_qgemm_args& p) {
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
         const int it = wave + i * waves, row = it / segs;
-        if (it < items) v[i].load((const T*)p.x + row * p.ldx, ((it - row * segs) * 64 + lane) * 16, p.k, p.vec & 2);
+        if (it < items) v[i].load((const T*)p.x + row * p.ldx, ((it - row * segs) * 64 + lane) * 16, p.k);
     }
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
@@ -222,7 +222,7 @@ template <typename T, int CH> SOX_DEV void qpanel_body(const sox_qgemm_args& p) 
         const T* x = (const T*)p.x + (int64_t)min(m0 + row, p.m - 1) * p.ldx;
         RawValues<T, 16> v[CH];
 #pragma unroll
-        for (int c = 0; c < CH; c++) v[c].load(x, (c * 16 + i16) * 16, p.k, p.vec & 2);
+        for (int c = 0; c < CH; c++) v[c].load(x, (c * 16 + i16) * 16, p.k);
         AbsMax<T> top;
 #pragma unroll
         for (int c = 0; c < CH; c++) top.add(v[c]);

@@ -90,7 +90,7 @@ KINDS = [("none", "rms"), ("rms", "rms"), ("layer", "layer"), ("none", "layer"),
                                              (2, 8192, 0, 0), (3, 8200, 0, 0), (2, 16384, 0, 0), (2, 16383, 0, 3),
                                              (3, 2304, 0, 0), (4, 2559, 3, 1), (2, 2560, 0, 0), (3, 2561, 7, 0), (3, 2568, 0, 0)])
 def test_sizes(hip, storage, rows, c, pad, skip):
-    """Every instance at both ends of its range, vector and scalar."""
+    """Every instance at both ends of its range, on 16-byte boundaries and off them."""
     print(f"[gpu] block norm {storage} {rows} x {c}", flush=True)
     kinds = KINDS[c % len(KINDS)]
     run_case(hip, c, rows, c, storage, params(c, c, *kinds, res_scale=0.75), gate_rows=rows, pad=pad, skip=skip)
