@@ -492,13 +492,14 @@ void quantize_columns(const float* weights, int inner, int columns, std::vector<
 // block_norm.hip's instances: threads of a row, chunks of 8 columns of a thread, workgroups per CU at most; `many`: for many
 // rows, with the parameters in LDS. The workgroups are what a CU holds at once of an instance (one more of 256 threads a row
 // waits for a second round: 16384 x 1536 60.8 us with 5, 45.5 with 4) or what its rows' streams run best with. Rows that
-// leave much of 256 threads' second chunk empty go to 128 threads with three: 30000 x 2304 132 us, 201 so, 180 with 320 threads.
+// leave much of 256 threads' second chunk empty go to 128 threads with three: 30000 x 2304 132 us, 201 so, 180 with 320 threads. Above 4096 columns likewise: 8192 x 5120 bf16 78 us
+// with three chunks of 256 threads, two workgroups to a CU; 120 with two of 512, of which it holds one.
 struct BnormShape {
     int tpr, ch, per_cu;
     bool many;
 };
 const BnormShape kBnormShapes[] = {{32, 1, 6, true},   {64, 1, 6, true},   {64, 2, 4, true},   {256, 1, 4, false},
-                                   {128, 3, 4, false}, {256, 2, 2, false}, {512, 2, 2, false}, {512, 4, 1, false}};
+                                   {128, 3, 4, false}, {256, 2, 2, false}, {256, 3, 2, false}, {512, 2, 2, false}, {512, 4, 1, false}};
 
 // The first instance that holds c columns; those for many rows only where there are many.
 int bnorm_shape(int c, bool many) {

@@ -209,9 +209,9 @@ template <typename T, int TPR, int CH, int PAR> SOX_DEV void bnorm_body(const so
             }
     };
     int set = 0;
-    // (a wave's row is one number: its addresses stay in scalar registers. With 256 threads a row it fits as it is, and lanes'
-    // own addresses are faster: 16384 x 4096 95.9 us, 99.5 with scalar ones)
-    const int sub = TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : BLOCK == TPR && TPR != 256 ? 0 : threadIdx.x / TPR;
+    // (a wave's row is one number: its addresses stay in scalar registers. With 256 threads and up to two chunks it fits as it
+    // is, and lanes' own addresses are faster: 16384 x 4096 95.9 us, 99.5 with scalar ones)
+    const int sub = TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : BLOCK == TPR && (TPR != 256 || N > 16) ? 0 : threadIdx.x / TPR;
     // Where a workgroup fills a CU (512 threads a row), the next row's values come while the row before is worked on; smaller
     // ones have each other's loads for that, and fewer registers: 4096 x 8192 bf16 55 us, 64 without; 40000 x 192 19.4, 14.8
     // without.
@@ -299,19 +299,19 @@ template <typename T, int TPR, int CH, int PAR> SOX_DEV void bnorm_body(const so
 }
 
 #define SOX_BNORM(NAME, T, TPR, CH, PAR)                                                                                   \
-    extern "C" __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR <= 64 ? 4 : TPR == 128 ? 2 : 1)                \
+    extern "C" __global__ void __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR <= 64 ? 4 : TPR <= 256 ? 2 : 1)                \
         sox_bnorm_##NAME##_t##TPR##c##CH(sox_bnorm_args p) {                                                               \
         bnorm_body<T, TPR, CH, PAR>(p);                                                                                    \
     }
-// threads of a row and chunks of a thread: 16-bit rows of up to 256, 512, 1024 columns for many rows, and of up to 2048, one
-// and a half times that, 4096, 8192, 16384 for few or long ones ...
+// threads of a row and chunks of a thread: 16-bit rows of up to 256, 512, 1024 columns for many rows, and of up to 2048, 4096,
+// 8192, 16384 and one and a half times 2048 and 4096 for few or long ones ...
 #define SOX_BNORM_16(NAME, T)                                                                                             \
     SOX_BNORM(NAME, T, 32, 1, PAR_LDS) SOX_BNORM(NAME, T, 64, 1, PAR_LDS) SOX_BNORM(NAME, T, 64, 2, PAR_LDS)              \
-    SOX_BNORM(NAME, T, 256, 1, PAR_REG) SOX_BNORM(NAME, T, 128, 3, PAR_REG) SOX_BNORM(NAME, T, 256, 2, PAR_REG) SOX_BNORM(NAME, T, 512, 2, PAR_REG)           \
+    SOX_BNORM(NAME, T, 256, 1, PAR_REG) SOX_BNORM(NAME, T, 128, 3, PAR_REG) SOX_BNORM(NAME, T, 256, 2, PAR_REG) SOX_BNORM(NAME, T, 256, 3, PAR_REG) SOX_BNORM(NAME, T, 512, 2, PAR_REG)           \
     SOX_BNORM(NAME, T, 512, 4, PAR_MEM)
 SOX_BNORM_16(f16, half_t)
 SOX_BNORM_16(bf16, bf16_t)
 // ... and the same in fp32, twice the chunks
 SOX_BNORM(f32, float, 32, 2, PAR_LDS) SOX_BNORM(f32, float, 64, 2, PAR_LDS) SOX_BNORM(f32, float, 64, 4, PAR_LDS)
-SOX_BNORM(f32, float, 256, 2, PAR_REG) SOX_BNORM(f32, float, 128, 6, PAR_REG) SOX_BNORM(f32, float, 256, 4, PAR_REG) SOX_BNORM(f32, float, 512, 4, PAR_REG)
+SOX_BNORM(f32, float, 256, 2, PAR_REG) SOX_BNORM(f32, float, 128, 6, PAR_REG) SOX_BNORM(f32, float, 256, 4, PAR_REG) SOX_BNORM(f32, float, 256, 6, PAR_REG) SOX_BNORM(f32, float, 512, 4, PAR_REG)
 SOX_BNORM(f32, float, 512, 8, PAR_MEM)
