@@ -112,6 +112,22 @@ def test_block(hip, b, t, c, f, storage, handed, monkeypatch):
             assert np.array_equal(got, block.by_calls(hip, x, gate, storage, handed))
 
 
+@pytest.mark.parametrize("b,t,c,f", [(2, 8, 4096, 64), (1, 30, 192, 384), (2, 300, 768, 520)])
+def test_replayed_session(hip, b, t, c, f):
+    """The captured list of dispatches gives each run's own results: tokens whose rows fill the LDS, panels, the ring."""
+    print(f"[gpu] replay {b}x{t}x{c} {f}", flush=True)
+    block = Block(b * t, b, t, c, f)
+    with HipInferenceSession(hip.graph(block.plan(), True)) as s, HipInferenceSession(hip.graph(block.plan(), True)) as eager:
+        s.set_replay(True)
+        for seed in range(4):
+            outs = []
+            for sess in (s, eager):
+                for i, v in enumerate(block.inputs(seed, "f16")):
+                    sess.set_input(v, i)
+                outs.append(sess.run().copy())
+            assert np.array_equal(*outs)
+
+
 def test_handed_rows_are_not_read_as_elements(hip, monkeypatch):
     """A session gives out a norm's y, but not where it holds 8-bit rows."""
     def session():
