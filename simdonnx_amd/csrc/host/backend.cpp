@@ -3591,6 +3591,20 @@ bool conv_pads_channels(const sox_graph& g, const PlanNode& n) {
     return pads_rows(g, (int64_t)xs[0] * a.ih * a.iw, ic, oc, taps);
 }
 
+// Reads of value v's buffer by any node, those folded into others too (the kernel that runs a folded node may still read its
+// operands: a fused MLP its Add's residual, or its projection's), plus the plan output when it lives there.
+int operand_reads(const sox_graph& g, int v) {
+    const auto& P = g.plan;
+    const int buf = P.values[v].buf;
+    auto here = [&](int x) { return x >= 0 && g.V(x).buf == buf; };
+    int u = here(P.output);
+    for (const PlanNode& n : P.nodes) {
+        for (int x : n.in) u += here(x);
+        if (n.op == SOX_OP_CONV) u += here(n.p<sox_conv_p>().add_value) + here(n.p<sox_conv_p>().bias_value);
+    }
+    return u;
+}
+
 // The nodes of the 8-bit layers. A BlockNorm's parameters become one const. An output that the plan put over an operand gets
 // a buffer of its own (workgroups write it while others still read). A BlockNorm whose y only QuantLinears read hands
 // them 8-bit rows, rounded once and from fp32, in y's own buffer: channels bytes a row and 4 for its scale fit where
@@ -3631,7 +3645,7 @@ void plan_layers8(sox_graph& g) {
                 const QuantLinearNode q(g, P.nodes[k]);
                 reads += q.x == b.y && q.residual != b.y;
             }
-        if (shared == 1 && reads > 0 && buffer_reads(g, b.y, -1) == reads) g.q8rows.insert(b.y);
+        if (shared == 1 && reads > 0 && operand_reads(g, b.y) == reads) g.q8rows.insert(b.y);
     }
 }
 

@@ -215,3 +215,45 @@ def test_units_side_by_side(hip):
         for i, a in zip(ids, alone):
             assert np.array_equal(run.output(i).reshape(a.shape), a)
     run.close()
+
+
+@pytest.mark.parametrize("tail", ["mlp residual", "projected", "projection residual"])
+@pytest.mark.parametrize("storage", ["f16", "bf16"])
+def test_norm_rows_in_fused_nodes(hip, tail, storage, monkeypatch):
+    """A norm's y that a product reads and that a fused MLP's or projection's kernel reads as well: the bits of the norm,
+    the product and the MLP as plans of their own."""
+    r = rng(21)
+    rows, c, hidden = 100, 192, 768
+    g = lambda *s: (r.normal(size=s) / np.sqrt(s[0])).astype(np.float32)  # noqa: E731
+    wq, w1, w2, wp, b1, b2 = g(c, c), g(c, hidden), g(hidden, c), g(c, c), g(hidden), g(c)
+    x, s = (rounded(r.normal(size=(rows, c)), storage) for _ in range(2))
+
+    def norm(pb, v):
+        return pb.block_norm(residual=v, h=False)[1]
+
+    def mlp(pb, y, v):
+        res = y
+        if tail != "mlp residual":
+            res = v = pb.add(pb.gemm(y if tail == "projected" else v, wp, b2), v if tail == "projected" else y)
+        m = pb.gemm(pb.layer_norm(v, np.ones(c, np.float32), np.zeros(c, np.float32)), w1, b1, act="gelu")
+        return pb.add(pb.gemm(m, w2, b2), res)
+
+    def run(build, *inputs):
+        pb = PlanBuilder()
+        plan = pb.build(build(pb, *[pb.input((rows, c)) for _ in inputs]))
+        with HipInferenceSession(hip.graph(plan, STORAGE[storage])) as sess:
+            for i, v in enumerate(inputs):
+                sess.set_input(v, i)
+            return sess.run().reshape(rows, c).copy()
+
+    def whole(pb, xv, sv):
+        y = norm(pb, xv)
+        return pb.add(pb.quant_linear(y, wq), mlp(pb, y, sv))
+
+    print(f"[gpu] norm beside a fused MLP, {tail} {storage}", flush=True)
+    got = run(whole, x, s)
+    y = run(norm, x)
+    z, out = run(lambda pb, v: pb.quant_linear(v, wq), y), run(mlp, y, s)
+    assert np.array_equal(got, rounded(z + out, storage))
+    monkeypatch.setenv("SIMDONNX_HIP_NO_QUANT_NORM", "1")
+    assert np.array_equal(run(whole, x, s), got)

@@ -78,6 +78,40 @@ def test_norm_keeps_its_rows_for_others(offline, monkeypatch):
     assert rows(output) == 1
 
 
+def mlp_after(pb, y, tail):
+    """A transformer MLP that runs as one kernel, and where y comes into it."""
+    ones, zeros = np.ones(192, np.float32), np.zeros(192, np.float32)
+
+    def mlp(x, res):
+        m = pb.gemm(pb.layer_norm(x, ones, zeros), weights(192, 768), np.zeros(768, np.float32), act="gelu")
+        return pb.add(pb.gemm(m, weights(768, 192), zeros), res)
+
+    s = pb.input((ROWS, 192))
+    if tail == "mlp residual":
+        return mlp(s, y)
+    o, r = (y, s) if tail == "projected" else (s, y)
+    x = pb.add(pb.gemm(o, weights(192, 192), zeros), r)
+    return mlp(x, x)
+
+
+@pytest.mark.parametrize("storage", [True, "bf16"])
+@pytest.mark.parametrize("tail", ["mlp residual", "projected", "projection residual"])
+def test_norm_keeps_its_rows_for_fused_nodes(offline, tail, storage, monkeypatch):
+    """A y that a fused MLP's or projection's kernel reads, through nodes folded into it, stays in storage elements."""
+    monkeypatch.setenv("SIMDONNX_HIP_QGEMM", "64x64_w4k128s4")  # (its floating rows need a launch of their own)
+
+    pb = PlanBuilder()
+    _, y = pb.block_norm(residual=pb.input((ROWS, 192)), h=False)
+    z = pb.quant_linear(y, weights(192, 192))
+    g = offline.graph(pb.build(pb.add(z, mlp_after(pb, y, tail))), storage)
+    at, size = g.value_place(y)
+    names = [d[0] for d in g.dispatches]
+    reads = [(n, b[2]) for i, n in enumerate(names) for b in g.binds(i) if b[0] == N.SLOT_ARENA and b[1] == at]
+    assert any(n.startswith("mlp") for n in names) and not any(n == "gemm" for n in names), names  # (folded)
+    assert ("block_norm", size) in reads and ("quant_rows", size) in reads, reads
+    assert len(reads) >= 3 and all(n == size for _, n in reads), reads
+
+
 def plan_over(at, outs):
     """A plan whose arena puts the values `outs` where `at` says (elements)."""
     pb = PlanBuilder()
