@@ -365,8 +365,8 @@ int sox_block_norm_run_quantized(sox_block_norm* norm, void* stream, int32_t sto
 
 /* Both as nodes of a plan, SOX_OP_EXT nodes named "QuantLinear" and "BlockNorm" (a consumer's registration of the name
  * wins). Values are rows over their last dimension, stored in the order of their shape. A BlockNorm whose y only
- * QuantLinears read, as x, hands them 8-bit rows (channels a multiple of 16), and a session refuses to read that value;
- * SIMDONNX_HIP_NO_QUANT_NORM leaves y in storage elements, rounded by each reader. */
+ * QuantLinears read, as x, hands them 8-bit rows (channels a multiple of 16, its buffer on a 16-byte boundary), and a
+ * session refuses to read that value; SIMDONNX_HIP_NO_QUANT_NORM leaves y in storage elements, rounded by each reader. */
 typedef struct sox_quant_linear_p { /* in: x, weights (const [inner][columns]), bias (const) if any, residual if any; out: y */
     int32_t act, has_bias, has_residual;
 } sox_quant_linear_p;

@@ -3638,6 +3638,7 @@ void plan_layers8(sox_graph& g) {
         P.values.push_back(std::move(v));
         g.bnorm_vectors[ni] = (int)P.values.size() - 1;
         if (b.y < 0 || b.channels % 16 || getenv("SIMDONNX_HIP_NO_QUANT_NORM")) continue;
+        if ((uint64_t)P.buf_offset[P.values[b.y].buf] * g.es % 16) continue;  // (8-bit rows move 8 and 16 bytes at a time)
         int shared = 0, reads = 0;
         for (const PlanValue& o : P.values) shared += o.buf == P.values[b.y].buf;
         for (int k = 0; k < (int)P.nodes.size(); k++)

@@ -257,3 +257,25 @@ def test_norm_rows_in_fused_nodes(hip, tail, storage, monkeypatch):
     assert np.array_equal(got, rounded(z + out, storage))
     monkeypatch.setenv("SIMDONNX_HIP_NO_QUANT_NORM", "1")
     assert np.array_equal(run(whole, x, s), got)
+
+
+@pytest.mark.parametrize("storage", list(STORAGE))
+@pytest.mark.parametrize("off", [1, 4, 6])
+def test_norm_rows_off_16_byte_boundaries(hip, storage, off):
+    """A plan whose arena puts a norm's y on any element: the bits of the same plan on a boundary. The y are 16-bit values, in
+    fp32 too, which norm and product bring to 8 bits alike, exactly."""
+    r = rng(off)
+    x, w = rounded(r.normal(size=(70, 64)), "bf16" if storage == "f32" else storage), r.normal(size=(64, 48)).astype(np.float32)
+
+    def run(off):
+        pb = PlanBuilder()
+        _, y = pb.block_norm(residual=pb.input((70, 64)), pre="none", h=False)
+        p = pb.build(pb.quant_linear(y, w, act="relu"))
+        p.buf_offset[p.values[y].buf] = p.arena_floats + off
+        p.arena_floats += 70 * 64 + off
+        print(f"[gpu] norm at element {off} {storage}", flush=True)
+        with HipInferenceSession(hip.graph(p, STORAGE[storage])) as s:
+            s.set_input(x, 0)
+            return s.run().copy()
+
+    assert np.array_equal(run(off), run(0))

@@ -112,6 +112,23 @@ def test_norm_keeps_its_rows_for_fused_nodes(offline, tail, storage, monkeypatch
     assert len(reads) >= 3 and all(n == size for _, n in reads), reads
 
 
+@pytest.mark.parametrize("storage", [False, True])
+def test_norm_keeps_its_rows_off_16_byte_boundaries(offline, storage, monkeypatch):
+    """8-bit rows are stored and read 8 and 16 bytes at a time: not in a buffer that the plan put off such a boundary."""
+    monkeypatch.setenv("SIMDONNX_HIP_QGEMM", "64x64_w4k128s4")
+    for off in range(9):
+        pb = PlanBuilder()
+        x = pb.input((ROWS, C))
+        _, y = pb.block_norm(residual=x, h=False)
+        p = pb.build(pb.quant_linear(y, weights(C, C)))
+        p.buf_offset[p.values[y].buf] = p.arena_floats + off
+        p.arena_floats += ROWS * C + off
+        g = offline.graph(p, storage)
+        boundary = g.value_place(y)[0] % 16 == 0
+        assert boundary == (off % (8 if storage else 4) == 0)
+        assert [d[0] for d in g.dispatches].count("quant_rows") == (0 if boundary else 1)
+
+
 def plan_over(at, outs):
     """A plan whose arena puts the values `outs` where `at` says (elements)."""
     pb = PlanBuilder()
