@@ -4179,6 +4179,7 @@ int sox_backend_register_ext(sox_backend* backend, const char* name, sox_ext_emi
 
 int sox_graph_bind(sox_graph* graph, int32_t value, int32_t const_kind, sox_bind* out) {
     return guarded([&] {
+        if (graph->q8rows.count(value)) fail(SOX_E_INVALID, "value holds 8-bit rows for the products that read it");
         Emitter e(*graph);
         *out = e.bind(value, const_kind);
     });

@@ -129,6 +129,31 @@ def test_norm_keeps_its_rows_off_16_byte_boundaries(offline, storage, monkeypatc
         assert [d[0] for d in g.dispatches].count("quant_rows") == (0 if boundary else 1)
 
 
+def test_handed_rows_are_not_bound_as_elements(offline, capsys):
+    """An extension operator that names a norm's y outside of its node's inputs gets an error where it holds 8-bit rows."""
+    seen = []
+
+    def emit(g, node):
+        seen.append(None)
+        seen[-1] = g.bind(N.c_int32.from_buffer_copy(g.node(node)[1]).value)
+
+    offline.register_ext("ReadsAnother", emit)
+
+    def lower(named):
+        pb = PlanBuilder()
+        x = pb.input((ROWS, C))
+        h, y = pb.block_norm(residual=x)
+        z = pb.quant_linear(y, weights(C, C))
+        e = pb.ext("ReadsAnother", [z], (ROWS, C), bytes(N.c_int32({"h": h, "y": y}[named])))
+        return offline.graph(pb.build(e), True)
+
+    lower("h")
+    assert seen[-1].size == ROWS * C * 2
+    with pytest.raises(N.SoxError, match="ReadsAnother emit failed"):
+        lower("y")
+    assert seen[-1] is None and "8-bit rows" in capsys.readouterr().out
+
+
 def plan_over(at, outs):
     """A plan whose arena puts the values `outs` where `at` says (elements)."""
     pb = PlanBuilder()
