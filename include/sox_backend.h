@@ -318,7 +318,8 @@ int sox_qlinear_create_int8(sox_backend* backend, const int8_t* weights, const f
 void sox_qlinear_destroy(sox_qlinear* linear);
 /* Bytes from row to row that sox_qlinear_run_quantized's rows are best held at (inner rounded up to 64). */
 int sox_qlinear_pitch(sox_qlinear* linear);
-/* Workspace bytes of sox_qlinear_run at this many rows (0: none needed). */
+/* Workspace bytes that are enough for sox_qlinear_run at any number of rows up to this one (0: none needed). A call that
+ * needs less takes less, and none where it brings its rows to 8 bits itself. */
 uint64_t sox_qlinear_workspace(sox_qlinear* linear, int32_t rows);
 /* y[r][c] = act(sum_k q[r][k] w[k][c] * scale[r] * ws[c] + bias[c] (+ residual[r][c])) over floating rows x [rows][inner].
  * act: enum sox_act; residual [rows][columns] or NULL (may be y itself, same ld). workspace: 16-byte-aligned device

@@ -621,7 +621,7 @@ class HipQuantLinear:
         self._run, self._run_quantized = N.backend().sox_qlinear_run, N.backend().sox_qlinear_run_quantized
 
     def workspace(self, rows: int) -> int:
-        """Bytes of workspace that `run` needs at this many rows."""
+        """Bytes of workspace that are enough for `run` at any number of rows up to this one."""
         return int(N.backend().sox_qlinear_workspace(self.h, rows))
 
     def run(self, x: int, rows: int, y: int, storage: str = "f16", ldx: Optional[int] = None, ldy: Optional[int] = None,

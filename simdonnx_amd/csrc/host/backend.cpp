@@ -328,7 +328,7 @@ struct QPlan {
     QPlan(int inner, int columns, int compute_units, int64_t m, int32_t storage, bool floating) {
         const int es = storage == SOX_STORAGE_F32 ? 4 : 2;
         const double cus = std::max(1, compute_units), n = columns, k = inner;
-        if (floating && m <= 16 && inner <= 4096) {
+        if (floating && few_floating(inner, m)) {
             way = FEWX;
             return;
         }
@@ -352,6 +352,7 @@ struct QPlan {
         }
         if (floating && inner <= 1024 && m <= 1 << 20 && panel_us((double)m, n, k, es, cus) < rows_us((double)m, k, es) + best) way = PANEL;
     }
+    static bool few_floating(int inner, int64_t m) { return m <= 16 && inner <= 4096; }
     bool rounds_itself() const { return way == FEWX || way == PANEL; }
     // workspace: rows [m][pitch], then their scales
     static int pitch(int inner) { return round_up(inner, 64); }
@@ -5499,16 +5500,11 @@ void sox_qlinear_destroy(sox_qlinear* L) { delete L; }
 
 int sox_qlinear_pitch(sox_qlinear* L) { return L ? QPlan::pitch(L->inner) : 0; }
 
+// What every call of up to `rows` rows is content with: whether a call rounds its rows itself is no steady function of their
+// number, so only the numbers that never need a workspace are told apart.
 uint64_t sox_qlinear_workspace(sox_qlinear* L, int32_t rows) {
-    if (!L || rows <= 0 || rows > 1 << 23) return 0;
-    uint64_t need = 0;  // for every storage type
-    for (int32_t s = 0; s < 3; s++) {
-        const int rc = guarded([&] {
-            if (!L->plan(rows, s, true).rounds_itself()) need = QPlan::bytes(L->inner, rows);
-        });
-        if (rc) return QPlan::bytes(L->inner, rows);
-    }
-    return need;
+    if (!L || rows <= 0 || rows > 1 << 23 || QPlan::few_floating(L->inner, rows)) return 0;
+    return QPlan::bytes(L->inner, rows);
 }
 
 int sox_qlinear_run(sox_qlinear* L, void* stream, int32_t storage, const void* x, int64_t ldx, int32_t rows, const void* residual,

@@ -194,3 +194,20 @@ def test_norm_creation(offline):
                                              N.ctypes.byref(N.c_void_p())) == N.SOX_E_UNSUPPORTED
     N.backend().sox_block_norm_destroy(None)
 
+
+@pytest.mark.parametrize("k,n", [(768, 768), (256, 4096), (512, 2048), (32, 16), (1024, 96), (1025, 40), (4096, 64), (4097, 64)])
+def test_workspace_for_the_largest_call(offline, k, n):
+    """A workspace taken for the largest number of rows is enough for every smaller call, whichever way each runs."""
+    lin = HipQuantLinear(offline, np.ones((k, n), np.int8), None, k, n, scales=np.ones(n, np.float32))
+    sizes = [lin.workspace(rows) for rows in range(2049)]
+    assert sizes == sorted(sizes) and sizes[0] == 0
+    assert (sizes[16] == 0) == (k <= 4096)
+    far = [lin.workspace(rows) for rows in (1 << 14, 100003, 1 << 20, (1 << 20) + 1, 1 << 23)]
+    assert far == sorted(far) and far[0] >= sizes[-1]
+    for most in (2048, 1600, 1118, 21, 17):
+        size = lin.workspace(most)
+        for rows in {1, 15, 16, 17, 18, 20, 21, 64, 65, 1117, 1118, 1471, 1472, 1574, 1575, most}:
+            if rows <= most:
+                for storage in ("f16", "bf16", "f32"):
+                    in_order(lin.run, x=at(0), rows=rows, y=at(4), storage=storage, workspace=at(8), workspace_bytes=size)
+    lin.close()
