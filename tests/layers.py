@@ -33,6 +33,12 @@ def rounded(x, storage):
     return from_bits(to_bits(x, storage), storage)
 
 
+# (rows, inner, columns) of floating products that one launch of 32 x 128 outputs rounds and multiplies, at both ends of the
+# range of K of each of its instances
+PANELS = [(90, 2, 40), (21, 256, 72), (90, 257, 72), (64, 512, 100), (70, 513, 33), (100, 768, 129), (100, 769, 136),
+          (65, 1000, 40), (257, 1023, 301), (786, 1024, 760), (66, 1024, 1)]
+
+
 class Matrix:
     """rows x cols of a storage type (or "i8") on the device, `ld` elements from row to row, `skip` elements behind an
     aligned base; every byte around the elements holds a pattern that `untouched` looks for."""

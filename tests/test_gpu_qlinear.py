@@ -14,7 +14,7 @@ from simdonnx_amd import native as N
 from simdonnx_amd import synth
 from simdonnx_amd.backend import HipQuantLinear
 from simdonnx_amd.native import SoxError
-from tests.layers import Matrix, from_bits, linear64, quantize, rounded, to_bits
+from tests.layers import PANELS, Matrix, from_bits, linear64, quantize, rounded, to_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -138,6 +138,16 @@ def test_many_tiles_per_workgroup(hip, monkeypatch, tile):
     rows, n = {"256": (12000, 3304), "128": (9000, 2500), "64x": (4200, 2200)}[tile[:3].rstrip("x") if tile[0] != "6" else "64x"]
     print(f"[gpu] qlinear {tile} {rows} x 40 -> {n}", flush=True)
     both_ways(hip, 2100, rows, 40, n, "bf16")
+
+
+@pytest.mark.parametrize("storage", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,k,n", PANELS)
+def test_panels(hip, storage, rows, k, n):
+    """Rows rounded and multiplied by one launch, at the ends of each instance's range of K: the bits of the same rows given
+    in 8 bits, with whole rows and with a residual and rows off every boundary."""
+    print(f"[gpu] qlinear panel {storage} {rows} x {k} -> {n}", flush=True)
+    both_ways(hip, 2200 + k, rows, k, n, storage)
+    both_ways(hip, 2300 + k, rows, k, n, storage, act="swish", bias=False, res=True, pad=3, skip=1)
 
 
 @pytest.mark.parametrize("act", ["none", "relu", "sigmoid", "gelu", "hardswish", "swish"])

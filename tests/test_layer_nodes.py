@@ -11,6 +11,7 @@ import pytest
 from simdonnx_amd import native as N
 from simdonnx_amd.backend import HipBackend
 from simdonnx_amd.plan import NHWC, PlanBuilder
+from tests.layers import PANELS
 
 ROWS, C, K = 100, 64, 48
 
@@ -152,6 +153,19 @@ def test_handed_rows_are_not_bound_as_elements(offline, capsys):
     with pytest.raises(N.SoxError, match="ReadsAnother emit failed"):
         lower("y")
     assert seen[-1] is None and "8-bit rows" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("storage", ["f32", "f16", "bf16"])
+def test_panels_take_moderate_numbers_of_rows(offline, storage):
+    """The shapes by which the panel kernel is tested run on it, each instance among them."""
+    taken = set()
+    for rows, k, n in PANELS:
+        pb = PlanBuilder()
+        plan = pb.build(pb.quant_linear(pb.input((rows, k)), weights(k, n)))
+        name = f"sox_qpanel_{storage}_c{-(-k // 256)}"
+        assert offline.graph(plan, storage != "f32" and storage).kernels == [name], (rows, k, n)
+        taken.add(name)
+    assert len(taken) == 4
 
 
 def plan_over(at, outs):
