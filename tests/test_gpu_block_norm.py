@@ -126,6 +126,16 @@ def test_rows_past_one_round(hip, rows, c, pad):
     run_case(hip, rows, rows, c, "f16", params(c, c, "rms", "layer", gate_act="sigmoid"), gate_rows=1, pad=pad)
 
 
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,c,pad,skip", [(5003, 192, 0, 0), (5003, 256, 4, 0), (5003, 189, 0, 1), (3001, 257, 0, 0), (3001, 512, 0, 0),
+                                             (3001, 391, 3, 0), (2050, 513, 0, 0), (2050, 768, 8, 0), (2050, 1023, 0, 1), (1024, 1024, 0, 0)])
+def test_many_rows(hip, storage, rows, c, pad, skip):
+    """The instances for many rows in the other types than fp16, at both ends of their ranges."""
+    print(f"[gpu] block norm {storage} {rows} x {c} + {pad}", flush=True)
+    kinds = KINDS[(rows + c) % len(KINDS)]
+    run_case(hip, rows + c, rows, c, storage, params(c, c, *kinds, gate_act="swish"), gate_rows=rows if c % 2 else 1, pad=pad, skip=skip)
+
+
 def test_large_means(hip):
     """Rows far from zero: the variance comes from the deviations, not from a difference of squares."""
     print("[gpu] block norm large means", flush=True)

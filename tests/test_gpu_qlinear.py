@@ -82,6 +82,14 @@ def test_few_rows(hip, storage, rows, k, n):
     both_ways(hip, 1000 + rows + k, rows, k, n, storage)
 
 
+@pytest.mark.parametrize("storage", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,k,n", [(1, 1025, 40), (2, 1100, 33), (16, 1536, 72), (5, 2047, 17), (16, 2048, 48)])
+def test_few_rows_of_two_steps_a_wave(hip, storage, rows, k, n):
+    print(f"[gpu] qlinear {storage} {rows} x {k} -> {n}", flush=True)
+    both_ways(hip, 1500 + rows + k, rows, k, n, storage)
+    both_ways(hip, 1600 + rows + k, rows, k, n, storage, act="gelu", bias=False, res=True, pad=5, skip=1)
+
+
 @pytest.mark.parametrize("tile", TILES)
 @pytest.mark.parametrize("storage,rows,k,n,pad,skip", [
     ("f16", 300, 768, 520, 0, 0), ("bf16", 65, 1, 1, 0, 0), ("bf16", 257, 64, 300, 8, 0), ("f16", 130, 200, 257, 3, 1),
