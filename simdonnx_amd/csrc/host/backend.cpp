@@ -869,6 +869,7 @@ int64_t axis_stride(const PlanValue& v, int axis);
 // ---------------------------------------------------------------------------------------------
 bool conv_pads_channels(const sox_graph& g, const PlanNode& n);
 bool gemm_pads_k(const sox_graph& g, int64_t m, int n, int k);
+int value_reads(const sox_graph& g, int v);
 
 struct Emitter {
     sox_graph& g;
@@ -965,19 +966,7 @@ struct Emitter {
     }
 
     // Reads of value v by any node (inputs and the value-id fields of the param records).
-    int uses(int v) const {
-        int u = 0;
-        for (int ni = 0; ni < (int)g.plan.nodes.size(); ni++) {
-            if (g.folded.count(ni)) continue;
-            const PlanNode& n = g.plan.nodes[ni];
-            for (int x : n.in) u += x == v;
-            if (n.op == SOX_OP_CONV) {
-                const auto& p = n.p<sox_conv_p>();
-                u += (p.add_value == v) + (p.bias_value == v);
-            }
-        }
-        return u + (v == g.plan.output);
-    }
+    int uses(int v) const { return value_reads(g, v); }
 
     // Arena byte range of an activation value (empty for consts).
     std::pair<uint64_t, uint64_t> arena_range(int v) {
@@ -2829,9 +2818,11 @@ int buffer_reads(const sox_graph& g, int v, int except) {
 }
 
 // Reads of value v by the nodes not folded away (inputs and the value-id fields of conv params) plus
-// the plan output.
+// the plan output. An activation's reads through its zero-copy views count too: a fusion that no longer
+// stores v takes the content of its views with it.
 int value_reads(const sox_graph& g, int v) {
     const auto& P = g.plan;
+    if (g.V(v).buf >= 0) return buffer_reads(g, v, -1);
     int u = v == P.output;
     for (int ni = 0; ni < (int)P.nodes.size(); ni++) {
         if (g.folded.count(ni)) continue;

@@ -279,3 +279,37 @@ def test_norm_rows_off_16_byte_boundaries(hip, storage, off):
             return s.run().copy()
 
     assert np.array_equal(run(off), run(0))
+
+
+@pytest.mark.parametrize("fusion", ["residual add", "layer norm", "mlp"])
+def test_views_of_fused_values(hip, fusion):
+    """A product that reads a view of a value which a fusion would not store: the bits of two plans, one after the other."""
+    r = rng(31)
+    g = lambda *s: (r.normal(size=s) / np.sqrt(s[0])).astype(np.float32)  # noqa: E731
+    rows, k, n = {"residual add": (128, 64, 64), "layer norm": (128, 64, 64), "mlp": (128, 192, 768)}[fusion]
+    x = rounded(r.normal(size=(rows, k)), "f16")
+    gamma, beta, w1, b1, w2, b2, wq = 1 + 0.1 * g(k), g(k), g(k, n), g(n), g(n, k), g(k), g(n, 48)
+
+    def value(pb, v):
+        if fusion == "residual add":
+            y = pb.gemm(v, w1, b1)
+            pb.add(y, v)
+        elif fusion == "layer norm":
+            y = pb.layer_norm(v, gamma, beta)
+            pb.gemm(y, w1, b1)
+        else:
+            y = pb.gemm(pb.layer_norm(v, gamma, beta), w1, b1, act="gelu")
+            pb.add(pb.gemm(y, w2, b2), v)
+        return y
+
+    def run(build, v):
+        pb = PlanBuilder()
+        plan = pb.build(build(pb, pb.input(v.shape)))
+        with HipInferenceSession(hip.graph(plan, True)) as s:
+            s.set_input(v, 0)
+            return s.run().copy()
+
+    print(f"[gpu] view of a fused value: {fusion}", flush=True)
+    got = run(lambda pb, v: pb.quant_linear(pb.alias(value(pb, v), (2, rows // 2, n)), wq), x)
+    y = run(value, x).reshape(rows, n)
+    assert np.array_equal(got.reshape(rows, 48), run(lambda pb, v: pb.quant_linear(v, wq), y).reshape(rows, 48))
