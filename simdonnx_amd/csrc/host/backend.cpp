@@ -2799,8 +2799,25 @@ int64_t axis_stride(const PlanValue& v, int axis) {
     return -1;
 }
 
+// The values that node k's dispatches read for the nodes folded into it: a fused transformer MLP's residual, its projection's
+// input and residual, the sources of a conv that gathers a concat of upsamples.
+std::vector<int> folded_reads(const sox_graph& g, int k) {
+    std::vector<int> r;
+    auto m = g.mlp.find(k);
+    if (m != g.mlp.end()) {
+        if (m->second.residual >= 0) r.push_back(m->second.residual);
+        if (m->second.proj >= 0) {
+            r.push_back(g.plan.nodes[m->second.proj].in[0]);
+            r.push_back(m->second.proj_res);
+        }
+    }
+    auto u = g.upcat.find(k);
+    if (u != g.upcat.end()) r.insert(r.end(), u->second.src, u->second.src + u->second.n);
+    return r;
+}
+
 // Reads of value v's buffer, through v or any alias of it, by the nodes not folded away other than
-// node `except`, plus the plan output when it lives there.
+// node `except` and for the nodes folded into them, plus the plan output when it lives there.
 int buffer_reads(const sox_graph& g, int v, int except) {
     const auto& P = g.plan;
     const int buf = P.values[v].buf;
@@ -2809,6 +2826,7 @@ int buffer_reads(const sox_graph& g, int v, int except) {
     for (int ni = 0; ni < (int)P.nodes.size(); ni++) {
         if (ni == except || g.folded.count(ni)) continue;
         for (int x : P.nodes[ni].in) u += P.values[x].buf == buf;
+        for (int x : folded_reads(g, ni)) u += P.values[x].buf == buf;
         if (P.nodes[ni].op == SOX_OP_CONV) {
             const auto& cp = P.nodes[ni].p<sox_conv_p>();
             for (int x : {cp.add_value, cp.bias_value}) u += x >= 0 && P.values[x].buf == buf;

@@ -85,3 +85,20 @@ def test_view_of_a_value_keeps_it(offline, fusion, end):
         assert kernels == plain and at == used  # as where the value itself has a second reader
     assert at and (end == "output" or at[0] < len(kernels) - 1)
     assert lowered(offline, fusion, "nobody")[0] != [k for k in plain if "unary" not in k], "no fusion to be kept out"
+
+
+@pytest.mark.parametrize("other", [True, False])
+def test_concat_that_a_fused_mlp_adds(offline, other):
+    """The concat of upsamples before a conv is stored where a fused MLP's kernel reads it as its residual."""
+    pb = PlanBuilder()
+    p, u = pb.input((1, 32, 16, 16), (0, 2, 3, 1)), pb.input((1, 32, 8, 8), (0, 2, 3, 1))
+    x = pb.concat_channels([pb.resize_nearest(u, 2), p])
+    s = pb.input((1, 16, 16, 64))
+    h = pb.gemm(pb.layer_norm(s, f(64) + 2, f(64)), f(64, 256), f(256), act="gelu")
+    pb.add(pb.gemm(h, f(256, 64), f(64)), x if other else s)
+    g = offline.graph(pb.build(pb.conv(x, f(16, 64, 3, 3), f(16), pad=1)), True)
+    assert any(k.startswith("sox_mlp") for k in g.kernels)
+    assert any("upcat" in k for k in g.kernels) != other
+    at, size = g.value_place(x)
+    touch = [k for i, k in enumerate(g.kernels) if any(b[0] == 0 and b[1] < at + size and at < b[1] + b[2] for b in g.binds(i))]
+    assert not other or not touch[0].startswith("sox_mlp"), touch  # (written before the MLP reads it)
