@@ -870,6 +870,8 @@ int64_t axis_stride(const PlanValue& v, int axis);
 bool conv_pads_channels(const sox_graph& g, const PlanNode& n);
 bool gemm_pads_k(const sox_graph& g, int64_t m, int n, int k);
 int value_reads(const sox_graph& g, int v);
+std::vector<int> folded_reads(const sox_graph& g, int k);
+std::vector<int> emitted_writes(const sox_graph& g, int k);
 
 struct Emitter {
     sox_graph& g;
@@ -934,10 +936,9 @@ struct Emitter {
                     if (g.folded.count(k)) continue;
                     for (int u : nodes[k].in) clear(u);
                     for (int u : nodes[k].out) clear(u);
+                    for (int u : folded_reads(g, k)) clear(u);
+                    for (int u : emitted_writes(g, k)) clear(u);
                     if (nodes[k].op == SOX_OP_CONV) clear(nodes[k].p<sox_conv_p>().add_value);
-                    auto uc = g.upcat.find(k);  // a conv that gathers its input from upsample sources
-                    if (uc != g.upcat.end())
-                        for (int i = 0; i < uc->second.n; i++) clear(uc->second.src[i]);
                     auto ua = g.upadd.find(k);  // a nearest-add run as its addend's conv reads that conv's input
                     if (ua != g.upadd.end()) clear(nodes[ua->second.first].in[0]);
                     // a conv fed by a gated product reads the gate's input instead

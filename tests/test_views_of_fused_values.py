@@ -102,3 +102,28 @@ def test_concat_that_a_fused_mlp_adds(offline, other):
     at, size = g.value_place(x)
     touch = [k for i, k in enumerate(g.kernels) if any(b[0] == 0 and b[1] < at + size and at < b[1] + b[2] for b in g.binds(i))]
     assert not other or not touch[0].startswith("sox_mlp"), touch  # (written before the MLP reads it)
+
+
+@pytest.mark.parametrize("over", ["out", "residual", "clear"])
+def test_slices_beside_a_fused_mlp(offline, over):
+    """A conv does not write its slice of a concat ahead of a fused MLP whose output or residual the plan put there."""
+    pb = PlanBuilder()
+    layout = (0, 2, 3, 1)
+    x = pb.input((1, 32, 16, 16), layout)
+    s, r = pb.input((256, 64)), pb.input((256, 64))
+    c = pb.conv(x, f(32, 32, 1, 1), f(32), pad=0)
+    h = pb.gemm(pb.layer_norm(s, f(64) + 2, f(64)), f(64, 256), f(256), act="gelu")
+    m = pb.add(pb.gemm(h, f(256, 64), f(64)), r)
+    pb.unary("Tanh", m)
+    cat = pb.concat_channels([c, x])
+    p = pb.build(cat)
+    place = p.arena_floats
+    for v in (cat, {"out": m, "residual": r}.get(over, cat)):
+        p.buf_offset[p.values[v].buf] = place
+    p.arena_floats += 256 * 64
+    g = offline.graph(p, True)
+    assert any(k.startswith("sox_mlp") for k in g.kernels)
+    at, size = g.value_place(cat)
+    inside = [[b for b in g.binds(i) if b[0] == 0 and at <= b[1] < at + size] for i in range(len(g.kernels))]
+    first = next(i for i, b in enumerate(inside) if b)
+    assert ("conv" in g.kernels[first] or "gemm" in g.kernels[first]) == (over == "clear"), g.kernels
