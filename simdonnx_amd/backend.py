@@ -622,12 +622,14 @@ class HipQuantLinear:
 
     def workspace(self, rows: int) -> int:
         """Bytes of workspace that are enough for `run` at any number of rows up to this one."""
-        return int(N.backend().sox_qlinear_workspace(self.h, rows))
+        return int(N.backend().sox_qlinear_workspace(self.h, -1 if rows >> 31 else rows))
 
     def run(self, x: int, rows: int, y: int, storage: str = "f16", ldx: Optional[int] = None, ldy: Optional[int] = None,
             act: str = "none", residual: Optional[int] = None, ldr: Optional[int] = None, workspace: Optional[int] = None,
             workspace_bytes: int = 0, stream: Optional[int] = None):
         """y [rows, columns] from floating rows x [rows, inner]."""
+        if rows >> 31:
+            rows = -1  # (only its lowest 32 bits would reach the library)
         rc = self._run(self.h, stream, STORAGE[storage], x, self.inner if ldx is None else ldx, rows, residual,
                        self.columns if ldr is None else ldr, y, self.columns if ldy is None else ldy, N.ACT[act], workspace,
                        workspace_bytes)
@@ -638,6 +640,8 @@ class HipQuantLinear:
                       ldy: Optional[int] = None, act: str = "none", residual: Optional[int] = None,
                       ldr: Optional[int] = None, stream: Optional[int] = None):
         """y [rows, columns] from 8-bit rows (`pitch` bytes apart unless ldq says so) and their scales [rows]."""
+        if rows >> 31:
+            rows = -1  # (only its lowest 32 bits would reach the library)
         rc = self._run_quantized(self.h, stream, q, self.pitch if ldq is None else ldq, scales, rows, STORAGE[storage],
                                  residual, self.columns if ldr is None else ldr, y, self.columns if ldy is None else ldy,
                                  N.ACT[act])
@@ -679,6 +683,8 @@ class HipBlockNorm:
             ldy: Optional[int] = None, stream: Optional[int] = None):
         """h and y [rows, channels] (either may be left out) from the residual and the branch x."""
         c = self.channels
+        if (rows | gate_rows) >> 31:
+            rows = -1  # (only their lowest 32 bits would reach the library)
         rc = self._run(self.h, stream, STORAGE[storage], rows, residual, c if ldr is None else ldr, x, c if ldx is None else ldx,
                        gate, c if ldg is None else ldg, gate_rows, h, c if ldh is None else ldh, y, c if ldy is None else ldy)
         if rc:
@@ -690,6 +696,8 @@ class HipBlockNorm:
                       ldh: Optional[int] = None, ldq: Optional[int] = None, stream: Optional[int] = None):
         """h, and y as 8-bit rows q (channels rounded up to 64 bytes apart unless ldq says so) and their scales [rows]."""
         c = self.channels
+        if (rows | gate_rows) >> 31:
+            rows = -1  # (only their lowest 32 bits would reach the library)
         rc = self._run_quantized(self.h, stream, STORAGE[storage], rows, residual, c if ldr is None else ldr, x,
                                  c if ldx is None else ldx, gate, c if ldg is None else ldg, gate_rows, h,
                                  c if ldh is None else ldh, q, -(-c // 64) * 64 if ldq is None else ldq, scales)

@@ -211,3 +211,14 @@ def test_workspace_for_the_largest_call(offline, k, n):
                 for storage in ("f16", "bf16", "f32"):
                     in_order(lin.run, x=at(0), rows=rows, y=at(4), storage=storage, workspace=at(8), workspace_bytes=size)
     lin.close()
+
+
+def test_counts_past_32_bits(linear, norm):
+    """Row counts whose lowest 32 bits are a count in order."""
+    for rows in (1 << 32, (1 << 32) + 16, 1 << 31):
+        refused("rows", linear.run, **run_args(rows=rows))
+        refused("rows", linear.run_quantized, q=at(0), scales=at(1), rows=rows, y=at(2))
+        refused("rows", norm.run, at(0), rows, h=at(2))
+        refused("rows", norm.run_quantized, at(0), rows, at(2), at(3))
+        refused("rows", norm.run, at(0), 16, x=at(1), gate=at(4), gate_rows=rows, h=at(2))
+        assert linear.workspace(rows) == 0
