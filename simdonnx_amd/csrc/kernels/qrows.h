@@ -24,7 +24,8 @@ template <typename T, int ACT> SOX_DEV float q_out(float v, int act = 0) {
         const float g = sox_gelu(v);
         return v != v ? v : g;
     } else if constexpr (ACT == Q_ACT_GATES) {
-        const float hard = fminf(fmaxf(__builtin_fmaf(v, 1.0f / 6.0f, 0.5f), 0.0f), 1.0f);
+        // (v + 3 is exact near its zero, where v / 6 + 1 / 2 would be left with the quotient's rounding)
+        const float hard = fminf(fmaxf((v + 3.0f) * (1.0f / 6.0f), 0.0f), 1.0f);
         const float gate = act == SOX_ACT_HARDSWISH ? hard : sox_sigmoid(v), r = act == SOX_ACT_SIGMOID ? gate : v * gate;
         return v != v ? v : r;
     } else {

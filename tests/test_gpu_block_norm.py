@@ -136,6 +136,25 @@ def test_many_rows(hip, storage, rows, c, pad, skip):
     run_case(hip, rows + c, rows, c, storage, params(c, c, *kinds, gate_act="swish"), gate_rows=rows if c % 2 else 1, pad=pad, skip=skip)
 
 
+def test_hardswish_next_to_its_zero(hip):
+    """v clip((v + 3) / 6, 0, 1) keeps its digits where it leaves zero: four roundings (the sum, the sixth, two products) of half
+    a unit each, h being the gate alone; 5 units leave room for their products."""
+    c = 2048
+    g = np.concatenate([-3 + 2.0 ** -22 * np.arange(-100, 700), -3 + 2.0 ** -np.arange(1, 21.0), 3 + 2.0 ** -22 * np.arange(-200, 200),
+                        np.linspace(-8, 8, 828)]).astype(np.float32)[None]
+    assert g.size == c
+    norm = HipBlockNorm(hip, c, pre="none", gate_act="hardswish")
+    X, G, H = Matrix(np.ones((1, c)), "f32"), Matrix(g, "f32"), Matrix(None, "f32", 1, c)
+    print("[gpu] block norm hardswish", flush=True)
+    norm.run(None, 1, "f32", x=X.ptr, gate=G.ptr, h=H.ptr)
+    v = g.astype(np.float64)
+    want = v * np.clip((v + 3) / 6, 0, 1)
+    assert (np.abs(H.read() - want) <= 5 * 2.0 ** -24 * np.abs(want)).all()
+    for m in (X, G, H):
+        m.free()
+    norm.close()
+
+
 def test_large_means(hip):
     """Rows far from zero: the variance comes from the deviations, not from a difference of squares."""
     print("[gpu] block norm large means", flush=True)
