@@ -368,7 +368,9 @@ int sox_block_norm_run_quantized(sox_block_norm* norm, void* stream, int32_t sto
  * wins). Values are rows over their last dimension, stored in the order of their shape. A BlockNorm whose y only
  * QuantLinears read, as x, hands them 8-bit rows (channels a multiple of 16, its buffer on a 16-byte boundary), and a
  * session refuses to read that value; SIMDONNX_HIP_NO_QUANT_NORM leaves y in storage elements, rounded by each reader. */
-typedef struct sox_quant_linear_p { /* in: x, weights (const [inner][columns]), bias (const) if any, residual if any; out: y */
+typedef struct sox_quant_linear_p { /* in: x, weights (const [inner][columns], floats: brought to 8 bits by column, so a column
+                                       of given 8-bit weights keeps them if its largest is 127), bias (const) if any,
+                                       residual if any; out: y */
     int32_t act, has_bias, has_residual;
 } sox_quant_linear_p;
 /* operands of a BlockNorm node: which values its in and out list, in this order. The vectors are consts [channels]. */

@@ -296,14 +296,18 @@ const QTile kQTiles[] = {
 const int kRowThreads[] = {32, 64, 256};  // of a row brought to 8 bits, each with four 16-byte chunks in registers
 constexpr int kQTileCount = (int)(sizeof kQTiles / sizeof *kQTiles);
 
-// How a product of m rows runs. Every way gives the same bits (whole numbers), so the choice is by time alone, each
-// estimate a fit to measurements on one MI355X:
-//   FEWX   up to 16 floating rows of up to 4096 values, one launch           1 x 768 -> 768: 3.9 us
-//   PANEL  floating rows of up to 1024 values, one launch that rounds them   786 x 768 -> 760: 7.3 us; rounded by a launch
-//          once per 128 columns                                              of its own 9.4. 8192 x 768 -> 2304: 51, 35
+// How a product of m rows runs. Every way gives the same bits (whole numbers), so the choice is by time alone: by estimates,
+// each a fit to measurements on one MI355X, but for FEWX.
+//   FEWX   up to 16 floating rows of up to 4096 values, one launch, always. Every workgroup rounds all rows for its 16 columns,
+//          which a launch of its own does once: with one row or layers of up to 4096 columns that is less than a launch,
+//          16 rows of wide layers pay more than twice. us, K -> N at 1 / 7 / 16 rows, FEWX and (rows, FEW):
+//            768 -> 768   4.0 / 4.5 / 5.6, 5.3 / 5.4 / 5.4      4096 -> 4096   6.1 / 8.3 / 12.3, 7.7 / 8.5 / 9.4
+//            768 -> 16384 8.7 / 10 / 14, 6.7 / 6.8 / 6.8        4096 -> 16384  15 / 21 / 43, 16 / 17 / 21
+//   PANEL  floating rows of up to 1024 values, one launch that rounds them   786 x 768 -> 760: 7.2 us; rounded by a launch
+//          once per 128 columns                                              of its own 9.4. 8192 x 768 -> 2304: 51, 33
 //   FEW    up to 64 8-bit rows, weights straight to registers                64 x 4096 -> 4096: 10.8 us, ring 13.5;
 //                                                                            64 x 1024 -> 8192: 6.9, ring 6.0
-//   RING   8-bit rows on the ring of the tiling with the smallest estimate. Over 170 random products the pick is 1.3% above
+//   RING   8-bit rows on the ring of the tiling with the smallest estimate. Over 170 random products the pick is 1.2% above
 //          the fastest tiling on average, at most 18%
 // FEW and RING take floating rows behind a launch that brings them to 8 bits in the workspace.
 struct QPlan {

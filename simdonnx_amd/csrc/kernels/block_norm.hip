@@ -13,8 +13,8 @@
 //  * few rows, or longer ones: TPR threads per row, which shortens the one row's chain of loads, sums and stores; the
 //    parameters stay in registers (or, for the longest rows, are read where they are used).
 // A workgroup walks rows a whole grid apart; the grid is held to what the rows' streams run best with: 16384 x 4096 bf16 in
-// 95 us (5.7 TB/s) on 2 workgroups per CU, 122 with one row each, and 135 to 300 with a wave per row. Registers decide how
-// many waves there are: 8192 x 768 with a gate 13.8 us (100 registers, 4 waves on a SIMD), 17.5 when it took 144.
+// 95 to 100 us by box (5.7 to 5.4 TB/s) on 2 workgroups per CU, 122 with one row each, and 135 to 300 with a wave per row.
+// Registers decide how many waves there are: 8192 x 768 with a gate 13.8 us (100 registers, 4 waves on a SIMD), 17.5 when it took 144.
 #include "qrows.h"
 
 enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };

@@ -21,11 +21,13 @@
 //    residual loads and output stores are whole row segments.
 //
 // Tiles by size (the host's estimates choose): 256 x 256 with its 8 waves holds a wave's 128 x 64 outputs in registers and
-// reads 1 byte of LDS for 128 multiply-adds; 256 x 192 for shapes that fill the CUs' rounds better (8192 x 768 -> 2304: 27 us,
-// 1.5 rounds; 256 x 128 33); down to 64 x 64, four slices deep, where there are few tiles and a slice's latency counts.
-// Bound: with long K by the matrix cores, 4096 x 4096 -> 8192 in 126 us (2.18e15 operations a second; a large library product of
-// 8-bit integers reaches 2.1e15 on the same card). With K = 4096 a 256 x 256 tile takes 52 us, 43 of them without its DMA and 35
-// without its MFMAs, the epilogue 4 us. With short K by the prologue (2 us), the epilogue and the outputs' stores.
+// multiplies 43 times for each byte of LDS that it reads, 128 times for each that comes from memory; 256 x 192 for shapes
+// whose tiles it deals to the CUs in fuller rounds (8192 x 1024 -> 1536: one round, 19.4 us; 256 x 256 21.5, 256 x 128 24.3,
+// 128 x 128 24.6); down to 64 x 64, four slices deep, where there are few tiles and a slice's latency counts.
+// Bound: with long K by DMA, LDS reads and MFMAs that overlap in part, 4096 x 4096 -> 8192 in 117 to 122 us by box (2.25 to
+// 2.35e15 operations a second; a large library product of 8-bit integers reaches 2.0 to 2.1e15). Of a 256 x 256 tile's 52 us at
+// K = 4096, 43 are left without its DMA and 35 without its MFMAs; its epilogue is 4. With short K by the prologue (2 us), the
+// epilogue (nothing multiplies meanwhile) and the outputs' stores.
 #pragma once
 #include "qrows.h"
 
@@ -58,8 +60,8 @@ template <typename T> SOX_DEV int stage_at(int r, int c) {
 
 // What a kernel knows of its outputs' rows:
 //   Q_LINES  they stand on 128-byte lines and hold whole 16-byte chunks. Their stores pass L2 by, which leaves it to the A and W
-//            lines that are read again: 4096 x 4096 -> 8192 124 us, 133 with stores through L2, 128 with the choice made in
-//            the kernel
+//            lines that are read again: 4096 x 4096 -> 8192 with its rounding 125 us, 133 with stores through L2, 128 with the
+//            choice made in the kernel
 //   Q_CHUNKS they hold whole chunks. Their stores go through L2: a line that different stores write in parts would reach memory
 //            in parts, 2954 x 320 -> 3112 19.8 us so and 13.3 through L2
 //   Q_PART   any
