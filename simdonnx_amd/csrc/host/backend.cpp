@@ -2827,14 +2827,16 @@ int buffer_reads(const sox_graph& g, int v, int except) {
     const auto& P = g.plan;
     const int buf = P.values[v].buf;
     if (buf < 0) return 1;
-    int u = P.values[P.output].buf == buf;
+    // (ids that a plan gets wrong are refused where its nodes are lowered)
+    auto on = [&](int x) { return x >= 0 && x < (int)P.values.size() && P.values[x].buf == buf; };
+    int u = on(P.output);
     for (int ni = 0; ni < (int)P.nodes.size(); ni++) {
         if (ni == except || g.folded.count(ni)) continue;
-        for (int x : P.nodes[ni].in) u += P.values[x].buf == buf;
-        for (int x : folded_reads(g, ni)) u += P.values[x].buf == buf;
+        for (int x : P.nodes[ni].in) u += on(x);
+        for (int x : folded_reads(g, ni)) u += on(x);
         if (P.nodes[ni].op == SOX_OP_CONV) {
             const auto& cp = P.nodes[ni].p<sox_conv_p>();
-            for (int x : {cp.add_value, cp.bias_value}) u += x >= 0 && P.values[x].buf == buf;
+            u += on(cp.add_value) + on(cp.bias_value);
         }
     }
     return u;

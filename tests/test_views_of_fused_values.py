@@ -3,6 +3,7 @@
 import numpy as np
 import pytest
 
+from simdonnx_amd import native as N
 from simdonnx_amd.backend import HipBackend
 from simdonnx_amd.plan import PlanBuilder
 
@@ -127,3 +128,16 @@ def test_slices_beside_a_fused_mlp(offline, over):
     inside = [[b for b in g.binds(i) if b[0] == 0 and at <= b[1] < at + size] for i in range(len(g.kernels))]
     first = next(i for i, b in enumerate(inside) if b)
     assert ("conv" in g.kernels[first] or "gemm" in g.kernels[first]) == (over == "clear"), g.kernels
+
+
+@pytest.mark.parametrize("wrong", [1000, 1 << 30, -1, -5])
+@pytest.mark.parametrize("fusion", FUSIONS, ids=[x.__name__ for x in FUSIONS])
+def test_readers_that_name_no_value(offline, fusion, wrong):
+    """A node over an id that is no value's is refused, not looked up, by the fusions before it."""
+    pb = PlanBuilder()
+    _, out = fusion(pb)
+    pb.unary("Tanh", out)
+    p = pb.build(out)
+    p.nodes[-1].ins = [wrong]
+    with pytest.raises(N.SoxError, match="out of range"):
+        offline.graph(p, True)
