@@ -617,6 +617,70 @@ typedef struct sox_bnorm_args {
     int32_t pad_;
 } sox_bnorm_args;
 
+/* ---- attention while a transformer serves: rotary positions, a paged cache, attention over it (no counterpart in the
+ * reference) ---- */
+
+/* A rotation by position: pair j < half of a head's first 2 half channels (channels j and half + j, or with interleaved 2 j
+ * and 2 j + 1) turned by position * turns[j] / 2^64 of a whole turn, times amplitude. half = 0: none. */
+typedef struct sox_turn_args {
+    const uint64_t* turns;
+    double amplitude;
+    int32_t half, interleaved;
+} sox_turn_args;
+
+/* sox_rotary_*: rows_per_block rows of x [rows][heads][dim] per workgroup of 256, 2^lanes lanes for each head (16 bytes of
+ * x a lane). positions[r] is row r's. */
+typedef struct sox_rotary_args {
+    const void* x;
+    void* y;
+    const int32_t* positions;
+    int64_t ldx, ldy;
+    int32_t rows, heads, dim, lanes, rows_per_block, pad_;
+    sox_turn_args turn;
+} sox_rotary_args;
+
+/* A batch over a paged cache. Page p is page_bytes at pool + p * page_bytes: K [heads][2^shift tokens][dim], at v_at V the
+ * same, and with 8-bit elements at ks_at / vs_at their scales [heads][2^shift] fp32. Sequence s: its new rows are
+ * starts[s] .. starts[s + 1] - 1, the last of its lengths[s] tokens; token t is in page tables[s * ldt + (t >> shift)]. */
+typedef struct sox_kv_view {
+    uint8_t* pool;
+    const int32_t* tables;
+    const int32_t* starts;
+    const int32_t* lengths;
+    int64_t ldt, page_bytes, v_at, ks_at, vs_at;
+    int32_t pages, table_pages, sequences, rows;
+    int32_t heads, dim, shift, pad_;
+} sox_kv_view;
+
+/* sox_kv_write_* (k, v: from; q, if any, turned into y) and sox_kv_read_* (k, v: to), tiled as sox_rotary_args. */
+typedef struct sox_kv_rows_args {
+    sox_kv_view b;
+    void* k;
+    void* v;
+    const void* q;
+    void* y;
+    int64_t ldk, ldv, ldq, ldy;
+    int32_t q_heads, lanes, rows_per_block, pad_;
+    sox_turn_args turn;
+} sox_kv_rows_args;
+
+/* sox_kv_few_* / sox_kv_many_* (kv_attend.h): workgroup = (split, row tile, kv head), kv head fastest, and their merge.
+ * Rows of a tile: 16 or 128 pairs (new row, query head of the kv head's group), in that order. only: every sequence's rows
+ * (0), or those of sequences of at most 16 pairs in the one kernel and of more in the other (1). With splits > 1 a row's
+ * partial results go to part [rows][q_heads][stride][dim] (sums of p v) and ml [rows][q_heads][stride][2] (reference, sum). */
+typedef struct sox_kv_attend_args {
+    sox_kv_view b;
+    const void* q;
+    void* y;
+    float* part;
+    float* ml;
+    int64_t ldq, ldy;
+    int32_t q_heads, group, window, only;
+    int32_t splits, stride, tiles, min_tokens; /* min_tokens: of a split */
+    float scale_log2;                 /* scale * log2(e) */
+    int32_t splits_few, splits_many;  /* of the merge: by a sequence's pairs */
+} sox_kv_attend_args;
+
 #ifdef __cplusplus
 }
 #endif

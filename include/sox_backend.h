@@ -383,6 +383,83 @@ typedef struct sox_block_norm_node_p {
     uint32_t operands;               /* SOX_BN_* */
 } sox_block_norm_node_p;
 
+/* ---- a transformer layer's attention while it serves (no counterpart in the reference) ----
+ * Rotary positions, a paged cache of keys and values with an 8-bit form, and the attention of new tokens over it. Objects,
+ * streams, matrices, threads, captures, errors and offline backends as for the 8-bit layers above; a matrix's row holds
+ * [heads][head_dim] elements. head_dim: a multiple of 8, 8 .. 256 (SOX_E_UNSUPPORTED for others up to 2^31 - 1).
+ * What a call reads of the device's integers (positions, a batch's tables, starts and lengths) it checks on the device: no
+ * value there leads outside of the buffers. */
+
+/* Pair j of a head (channels j and rotary_dim / 2 + j, or with interleaved 2 j and 2 j + 1), j < rotary_dim / 2, turned by
+ * position * frequency[j] radians and multiplied by amplitude; the channels from rotary_dim on stay as they are.
+ * frequency[j] = f (keep + (1 - keep) / factor), f = base^(-2 j / rotary_dim), and with original > 0, keep = (original * f /
+ * (2 pi) - low) / (high - low) held to 0 .. 1: frequencies that turn less than `low` times within `original` positions
+ * are divided by the factor, those of more than `high` turns kept; without (original = 0), keep = 0. Or frequencies given
+ * one by one. Angles are exact to 2^-33 of a turn at any position. */
+typedef struct sox_rotary_p {
+    int32_t head_dim, rotary_dim; /* rotary_dim: even, 2 .. head_dim */
+    int32_t interleaved;
+    int32_t original;             /* positions, 0: every frequency divided by the factor */
+    double base, factor, low, high, amplitude;
+} sox_rotary_p;
+typedef struct sox_rotary sox_rotary;
+/* frequencies [rotary_dim / 2] (finite) or NULL: from base, factor, original, low and high. */
+int sox_rotary_create(sox_backend* backend, const sox_rotary_p* params, const double* frequencies, sox_rotary** rotary);
+/* After the last call's work has run (and every captured one's last replay); as all of these. */
+void sox_rotary_destroy(sox_rotary* rotary);
+/* The frequencies in use, [rotary_dim / 2]. */
+int sox_rotary_frequencies(sox_rotary* rotary, double* frequencies);
+/* y = x turned, [rows][heads][head_dim]; positions: int32 [rows] on the device, any sign. y may be x itself (same ld). */
+int sox_rotary_run(sox_rotary* rotary, void* stream, int32_t storage, const int32_t* positions, const void* x, int64_t ldx,
+                   int32_t rows, int32_t heads, void* y, int64_t ldy);
+
+/* K and V of `page` tokens (a power of two, 1 .. 4096) of all kv_heads stand in one page of a pool that the caller owns, pages
+ * sox_kv_cache_page_bytes apart; their order within a page is the library's. format: the elements' SOX_STORAGE_* (then
+ * also of the rows written, read and attended with), or SOX_KV_INT8: 8 bits with a scale for each token and head,
+ * as sox_qlinear's rows (scale = amax / 127, q = rint(127 x / amax) of the head's values in fp32; a head with a NaN or an
+ * infinity is held as NaN), with rows of any storage. */
+enum { SOX_KV_INT8 = 3 };
+typedef struct sox_kv_cache_p {
+    int32_t kv_heads, head_dim, page, format;
+} sox_kv_cache_p;
+typedef struct sox_kv_cache sox_kv_cache;
+int sox_kv_cache_create(sox_backend* backend, const sox_kv_cache_p* params, sox_kv_cache** cache);
+void sox_kv_cache_destroy(sox_kv_cache* cache);
+uint64_t sox_kv_cache_page_bytes(sox_kv_cache* cache);
+
+/* A batch of sequences, on the device but for the counts. Sequence s has lengths[s] tokens, token t in page tables[s * ldt +
+ * t / page] of the pool, at t % page. Rows starts[s] .. starts[s + 1] - 1 of a call's matrices are its last tokens (row
+ * starts[s + 1] - 1 is token lengths[s] - 1); starts ascends from 0 or more to `rows` or less, and rows that are no
+ * sequence's, or of a token before its first, are left as they are. A table entry outside of 0 .. pages - 1, and a token past
+ * table_pages, is in no page: it is not written, read as zeros and not attended to. Two sequences may share pages that
+ * neither writes. */
+typedef struct sox_kv_batch {
+    void* pool;             /* pages * page_bytes, on a 256-byte boundary */
+    const int32_t* tables;  /* [sequences][table_pages], rows ldt apart */
+    const int32_t* starts;  /* [sequences + 1] */
+    const int32_t* lengths; /* [sequences] */
+    int64_t ldt;
+    int32_t pages, table_pages, sequences, rows;
+} sox_kv_batch;
+/* Writes the rows' k and v [rows][kv_heads][head_dim] to their pages, k turned by its token's position if there is a rotary
+ * (of this head_dim). q (or NULL) [rows][q_heads][head_dim]: y = q turned alike, in the same launch; y may be q itself (same ld). */
+int sox_kv_cache_write(sox_kv_cache* cache, void* stream, const sox_kv_batch* batch, int32_t storage, sox_rotary* rotary,
+                       const void* k, int64_t ldk, const void* v, int64_t ldv, const void* q, int64_t ldq, int32_t q_heads,
+                       void* y, int64_t ldy);
+/* Reads the rows' k and v back out of their pages. */
+int sox_kv_cache_read(sox_kv_cache* cache, void* stream, const sox_kv_batch* batch, int32_t storage, void* k, int64_t ldk,
+                      void* v, int64_t ldv);
+/* Workspace bytes that are enough for sox_kv_cache_attend at any number of rows and sequences up to these. */
+uint64_t sox_kv_cache_workspace(sox_kv_cache* cache, int32_t rows, int32_t sequences, int32_t q_heads);
+/* y [rows][q_heads][head_dim]: query head h (q_heads a multiple of kv_heads) attends with kv head h / (q_heads / kv_heads),
+ *   y = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j)  over the tokens j <= its own position,
+ * and with window > 0 over the last `window` of them. scale > 0; 0: 1 / sqrt(head_dim). Sums in fp32. A row without such a
+ * token (or with none but scores of minus infinity) gives zeros; tokens that a row does not see do not reach it, whatever they
+ * hold. The tokens' k and v have to be in the cache (the rows' own too). workspace: 16-byte aligned, held until the work has run. */
+int sox_kv_cache_attend(sox_kv_cache* cache, void* stream, const sox_kv_batch* batch, int32_t storage, const void* q, int64_t ldq,
+                        int32_t q_heads, void* y, int64_t ldy, float scale, int32_t window, void* workspace,
+                        uint64_t workspace_bytes);
+
 /* ---- image session (VkImageSession, Backends/Vulkan/VkImageSession.cs:7-297) ----
  * Image-to-image inference with the pixel conversions on the device, in the same stream as the model:
  * one upload of the bytes, the dispatches, one download. The model maps [1, 3, H, W] to [1, 3, H, W];

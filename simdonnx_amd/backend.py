@@ -714,3 +714,128 @@ class HipBlockNorm:
             self.close()
         except Exception:
             pass
+
+
+def _count(n: int) -> int:
+    """A count for a 32-bit argument: one that does not fit becomes -1, which the library refuses."""
+    return -1 if n >> 31 else n
+
+
+class HipRotary:
+    """Rotary positions (sox_rotary_* of include/sox_backend.h): pairs of a head's first `rotary_dim` channels turned by
+    position * frequency. `frequencies` [rotary_dim / 2] given, or base^(-2 j / rotary_dim), divided by `factor` (with
+    `original` > 0 only those that turn less than `high` times within that many positions, wholly below `low`).
+    Addresses and streams as for HipQuantLinear."""
+
+    def __init__(self, backend: HipBackend, head_dim: int, rotary_dim: Optional[int] = None, interleaved: bool = False,
+                 base: float = 10000.0, frequencies=None, factor: float = 1.0, original: int = 0, low: float = 1.0,
+                 high: float = 4.0, amplitude: float = 1.0):
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        f = None
+        if frequencies is not None:
+            f = np.ascontiguousarray(frequencies, dtype=np.float64).reshape(-1)
+            if f.size != rotary_dim // 2:
+                raise ValueError("frequencies must hold rotary_dim / 2 values")
+        p = N.RotaryP(_count(head_dim), _count(rotary_dim), int(bool(interleaved)), _count(original), base, factor, low, high,
+                      amplitude)
+        h = N.c_void_p()
+        N.check(N.backend().sox_rotary_create(backend.h, ctypes.byref(p), _address(f), ctypes.byref(h)), "Rotary")
+        self.h, self.head_dim, self.rotary_dim = h, head_dim, rotary_dim
+        self._run = N.backend().sox_rotary_run
+
+    @property
+    def frequencies(self) -> np.ndarray:
+        """The frequencies in use, [rotary_dim / 2], in radians a position."""
+        f = np.empty(self.rotary_dim // 2, np.float64)
+        N.check(N.backend().sox_rotary_frequencies(self.h, f.ctypes.data), "Rotary.Frequencies")
+        return f
+
+    def run(self, x: int, positions: int, rows: int, heads: int, y: int, storage: str = "f16", ldx: Optional[int] = None,
+            ldy: Optional[int] = None, stream: Optional[int] = None):
+        """y [rows, heads, head_dim] = x turned; positions: int32 [rows] on the device."""
+        n = heads * self.head_dim
+        rc = self._run(self.h, stream, STORAGE[storage], positions, x, n if ldx is None else ldx, _count(rows), _count(heads), y,
+                       n if ldy is None else ldy)
+        if rc:
+            N.check(rc, "Rotary.Run")
+
+    def close(self):
+        if self.h:
+            N.backend().sox_rotary_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class HipKvBatch:
+    """A batch of sequences over a HipKvCache's pages (sox_kv_batch of include/sox_backend.h), device addresses but for the
+    counts: tables int32 [sequences, table_pages] (rows `ldt` apart), starts int32 [sequences + 1], lengths int32 [sequences]."""
+
+    def __init__(self, pool: int, pages: int, tables: int, table_pages: int, starts: int, lengths: int, sequences: int, rows: int,
+                 ldt: Optional[int] = None):
+        self.p = N.KvBatch(pool, tables, starts, lengths, table_pages if ldt is None else ldt, _count(pages), _count(table_pages),
+                           _count(sequences), _count(rows))
+        self.ref = ctypes.byref(self.p)
+
+
+class HipKvCache:
+    """A paged cache of keys and values and the attention over it (sox_kv_cache_* of include/sox_backend.h). `format`: the
+    elements' storage type, or "i8": 8 bits with a scale for each token and head. The caller owns the pool, `page_bytes` for
+    each page. Addresses and streams as for HipQuantLinear; each call works on a HipKvBatch."""
+
+    def __init__(self, backend: HipBackend, kv_heads: int, head_dim: int, page: int = 16, format: str = "f16"):
+        p = N.KvCacheP(_count(kv_heads), _count(head_dim), _count(page), N.KV_INT8 if format == "i8" else STORAGE[format])
+        h = N.c_void_p()
+        N.check(N.backend().sox_kv_cache_create(backend.h, ctypes.byref(p), ctypes.byref(h)), "KvCache")
+        self.h, self.kv_heads, self.head_dim, self.page, self.format = h, kv_heads, head_dim, page, format
+        self.page_bytes = int(N.backend().sox_kv_cache_page_bytes(h))
+        b = N.backend()
+        self._write, self._read, self._attend = b.sox_kv_cache_write, b.sox_kv_cache_read, b.sox_kv_cache_attend
+
+    def write(self, batch: HipKvBatch, k: int, v: int, storage: str = "f16", ldk: Optional[int] = None, ldv: Optional[int] = None,
+              rotary: Optional[HipRotary] = None, q: Optional[int] = None, ldq: Optional[int] = None, q_heads: int = 0,
+              y: Optional[int] = None, ldy: Optional[int] = None, stream: Optional[int] = None):
+        """The rows' k (turned by `rotary`, if any) and v into their pages; with q, y = q turned in the same launch."""
+        n, m = self.kv_heads * self.head_dim, q_heads * self.head_dim
+        rc = self._write(self.h, stream, batch.ref, STORAGE[storage], None if rotary is None else rotary.h, k, n if ldk is None else ldk,
+                         v, n if ldv is None else ldv, q, m if ldq is None else ldq, _count(q_heads), y, m if ldy is None else ldy)
+        if rc:
+            N.check(rc, "KvCache.Write")
+
+    def read(self, batch: HipKvBatch, k: int, v: int, storage: str = "f16", ldk: Optional[int] = None, ldv: Optional[int] = None,
+             stream: Optional[int] = None):
+        """The rows' k and v [rows, kv_heads, head_dim] out of their pages."""
+        n = self.kv_heads * self.head_dim
+        rc = self._read(self.h, stream, batch.ref, STORAGE[storage], k, n if ldk is None else ldk, v, n if ldv is None else ldv)
+        if rc:
+            N.check(rc, "KvCache.Read")
+
+    def workspace(self, rows: int, sequences: int, q_heads: int) -> int:
+        """Bytes of workspace that are enough for `attend` at any number of rows and sequences up to these."""
+        return int(N.backend().sox_kv_cache_workspace(self.h, _count(rows), _count(sequences), _count(q_heads)))
+
+    def attend(self, batch: HipKvBatch, q: int, q_heads: int, y: int, storage: str = "f16", ldq: Optional[int] = None,
+               ldy: Optional[int] = None, scale: float = 0.0, window: int = 0, workspace: Optional[int] = None,
+               workspace_bytes: int = 0, stream: Optional[int] = None):
+        """y [rows, q_heads, head_dim]: the rows' attention over their sequences, causal, with window > 0 over the last `window`
+        tokens; scale 0: 1 / sqrt(head_dim)."""
+        n = q_heads * self.head_dim
+        rc = self._attend(self.h, stream, batch.ref, STORAGE[storage], q, n if ldq is None else ldq, _count(q_heads), y,
+                          n if ldy is None else ldy, scale, _count(window), workspace, workspace_bytes)
+        if rc:
+            N.check(rc, "KvCache.Attend")
+
+    def close(self):
+        if self.h:
+            N.backend().sox_kv_cache_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

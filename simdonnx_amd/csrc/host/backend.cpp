@@ -5635,3 +5635,377 @@ int sox_block_norm_run_quantized(sox_block_norm* N, void* stream, int32_t storag
 }
 
 }  // extern "C"
+
+// ---- a transformer layer's attention while it serves (kernels in kv_cache.hip, kv_attend.h) ----
+struct sox_rotary {
+    sox_backend* be = nullptr;
+    sox_rotary_p p{};
+    std::vector<double> frequencies;
+    DeviceBlock mem;  // their 64-bit fractions of a turn
+    void* fns[3] = {};
+
+    sox_turn_args turn() const { return {(const uint64_t*)mem.p, p.amplitude, p.rotary_dim / 2, p.interleaved != 0}; }
+};
+
+struct sox_kv_cache {
+    sox_backend* be = nullptr;
+    sox_kv_cache_p p{};
+    int shift = 0;
+    int64_t page_bytes = 0, v_at = 0, ks_at = 0, vs_at = 0;
+    void *write[3] = {}, *read[3] = {}, *few[3] = {}, *many[3] = {}, *merge[3] = {};  // by storage, null where the format has none
+};
+
+namespace {
+
+const char* const STORAGE_NAME[] = {"f32", "f16", "bf16"};  // by SOX_STORAGE_*
+
+void check_head_dim(const char* name, int32_t dim) {
+    if (dim <= 0) fail(SOX_E_INVALID, std::string(name) + ": head_dim");
+    if (dim > 256 || dim % 8) unsupported(std::string(name) + ": head_dim " + std::to_string(dim) + " is no multiple of 8 up to 256");
+}
+
+// 2^lanes lanes of 16 bytes hold a head's row
+int head_lanes(int dim, int64_t es) {
+    int lanes = 0;
+    while ((16 << lanes) < dim * es) lanes++;
+    return lanes;
+}
+// Rows of a workgroup: one where there are few, so that they spread over the CUs; four otherwise, which share the table's work
+int rows_per_block(int64_t rows, int cus) { return rows > 8 * cus ? 4 : 1; }
+
+// What a batch's calls check alike.
+struct KvCall : LayerCall {
+    const sox_kv_cache* cache;
+    const sox_kv_batch* batch;
+    Rows pool{"pool"}, tables{"tables"}, starts{"starts"}, lengths{"lengths"};
+
+    KvCall(sox_kv_cache* c, const sox_kv_batch* b, const char* name, int32_t storage)
+        : LayerCall(valid(c, b, name)->be, name, b->rows, storage), cache(c), batch(b) {
+        if (c->p.format != SOX_KV_INT8 && c->p.format != storage) bad("a cache of another storage");
+        if (b->sequences < 0 || b->sequences > 1 << 20) bad("sequences");
+        if (b->pages <= 0 || b->pages > ((int64_t)1 << 48) / c->page_bytes) bad("pages");
+        if (b->table_pages <= 0 || ((int64_t)b->table_pages << c->shift) > 1 << 30) bad("table_pages");
+        if (idle()) return;
+        pool = matrix("pool", b->pool, c->page_bytes * b->pages, c->page_bytes * b->pages, 1, 256, false, 1);
+        tables = matrix("tables", b->tables, b->ldt, b->table_pages, 4, 4, false, b->sequences);
+        starts = matrix("starts", b->starts, b->sequences + 1, b->sequences + 1, 4, 4, false, 1);
+        lengths = matrix("lengths", b->lengths, b->sequences, b->sequences, 4, 4, false, 1);
+    }
+    static sox_kv_cache* valid(sox_kv_cache* c, const sox_kv_batch* b, const char* name) {
+        if (!c || !b) fail(SOX_E_INVALID, std::string(name) + ": arguments");
+        return c;
+    }
+    bool idle() const { return rows == 0 || batch->sequences == 0; }  // (no row is a sequence's)
+    Rows heads(const char* what, const void* p, int64_t ld, int32_t n, bool optional = false) const {
+        return matrix(what, p, ld, (int64_t)n * cache->p.head_dim, optional);
+    }
+    sox_kv_view view() const {
+        sox_kv_view v{};
+        v.pool = (uint8_t*)batch->pool;
+        v.tables = batch->tables;
+        v.starts = batch->starts;
+        v.lengths = batch->lengths;
+        v.ldt = batch->ldt;
+        v.page_bytes = cache->page_bytes;
+        v.v_at = cache->v_at;
+        v.ks_at = cache->ks_at;
+        v.vs_at = cache->vs_at;
+        v.pages = batch->pages;
+        v.table_pages = batch->table_pages;
+        v.sequences = batch->sequences;
+        v.rows = (int32_t)rows;
+        v.heads = cache->p.kv_heads;
+        v.dim = cache->p.head_dim;
+        v.shift = cache->shift;
+        return v;
+    }
+    uint32_t grid(int64_t workgroups) const {
+        if (workgroups > 0x7fffffff) fail(SOX_E_UNSUPPORTED, std::string(name) + ": too many rows");
+        return (uint32_t)workgroups;
+    }
+};
+
+// Which kernels attend, with how many row tiles and splits each.
+//   few   tiles of 16 pairs (row, query head of a kv head's group): where single tokens are all there is
+//   many  tiles of 128
+//   both, each for its sequences, where a batch may hold single tokens and longer pieces
+// The host knows the rows of the whole batch alone; each kernel is right for every sequence.
+// Splits: so many that the workgroups fill the CUs about `fill` times, while a row's partial results stay within PARTIALS.
+struct AttendPlan {
+    static constexpr int64_t PARTIALS = 65536, MAX_SPLITS = 512;
+    bool use_few = false, use_many = false;
+    int64_t few_tiles = 0, many_tiles = 0;
+    int few_splits = 1, many_splits = 1;
+
+    AttendPlan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t tokens, int cus) {
+        const int64_t pairs = rows * (q_heads / kv_heads);
+        if (pairs <= 16 || (pairs <= 16 * sequences && rows <= 4 * sequences))
+            use_few = true;
+        else if (sequences == 1)
+            use_many = true;
+        else
+            use_few = use_many = true;
+        few_tiles = use_many ? sequences : pairs / 16 + sequences;
+        many_tiles = pairs / 128 + (use_few ? std::min(sequences, pairs / 17) : sequences);
+        if (use_few) few_splits = splits(few_tiles * kv_heads, rows * q_heads, tokens / MIN_FEW, 8 * cus);
+        if (use_many) many_splits = splits(many_tiles * kv_heads, rows * q_heads, tokens / MIN_MANY, 2 * cus);
+    }
+    static constexpr int MIN_FEW = 256, MIN_MANY = 256;  // tokens of a split at least
+    static int splits(int64_t workgroups, int64_t heads, int64_t most, int64_t fill) {
+        const int64_t n = std::min({(fill + workgroups - 1) / workgroups, most, MAX_SPLITS, PARTIALS / heads});
+        return (int)std::max<int64_t>(n, 1);
+    }
+    int stride() const { return std::max(few_splits, many_splits); }
+    static uint64_t of(int64_t partials, int dim) { return ((uint64_t)partials * ((uint64_t)dim * 4 + 8) + 15) / 16 * 16; }
+    static uint64_t bytes(int64_t heads, int dim) { return of(std::min(heads * MAX_SPLITS, PARTIALS), dim); }
+    uint64_t need(int64_t heads, int dim) const { return stride() > 1 ? of(heads * stride(), dim) : 0; }
+};
+
+// kv_attend.h's LDS
+uint32_t attend_lds(bool many, int dp, int es) {
+    const int pitch = dp * es;
+    if (many) {
+        const int tt = pitch >= 512 ? 32 : 64;
+        return (uint32_t)(4 * tt * pitch + 2 * 3 * tt * 4 + 64);
+    }
+    const int tt = es == 4 ? 16 : 32;
+    return (uint32_t)(4 * std::max(tt * pitch, 16 * (dp + 4) * 4) + 4 * 16 * 2 * 4);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sox_rotary_create(sox_backend* be, const sox_rotary_p* p, const double* frequencies, sox_rotary** out) {
+    return guarded([&] {
+        if (!be || !p || !out) fail(SOX_E_INVALID, "Rotary: arguments");
+        check_head_dim("Rotary", p->head_dim);
+        if (p->rotary_dim < 2 || p->rotary_dim > p->head_dim || p->rotary_dim % 2) fail(SOX_E_INVALID, "Rotary: rotary_dim has to be even, 2 to head_dim");
+        if (!std::isfinite(p->amplitude)) fail(SOX_E_INVALID, "Rotary: amplitude");
+        if (p->original < 0) fail(SOX_E_INVALID, "Rotary: original");
+        if (!frequencies) {
+            if (!(p->base > 0) || !std::isfinite(p->base)) fail(SOX_E_INVALID, "Rotary: base");
+            if (!(p->factor > 0) || !std::isfinite(p->factor)) fail(SOX_E_INVALID, "Rotary: factor");
+            if (p->original > 0 && (!std::isfinite(p->low) || !(p->high > p->low) || !std::isfinite(p->high))) fail(SOX_E_INVALID, "Rotary: low and high");
+        }
+        auto R = std::make_unique<sox_rotary>();
+        R->be = be;
+        R->p = *p;
+        const int half = p->rotary_dim / 2;
+        std::vector<uint64_t> turns;
+        for (int j = 0; j < half; j++) {
+            double f;
+            if (frequencies) {
+                f = frequencies[j];
+            } else {
+                f = std::pow(p->base, -(double)j / half);
+                double keep = 0;
+                if (p->original > 0) keep = std::min(1.0, std::max(0.0, (p->original * f / (2 * M_PI) - p->low) / (p->high - p->low)));
+                f *= keep + (1 - keep) / p->factor;
+            }
+            if (!std::isfinite(f)) fail(SOX_E_INVALID, "Rotary: frequencies have to be finite");
+            R->frequencies.push_back(f);
+            // whole turns do not matter, as positions are whole numbers
+            const long double turn = (long double)f / 6.283185307179586476925286766559L, part = turn - std::floor(turn);
+            turns.push_back(part >= 1.0L ? 0 : (uint64_t)(part * 18446744073709551616.0L));
+        }
+        R->mem.upload(be, turns.data(), turns.size() * 8, "Rotary frequencies");
+        for (int s = 0; s < 3; s++) R->fns[s] = be->fn(std::string("sox_rotary_") + STORAGE_NAME[s]);
+        *out = R.release();
+    });
+}
+
+void sox_rotary_destroy(sox_rotary* R) { delete R; }
+
+int sox_rotary_frequencies(sox_rotary* R, double* frequencies) {
+    if (!R || !frequencies) return SOX_E_INVALID;
+    memcpy(frequencies, R->frequencies.data(), R->frequencies.size() * 8);
+    return SOX_OK;
+}
+
+int sox_rotary_run(sox_rotary* R, void* stream, int32_t storage, const int32_t* positions, const void* x, int64_t ldx, int32_t rows,
+                   int32_t heads, void* y, int64_t ldy) {
+    return guarded([&] {
+        const char* name = "Rotary.Run";
+        if (!R) fail(SOX_E_INVALID, std::string(name) + ": arguments");
+        const LayerCall c(R->be, name, rows, storage);
+        if (heads <= 0 || heads > 1 << 16) c.bad("heads");
+        if (rows == 0) return;
+        const int64_t width = (int64_t)heads * R->p.head_dim;
+        const Rows P = c.matrix("positions", positions, rows, rows, 4, 4, false, 1), X = c.matrix("x", x, ldx, width), Y = c.matrix("y", y, ldy, width);
+        c.apart(Y, {&P}, {&X});
+        c.device(stream, {&P, &X, &Y});
+        sox_rotary_args a{};
+        a.x = x;
+        a.y = y;
+        a.positions = positions;
+        a.ldx = ldx;
+        a.ldy = ldy;
+        a.rows = rows;
+        a.heads = heads;
+        a.dim = R->p.head_dim;
+        a.lanes = head_lanes(a.dim, c.es);
+        a.rows_per_block = rows_per_block(rows, c.be->info.compute_units);
+        a.turn = R->turn();
+        c.launch(R->fns[storage], (uint32_t)((rows + a.rows_per_block - 1) / a.rows_per_block), 1, 256, stream, a);
+    });
+}
+
+int sox_kv_cache_create(sox_backend* be, const sox_kv_cache_p* p, sox_kv_cache** out) {
+    return guarded([&] {
+        if (!be || !p || !out) fail(SOX_E_INVALID, "KvCache: arguments");
+        check_head_dim("KvCache", p->head_dim);
+        if (p->kv_heads <= 0 || p->kv_heads > 1024) fail(SOX_E_INVALID, "KvCache: kv_heads");
+        if (p->page <= 0 || p->page > 4096 || (p->page & (p->page - 1))) fail(SOX_E_INVALID, "KvCache: page has to be a power of two up to 4096");
+        if (p->format < SOX_STORAGE_F32 || p->format > SOX_KV_INT8) fail(SOX_E_INVALID, "KvCache: format");
+        auto K = std::make_unique<sox_kv_cache>();
+        K->be = be;
+        K->p = *p;
+        while ((1 << K->shift) < p->page) K->shift++;
+        const bool quant = p->format == SOX_KV_INT8;
+        const int es = quant ? 1 : p->format == SOX_STORAGE_F32 ? 4 : 2;
+        const int64_t tokens = (int64_t)p->kv_heads * p->page;
+        auto up = [](int64_t v, int64_t to) { return (v + to - 1) / to * to; };
+        K->v_at = up(tokens * p->head_dim * es, 16);
+        K->ks_at = 2 * K->v_at;
+        K->vs_at = K->ks_at + up(quant ? tokens * 4 : 0, 16);
+        K->page_bytes = up(K->vs_at + (quant ? tokens * 4 : 0), 256);
+        const int dp = p->head_dim <= 64 ? 64 : p->head_dim <= 128 ? 128 : 256;
+        for (int s = 0; s < 3; s++) {
+            if (!quant && s != p->format) continue;
+            const std::string n = STORAGE_NAME[s] + std::string(quant ? "_i8" : ""), d = "_d" + std::to_string(dp);
+            K->write[s] = be->fn("sox_kv_write_" + n);
+            K->read[s] = be->fn("sox_kv_read_" + n);
+            K->few[s] = be->fn("sox_kv_few_" + n + d);
+            K->many[s] = be->fn("sox_kv_many_" + n + d);
+            K->merge[s] = be->fn(std::string("sox_kv_merge_") + STORAGE_NAME[s]);
+        }
+        *out = K.release();
+    });
+}
+
+void sox_kv_cache_destroy(sox_kv_cache* K) { delete K; }
+
+uint64_t sox_kv_cache_page_bytes(sox_kv_cache* K) { return K ? (uint64_t)K->page_bytes : 0; }
+
+int sox_kv_cache_write(sox_kv_cache* K, void* stream, const sox_kv_batch* batch, int32_t storage, sox_rotary* rotary, const void* k,
+                       int64_t ldk, const void* v, int64_t ldv, const void* q, int64_t ldq, int32_t q_heads, void* y, int64_t ldy) {
+    return guarded([&] {
+        const KvCall c(K, batch, "KvCache.Write", storage);
+        if (rotary && (rotary->be != K->be || rotary->p.head_dim != K->p.head_dim)) c.bad("a rotary of another head_dim or backend");
+        if (q && !rotary) c.bad("q without a rotary");
+        if (q && (q_heads <= 0 || q_heads > 1 << 16)) c.bad("q_heads");
+        if (c.idle()) return;
+        const Rows Kr = c.heads("k", k, ldk, K->p.kv_heads), V = c.heads("v", v, ldv, K->p.kv_heads);
+        Rows Q{"q"}, Y{"y"};
+        if (q) {
+            Q = c.heads("q", q, ldq, q_heads);
+            Y = c.heads("y", y, ldy, q_heads);
+        }
+        c.apart(c.pool, {&Kr, &V, &Q, &Y, &c.tables, &c.starts, &c.lengths});
+        c.apart(Y, {&Kr, &V, &c.tables, &c.starts, &c.lengths}, {&Q});
+        c.device(stream, {&c.pool, &c.tables, &c.starts, &c.lengths, &Kr, &V, &Q, &Y});
+        sox_kv_rows_args a{};
+        a.b = c.view();
+        a.k = const_cast<void*>(k);
+        a.v = const_cast<void*>(v);
+        a.q = q;
+        a.y = y;
+        a.ldk = ldk;
+        a.ldv = ldv;
+        a.ldq = ldq;
+        a.ldy = ldy;
+        a.q_heads = q ? q_heads : 0;
+        a.lanes = head_lanes(K->p.head_dim, c.es);
+        a.rows_per_block = rows_per_block(c.rows, c.be->info.compute_units);
+        if (rotary) a.turn = rotary->turn();
+        c.launch(K->write[storage], (uint32_t)((c.rows + a.rows_per_block - 1) / a.rows_per_block), 1, 256, stream, a);
+    });
+}
+
+int sox_kv_cache_read(sox_kv_cache* K, void* stream, const sox_kv_batch* batch, int32_t storage, void* k, int64_t ldk, void* v, int64_t ldv) {
+    return guarded([&] {
+        const KvCall c(K, batch, "KvCache.Read", storage);
+        if (c.idle()) return;
+        const Rows Kr = c.heads("k", k, ldk, K->p.kv_heads), V = c.heads("v", v, ldv, K->p.kv_heads);
+        c.apart(Kr, {&V, &c.pool, &c.tables, &c.starts, &c.lengths});
+        c.apart(V, {&c.pool, &c.tables, &c.starts, &c.lengths});
+        c.device(stream, {&c.pool, &c.tables, &c.starts, &c.lengths, &Kr, &V});
+        sox_kv_rows_args a{};
+        a.b = c.view();
+        a.k = k;
+        a.v = v;
+        a.ldk = ldk;
+        a.ldv = ldv;
+        a.lanes = head_lanes(K->p.head_dim, c.es);
+        a.rows_per_block = rows_per_block(c.rows, c.be->info.compute_units);
+        c.launch(K->read[storage], (uint32_t)((c.rows + a.rows_per_block - 1) / a.rows_per_block), 1, 256, stream, a);
+    });
+}
+
+uint64_t sox_kv_cache_workspace(sox_kv_cache* K, int32_t rows, int32_t sequences, int32_t q_heads) {
+    if (!K || rows <= 0 || rows > 1 << 23 || sequences <= 0 || q_heads <= 0 || q_heads > 1 << 16) return 0;
+    return AttendPlan::bytes((int64_t)rows * q_heads, K->p.head_dim);
+}
+
+int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch, int32_t storage, const void* q, int64_t ldq,
+                        int32_t q_heads, void* y, int64_t ldy, float scale, int32_t window, void* workspace, uint64_t workspace_bytes) {
+    return guarded([&] {
+        const KvCall c(K, batch, "KvCache.Attend", storage);
+        const int kv = K->p.kv_heads, dim = K->p.head_dim;
+        if (q_heads <= 0 || q_heads > 1 << 16 || q_heads % kv) c.bad("q_heads has to be a multiple of kv_heads");
+        if (!(scale >= 0) || !std::isfinite(scale)) c.bad("scale");
+        if (window < 0) c.bad("window");
+        if (c.idle()) return;
+        const Rows Q = c.heads("q", q, ldq, q_heads), Y = c.heads("y", y, ldy, q_heads);
+        const int64_t heads = c.rows * q_heads;
+        int64_t tokens = (int64_t)batch->table_pages << K->shift;
+        if (window) tokens = std::min(tokens, (int64_t)window + c.rows);
+        const AttendPlan plan(c.rows, batch->sequences, q_heads, kv, tokens, c.be->info.compute_units);
+        Rows W{"workspace"};
+        if (const uint64_t need = plan.need(heads, dim)) {
+            if (!workspace || workspace_bytes < need)
+                c.bad("needs " + std::to_string(need) + " bytes of workspace, has " + std::to_string(workspace ? workspace_bytes : 0));
+            W = c.matrix("workspace", workspace, (int64_t)need, (int64_t)need, 1, 16, false, 1);
+        }
+        c.apart(Y, {&Q, &W, &c.pool, &c.tables, &c.starts, &c.lengths});
+        c.apart(W, {&Q, &c.pool, &c.tables, &c.starts, &c.lengths});
+        c.device(stream, {&c.pool, &c.tables, &c.starts, &c.lengths, &Q, &Y, &W});
+        sox_kv_attend_args a{};
+        a.b = c.view();
+        a.q = q;
+        a.y = y;
+        a.ldq = ldq;
+        a.ldy = ldy;
+        a.q_heads = q_heads;
+        a.group = q_heads / kv;
+        a.window = window;
+        a.only = plan.use_few && plan.use_many;
+        a.stride = plan.stride();
+        a.part = (float*)workspace;
+        a.ml = workspace ? (float*)workspace + heads * a.stride * dim : nullptr;
+        a.scale_log2 = (float)((scale == 0 ? 1.0 / std::sqrt((double)dim) : (double)scale) * 1.4426950408889634);
+        a.splits_few = plan.few_splits;
+        a.splits_many = plan.many_splits;
+        if (!plan.use_few) a.splits_few = a.splits_many;  // (the merge asks by a sequence's pairs)
+        if (!plan.use_many) a.splits_many = a.splits_few;
+        const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256, es = (int)c.es;
+        const uint32_t few = c.grid(plan.few_tiles * kv * plan.few_splits), many = c.grid(plan.many_tiles * kv * plan.many_splits);
+        const uint32_t merge = a.stride > 1 ? c.grid(heads) : 0;
+        if (plan.use_many) {
+            a.splits = plan.many_splits;
+            a.tiles = (int32_t)plan.many_tiles;
+            a.min_tokens = AttendPlan::MIN_MANY;
+            c.launch(K->many[storage], many, 1, 256, stream, a, attend_lds(true, dp, es));
+        }
+        if (plan.use_few) {
+            a.splits = plan.few_splits;
+            a.tiles = (int32_t)plan.few_tiles;
+            a.min_tokens = AttendPlan::MIN_FEW;
+            c.launch(K->few[storage], few, 1, 256, stream, a, attend_lds(false, dp, es));
+        }
+        if (merge) c.launch(K->merge[storage], merge, 1, 256, stream, a);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,915 @@
+// Attention of new tokens over a paged cache: for each new row at position t of its sequence and each query head,
+//   y = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - reference),  j <= t and, with a window w, j > t - w
+// in one pass over the sequence's tokens with the running reference of a softmax. Two kernels:
+//   many  a workgroup takes 128 pairs (new row, query head of one kv head's group), 32 a wave, and walks the tokens tile by
+//         tile through LDS, which all of its waves read; bound by the matrix cores and the softmax between them
+//   few   16 pairs (a single new token's group): its waves walk different tokens, K straight to registers; bound by reading the
+//         cache
+// Both compute S^T = K Q^T, so a lane holds one pair's scores, 16 (or 8) tokens in its registers: the softmax needs no other
+// lane but for the maximum, and the scores, rounded, are as they stand the operand of O^T += V^T P^T. The token order within a
+// step is that of the score registers; V's rows are read to match it (transposing LDS reads for 16 bits).
+// The reference moves only when a score passes it by 2^8: what it leaves in p is divided out by the sum, and the outputs are
+// rescaled a few times, not once a tile. Sums and outputs in fp32; p is rounded to the storage type for its product (half a
+// step each, unbiased, on terms that the sum averages).
+// An 8-bit cache: k and v go into the products as whole numbers (exact in every storage type); k's scale multiplies the score,
+// v's p, before its rounding. In fp16, whose exponents end soon, v's scale goes into the exponent instead (2^(s + log2
+// scale), the reference bounds p times scale) and the sum divides it out again: exact while the scales span less than
+// 2^110, as fp16 rows' do (2^-31 to 2^9; scales below 2^-100 count as that).
+// Tokens that a row does not see add nothing, whatever their K and V hold: tokens that no row of the tile sees are not read,
+// masked scores are replaced, and a V that is not finite within a tile that is masked in part goes through without its values that are not finite (special4).
+#pragma once
+#include "kv_cache.h"
+
+constexpr int AT_THREADS = 256;
+constexpr float AT_SLACK = 8.0f;  // powers of two that p may stand above the reference
+
+// ---- storage types' steps ----
+template <typename T> struct Frag {  // 16 bytes of a row
+    static constexpr int E = 16 / sizeof(T);
+    typedef vec_t<T, E> V;
+};
+template <typename T> SOX_DEV float16v mma32(typename Frag<T>::V a, typename Frag<T>::V b, float16v c) {
+    if constexpr (sizeof(T) == 2) {
+        c = mfma32x32x16(a, b, c);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+    }
+    return c;
+}
+template <typename T> SOX_DEV float4v mma16(typename Frag<T>::V a, typename Frag<T>::V b, float4v c) {
+    if constexpr (sizeof(T) == 2) {
+        c = mfma16x16x32(a, b, c);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    }
+    return c;
+}
+
+// 16 bytes of the cache as they go to LDS: values of T
+template <typename T, typename C> struct Wide {
+    static constexpr int N = sizeof(T) / sizeof(C);  // 16-byte chunks of them
+    typename Frag<T>::V v[N];
+    SOX_DEV Wide of(int4v raw) {
+        Wide w;
+        if constexpr (N == 1) {
+            w.v[0] = __builtin_bit_cast(typename Frag<T>::V, raw);
+        } else {
+            constexpr int E = Frag<T>::E;
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int e = 0; e < E; e++) w.v[n][e] = (T)(float)(int8_t)(raw[(n * E + e) / 4] >> (n * E + e) % 4 * 8);
+        }
+        return w;
+    }
+};
+
+template <typename T> SOX_DEV bool any_not_finite(int4v raw) {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = (uint32_t)raw[i];
+        if constexpr (sizeof(T) == 4) {
+            bad |= (w & 0x7f800000u) == 0x7f800000u;
+        } else {
+            constexpr uint32_t EXP = std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
+            bad |= (w & EXP) == EXP || ((w >> 16) & EXP) == EXP;
+        }
+    }
+    return bad;
+}
+
+// Places of 16-byte chunks within LDS rows of CH chunks, so that what one read touches spreads over all banks: K's chunk by 16
+// rows (a chunk of 16 or 32 rows at once); V's, in 16 bits by 4 rows x 4 chunks (many) or 8 rows x 2 (few) of the transposing
+// reads, in 32 by rows 4 apart (8 chunks of two, or 4 of four)
+template <int CH> SOX_DEV int at_k(int row) { return CH >= 16 ? row & 15 : (row >> 1) & 7; }
+template <int CH, int BYTES, bool FEW> SOX_DEV int at_v(int row) {
+    if (BYTES == 4) return FEW ? row & 12 : (row & 4) << 1;
+    return CH >= 16 ? ((row & 3) << 2) | ((row >> 1) & 2) : (((row >> 1) & 1) << 2) | ((row >> 1) & 2);
+}
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+// Four values of a column from four rows for each lane: in each 16 lanes, lane l gives the address of columns 4 (l & 3) .. + 3
+// of row l / 4 and gets column l of the four
+SOX_DEV short4v read_columns(const unsigned char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p);
+}
+template <typename T> SOX_DEV typename Frag<T>::V join(short4v lo, short4v hi) {
+    typedef short short8v __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(typename Frag<T>::V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// ---- a value of V that is not finite, in a tile that some rows see in part ----
+// The matrix cores would carry 0 * inf into rows that do not see it, so such a tile goes through the product with those
+// values replaced by 0, and rows that see them get them from memory (special4).
+template <typename T> SOX_DEV int4v finite_only(int4v raw) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = (uint32_t)raw[i];
+        if constexpr (sizeof(T) == 4) {
+            raw[i] = (w & 0x7f800000u) == 0x7f800000u ? 0 : (int)w;
+        } else {
+            constexpr uint32_t EXP = std::is_same<T, half_t>::value ? 0x7c00u : 0x7f80u;
+            raw[i] = (int)(((w & EXP) == EXP ? 0u : w & 0xffffu) | ((w >> 16 & EXP) == EXP ? 0u : w & 0xffff0000u));
+        }
+    }
+    return raw;
+}
+// What four channels of a token's V add to a row that sees it: their values that are not finite
+template <typename T> SOX_DEV float4v special4(const T* v) {
+    typedef vec_t<T, 4> V4;
+    typedef V4 At __attribute__((aligned(sizeof(T))));
+    const V4 x = *(const At*)v;
+    float4v o;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float f = (float)x[e];
+        o[e] = abs_bits(f) < 0x7f800000u ? 0.0f : f;
+    }
+    return o;
+}
+
+template <int I, int N, class F> SOX_DEV void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<I + 1, N>(f);
+    }
+}
+
+// How v's scale in 8 bits takes part: not at all, as a factor of p, or in its exponent
+enum { SCALE_NONE, SCALE_FACTOR, SCALE_EXPONENT };
+template <typename T, typename C> constexpr int scale_form() {
+    return sizeof(C) == 1 ? std::is_same<T, half_t>::value ? SCALE_EXPONENT : SCALE_FACTOR : SCALE_NONE;
+}
+SOX_DEV float exponent_scale(float scale) { return __builtin_elementwise_maximum(scale, 0x1p-100f); }  // (a NaN stays one)
+
+// f of this lane's value and that of the lane 32 (or 16) away, in both
+template <class F> SOX_DEV float over_32(float v, F&& f) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <class F> SOX_DEV float over_16(float v, F&& f) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+SOX_DEV float larger(float a, float b) { return fmaxf(a, b); }
+SOX_DEV float added(float a, float b) { return a + b; }
+
+// ---- which rows a workgroup has ----
+struct RowTile {
+    int sequence, first;      // first: its first new row
+    int rows, pairs, m0;      // new rows and pairs of the sequence, first pair of the tile
+    int64_t length;           // tokens
+    bool some;
+};
+// The t-th tile of PAIRS pairs, counted over the sequences; every lane finds the same. `only` leaves out sequences of at most 16
+// pairs (LARGE) or of more.
+template <int PAIRS, bool LARGE> SOX_DEV RowTile row_tile(const sox_kv_attend_args& p, int t, int lane) {
+    RowTile r{};
+    int base = 0;
+    for (int c = 0; c < p.b.sequences; c += 64) {
+        int tiles = 0, first = 0, rows = 0;
+        if (c + lane < p.b.sequences) {
+            first = min(max(p.b.starts[c + lane], 0), p.b.rows);
+            rows = max(min(p.b.starts[c + lane + 1], p.b.rows) - first, 0);
+            const int64_t pairs = (int64_t)rows * p.group;
+            if (!p.only || (pairs > 16) == LARGE) tiles = (int)((pairs + PAIRS - 1) / PAIRS);
+        }
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(sum, o);
+            if (lane >= o) sum += v;
+        }
+        const uint64_t past = __ballot(base + sum > t);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            r.sequence = c + l;
+            r.first = __builtin_amdgcn_readlane(first, l);
+            r.rows = __builtin_amdgcn_readlane(rows, l);
+            r.pairs = r.rows * p.group;
+            // (a sequence's later tiles, which see more, start first)
+            const int before = base + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l);
+            r.m0 = (__builtin_amdgcn_readlane(tiles, l) - 1 - (t - before)) * PAIRS;
+            r.length = max(p.b.lengths[r.sequence], 0);
+            r.some = true;
+            return r;
+        }
+        base += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return r;
+}
+
+// The tokens of a tile of rows, and a split's share of them in steps of TT
+struct Span {
+    int lo, hi;              // tokens that any row sees
+    int begin, end;          // of this split, begin a multiple of TT
+    int pos_first, pos_last; // positions of the tile's first and last row
+};
+template <int PAIRS, int TT> SOX_DEV Span span_of(const sox_kv_attend_args& p, const RowTile& r, int split, int splits) {
+    Span s;
+    const int64_t base = r.length - r.rows;
+    const int last = min(r.m0 + PAIRS, r.pairs) - 1;
+    s.pos_first = (int)(base + r.m0 / p.group);
+    s.pos_last = (int)(base + last / p.group);
+    s.lo = p.window > 0 ? max(s.pos_first - p.window + 1, 0) : 0;
+    s.hi = (int)min((int64_t)s.pos_last + 1, (int64_t)p.b.table_pages << p.b.shift);
+    const int from = s.lo / TT * TT, tiles = max((s.hi - from + TT - 1) / TT, 0);
+    const int per = max((tiles + splits - 1) / splits, (p.min_tokens + TT - 1) / TT);
+    s.begin = min(from + (int)min((int64_t)split * per * TT, (int64_t)1 << 30), max(s.hi, from));
+    s.end = min(s.begin + per * TT, s.hi);
+    return s;
+}
+
+// A lane's token of a tile: its page, or -1; only tokens of [lo, hi) are looked up
+SOX_DEV int tile_page(const sox_kv_view& b, const int32_t* table, int token, int lo, int hi) {
+    return token >= lo && token < hi ? kv_page(b, table, token) : -1;
+}
+
+// Where a row's results go
+template <typename T> struct RowOut {
+    T* y;
+    float* part;
+    float* ml;
+};
+template <typename T> SOX_DEV RowOut<T> row_out(const sox_kv_attend_args& p, const RowTile& r, int kvh, int m, int split) {
+    const int64_t row = r.first + m / p.group;
+    const int head = kvh * p.group + m % p.group;
+    const int64_t at = (row * p.q_heads + head) * p.stride + split;
+    return {(T*)p.y + row * p.ldy + (int64_t)head * p.b.dim, p.part + at * p.b.dim, p.ml + at * 2};
+}
+template <typename T> SOX_DEV const T* row_q(const sox_kv_attend_args& p, const RowTile& r, int kvh, int m) {
+    return (const T*)p.q + (int64_t)(r.first + m / p.group) * p.ldq + (int64_t)(kvh * p.group + m % p.group) * p.b.dim;
+}
+template <typename T> SOX_DEV void store4(T* to, float4v v) {
+    typedef vec_t<T, 4> V4;
+    typedef V4 At __attribute__((aligned(sizeof(T))));
+    fp32_rounded(v);
+    *(At*)to = __builtin_convertvector(v, V4);
+}
+// A chunk of q, zeros past the head's channels
+template <typename T> SOX_DEV typename Frag<T>::V load_q(const T* q, int ch, int dim, bool valid) {
+    typename Frag<T>::V v = {};
+    if (valid && ch < dim) v = *(const typename Chunk16<T>::At*)(q + ch);
+    return v;
+}
+
+// The running reference and sum of a lane's pair. Scores in powers of two.
+struct Soft {
+    float ref = -__builtin_inff(), sum = 0.0f;
+    SOX_DEV float of(float ref) { return ref == -__builtin_inff() ? 0.0f : ref; }  // (nothing seen yet: any reference will do)
+    // moves the reference to `top` where it passes it by AT_SLACK; what the sum and the outputs are to be multiplied by
+    __device__ __forceinline__ float move(float top) {
+        const float now = fmaxf(ref, top);
+        const float by = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - now);
+        ref = now;
+        sum *= by;
+        return by;
+    }
+};
+
+// =====================================================================================================================
+// many: 128 pairs, 4 waves of 32, tiles of TT tokens through LDS
+// =====================================================================================================================
+template <typename T, typename C, int DP> struct Many {
+    static constexpr int FORM = scale_form<T, C>();
+    static constexpr bool QUANT = FORM != SCALE_NONE;
+    static constexpr int E = Frag<T>::E, CH = DP / E, KS = CH / 2, PITCH = DP * (int)sizeof(T);
+    static constexpr int TT = PITCH >= 512 ? 32 : 64, TB = TT / 32, DB = DP / 32;
+    static constexpr int EC = 16 / (int)sizeof(C), UR = DP / EC, NCH = Wide<T, C>::N;  // values of a unit of 16 bytes of the cache, units of a row
+    static constexpr int SU = TT * UR / AT_THREADS;                                     // units a thread stages
+    static constexpr int BUF = 2 * TT * PITCH;                                          // K and V of a tile
+    static constexpr int LDS = 2 * BUF + 2 * 3 * TT * 4 + 64;
+    static constexpr int WAVES = PITCH > 256 ? 1 : 2;  // on a SIMD
+    static constexpr bool AHEAD = PITCH <= 512;        // the next tile's loads in flight behind a tile (beyond, registers are short)
+    static_assert(SU >= 1 && TT * UR % AT_THREADS == 0, "staging");
+};
+
+template <typename T, typename C, int DP> __device__ __forceinline__ void attend_many(const sox_kv_attend_args& p) {
+    typedef Many<T, C, DP> M;
+    typedef typename Frag<T>::V FV;
+    constexpr bool QUANT = M::QUANT;
+    constexpr int FORM = M::FORM;
+    constexpr int TT = M::TT, TB = M::TB, DB = M::DB, E = M::E;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    float(*const scales)[3][TT] = (float(*)[3][TT])(lds + 2 * M::BUF);
+    int* const flags = (int*)(lds + 2 * M::BUF + 2 * 3 * TT * 4);  // [buffer][wave]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
+    const sox_kv_view& b = p.b;
+    const int kvh = blockIdx.x % b.heads, rest = blockIdx.x / b.heads, split = rest % p.splits;
+    const RowTile r = row_tile<128, true>(p, rest / p.splits, lane);
+    if (!r.some) return;
+    const Span s = span_of<128, TT>(p, r, split, p.splits);
+    const int32_t* const table = b.tables + r.sequence * b.ldt;
+    const int mask = (1 << b.shift) - 1, es = (int)sizeof(C);
+    const int64_t scale_at = tid < TT ? b.ks_at : b.vs_at;  // of what this thread stages of the scales
+
+    // this lane's pair
+    const int m = r.m0 + 32 * wave + col;
+    const bool mine = m < r.pairs;
+    const int pos = mine ? (int)(r.length - r.rows + m / p.group) : -1, low = p.window > 0 ? pos - p.window : -1;
+    const int wave_last = r.m0 + 32 * wave < r.pairs ? (int)(r.length - r.rows + (min(r.m0 + 32 * wave + 32, r.pairs) - 1) / p.group) : -1;
+    FV qf[M::KS];
+    {
+        const T* const q = row_q<T>(p, r, kvh, mine ? m : r.m0);
+#pragma unroll
+        for (int ks = 0; ks < M::KS; ks++) qf[ks] = load_q<T>(q, (2 * ks + half) * E, b.dim, mine);
+    }
+    float16v out[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++) out[d] = float16v{};
+    Soft soft;
+
+    // ---- staging ----
+    int4v raw_k[M::SU], raw_v[M::SU];
+    float raw_s = 0.0f;  // threads 0 .. TT - 1: K's scale of their token, TT .. 2 TT - 1: V's
+    auto lookup = [&](int t0) { return lane < TT ? tile_page(b, table, t0 + lane, s.lo, s.end) : -1; };
+    auto thread = [&] {  // (in the widest instances not to be worked with ahead of the loop: registers are short)
+        int t = tid;
+        if constexpr (!M::AHEAD) asm volatile("" : "+v"(t));
+        return t;
+    };
+    auto load = [&](int t0, int pages, int from = 0, int to = M::SU) {
+        const int tid = thread();
+#pragma unroll
+        for (int j = from; j < to; j++) {
+            const int u = j * AT_THREADS + tid, row = u / M::UR, c = u % M::UR;
+            const int page = M::UR == 64 ? __builtin_amdgcn_readlane(pages, 4 * j + wave) : __shfl(pages, row);
+            raw_k[j] = raw_v[j] = int4v{};
+            if (page >= 0 && c * M::EC < b.dim) {
+                typedef int4v At __attribute__((aligned(4)));
+                const uint8_t* at = b.pool + page * b.page_bytes + ((((int64_t)kvh << b.shift) + ((t0 + row) & mask)) * b.dim + c * M::EC) * es;
+                raw_k[j] = *(const At*)at;
+                raw_v[j] = *(const At*)(at + b.v_at);
+            }
+        }
+        if constexpr (QUANT) {
+            const int page = __shfl(pages, tid & (TT - 1));
+            raw_s = 0.0f;
+            if (tid < 2 * TT && page >= 0)
+                raw_s = *(const float*)(b.pool + page * b.page_bytes + scale_at + (((int64_t)kvh << b.shift) + ((t0 + (tid & (TT - 1))) & mask)) * 4);
+        }
+    };
+    bool bad = false;
+    auto store = [&](int buf, bool check, int from = 0, int to = M::SU) {
+        const int tid = thread();
+        unsigned char* const lk = lds + buf * M::BUF;
+        unsigned char* const lv = lk + TT * M::PITCH;
+        if (from == 0) bad = false;
+#pragma unroll
+        for (int j = from; j < to; j++) {
+            const int u = j * AT_THREADS + tid, row = u / M::UR, c = (u % M::UR) * M::NCH;
+            if constexpr (!QUANT) {
+                if (check) {
+                    bad |= any_not_finite<T>(raw_v[j]);
+                    raw_v[j] = finite_only<T>(raw_v[j]);
+                }
+            }
+            const Wide<T, C> k = Wide<T, C>::of(raw_k[j]), v = Wide<T, C>::of(raw_v[j]);
+#pragma unroll
+            for (int n = 0; n < M::NCH; n++) {
+                *(FV*)(lk + row * M::PITCH + (((c + n) ^ at_k<M::CH>(row)) << 4)) = k.v[n];
+                *(FV*)(lv + row * M::PITCH + (((c + n) ^ at_v<M::CH, sizeof(T), false>(row)) << 4)) = v.v[n];
+            }
+            if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (QUANT) {
+            if (tid < TT) {
+                scales[buf][0][tid] = raw_s * p.scale_log2;
+            } else if (tid < 2 * TT) {
+                if constexpr (FORM == SCALE_EXPONENT) {
+                    const float v = exponent_scale(raw_s);
+                    scales[buf][1][tid - TT] = __builtin_amdgcn_logf(v);
+                    scales[buf][2][tid - TT] = 1.0f / v;
+                } else {
+                    scales[buf][1][tid - TT] = raw_s;
+                }
+            }
+        } else if (check) {
+            const bool any = __any(bad);
+            if (lane == 0) flags[buf * 4 + wave] = any;
+        }
+    };
+    // a tile that some row sees in part
+    auto in_part = [&](int t0, uint64_t valid) {
+        return t0 + TT - 1 > s.pos_first || (p.window > 0 && t0 <= s.pos_last - p.window) || ~valid << (64 - TT) != 0;
+    };
+
+    // ---- a tile ----
+    auto tile = [&](int t0, int buf, uint64_t valid, bool part) {
+        const unsigned char* const lk = lds + buf * M::BUF;
+        const unsigned char* const lv = lk + TT * M::PITCH;
+        float16v acc[TB];
+#pragma unroll
+        for (int tb = 0; tb < TB; tb++) acc[tb] = float16v{};
+#pragma unroll
+        for (int ks = 0; ks < M::KS; ks++)
+#pragma unroll
+            for (int tb = 0; tb < TB; tb++) {
+                const int row = 32 * tb + col;
+                const FV kf = *(const FV*)(lk + row * M::PITCH + (((2 * ks + half) ^ at_k<M::CH>(row)) << 4));
+                acc[tb] = mma32<T>(kf, qf[ks], acc[tb]);
+                if ((ks % 2 || sizeof(T) == 4) && tb == TB - 1) __builtin_amdgcn_sched_barrier(0);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        // register i of block tb: token t0 + 32 tb + 8 (i / 4) + 4 half + i % 4
+        auto token = [&](int tb, int i) { return 32 * tb + 8 * (i >> 2) + 4 * half + (i & 3); };
+        // tokens as this lane counts them, from its first one on: constants below
+        const uint64_t there = valid >> (4 * half);
+        const int until = pos - t0 - 4 * half, after = low - t0 - 4 * half;
+        auto seen = [&](int tb, int i) {
+            const int t = 32 * tb + 8 * (i >> 2) + (i & 3);
+            return (t <= until) & (t > after) & (int)((t < 32 ? (uint32_t)there : (uint32_t)(there >> 32)) >> t % 32 & 1);
+        };
+        float x[TB][16];
+#pragma unroll
+        for (int tb = 0; tb < TB; tb++)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; i4++) {
+                float4v ks4, lv4;
+                if constexpr (QUANT) ks4 = *(const float4v*)&scales[buf][0][token(tb, 4 * i4)];
+                if constexpr (FORM == SCALE_EXPONENT) lv4 = *(const float4v*)&scales[buf][1][token(tb, 4 * i4)];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float a = acc[tb][4 * i4 + e];
+                    x[tb][4 * i4 + e] = FORM == SCALE_EXPONENT ? __builtin_fmaf(a, ks4[e], lv4[e]) : a * (QUANT ? ks4[e] : p.scale_log2);
+                }
+                if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
+            }
+        if (part) {
+#pragma unroll
+            for (int tb = 0; tb < TB; tb++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[tb][i] = seen(tb, i) ? x[tb][i] : -__builtin_inff();
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int tb = 0; tb < TB; tb++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, x[tb][i]);
+        if (__any(top > soft.ref + AT_SLACK)) {
+            const float by = soft.move(over_32(top, larger));
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                out[d] *= by;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        const float ref = Soft::of(soft.ref);
+#pragma unroll
+        for (int tb = 0; tb < TB; tb++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[tb][i] = __builtin_amdgcn_exp2f(x[tb][i] - ref);
+        // the sum, and p as it meets v (a hidden token's scale may be a NaN)
+#pragma unroll
+        for (int tb = 0; tb < TB; tb++)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; i4++) {
+                float4v v4;
+                if constexpr (QUANT) v4 = *(const float4v*)&scales[buf][FORM == SCALE_EXPONENT ? 2 : 1][token(tb, 4 * i4)];
+                if (QUANT && part) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v4[e] = seen(tb, 4 * i4 + e) ? v4[e] : 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float& a = x[tb][4 * i4 + e];
+                    soft.sum = FORM == SCALE_EXPONENT ? __builtin_fmaf(a, v4[e], soft.sum) : soft.sum + a;
+                    if constexpr (FORM == SCALE_FACTOR) a *= v4[e];
+                }
+                if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
+            }
+        // O^T += V^T P^T
+        auto v_at = [&](int row, int ch) { return lv + row * M::PITCH + (((ch / E) ^ at_v<M::CH, sizeof(T), false>(row)) << 4) + ch % E * (int)sizeof(T); };
+        if constexpr (sizeof(T) == 2) {
+            auto v_frag = [&](int tb, int s2, int d) {
+                const int row = 32 * tb + 16 * s2 + 4 * half + ((lane & 15) >> 2), ch = 32 * d + (lane & 16) + 4 * (lane & 3);
+                return join<T>(read_columns(v_at(row, ch)), read_columns(v_at(row + 8, ch)));
+            };
+#pragma unroll
+            for (int tb = 0; tb < TB; tb++)
+#pragma unroll
+                for (int s2 = 0; s2 < 2; s2++) {
+                    FV pf;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) pf[e] = (T)x[tb][8 * s2 + e];
+#pragma unroll
+                    for (int d = 0; d < DB; d++) out[d] = mfma32x32x16(v_frag(tb, s2, d), pf, out[d]);
+                    __builtin_amdgcn_sched_barrier(0);  // a step's fragments at a time: bounded register pressure
+                }
+        } else {
+#pragma unroll
+            for (int tb = 0; tb < TB; tb++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+#pragma unroll
+                    for (int d = 0; d < DB; d++) {
+                        out[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*(const T*)v_at(token(tb, i), 32 * d + col), x[tb][i], out[d], 0, 0, 0);
+                        if (d % 4 == 3 || d == DB - 1) __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+        }
+        if constexpr (!QUANT) {
+            if (part && (flags[buf * 4] | flags[buf * 4 + 1] | flags[buf * 4 + 2] | flags[buf * 4 + 3])) {
+#pragma unroll 1
+                for (int t = 0; t < TT; t++) {
+                    if (!((valid >> t) & 1)) continue;
+                    const T* const v = (const T*)(b.pool + kv_page(b, table, t0 + t) * b.page_bytes + b.v_at) + (((int64_t)kvh << b.shift) + ((t0 + t) & mask)) * b.dim;
+                    if (t0 + t > pos || t0 + t <= low) continue;
+#pragma unroll
+                    for (int d = 0; d < DB; d++)
+#pragma unroll
+                        for (int i4 = 0; i4 < 4; i4++) {
+                            const int ch = 32 * d + 8 * i4 + 4 * half;
+                            if (ch >= b.dim) continue;
+                            const float4v add = special4(v + ch);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) out[d][4 * i4 + e] += add[e];
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                }
+            }
+        }
+    };
+
+    // ---- the tokens ----
+    if (s.begin < s.end) {
+        int pages = lookup(s.begin);
+        uint64_t valid = __ballot(pages >= 0);
+        bool part = in_part(s.begin, valid);
+        // a tile's units one after the other
+        auto load_and_store = [&](int t0, int buf, bool check) {
+            static_for<0, M::SU>([&](auto j) {
+                constexpr int at = decltype(j)::value;
+                __builtin_amdgcn_sched_barrier(0);
+                load(t0, pages, at, at + 1);
+                store(buf, check, at, at + 1);
+            });
+        };
+        if constexpr (M::AHEAD) {
+            load(s.begin, pages);
+            store(0, part);
+        } else {
+            load_and_store(s.begin, 0, part);
+        }
+        pages = lookup(s.begin + TT);
+        __syncthreads();
+        int buf = 0;
+        for (int t0 = s.begin; t0 < s.end; t0 += TT, buf ^= 1) {
+            const bool more = t0 + TT < s.end;
+            const uint64_t next_valid = __ballot(pages >= 0);
+            const bool next_part = in_part(t0 + TT, next_valid);
+            if (M::AHEAD && more) {
+                load(t0 + TT, pages);
+                pages = lookup(t0 + 2 * TT);
+            }
+            if (t0 <= wave_last) tile(t0, buf, valid, part);
+            if (!M::AHEAD && more) {
+                pages = lookup(t0 + TT);  // (again, rather than held behind the tile)
+                load_and_store(t0 + TT, buf ^ 1, next_part);
+                pages = lookup(t0 + 2 * TT);
+            }
+            if (M::AHEAD && more) store(buf ^ 1, next_part);
+            __syncthreads();
+            valid = next_valid;
+            part = next_part;
+        }
+    }
+
+    // ---- out ----  (the pair from the lane number anew: held through the loop, it would cost the widest instances a spill)
+    soft.sum = over_32(soft.sum, added);
+    const int me = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), to = r.m0 + 32 * wave + (me & 31), upper = me >> 5;
+    if (to >= r.pairs || r.length - r.rows + to / p.group < 0) return;
+    const RowOut<T> o = row_out<T>(p, r, kvh, to, split);
+    if (p.splits > 1) {
+        if (upper == 0) o.ml[0] = soft.ref, o.ml[1] = soft.sum;
+        if (s.begin >= s.end) return;
+    }
+    const float inv = p.splits > 1 ? 1.0f : soft.sum == 0.0f ? 0.0f : 1.0f / soft.sum;
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; i4++) {
+            const int ch = 32 * d + 8 * i4 + 4 * upper;
+            float4v v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = out[d][4 * i4 + e] * inv;
+            if (ch >= b.dim) continue;
+            if (p.splits > 1)
+                *(float4v*)(o.part + ch) = v;
+            else
+                store4(o.y + ch, v);
+        }
+}
+
+// =====================================================================================================================
+// few: 16 pairs, 4 waves that walk every fourth tile of TT tokens each
+// =====================================================================================================================
+template <typename T, typename C, int DP> struct Few {
+    static constexpr int FORM = scale_form<T, C>();
+    static constexpr bool QUANT = FORM != SCALE_NONE;
+    static constexpr int E = Frag<T>::E, CH = DP / E, PITCH = DP * (int)sizeof(T);
+    static constexpr int TT = sizeof(T) == 4 ? 16 : 32 /* at most 32: the bits of a word */, NB = TT / 16, DB = DP / 16;
+    static constexpr int EC = 16 / (int)sizeof(C), UR = DP / EC, NCH = Wide<T, C>::N;
+    static constexpr int SU = TT * UR / 64;  // units of V a lane stages
+    static constexpr int KU = UR / 4;        // units of K a lane loads of each of its rows
+    static constexpr int OP = DP + 4;        // floats from pair to pair of a wave's results
+    static constexpr int BUF = TT * PITCH > 16 * OP * 4 ? TT * PITCH : 16 * OP * 4;
+    static constexpr int LDS = 4 * BUF + 4 * 16 * 2 * 4;
+    static constexpr int WAVES = PITCH > 256 ? 1 : 2;
+    static_assert(SU >= 1 && TT * UR % 64 == 0 && KU >= 1, "staging");
+};
+
+template <typename T, typename C, int DP> __device__ __forceinline__ void attend_few(const sox_kv_attend_args& p) {
+    typedef Few<T, C, DP> F;
+    typedef typename Frag<T>::V FV;
+    constexpr bool QUANT = F::QUANT;
+    constexpr int FORM = F::FORM;
+    constexpr int TT = F::TT, NB = F::NB, DB = F::DB, E = F::E;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, col = lane & 15;
+    const sox_kv_view& b = p.b;
+    const int kvh = blockIdx.x % b.heads, rest = blockIdx.x / b.heads, split = rest % p.splits;
+    const RowTile r = row_tile<16, false>(p, rest / p.splits, lane);
+    if (!r.some) return;
+    const Span s = span_of<16, TT>(p, r, split, p.splits);
+    const int32_t* const table = b.tables + r.sequence * b.ldt;
+    const int mask = (1 << b.shift) - 1, es = (int)sizeof(C);
+    unsigned char* const lv = lds + wave * F::BUF;
+    float* const ends = (float*)(lds + 4 * F::BUF);  // [wave][pair][reference, sum]
+
+    const int m = r.m0 + col;
+    const bool mine = m < r.pairs;
+    const int pos = mine ? (int)(r.length - r.rows + m / p.group) : -1, low = p.window > 0 ? pos - p.window : -1;
+    FV qf[F::KU][F::NCH];
+    {
+        const T* const q = row_q<T>(p, r, kvh, mine ? m : r.m0);
+#pragma unroll
+        for (int u = 0; u < F::KU; u++)
+#pragma unroll
+            for (int n = 0; n < F::NCH; n++) qf[u][n] = load_q<T>(q, (4 * u + quad) * F::EC + n * E, b.dim, mine);
+    }
+    float4v out[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++) out[d] = float4v{};
+    Soft soft;
+
+    int4v raw_k[NB][F::KU], raw_v[F::SU];
+    float4v ks4[NB], vs4[NB];  // scales of the tokens of this lane's scores
+    typedef int4v At __attribute__((aligned(4)));
+    auto lookup = [&](int t0) { return lane < TT ? tile_page(b, table, t0 + lane, s.lo, s.end) : -1; };
+    auto row_at = [&](int t0, int page, int row) { return b.pool + page * b.page_bytes + (((int64_t)kvh << b.shift) + ((t0 + row) & mask)) * (int64_t)(b.dim * es); };
+    auto load_k = [&](int t0, int pages) {
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+            const int row = 16 * n + col, page = __shfl(pages, row);
+            const uint8_t* const at = row_at(t0, page, row);
+#pragma unroll
+            for (int u = 0; u < F::KU; u++) {
+                raw_k[n][u] = int4v{};
+                if (page >= 0 && (4 * u + quad) * F::EC < b.dim) raw_k[n][u] = *(const At*)(at + (4 * u + quad) * 16);
+            }
+            if constexpr (QUANT) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int t = 16 * n + 4 * quad + e, pg = __shfl(pages, t);
+                    ks4[n][e] = vs4[n][e] = 0.0f;
+                    if (pg >= 0) {
+                        const uint8_t* const sc = b.pool + pg * b.page_bytes + (((int64_t)kvh << b.shift) + ((t0 + t) & mask)) * 4;
+                        ks4[n][e] = *(const float*)(sc + b.ks_at);
+                        vs4[n][e] = *(const float*)(sc + b.vs_at);
+                    }
+                }
+            }
+        }
+    };
+    auto load_v = [&](int t0, int pages) {
+#pragma unroll
+        for (int j = 0; j < F::SU; j++) {
+            const int u = j * 64 + lane, row = u / F::UR, c = u % F::UR, page = __shfl(pages, row);
+            raw_v[j] = int4v{};
+            if (page >= 0 && c * F::EC < b.dim) raw_v[j] = *(const At*)(row_at(t0, page, row) + b.v_at + c * 16);
+        }
+    };
+    auto v_at = [&](int row, int ch) { return lv + row * F::PITCH + (((ch / E) ^ at_v<F::CH, sizeof(T), true>(row)) << 4) + ch % E * (int)sizeof(T); };
+
+    const int stride = 4 * TT;
+    int t0 = s.begin + wave * TT;
+    int pages = lookup(t0), next_pages = lookup(t0 + stride);
+    if (t0 < s.end) {
+        load_k(t0, pages);
+        load_v(t0, pages);
+    }
+    for (; t0 < s.end; t0 += stride) {
+        const uint64_t valid = __ballot(pages >= 0);
+        const bool part = t0 + TT - 1 > s.pos_first || (p.window > 0 && t0 <= s.pos_last - p.window) || ~valid << (64 - TT) != 0;
+        const bool more = t0 + stride < s.end;
+        // S^T = K Q^T: register e of block n is token t0 + 16 n + 4 quad + e
+        float4v acc[NB];
+        float vsc[NB][4];  // what v's scales are to p or the sum
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+            acc[n] = float4v{};
+#pragma unroll
+            for (int u = 0; u < F::KU; u++) {
+                const Wide<T, C> k = Wide<T, C>::of(raw_k[n][u]);
+#pragma unroll
+                for (int x = 0; x < F::NCH; x++) acc[n] = mma16<T>(k.v[x], qf[u][x], acc[n]);
+                if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        bool special = false;
+        if constexpr (!QUANT) {
+            if (part) {
+                bool bad = false;
+#pragma unroll
+                for (int j = 0; j < F::SU; j++) {
+                    bad |= any_not_finite<T>(raw_v[j]);
+                    raw_v[j] = finite_only<T>(raw_v[j]);
+                }
+                special = __any(bad);
+            }
+        }
+        // tokens as this lane counts them, from its first one on: constants below
+        const uint32_t there = (uint32_t)(valid >> (4 * quad));
+        const int until = pos - t0 - 4 * quad, after = low - t0 - 4 * quad;
+        auto seen = [&](int t) { return (t <= until) & (t > after) & (int)(there >> t & 1); };
+        float x[NB][4];
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (FORM == SCALE_EXPONENT) {
+                    const float v = exponent_scale(vs4[n][e]);
+                    vsc[n][e] = __builtin_amdgcn_rcpf(v);
+                    x[n][e] = __builtin_fmaf(acc[n][e], ks4[n][e] * p.scale_log2, __builtin_amdgcn_logf(v));
+                } else {
+                    if constexpr (QUANT) vsc[n][e] = vs4[n][e];
+                    x[n][e] = acc[n][e] * (QUANT ? ks4[n][e] * p.scale_log2 : p.scale_log2);
+                }
+            }
+        if (part) {
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const bool hidden = !seen(16 * n + e);
+                    x[n][e] = hidden ? -__builtin_inff() : x[n][e];
+                    if constexpr (QUANT) vsc[n][e] = hidden ? 0.0f : vsc[n][e];  // (it may be a NaN)
+                }
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = fmaxf(top, x[n][e]);
+        // V into LDS, the next tile's loads behind it
+#pragma unroll
+        for (int j = 0; j < F::SU; j++) {
+            const int u = j * 64 + lane, row = u / F::UR, c = (u % F::UR) * F::NCH;
+            const Wide<T, C> v = Wide<T, C>::of(raw_v[j]);
+#pragma unroll
+            for (int n = 0; n < F::NCH; n++) *(FV*)(lv + row * F::PITCH + (((c + n) ^ at_v<F::CH, sizeof(T), true>(row)) << 4)) = v.v[n];
+            if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
+        }
+        pages = next_pages;
+        if (more) {
+            load_k(t0 + stride, pages);
+            load_v(t0 + stride, pages);
+            next_pages = lookup(t0 + 2 * stride);
+        }
+        if (__any(top > soft.ref + AT_SLACK)) {
+            const float by = soft.move(over_32(over_16(top, larger), larger));
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                out[d] *= by;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        const float ref = Soft::of(soft.ref);
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[n][e] = __builtin_amdgcn_exp2f(x[n][e] - ref);
+                soft.sum = FORM == SCALE_EXPONENT ? __builtin_fmaf(x[n][e], vsc[n][e], soft.sum) : soft.sum + x[n][e];
+                if constexpr (FORM == SCALE_FACTOR) x[n][e] *= vsc[n][e];
+            }
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int n = 0; n < NB; n += 2) {
+                FV pf;
+#pragma unroll
+                for (int e = 0; e < 8; e++) pf[e] = (T)x[n + e / 4][e % 4];
+                auto v_frag = [&](int d) {
+                    const int row = 16 * n + 4 * quad + (col >> 2), ch = 16 * d + 4 * (lane & 3);
+                    return join<T>(read_columns(v_at(row, ch)), read_columns(v_at(row + 16, ch)));
+                };
+#pragma unroll
+                for (int d = 0; d < DB; d++) {
+                    out[d] = mfma16x16x32(v_frag(d), pf, out[d]);
+                    if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int d = 0; d < DB; d++) {
+                        out[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(*(const T*)v_at(16 * n + 4 * quad + e, 16 * d + col), x[n][e], out[d], 0, 0, 0);
+                        if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
+        }
+        if constexpr (!QUANT) {
+            if (special) {
+#pragma unroll 1
+                for (int t = 0; t < TT; t++) {
+                    if (!((valid >> t) & 1)) continue;
+                    const T* const v = (const T*)(row_at(t0, kv_page(b, table, t0 + t), t) + b.v_at);
+                    if (t0 + t > pos || t0 + t <= low) continue;
+#pragma unroll
+                    for (int d = 0; d < DB; d++)
+                        if (16 * d + 4 * quad < b.dim) out[d] += special4(v + 16 * d + 4 * quad);
+                }
+            }
+        }
+    }
+
+    // ---- the waves' results joined ----
+    soft.sum = over_32(over_16(soft.sum, added), added);
+    float* const mine_o = (float*)lv + col * F::OP;
+#pragma unroll
+    for (int d = 0; d < DB; d++) *(float4v*)(mine_o + 16 * d + 4 * quad) = out[d];
+    if (quad == 0) ends[(wave * 16 + col) * 2] = soft.ref, ends[(wave * 16 + col) * 2 + 1] = soft.sum;
+    __syncthreads();
+    for (int u = tid; u < 16 * (DP / 4); u += AT_THREADS) {
+        const int pair = u / (DP / 4), ch = u % (DP / 4) * 4;
+        if (r.m0 + pair >= r.pairs || ch >= b.dim || r.length - r.rows + (r.m0 + pair) / p.group < 0) continue;
+        float ref = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) ref = fmaxf(ref, ends[(w * 16 + pair) * 2]);
+        float4v v = {};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float l = ends[(w * 16 + pair) * 2 + 1], from = ends[(w * 16 + pair) * 2];
+            const float by = l == 0.0f ? 0.0f : from == ref ? 1.0f : __builtin_amdgcn_exp2f(from - ref);
+            sum += by * l;
+            if (l != 0.0f) v += by * *(const float4v*)((const float*)(lds + w * F::BUF) + pair * F::OP + ch);
+        }
+        const RowOut<T> o = row_out<T>(p, r, kvh, r.m0 + pair, split);
+        if (p.splits > 1) {
+            if (ch == 0) o.ml[0] = ref, o.ml[1] = sum;
+            if (s.begin < s.end) *(float4v*)(o.part + ch) = v;
+        } else {
+            store4(o.y + ch, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
+        }
+    }
+}
+
+// =====================================================================================================================
+// the splits' results joined: a workgroup for each (row, query head)
+// =====================================================================================================================
+template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_attend_args& p) {
+    const sox_kv_view& b = p.b;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x / p.q_heads, head = blockIdx.x % p.q_heads;
+    const int s = kv_sequence(b, row, lane);
+    if (s < 0) return;
+    const int first = min(max(b.starts[s], 0), b.rows), rows = max(min(b.starts[s + 1], b.rows) - first, 0);
+    const int splits = (int64_t)rows * p.group > 16 ? p.splits_many : p.splits_few;
+    if (splits < 2 || (int64_t)max(b.lengths[s], 0) - rows + (row - first) < 0) return;
+    const int64_t at = ((int64_t)row * p.q_heads + head) * p.stride;
+    const float* const ml = p.ml + at * 2;
+    const float* const part = p.part + at * b.dim;
+    float ref = -__builtin_inff();
+    for (int i = lane; i < splits; i += 64) ref = fmaxf(ref, ml[2 * i]);
+    for (int o = 1; o < 64; o <<= 1) ref = fmaxf(ref, __shfl_xor(ref, o));
+    float sum = 0.0f;
+    float4v v = {};
+    const int ch = lane * 4;
+    for (int i = wave; i < splits; i += 4) {
+        const float from = ml[2 * i], l = ml[2 * i + 1];
+        if (l == 0.0f) continue;
+        const float by = from == ref ? 1.0f : __builtin_amdgcn_exp2f(from - ref);
+        sum += by * l;
+        if (ch < b.dim) v += by * *(const float4v*)(part + (int64_t)i * b.dim + ch);
+    }
+    __shared__ float4v all[4][64];
+    __shared__ float sums[4];
+    all[wave][lane] = v;
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    if (wave || ch >= b.dim) return;
+    v = (all[0][lane] + all[1][lane]) + (all[2][lane] + all[3][lane]);
+    sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    store4((T*)p.y + (int64_t)row * p.ldy + (int64_t)head * b.dim + ch, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
+}
+
+#define KV_ATTEND(NAME, T, C, DP)                                                                                              \
+    extern "C" __global__ void __launch_bounds__(256, (Many<T, C, DP>::WAVES)) sox_kv_many_##NAME##_d##DP(sox_kv_attend_args p) { attend_many<T, C, DP>(p); } \
+    extern "C" __global__ void __launch_bounds__(256, (Few<T, C, DP>::WAVES)) sox_kv_few_##NAME##_d##DP(sox_kv_attend_args p) { attend_few<T, C, DP>(p); }
+#define KV_ATTEND_DIMS(NAME, T, C) KV_ATTEND(NAME, T, C, 64) KV_ATTEND(NAME, T, C, 128) KV_ATTEND(NAME, T, C, 256)

@@ -33,6 +33,7 @@ SLOT_ARENA, SLOT_CONSTS, SLOT_DUMMY, SLOT_SYNC = 0, 1, 2, 3
 PIX = dict(Bgr24=0, Rgb24=1, Bgra32=2, Rgba32=3)  # PixelFormat (Imaging/ImageTensor.cs:8-20)
 RUN_STAGING, RUN_DISPATCHES = 1, 2
 NORM = dict(none=0, rms=1, layer=2)  # SOX_NORM_*
+KV_INT8 = 3  # SOX_KV_INT8
 
 
 class DeviceInfo(ctypes.Structure):
@@ -148,6 +149,21 @@ class QuantLinearP(ctypes.Structure):
 
 class BlockNormNodeP(ctypes.Structure):
     _fields_ = [("norm", BlockNormP), ("operands", c_uint32)]
+
+
+class RotaryP(ctypes.Structure):
+    _fields_ = [("head_dim", c_int32), ("rotary_dim", c_int32), ("interleaved", c_int32), ("original", c_int32),
+                ("base", ctypes.c_double), ("factor", ctypes.c_double), ("low", ctypes.c_double), ("high", ctypes.c_double),
+                ("amplitude", ctypes.c_double)]
+
+
+class KvCacheP(ctypes.Structure):
+    _fields_ = [("kv_heads", c_int32), ("head_dim", c_int32), ("page", c_int32), ("format", c_int32)]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [("pool", c_void_p), ("tables", c_void_p), ("starts", c_void_p), ("lengths", c_void_p), ("ldt", c_int64),
+                ("pages", c_int32), ("table_pages", c_int32), ("sequences", c_int32), ("rows", c_int32)]
 
 
 class Bind(ctypes.Structure):
@@ -305,6 +321,21 @@ BACKEND_API = {
     "sox_block_norm_run_quantized": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p,
                                                c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_int64,
                                                c_void_p]),
+    "sox_rotary_create": (c_int32, [c_void_p, ctypes.POINTER(RotaryP), c_void_p, ctypes.POINTER(c_void_p)]),
+    "sox_rotary_destroy": (None, [c_void_p]),
+    "sox_rotary_frequencies": (c_int32, [c_void_p, c_void_p]),
+    "sox_rotary_run": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p,
+                                 c_int64]),
+    "sox_kv_cache_create": (c_int32, [c_void_p, ctypes.POINTER(KvCacheP), ctypes.POINTER(c_void_p)]),
+    "sox_kv_cache_destroy": (None, [c_void_p]),
+    "sox_kv_cache_page_bytes": (c_uint64, [c_void_p]),
+    "sox_kv_cache_write": (c_int32, [c_void_p, c_void_p, ctypes.POINTER(KvBatch), c_int32, c_void_p, c_void_p, c_int64,
+                                     c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64]),
+    "sox_kv_cache_read": (c_int32, [c_void_p, c_void_p, ctypes.POINTER(KvBatch), c_int32, c_void_p, c_int64, c_void_p,
+                                    c_int64]),
+    "sox_kv_cache_workspace": (c_uint64, [c_void_p, c_int32, c_int32, c_int32]),
+    "sox_kv_cache_attend": (c_int32, [c_void_p, c_void_p, ctypes.POINTER(KvBatch), c_int32, c_void_p, c_int64, c_int32,
+                                      c_void_p, c_int64, c_float, c_int32, c_void_p, c_uint64]),
 }
 
 _thin = None
