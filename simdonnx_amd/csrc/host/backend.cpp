@@ -5747,7 +5747,7 @@ struct AttendPlan {
             use_few = use_many = true;
         few_tiles = use_many ? sequences : pairs / 16 + sequences;
         many_tiles = pairs / 128 + (use_few ? std::min(sequences, pairs / 17) : sequences);
-        if (use_few) few_splits = splits(few_tiles * kv_heads, rows * q_heads, tokens / MIN_FEW, 8 * cus);
+        if (use_few) few_splits = splits(few_tiles * kv_heads, rows * q_heads, tokens / MIN_FEW, 4 * cus);
         if (use_many) many_splits = splits(many_tiles * kv_heads, rows * q_heads, tokens / MIN_MANY, 2 * cus);
     }
     static constexpr int MIN_FEW = 256, MIN_MANY = 256;  // tokens of a split at least
@@ -5870,6 +5870,7 @@ int sox_kv_cache_create(sox_backend* be, const sox_kv_cache_p* p, sox_kv_cache**
         K->ks_at = 2 * K->v_at;
         K->vs_at = K->ks_at + up(quant ? tokens * 4 : 0, 16);
         K->page_bytes = up(K->vs_at + (quant ? tokens * 4 : 0), 256);
+        if (K->page_bytes >> 32) unsupported("KvCache: a page of 4 GiB or more");
         const int dp = p->head_dim <= 64 ? 64 : p->head_dim <= 128 ? 128 : 256;
         for (int s = 0; s < 3; s++) {
             if (!quant && s != p->format) continue;
@@ -5954,7 +5955,7 @@ int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch
         const KvCall c(K, batch, "KvCache.Attend", storage);
         const int kv = K->p.kv_heads, dim = K->p.head_dim;
         if (q_heads <= 0 || q_heads > 1 << 16 || q_heads % kv) c.bad("q_heads has to be a multiple of kv_heads");
-        if (!(scale >= 0) || !std::isfinite(scale)) c.bad("scale");
+        if (!(scale >= 0) || !std::isfinite(scale * 1.5f)) c.bad("scale");
         if (window < 0) c.bad("window");
         if (c.idle()) return;
         const Rows Q = c.heads("q", q, ldq, q_heads), Y = c.heads("y", y, ldy, q_heads);
@@ -5991,7 +5992,8 @@ int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch
         if (!plan.use_many) a.splits_many = a.splits_few;
         const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256, es = (int)c.es;
         const uint32_t few = c.grid(plan.few_tiles * kv * plan.few_splits), many = c.grid(plan.many_tiles * kv * plan.many_splits);
-        const uint32_t merge = a.stride > 1 ? c.grid(heads) : 0;
+        const int each = a.stride > 8 ? 1 : 4;  // (row, head)s of a workgroup that joins
+        const uint32_t merge = a.stride > 1 ? c.grid((heads + each - 1) / each) : 0;
         if (plan.use_many) {
             a.splits = plan.many_splits;
             a.tiles = (int32_t)plan.many_tiles;
@@ -6004,7 +6006,10 @@ int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch
             a.min_tokens = AttendPlan::MIN_FEW;
             c.launch(K->few[storage], few, 1, 256, stream, a, attend_lds(false, dp, es));
         }
-        if (merge) c.launch(K->merge[storage], merge, 1, 256, stream, a);
+        if (merge) {
+            a.tiles = each;
+            c.launch(K->merge[storage], merge, 1, 256, stream, a);
+        }
     });
 }
 

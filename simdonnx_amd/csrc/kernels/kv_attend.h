@@ -223,9 +223,18 @@ template <int PAIRS, int TT> SOX_DEV Span span_of(const sox_kv_attend_args& p, c
     return s;
 }
 
-// A lane's token of a tile: its page, or -1; only tokens of [lo, hi) are looked up
-SOX_DEV int tile_page(const sox_kv_view& b, const int32_t* table, int token, int lo, int hi) {
-    return token >= lo && token < hi ? kv_page(b, table, token) : -1;
+// A lane's token of a tile: its table entry, from the table's nearest one where it has none, so that the load needs no branch
+// and nothing waits for it until tile_page looks at it, a tile later
+SOX_DEV int tile_entry(const sox_kv_view& b, const int32_t* table, int token) {
+    return table[min(max(token, 0) >> b.shift, b.table_pages - 1)];
+}
+// and its page, or -1: no page of the pool, or a token outside of [lo, hi) (which lies within the table)
+SOX_DEV int tile_page(const sox_kv_view& b, int entry, int token, int lo, int hi) {
+    return token >= lo && token < hi && (uint32_t)entry < (uint32_t)b.pages ? entry : -1;
+}
+// The head's rows of a page, `bytes` into their region: a page is below 4 GiB
+SOX_DEV const uint8_t* head_rows(const sox_kv_view& b, const uint8_t* head, int page, uint32_t bytes) {
+    return head + (uint64_t)(uint32_t)page * (uint32_t)b.page_bytes + bytes;
 }
 
 // Where a row's results go
@@ -283,6 +292,7 @@ template <typename T, typename C, int DP> struct Many {
     static constexpr int BUF = 2 * TT * PITCH;                                          // K and V of a tile
     static constexpr int LDS = 2 * BUF + 2 * 3 * TT * 4 + 64;
     static constexpr int WAVES = PITCH > 256 ? 1 : 2;  // on a SIMD
+    static constexpr int GROUP = sizeof(T) == 2 ? 4 : 2, VGROUP = 4;  // fragments read at once
     static constexpr bool AHEAD = PITCH <= 512;        // the next tile's loads in flight behind a tile (beyond, registers are short)
     static_assert(SU >= 1 && TT * UR % AT_THREADS == 0, "staging");
 };
@@ -303,7 +313,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     if (!r.some) return;
     const Span s = span_of<128, TT>(p, r, split, p.splits);
     const int32_t* const table = b.tables + r.sequence * b.ldt;
-    const int mask = (1 << b.shift) - 1, es = (int)sizeof(C);
+    const int mask = (1 << b.shift) - 1;
     const int64_t scale_at = tid < TT ? b.ks_at : b.vs_at;  // of what this thread stages of the scales
 
     // this lane's pair
@@ -325,7 +335,11 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     // ---- staging ----
     int4v raw_k[M::SU], raw_v[M::SU];
     float raw_s = 0.0f;  // threads 0 .. TT - 1: K's scale of their token, TT .. 2 TT - 1: V's
-    auto lookup = [&](int t0) { return lane < TT ? tile_page(b, table, t0 + lane, s.lo, s.end) : -1; };
+    const uint32_t row_bytes = (uint32_t)b.dim * sizeof(C);
+    const uint8_t* const head = b.pool + ((int64_t)kvh << b.shift) * row_bytes;
+    const uint8_t* const head_s = b.pool + ((int64_t)kvh << b.shift) * 4;
+    auto entry = [&](int t0) { return tile_entry(b, table, t0 + min(lane, TT - 1)); };
+    auto page_of = [&](int t0, int entry) { return lane < TT ? tile_page(b, entry, t0 + lane, s.lo, s.end) : -1; };
     auto thread = [&] {  // (in the widest instances not to be worked with ahead of the loop: registers are short)
         int t = tid;
         if constexpr (!M::AHEAD) asm volatile("" : "+v"(t));
@@ -333,14 +347,16 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     };
     auto load = [&](int t0, int pages, int from = 0, int to = M::SU) {
         const int tid = thread();
+        int of[M::SU];
+#pragma unroll
+        for (int j = from; j < to; j++) of[j] = M::UR == 64 ? __builtin_amdgcn_readlane(pages, 4 * j + wave) : __shfl(pages, (j * AT_THREADS + tid) / M::UR);
 #pragma unroll
         for (int j = from; j < to; j++) {
-            const int u = j * AT_THREADS + tid, row = u / M::UR, c = u % M::UR;
-            const int page = M::UR == 64 ? __builtin_amdgcn_readlane(pages, 4 * j + wave) : __shfl(pages, row);
+            const int u = j * AT_THREADS + tid, row = u / M::UR, c = u % M::UR, page = of[j];
             raw_k[j] = raw_v[j] = int4v{};
             if (page >= 0 && c * M::EC < b.dim) {
                 typedef int4v At __attribute__((aligned(4)));
-                const uint8_t* at = b.pool + page * b.page_bytes + ((((int64_t)kvh << b.shift) + ((t0 + row) & mask)) * b.dim + c * M::EC) * es;
+                const uint8_t* const at = head_rows(b, head, page, ((t0 + row) & mask) * row_bytes + c * 16);
                 raw_k[j] = *(const At*)at;
                 raw_v[j] = *(const At*)(at + b.v_at);
             }
@@ -349,7 +365,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
             const int page = __shfl(pages, tid & (TT - 1));
             raw_s = 0.0f;
             if (tid < 2 * TT && page >= 0)
-                raw_s = *(const float*)(b.pool + page * b.page_bytes + scale_at + (((int64_t)kvh << b.shift) + ((t0 + (tid & (TT - 1))) & mask)) * 4);
+                raw_s = *(const float*)(head_rows(b, head_s, page, ((t0 + (tid & (TT - 1))) & mask) * 4) + scale_at);
         }
     };
     bool bad = false;
@@ -404,15 +420,46 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         float16v acc[TB];
 #pragma unroll
         for (int tb = 0; tb < TB; tb++) acc[tb] = float16v{};
+        // K's fragments a group ahead of their MFMAs (left alone, the compiler waits for each where it is used)
+        {
+            constexpr int G = M::GROUP, GROUPS = M::KS * TB / G;
+            FV kf[2][G];
+            auto read_k = [&](int g, FV(&f)[G]) {
 #pragma unroll
-        for (int ks = 0; ks < M::KS; ks++)
+                for (int i = 0; i < G; i++) {
+                    const int ks = (g * G + i) / TB, row = 32 * ((g * G + i) % TB) + col;
+                    f[i] = *(const FV*)(lk + row * M::PITCH + (((2 * ks + half) ^ at_k<M::CH>(row)) << 4));
+                }
+            };
+            read_k(0, kf[0]);
 #pragma unroll
-            for (int tb = 0; tb < TB; tb++) {
-                const int row = 32 * tb + col;
-                const FV kf = *(const FV*)(lk + row * M::PITCH + (((2 * ks + half) ^ at_k<M::CH>(row)) << 4));
-                acc[tb] = mma32<T>(kf, qf[ks], acc[tb]);
-                if ((ks % 2 || sizeof(T) == 4) && tb == TB - 1) __builtin_amdgcn_sched_barrier(0);
+            for (int g = 0; g < GROUPS; g++) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (g + 1 < GROUPS) read_k(g + 1, kf[(g + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < G; i++) {
+                    const int ks = (g * G + i) / TB, tb = (g * G + i) % TB;
+                    acc[tb] = mma32<T>(kf[g & 1][i], qf[ks], acc[tb]);
+                }
             }
+        }
+        // V's likewise, the first group behind the softmax
+        auto v_at = [&](int row, int ch) { return lv + row * M::PITCH + (((ch / E) ^ at_v<M::CH, sizeof(T), false>(row)) << 4) + ch % E * (int)sizeof(T); };
+        constexpr int VG = M::VGROUP, VGROUPS = TB * 2 * DB / VG;
+        FV vf[2][sizeof(T) == 2 ? VG : 1];
+        auto read_v = [&](int g, FV(&f)[sizeof(T) == 2 ? VG : 1]) {
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int i = 0; i < VG; i++) {
+                    const int at = g * VG + i, step = at / DB, d = at % DB;  // steps of 16 tokens
+                    const int row = 16 * step + 4 * half + ((lane & 15) >> 2), ch = 32 * d + (lane & 16) + 4 * (lane & 3);
+                    f[i] = join<T>(read_columns(v_at(row, ch)), read_columns(v_at(row + 8, ch)));
+                }
+            }
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        read_v(0, vf[0]);
         __builtin_amdgcn_sched_barrier(0);
         // register i of block tb: token t0 + 32 tb + 8 (i / 4) + 4 half + i % 4
         auto token = [&](int tb, int i) { return 32 * tb + 8 * (i >> 2) + 4 * half + (i & 3); };
@@ -434,7 +481,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float a = acc[tb][4 * i4 + e];
-                    x[tb][4 * i4 + e] = FORM == SCALE_EXPONENT ? __builtin_fmaf(a, ks4[e], lv4[e]) : a * (QUANT ? ks4[e] : p.scale_log2);
+                    x[tb][4 * i4 + e] = FORM == SCALE_EXPONENT ? __builtin_fmaf(a, ks4[e], lv4[e]) : QUANT ? a * ks4[e] : a;
                 }
                 if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
             }
@@ -449,6 +496,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         for (int tb = 0; tb < TB; tb++)
 #pragma unroll
             for (int i = 0; i < 16; i++) top = fmaxf(top, x[tb][i]);
+        if constexpr (!QUANT) top *= p.scale_log2;
         if (__any(top > soft.ref + AT_SLACK)) {
             const float by = soft.move(over_32(top, larger));
 #pragma unroll
@@ -461,7 +509,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 #pragma unroll
         for (int tb = 0; tb < TB; tb++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[tb][i] = __builtin_amdgcn_exp2f(x[tb][i] - ref);
+            for (int i = 0; i < 16; i++) x[tb][i] = __builtin_amdgcn_exp2f(QUANT ? x[tb][i] - ref : __builtin_fmaf(x[tb][i], p.scale_log2, -ref));
         // the sum, and p as it meets v (a hidden token's scale may be a NaN)
 #pragma unroll
         for (int tb = 0; tb < TB; tb++)
@@ -482,23 +530,23 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                 if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
             }
         // O^T += V^T P^T
-        auto v_at = [&](int row, int ch) { return lv + row * M::PITCH + (((ch / E) ^ at_v<M::CH, sizeof(T), false>(row)) << 4) + ch % E * (int)sizeof(T); };
         if constexpr (sizeof(T) == 2) {
-            auto v_frag = [&](int tb, int s2, int d) {
-                const int row = 32 * tb + 16 * s2 + 4 * half + ((lane & 15) >> 2), ch = 32 * d + (lane & 16) + 4 * (lane & 3);
-                return join<T>(read_columns(v_at(row, ch)), read_columns(v_at(row + 8, ch)));
-            };
+            FV pf[2 * TB];
 #pragma unroll
-            for (int tb = 0; tb < TB; tb++)
+            for (int st = 0; st < 2 * TB; st++)
 #pragma unroll
-                for (int s2 = 0; s2 < 2; s2++) {
-                    FV pf;
+                for (int e = 0; e < 8; e++) pf[st][e] = (T)x[st / 2][8 * (st % 2) + e];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) pf[e] = (T)x[tb][8 * s2 + e];
+            for (int g = 0; g < VGROUPS; g++) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (g + 1 < VGROUPS) read_v(g + 1, vf[(g + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int d = 0; d < DB; d++) out[d] = mfma32x32x16(v_frag(tb, s2, d), pf, out[d]);
-                    __builtin_amdgcn_sched_barrier(0);  // a step's fragments at a time: bounded register pressure
+                for (int i = 0; i < VG; i++) {
+                    const int at = g * VG + i;
+                    out[at % DB] = mfma32x32x16(vf[g & 1][i], pf[at / DB], out[at % DB]);
                 }
+            }
         } else {
 #pragma unroll
             for (int tb = 0; tb < TB; tb++)
@@ -536,7 +584,8 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 
     // ---- the tokens ----
     if (s.begin < s.end) {
-        int pages = lookup(s.begin);
+        int pages = page_of(s.begin, entry(s.begin));
+        int next = entry(s.begin + TT);
         uint64_t valid = __ballot(pages >= 0);
         bool part = in_part(s.begin, valid);
         // a tile's units one after the other
@@ -554,23 +603,17 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         } else {
             load_and_store(s.begin, 0, part);
         }
-        pages = lookup(s.begin + TT);
         __syncthreads();
         int buf = 0;
         for (int t0 = s.begin; t0 < s.end; t0 += TT, buf ^= 1) {
             const bool more = t0 + TT < s.end;
+            pages = page_of(t0 + TT, next);
             const uint64_t next_valid = __ballot(pages >= 0);
             const bool next_part = in_part(t0 + TT, next_valid);
-            if (M::AHEAD && more) {
-                load(t0 + TT, pages);
-                pages = lookup(t0 + 2 * TT);
-            }
+            next = entry(t0 + 2 * TT);
+            if (M::AHEAD && more) load(t0 + TT, pages);
             if (t0 <= wave_last) tile(t0, buf, valid, part);
-            if (!M::AHEAD && more) {
-                pages = lookup(t0 + TT);  // (again, rather than held behind the tile)
-                load_and_store(t0 + TT, buf ^ 1, next_part);
-                pages = lookup(t0 + 2 * TT);
-            }
+            if (!M::AHEAD && more) load_and_store(t0 + TT, buf ^ 1, next_part);
             if (M::AHEAD && more) store(buf ^ 1, next_part);
             __syncthreads();
             valid = next_valid;
@@ -584,7 +627,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     if (to >= r.pairs || r.length - r.rows + to / p.group < 0) return;
     const RowOut<T> o = row_out<T>(p, r, kvh, to, split);
     if (p.splits > 1) {
-        if (upper == 0) o.ml[0] = soft.ref, o.ml[1] = soft.sum;
+        if (upper == 0) o.ml[0] = soft.ref, o.ml[1] = s.begin < s.end ? soft.sum : -1.0f;
         if (s.begin >= s.end) return;
     }
     const float inv = p.splits > 1 ? 1.0f : soft.sum == 0.0f ? 0.0f : 1.0f / soft.sum;
@@ -636,7 +679,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     if (!r.some) return;
     const Span s = span_of<16, TT>(p, r, split, p.splits);
     const int32_t* const table = b.tables + r.sequence * b.ldt;
-    const int mask = (1 << b.shift) - 1, es = (int)sizeof(C);
+    const int mask = (1 << b.shift) - 1;
     unsigned char* const lv = lds + wave * F::BUF;
     float* const ends = (float*)(lds + 4 * F::BUF);  // [wave][pair][reference, sum]
 
@@ -659,8 +702,12 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     int4v raw_k[NB][F::KU], raw_v[F::SU];
     float4v ks4[NB], vs4[NB];  // scales of the tokens of this lane's scores
     typedef int4v At __attribute__((aligned(4)));
-    auto lookup = [&](int t0) { return lane < TT ? tile_page(b, table, t0 + lane, s.lo, s.end) : -1; };
-    auto row_at = [&](int t0, int page, int row) { return b.pool + page * b.page_bytes + (((int64_t)kvh << b.shift) + ((t0 + row) & mask)) * (int64_t)(b.dim * es); };
+    const uint32_t row_bytes = (uint32_t)b.dim * sizeof(C);
+    const uint8_t* const head = b.pool + ((int64_t)kvh << b.shift) * row_bytes;
+    const uint8_t* const head_s = b.pool + ((int64_t)kvh << b.shift) * 4;
+    auto entry = [&](int t0) { return tile_entry(b, table, t0 + min(lane, TT - 1)); };
+    auto page_of = [&](int t0, int entry) { return lane < TT ? tile_page(b, entry, t0 + lane, s.lo, s.end) : -1; };
+    auto row_at = [&](int t0, int page, int row) { return head_rows(b, head, page, ((t0 + row) & mask) * row_bytes); };
     auto load_k = [&](int t0, int pages) {
 #pragma unroll
         for (int n = 0; n < NB; n++) {
@@ -677,7 +724,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                     const int t = 16 * n + 4 * quad + e, pg = __shfl(pages, t);
                     ks4[n][e] = vs4[n][e] = 0.0f;
                     if (pg >= 0) {
-                        const uint8_t* const sc = b.pool + pg * b.page_bytes + (((int64_t)kvh << b.shift) + ((t0 + t) & mask)) * 4;
+                        const uint8_t* const sc = head_rows(b, head_s, pg, ((t0 + t) & mask) * 4);
                         ks4[n][e] = *(const float*)(sc + b.ks_at);
                         vs4[n][e] = *(const float*)(sc + b.vs_at);
                     }
@@ -697,7 +744,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 
     const int stride = 4 * TT;
     int t0 = s.begin + wave * TT;
-    int pages = lookup(t0), next_pages = lookup(t0 + stride);
+    int pages = page_of(t0, entry(t0)), next = entry(t0 + stride);
     if (t0 < s.end) {
         load_k(t0, pages);
         load_v(t0, pages);
@@ -774,11 +821,11 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
             for (int n = 0; n < F::NCH; n++) *(FV*)(lv + row * F::PITCH + (((c + n) ^ at_v<F::CH, sizeof(T), true>(row)) << 4)) = v.v[n];
             if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
         }
-        pages = next_pages;
+        pages = page_of(t0 + stride, next);
+        next = entry(t0 + 2 * stride);
         if (more) {
             load_k(t0 + stride, pages);
             load_v(t0 + stride, pages);
-            next_pages = lookup(t0 + 2 * stride);
         }
         if (__any(top > soft.ref + AT_SLACK)) {
             const float by = soft.move(over_32(over_16(top, larger), larger));
@@ -862,7 +909,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         }
         const RowOut<T> o = row_out<T>(p, r, kvh, r.m0 + pair, split);
         if (p.splits > 1) {
-            if (ch == 0) o.ml[0] = ref, o.ml[1] = sum;
+            if (ch == 0) o.ml[0] = ref, o.ml[1] = s.begin < s.end ? sum : -1.0f;
             if (s.begin < s.end) *(float4v*)(o.part + ch) = v;
         } else {
             store4(o.y + ch, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
@@ -871,41 +918,68 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 }
 
 // =====================================================================================================================
-// the splits' results joined: a workgroup for each (row, query head)
+// the splits' results joined
 // =====================================================================================================================
+// 64 threads for each (row, query head), 256 where there are many splits (p.tiles: (row, head)s of a workgroup). A row of
+// partial results takes dim / 4 lanes, so 64 / (dim / 4) of them are in flight for each wave's load, four loads at a time. A split
+// that had no tokens left a sum of -1 and nothing else; such splits are the last.
 template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_attend_args& p) {
     const sox_kv_view& b = p.b;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = blockIdx.x / p.q_heads, head = blockIdx.x % p.q_heads;
-    const int s = kv_sequence(b, row, lane);
-    if (s < 0) return;
-    const int first = min(max(b.starts[s], 0), b.rows), rows = max(min(b.starts[s + 1], b.rows) - first, 0);
-    const int splits = (int64_t)rows * p.group > 16 ? p.splits_many : p.splits_few;
-    if (splits < 2 || (int64_t)max(b.lengths[s], 0) - rows + (row - first) < 0) return;
+    const int each = p.tiles, threads = AT_THREADS / each, tid = threadIdx.x, lane = tid & 63;
+    const int64_t which = (int64_t)blockIdx.x * each + tid / threads;
+    const int row = __builtin_amdgcn_readfirstlane((int)(which / p.q_heads)), head = __builtin_amdgcn_readfirstlane((int)(which % p.q_heads));
+    const int s = row < b.rows ? kv_sequence(b, row, lane) : -1;
+    int splits = 0;
+    if (s >= 0) {
+        const int first = min(max(b.starts[s], 0), b.rows), rows = max(min(b.starts[s + 1], b.rows) - first, 0);
+        splits = (int64_t)rows * p.group > 16 ? p.splits_many : p.splits_few;
+        if (splits < 2 || (int64_t)max(b.lengths[s], 0) - rows + (row - first) < 0) splits = 0;
+    }
     const int64_t at = ((int64_t)row * p.q_heads + head) * p.stride;
     const float* const ml = p.ml + at * 2;
-    const float* const part = p.part + at * b.dim;
     float ref = -__builtin_inff();
-    for (int i = lane; i < splits; i += 64) ref = fmaxf(ref, ml[2 * i]);
+    int n = 0;
+    for (int i0 = 0; i0 < splits; i0 += 64) {
+        const bool some = i0 + lane < splits && ml[2 * (i0 + lane) + 1] != -1.0f;
+        if (some) ref = fmaxf(ref, ml[2 * (i0 + lane)]);
+        n += __popcll(__ballot(some));
+    }
     for (int o = 1; o < 64; o <<= 1) ref = fmaxf(ref, __shfl_xor(ref, o));
+    const int lanes = b.dim <= 64 ? 16 : b.dim <= 128 ? 32 : 64, groups = threads / lanes;
+    const int mine = tid % threads, group = mine / lanes, ch = mine % lanes * 4;
+    const float* const part = p.part + at * b.dim + ch;
     float sum = 0.0f;
     float4v v = {};
-    const int ch = lane * 4;
-    for (int i = wave; i < splits; i += 4) {
-        const float from = ml[2 * i], l = ml[2 * i + 1];
-        if (l == 0.0f) continue;
-        const float by = from == ref ? 1.0f : __builtin_amdgcn_exp2f(from - ref);
-        sum += by * l;
-        if (ch < b.dim) v += by * *(const float4v*)(part + (int64_t)i * b.dim + ch);
+    for (int i0 = group; i0 < n; i0 += 4 * groups) {
+        float4v o[4];
+        float from[4], l[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + k * groups;
+            o[k] = float4v{};
+            from[k] = ref, l[k] = 0.0f;
+            if (i < n) {
+                from[k] = ml[2 * i], l[k] = ml[2 * i + 1];
+                if (ch < b.dim) o[k] = *(const float4v*)(part + (int64_t)i * b.dim);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float by = l[k] == 0.0f ? 0.0f : from[k] == ref ? 1.0f : __builtin_amdgcn_exp2f(from[k] - ref);
+            sum += by * l[k];
+            v += by * o[k];
+        }
     }
-    __shared__ float4v all[4][64];
-    __shared__ float sums[4];
-    all[wave][lane] = v;
-    if (lane == 0) sums[wave] = sum;
+    __shared__ float4v all[AT_THREADS];
+    __shared__ float sums[AT_THREADS];
+    all[tid] = v;
+    sums[tid] = sum;
     __syncthreads();
-    if (wave || ch >= b.dim) return;
-    v = (all[0][lane] + all[1][lane]) + (all[2][lane] + all[3][lane]);
-    sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    if (splits == 0 || group || ch >= b.dim) return;
+    for (int g = 1; g < groups; g++) {
+        v += all[tid + g * lanes];
+        sum += sums[tid + g * lanes];
+    }
     store4((T*)p.y + (int64_t)row * p.ldy + (int64_t)head * b.dim + ch, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
 }
 
