@@ -16,7 +16,8 @@
 // scale), the reference bounds p times scale) and the sum divides it out again: exact while the scales span less than
 // 2^110, as fp16 rows' do (2^-31 to 2^9; scales below 2^-100 count as that).
 // Tokens that a row does not see add nothing, whatever their K and V hold: tokens that no row of the tile sees are not read,
-// masked scores are replaced, and a V that is not finite within a tile that is masked in part goes through without its values that are not finite (special4).
+// masked scores are replaced, and a V that is not finite within a tile that is masked in part goes through without its values
+// that are not finite (special4).
 #pragma once
 #include "kv_cache.h"
 
@@ -144,6 +145,18 @@ template <typename T, typename C> constexpr int scale_form() {
     return sizeof(C) == 1 ? std::is_same<T, half_t>::value ? SCALE_EXPONENT : SCALE_FACTOR : SCALE_NONE;
 }
 SOX_DEV float exponent_scale(float scale) { return __builtin_elementwise_maximum(scale, 0x1p-100f); }  // (a NaN stays one)
+
+// c + the sum of eight values
+SOX_DEV float sum8(half8 v, float c) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) c = __builtin_amdgcn_fdot2(half2v{v[i], v[i + 1]}, half2v{(half_t)1.0f, (half_t)1.0f}, c, false);
+    return c;
+}
+SOX_DEV float sum8(bf16x8 v, float c) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) c = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[i], v[i + 1]}, bf16x2{(bf16_t)1.0f, (bf16_t)1.0f}, c, false);
+    return c;
+}
 
 // f of this lane's value and that of the lane 32 (or 16) away, in both
 template <class F> SOX_DEV float over_32(float v, F&& f) {
@@ -305,7 +318,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     constexpr int TT = M::TT, TB = M::TB, DB = M::DB, E = M::E;
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     float(*const scales)[3][TT] = (float(*)[3][TT])(lds + 2 * M::BUF);
-    int* const flags = (int*)(lds + 2 * M::BUF + 2 * 3 * TT * 4);  // [buffer][wave]
+    int* const flags = (int*)(lds + 2 * M::BUF + 2 * 3 * TT * 4);  // a wave found V not finite in a tile that is cut
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const sox_kv_view& b = p.b;
     const int kvh = blockIdx.x % b.heads, rest = blockIdx.x / b.heads, split = rest % p.splits;
@@ -319,7 +332,8 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     // this lane's pair
     const int m = r.m0 + 32 * wave + col;
     const bool mine = m < r.pairs;
-    const int pos = mine ? (int)(r.length - r.rows + m / p.group) : -1, low = p.window > 0 ? pos - p.window : -1;
+    // (a lane without a pair sees all: nothing, and its wave would look for a reference in every tile)
+    const int pos = mine ? (int)(r.length - r.rows + m / p.group) : 0x7fffffff, low = mine && p.window > 0 ? pos - p.window : -1;
     const int wave_last = r.m0 + 32 * wave < r.pairs ? (int)(r.length - r.rows + (min(r.m0 + 32 * wave + 32, r.pairs) - 1) / p.group) : -1;
     FV qf[M::KS];
     {
@@ -345,20 +359,31 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         if constexpr (!M::AHEAD) asm volatile("" : "+v"(t));
         return t;
     };
-    auto load = [&](int t0, int pages, int from = 0, int to = M::SU) {
-        const int tid = thread();
-        int of[M::SU];
+    const bool wide_pages = (1 << b.shift) >= 64 / M::UR && b.dim == DP;  // what a wave loads at once of a tile seen whole stands in one page
+    auto load = [&](int t0, int pages, bool part, int from = 0, int to = M::SU) {
+        typedef int4v At __attribute__((aligned(4)));
+        if (wide_pages && !part) {
 #pragma unroll
-        for (int j = from; j < to; j++) of[j] = M::UR == 64 ? __builtin_amdgcn_readlane(pages, 4 * j + wave) : __shfl(pages, (j * AT_THREADS + tid) / M::UR);
+            for (int j = from; j < to; j++) {
+                const int row = (j * AT_THREADS + wave * 64) / M::UR, page = __builtin_amdgcn_readlane(pages, row);
+                const uint8_t* const at = head_rows(b, head, page, ((t0 + row) & mask) * (DP * (int)sizeof(C)));
+                raw_k[j] = *(const At*)(at + lane * 16);
+                raw_v[j] = *(const At*)(at + b.v_at + lane * 16);
+            }
+        } else {
+            const int tid = thread();
+            int of[M::SU];
 #pragma unroll
-        for (int j = from; j < to; j++) {
-            const int u = j * AT_THREADS + tid, row = u / M::UR, c = u % M::UR, page = of[j];
-            raw_k[j] = raw_v[j] = int4v{};
-            if (page >= 0 && c * M::EC < b.dim) {
-                typedef int4v At __attribute__((aligned(4)));
-                const uint8_t* const at = head_rows(b, head, page, ((t0 + row) & mask) * row_bytes + c * 16);
-                raw_k[j] = *(const At*)at;
-                raw_v[j] = *(const At*)(at + b.v_at);
+            for (int j = from; j < to; j++) of[j] = M::UR == 64 ? __builtin_amdgcn_readlane(pages, 4 * j + wave) : __shfl(pages, (j * AT_THREADS + tid) / M::UR);
+#pragma unroll
+            for (int j = from; j < to; j++) {
+                const int u = j * AT_THREADS + tid, row = u / M::UR, c = u % M::UR, page = of[j];
+                raw_k[j] = raw_v[j] = int4v{};
+                if (page >= 0 && c * M::EC < b.dim) {
+                    const uint8_t* const at = head_rows(b, head, page, ((t0 + row) & mask) * row_bytes + c * 16);
+                    raw_k[j] = *(const At*)at;
+                    raw_v[j] = *(const At*)(at + b.v_at);
+                }
             }
         }
         if constexpr (QUANT) {
@@ -368,21 +393,26 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                 raw_s = *(const float*)(head_rows(b, head_s, page, ((t0 + (tid & (TT - 1))) & mask) * 4) + scale_at);
         }
     };
-    bool bad = false;
-    auto store = [&](int buf, bool check, int from = 0, int to = M::SU) {
+    bool found = false;  // a value of V that is not finite, in a tile that is cut
+    // cut: a tile that some rows see less of than others, whose V goes without such values
+    auto store = [&](int buf, bool cut, int from = 0, int to = M::SU) {
         const int tid = thread();
         unsigned char* const lk = lds + buf * M::BUF;
         unsigned char* const lv = lk + TT * M::PITCH;
-        if (from == 0) bad = false;
+        if constexpr (!QUANT) {
+            if (cut) {
+                uint32_t bad = 0;
 #pragma unroll
-        for (int j = from; j < to; j++) {
-            const int u = j * AT_THREADS + tid, row = u / M::UR, c = (u % M::UR) * M::NCH;
-            if constexpr (!QUANT) {
-                if (check) {
+                for (int j = from; j < to; j++) {
                     bad |= any_not_finite<T>(raw_v[j]);
                     raw_v[j] = finite_only<T>(raw_v[j]);
                 }
+                found |= __any(bad);
             }
+        }
+#pragma unroll
+        for (int j = from; j < to; j++) {
+            const int u = j * AT_THREADS + tid, row = u / M::UR, c = (u % M::UR) * M::NCH;
             const Wide<T, C> k = Wide<T, C>::of(raw_k[j]), v = Wide<T, C>::of(raw_v[j]);
 #pragma unroll
             for (int n = 0; n < M::NCH; n++) {
@@ -403,15 +433,10 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                     scales[buf][1][tid - TT] = raw_s;
                 }
             }
-        } else if (check) {
-            const bool any = __any(bad);
-            if (lane == 0) flags[buf * 4 + wave] = any;
         }
     };
-    // a tile that some row sees in part
-    auto in_part = [&](int t0, uint64_t valid) {
-        return t0 + TT - 1 > s.pos_first || (p.window > 0 && t0 <= s.pos_last - p.window) || ~valid << (64 - TT) != 0;
-    };
+    auto is_cut = [&](int t0) { return t0 + TT - 1 > s.pos_first || (p.window > 0 && t0 <= s.pos_last - p.window); };
+    auto in_part = [&](int t0, uint64_t valid) { return is_cut(t0) || ~valid << (64 - TT) != 0; };  // (or without some of its tokens)
 
     // ---- a tile ----
     auto tile = [&](int t0, int buf, uint64_t valid, bool part) {
@@ -524,18 +549,22 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     float& a = x[tb][4 * i4 + e];
-                    soft.sum = FORM == SCALE_EXPONENT ? __builtin_fmaf(a, v4[e], soft.sum) : soft.sum + a;
+                    if constexpr (QUANT || sizeof(T) == 4) soft.sum = FORM == SCALE_EXPONENT ? __builtin_fmaf(a, v4[e], soft.sum) : soft.sum + a;
                     if constexpr (FORM == SCALE_FACTOR) a *= v4[e];
                 }
                 if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
             }
-        // O^T += V^T P^T
+        FV pf[2 * TB];
         if constexpr (sizeof(T) == 2) {
-            FV pf[2 * TB];
 #pragma unroll
-            for (int st = 0; st < 2 * TB; st++)
+            for (int st = 0; st < 2 * TB; st++) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) pf[st][e] = (T)x[st / 2][8 * (st % 2) + e];
+                if constexpr (!QUANT) soft.sum = sum8(pf[st], soft.sum);  // (of p as it meets v, two at a time)
+            }
+        }
+        // O^T += V^T P^T
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int g = 0; g < VGROUPS; g++) {
                 __builtin_amdgcn_sched_barrier(0);
@@ -559,27 +588,6 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                     }
                 }
         }
-        if constexpr (!QUANT) {
-            if (part && (flags[buf * 4] | flags[buf * 4 + 1] | flags[buf * 4 + 2] | flags[buf * 4 + 3])) {
-#pragma unroll 1
-                for (int t = 0; t < TT; t++) {
-                    if (!((valid >> t) & 1)) continue;
-                    const T* const v = (const T*)(b.pool + kv_page(b, table, t0 + t) * b.page_bytes + b.v_at) + (((int64_t)kvh << b.shift) + ((t0 + t) & mask)) * b.dim;
-                    if (t0 + t > pos || t0 + t <= low) continue;
-#pragma unroll
-                    for (int d = 0; d < DB; d++)
-#pragma unroll
-                        for (int i4 = 0; i4 < 4; i4++) {
-                            const int ch = 32 * d + 8 * i4 + 4 * half;
-                            if (ch >= b.dim) continue;
-                            const float4v add = special4(v + ch);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) out[d][4 * i4 + e] += add[e];
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                }
-            }
-        }
     };
 
     // ---- the tokens ----
@@ -589,17 +597,17 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         uint64_t valid = __ballot(pages >= 0);
         bool part = in_part(s.begin, valid);
         // a tile's units one after the other
-        auto load_and_store = [&](int t0, int buf, bool check) {
+        auto load_and_store = [&](int t0, int buf, bool part) {
             static_for<0, M::SU>([&](auto j) {
                 constexpr int at = decltype(j)::value;
                 __builtin_amdgcn_sched_barrier(0);
-                load(t0, pages, at, at + 1);
-                store(buf, check, at, at + 1);
+                load(t0, pages, part, at, at + 1);
+                store(buf, is_cut(t0), at, at + 1);
             });
         };
         if constexpr (M::AHEAD) {
-            load(s.begin, pages);
-            store(0, part);
+            load(s.begin, pages, part);
+            store(0, is_cut(s.begin));
         } else {
             load_and_store(s.begin, 0, part);
         }
@@ -611,10 +619,10 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
             const uint64_t next_valid = __ballot(pages >= 0);
             const bool next_part = in_part(t0 + TT, next_valid);
             next = entry(t0 + 2 * TT);
-            if (M::AHEAD && more) load(t0 + TT, pages);
+            if (M::AHEAD && more) load(t0 + TT, pages, next_part);
             if (t0 <= wave_last) tile(t0, buf, valid, part);
             if (!M::AHEAD && more) load_and_store(t0 + TT, buf ^ 1, next_part);
-            if (M::AHEAD && more) store(buf ^ 1, next_part);
+            if (M::AHEAD && more) store(buf ^ 1, is_cut(t0 + TT));
             __syncthreads();
             valid = next_valid;
             part = next_part;
@@ -623,8 +631,15 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 
     // ---- out ----  (the pair from the lane number anew: held through the loop, it would cost the widest instances a spill)
     soft.sum = over_32(soft.sum, added);
+    bool special = false;
+    if constexpr (!QUANT) {
+        if (lane == 0) flags[wave] = found;
+        __syncthreads();
+        special = flags[0] | flags[1] | flags[2] | flags[3];
+    }
     const int me = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), to = r.m0 + 32 * wave + (me & 31), upper = me >> 5;
-    if (to >= r.pairs || r.length - r.rows + to / p.group < 0) return;
+    const int64_t at = r.length - r.rows + to / p.group;
+    if (to >= r.pairs || at < 0) return;
     const RowOut<T> o = row_out<T>(p, r, kvh, to, split);
     if (p.splits > 1) {
         if (upper == 0) o.ml[0] = soft.ref, o.ml[1] = s.begin < s.end ? soft.sum : -1.0f;
@@ -640,6 +655,18 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = out[d][4 * i4 + e] * inv;
             if (ch >= b.dim) continue;
+            if (!QUANT && special) {  // what the row sees of the values left out
+#pragma unroll 1
+                for (int t = s.begin; t < s.end; t++) {
+                    if (!is_cut((t - s.begin) / TT * TT + s.begin)) {
+                        t += TT - 1;
+                        continue;
+                    }
+                    const int page = t >= s.lo ? kv_page(b, table, t) : -1;
+                    if (page >= 0 && t <= at && (p.window <= 0 || t > at - p.window))
+                        v += special4((const T*)(head_rows(b, head, page, (t & mask) * row_bytes) + b.v_at) + ch);
+                }
+            }
             if (p.splits > 1)
                 *(float4v*)(o.part + ch) = v;
             else
