@@ -5769,7 +5769,7 @@ uint32_t attend_lds(bool many, int dp, int es) {
         return (uint32_t)(4 * tt * pitch + 2 * 3 * tt * 4 + 64);
     }
     const int tt = es == 4 ? 16 : 32;
-    return (uint32_t)(4 * std::max(tt * pitch, 16 * (dp + 4) * 4) + 4 * 16 * 2 * 4);
+    return (uint32_t)(4 * std::max(tt * pitch, 16 * (dp + 4) * 4) + 4 * 16 * 2 * 4 + 4 * 3 * tt * 4);
 }
 
 }  // namespace

@@ -58,6 +58,7 @@ template <typename T, typename C> struct Wide {
             w.v[0] = __builtin_bit_cast(typename Frag<T>::V, raw);
         } else {
             constexpr int E = Frag<T>::E;
+            asm("" : "+v"(raw));  // (here, not where it was loaded: the compiler takes shifts there, and waits)
 #pragma unroll
             for (int n = 0; n < N; n++)
 #pragma unroll
@@ -687,7 +688,7 @@ template <typename T, typename C, int DP> struct Few {
     static constexpr int KU = UR / 4;        // units of K a lane loads of each of its rows
     static constexpr int OP = DP + 4;        // floats from pair to pair of a wave's results
     static constexpr int BUF = TT * PITCH > 16 * OP * 4 ? TT * PITCH : 16 * OP * 4;
-    static constexpr int LDS = 4 * BUF + 4 * 16 * 2 * 4;
+    static constexpr int LDS = 4 * BUF + 4 * 16 * 2 * 4 + 4 * 3 * TT * 4;
     static constexpr int WAVES = PITCH > 256 ? 1 : 2;
     static_assert(SU >= 1 && TT * UR % 64 == 0 && KU >= 1, "staging");
 };
@@ -709,6 +710,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     const int mask = (1 << b.shift) - 1;
     unsigned char* const lv = lds + wave * F::BUF;
     float* const ends = (float*)(lds + 4 * F::BUF);  // [wave][pair][reference, sum]
+    float* const scales = ends + 4 * 16 * 2 + wave * 3 * TT;  // k's times the score's, log2 of v's, what v's are to p or the sum
 
     const int m = r.m0 + col;
     const bool mine = m < r.pairs;
@@ -727,7 +729,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     Soft soft;
 
     int4v raw_k[NB][F::KU], raw_v[F::SU];
-    float4v ks4[NB], vs4[NB];  // scales of the tokens of this lane's scores
+    float raw_s = 0.0f;  // lanes 0 .. TT - 1: K's scale of their token, TT .. 2 TT - 1: V's
     typedef int4v At __attribute__((aligned(4)));
     const uint32_t row_bytes = (uint32_t)b.dim * sizeof(C);
     const uint8_t* const head = b.pool + ((int64_t)kvh << b.shift) * row_bytes;
@@ -735,36 +737,45 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     auto entry = [&](int t0) { return tile_entry(b, table, t0 + min(lane, TT - 1)); };
     auto page_of = [&](int t0, int entry) { return lane < TT ? tile_page(b, entry, t0 + lane, s.lo, s.end) : -1; };
     auto row_at = [&](int t0, int page, int row) { return head_rows(b, head, page, ((t0 + row) & mask) * row_bytes); };
-    auto load_k = [&](int t0, int pages) {
+    const int scale_at = lane < TT ? b.ks_at : b.vs_at;
+    const uint32_t lane_k = (uint32_t)(col * DP * (int)sizeof(C) + quad * 16);
+    const bool wide_pages = b.shift >= 4 && b.dim == DP;  // 16 tokens of a tile seen whole stand in one page
+    auto load = [&](int t0, int pages, bool part) {
+        if (wide_pages && !part) {
 #pragma unroll
-        for (int n = 0; n < NB; n++) {
-            const int row = 16 * n + col, page = __shfl(pages, row);
-            const uint8_t* const at = row_at(t0, page, row);
+            for (int n = 0; n < NB; n++) {
+                const uint8_t* const at = head_rows(b, head, __builtin_amdgcn_readlane(pages, 16 * n), ((t0 + 16 * n) & mask) * (DP * (int)sizeof(C)));
 #pragma unroll
-            for (int u = 0; u < F::KU; u++) {
-                raw_k[n][u] = int4v{};
-                if (page >= 0 && (4 * u + quad) * F::EC < b.dim) raw_k[n][u] = *(const At*)(at + (4 * u + quad) * 16);
+                for (int u = 0; u < F::KU; u++) raw_k[n][u] = *(const At*)(at + u * 64 + lane_k);
             }
-            if constexpr (QUANT) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int t = 16 * n + 4 * quad + e, pg = __shfl(pages, t);
-                    ks4[n][e] = vs4[n][e] = 0.0f;
-                    if (pg >= 0) {
-                        const uint8_t* const sc = head_rows(b, head_s, pg, ((t0 + t) & mask) * 4);
-                        ks4[n][e] = *(const float*)(sc + b.ks_at);
-                        vs4[n][e] = *(const float*)(sc + b.vs_at);
-                    }
+            for (int j = 0; j < F::SU; j++) {
+                const int row = j * 64 / F::UR;
+                const uint8_t* const at = head_rows(b, head, __builtin_amdgcn_readlane(pages, row), ((t0 + row) & mask) * (DP * (int)sizeof(C))) + b.v_at;
+                raw_v[j] = *(const At*)(at + lane * 16);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                const int row = 16 * n + col, page = __shfl(pages, row);
+                const uint8_t* const at = row_at(t0, page, row);
+#pragma unroll
+                for (int u = 0; u < F::KU; u++) {
+                    raw_k[n][u] = int4v{};
+                    if (page >= 0 && (4 * u + quad) * F::EC < b.dim) raw_k[n][u] = *(const At*)(at + (4 * u + quad) * 16);
                 }
             }
-        }
-    };
-    auto load_v = [&](int t0, int pages) {
 #pragma unroll
-        for (int j = 0; j < F::SU; j++) {
-            const int u = j * 64 + lane, row = u / F::UR, c = u % F::UR, page = __shfl(pages, row);
-            raw_v[j] = int4v{};
-            if (page >= 0 && c * F::EC < b.dim) raw_v[j] = *(const At*)(row_at(t0, page, row) + b.v_at + c * 16);
+            for (int j = 0; j < F::SU; j++) {
+                const int u = j * 64 + lane, row = u / F::UR, c = u % F::UR, page = __shfl(pages, row);
+                raw_v[j] = int4v{};
+                if (page >= 0 && c * F::EC < b.dim) raw_v[j] = *(const At*)(row_at(t0, page, row) + b.v_at + c * 16);
+            }
+        }
+        if constexpr (QUANT) {
+            const int page = __shfl(pages, lane & (TT - 1));
+            raw_s = 0.0f;
+            if (page >= 0 && lane < 2 * TT) raw_s = *(const float*)(head_rows(b, head_s, page, ((t0 + (lane & (TT - 1))) & mask) * 4) + scale_at);
         }
     };
     auto v_at = [&](int row, int ch) { return lv + row * F::PITCH + (((ch / E) ^ at_v<F::CH, sizeof(T), true>(row)) << 4) + ch % E * (int)sizeof(T); };
@@ -772,17 +783,32 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     const int stride = 4 * TT;
     int t0 = s.begin + wave * TT;
     int pages = page_of(t0, entry(t0)), next = entry(t0 + stride);
-    if (t0 < s.end) {
-        load_k(t0, pages);
-        load_v(t0, pages);
-    }
+    auto in_part = [&](int t0, uint64_t valid) {  // a tile that not every row sees whole
+        return t0 + TT - 1 > s.pos_first || (p.window > 0 && t0 <= s.pos_last - p.window) || ~valid << (64 - TT) != 0;
+    };
+    uint64_t next_valid = __ballot(pages >= 0);
+    bool next_part = in_part(t0, next_valid);
+    if (t0 < s.end) load(t0, pages, next_part);
     for (; t0 < s.end; t0 += stride) {
-        const uint64_t valid = __ballot(pages >= 0);
-        const bool part = t0 + TT - 1 > s.pos_first || (p.window > 0 && t0 <= s.pos_last - p.window) || ~valid << (64 - TT) != 0;
+        const uint64_t valid = next_valid;
+        const bool part = next_part;
         const bool more = t0 + stride < s.end;
+        if constexpr (QUANT) {
+            if (lane < TT) {
+                scales[lane] = raw_s * p.scale_log2;
+            } else if (lane < 2 * TT) {
+                if constexpr (FORM == SCALE_EXPONENT) {
+                    const float v = exponent_scale(raw_s);
+                    scales[lane] = __builtin_amdgcn_logf(v);
+                    scales[TT + lane] = __builtin_amdgcn_rcpf(v);
+                } else {
+                    scales[TT + lane] = raw_s;
+                }
+            }
+        }
         // S^T = K Q^T: register e of block n is token t0 + 16 n + 4 quad + e
         float4v acc[NB];
-        float vsc[NB][4];  // what v's scales are to p or the sum
+        float4v vsc[NB];
 #pragma unroll
         for (int n = 0; n < NB; n++) {
             acc[n] = float4v{};
@@ -812,18 +838,14 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         auto seen = [&](int t) { return (t <= until) & (t > after) & (int)(there >> t & 1); };
         float x[NB][4];
 #pragma unroll
-        for (int n = 0; n < NB; n++)
+        for (int n = 0; n < NB; n++) {
+            float4v ks, lv;
+            if constexpr (QUANT) ks = *(const float4v*)(scales + 16 * n + 4 * quad), vsc[n] = *(const float4v*)(scales + 2 * TT + 16 * n + 4 * quad);
+            if constexpr (FORM == SCALE_EXPONENT) lv = *(const float4v*)(scales + TT + 16 * n + 4 * quad);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if constexpr (FORM == SCALE_EXPONENT) {
-                    const float v = exponent_scale(vs4[n][e]);
-                    vsc[n][e] = __builtin_amdgcn_rcpf(v);
-                    x[n][e] = __builtin_fmaf(acc[n][e], ks4[n][e] * p.scale_log2, __builtin_amdgcn_logf(v));
-                } else {
-                    if constexpr (QUANT) vsc[n][e] = vs4[n][e];
-                    x[n][e] = acc[n][e] * (QUANT ? ks4[n][e] * p.scale_log2 : p.scale_log2);
-                }
-            }
+            for (int e = 0; e < 4; e++)
+                x[n][e] = FORM == SCALE_EXPONENT ? __builtin_fmaf(acc[n][e], ks[e], lv[e]) : acc[n][e] * (QUANT ? ks[e] : p.scale_log2);
+        }
         if (part) {
 #pragma unroll
             for (int n = 0; n < NB; n++)
@@ -850,10 +872,9 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         }
         pages = page_of(t0 + stride, next);
         next = entry(t0 + 2 * stride);
-        if (more) {
-            load_k(t0 + stride, pages);
-            load_v(t0 + stride, pages);
-        }
+        next_valid = __ballot(pages >= 0);
+        next_part = in_part(t0 + stride, next_valid);
+        if (more) load(t0 + stride, pages, next_part);
         if (__any(top > soft.ref + AT_SLACK)) {
             const float by = soft.move(over_32(over_16(top, larger), larger));
 #pragma unroll
