@@ -5652,7 +5652,7 @@ struct sox_kv_cache {
     sox_kv_cache_p p{};
     int shift = 0;
     int64_t page_bytes = 0, v_at = 0, ks_at = 0, vs_at = 0;
-    void *write[3] = {}, *read[3] = {}, *few[3] = {}, *many[3] = {}, *merge[3] = {};  // by storage, null where the format has none
+    void *write[3] = {}, *read[3] = {}, *few[3] = {}, *many[3] = {}, *both[3] = {}, *merge[3] = {};  // by storage, null where the format has none
 };
 
 namespace {
@@ -5747,10 +5747,11 @@ struct AttendPlan {
             use_few = use_many = true;
         few_tiles = use_many ? sequences : pairs / 16 + sequences;
         many_tiles = pairs / 128 + (use_few ? std::min(sequences, pairs / 17) : sequences);
-        if (use_few) few_splits = splits(few_tiles * kv_heads, rows * q_heads, tokens / MIN_FEW, 4 * cus);
-        if (use_many) many_splits = splits(many_tiles * kv_heads, rows * q_heads, tokens / MIN_MANY, 2 * cus);
+        if (use_few) few_splits = splits(few_tiles * kv_heads, rows * q_heads, tokens / MIN_TOKENS, 4 * cus);
+        // (beside single tokens the many rows are most often one sequence's: the tiles that there are, not those that there may be)
+        if (use_many) many_splits = splits((use_few ? pairs / 128 + 1 : many_tiles) * kv_heads, rows * q_heads, tokens / MIN_TOKENS, 2 * cus);
     }
-    static constexpr int MIN_FEW = 256, MIN_MANY = 256;  // tokens of a split at least
+    static constexpr int MIN_TOKENS = 256;  // of a split, at least
     static int splits(int64_t workgroups, int64_t heads, int64_t most, int64_t fill) {
         const int64_t n = std::min({(fill + workgroups - 1) / workgroups, most, MAX_SPLITS, PARTIALS / heads});
         return (int)std::max<int64_t>(n, 1);
@@ -5879,6 +5880,7 @@ int sox_kv_cache_create(sox_backend* be, const sox_kv_cache_p* p, sox_kv_cache**
             K->read[s] = be->fn("sox_kv_read_" + n);
             K->few[s] = be->fn("sox_kv_few_" + n + d);
             K->many[s] = be->fn("sox_kv_many_" + n + d);
+            K->both[s] = be->fn("sox_kv_both_" + n + d);
             K->merge[s] = be->fn(std::string("sox_kv_merge_") + STORAGE_NAME[s]);
         }
         *out = K.release();
@@ -5986,29 +5988,22 @@ int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch
         a.part = (float*)workspace;
         a.ml = workspace ? (float*)workspace + heads * a.stride * dim : nullptr;
         a.scale_log2 = (float)((scale == 0 ? 1.0 / std::sqrt((double)dim) : (double)scale) * 1.4426950408889634);
-        a.splits_few = plan.few_splits;
-        a.splits_many = plan.many_splits;
-        if (!plan.use_few) a.splits_few = a.splits_many;  // (the merge asks by a sequence's pairs)
-        if (!plan.use_many) a.splits_many = a.splits_few;
+        a.splits_few = plan.use_few ? plan.few_splits : plan.many_splits;  // (the merge asks by a sequence's pairs)
+        a.splits_many = plan.use_many ? plan.many_splits : plan.few_splits;
+        a.min_tokens = AttendPlan::MIN_TOKENS;
         const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256, es = (int)c.es;
         const uint32_t few = c.grid(plan.few_tiles * kv * plan.few_splits), many = c.grid(plan.many_tiles * kv * plan.many_splits);
-        const int each = a.stride > 8 ? 1 : 4;  // (row, head)s of a workgroup that joins
-        const uint32_t merge = a.stride > 1 ? c.grid((heads + each - 1) / each) : 0;
-        if (plan.use_many) {
-            a.splits = plan.many_splits;
-            a.tiles = (int32_t)plan.many_tiles;
-            a.min_tokens = AttendPlan::MIN_MANY;
+        if (a.only) {
+            a.many = (int32_t)many;
+            c.launch(K->both[storage], c.grid((int64_t)many + few), 1, 256, stream, a, std::max(attend_lds(true, dp, es), attend_lds(false, dp, es)));
+        } else if (plan.use_many) {
             c.launch(K->many[storage], many, 1, 256, stream, a, attend_lds(true, dp, es));
-        }
-        if (plan.use_few) {
-            a.splits = plan.few_splits;
-            a.tiles = (int32_t)plan.few_tiles;
-            a.min_tokens = AttendPlan::MIN_FEW;
+        } else {
             c.launch(K->few[storage], few, 1, 256, stream, a, attend_lds(false, dp, es));
         }
-        if (merge) {
-            a.tiles = each;
-            c.launch(K->merge[storage], merge, 1, 256, stream, a);
+        if (a.stride > 1) {
+            a.each = a.stride > 8 ? 1 : 4;  // (row, head)s of a workgroup that joins
+            c.launch(K->merge[storage], c.grid((heads + a.each - 1) / a.each), 1, 256, stream, a);
         }
     });
 }

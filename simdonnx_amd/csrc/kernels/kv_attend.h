@@ -311,7 +311,7 @@ template <typename T, typename C, int DP> struct Many {
     static_assert(SU >= 1 && TT * UR % AT_THREADS == 0, "staging");
 };
 
-template <typename T, typename C, int DP> __device__ __forceinline__ void attend_many(const sox_kv_attend_args& p) {
+template <typename T, typename C, int DP> __device__ __forceinline__ void attend_many(const sox_kv_attend_args& p, uint32_t block) {
     typedef Many<T, C, DP> M;
     typedef typename Frag<T>::V FV;
     constexpr bool QUANT = M::QUANT;
@@ -322,10 +322,10 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     int* const flags = (int*)(lds + 2 * M::BUF + 2 * 3 * TT * 4);  // a wave found V not finite in a tile that is cut
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const sox_kv_view& b = p.b;
-    const int kvh = blockIdx.x % b.heads, rest = blockIdx.x / b.heads, split = rest % p.splits;
-    const RowTile r = row_tile<128, true>(p, rest / p.splits, lane);
+    const int kvh = block % b.heads, rest = block / b.heads, splits = p.splits_many, split = rest % splits;
+    const RowTile r = row_tile<128, true>(p, rest / splits, lane);
     if (!r.some) return;
-    const Span s = span_of<128, TT>(p, r, split, p.splits);
+    const Span s = span_of<128, TT>(p, r, split, splits);
     const int32_t* const table = b.tables + r.sequence * b.ldt;
     const int mask = (1 << b.shift) - 1;
     const int64_t scale_at = tid < TT ? b.ks_at : b.vs_at;  // of what this thread stages of the scales
@@ -642,11 +642,11 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     const int64_t at = r.length - r.rows + to / p.group;
     if (to >= r.pairs || at < 0) return;
     const RowOut<T> o = row_out<T>(p, r, kvh, to, split);
-    if (p.splits > 1) {
+    if (splits > 1) {
         if (upper == 0) o.ml[0] = soft.ref, o.ml[1] = s.begin < s.end ? soft.sum : -1.0f;
         if (s.begin >= s.end) return;
     }
-    const float inv = p.splits > 1 ? 1.0f : soft.sum == 0.0f ? 0.0f : 1.0f / soft.sum;
+    const float inv = splits > 1 ? 1.0f : soft.sum == 0.0f ? 0.0f : 1.0f / soft.sum;
 #pragma unroll
     for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -668,7 +668,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                         v += special4((const T*)(head_rows(b, head, page, (t & mask) * row_bytes) + b.v_at) + ch);
                 }
             }
-            if (p.splits > 1)
+            if (splits > 1)
                 *(float4v*)(o.part + ch) = v;
             else
                 store4(o.y + ch, v);
@@ -693,7 +693,7 @@ template <typename T, typename C, int DP> struct Few {
     static_assert(SU >= 1 && TT * UR % 64 == 0 && KU >= 1, "staging");
 };
 
-template <typename T, typename C, int DP> __device__ __forceinline__ void attend_few(const sox_kv_attend_args& p) {
+template <typename T, typename C, int DP> __device__ __forceinline__ void attend_few(const sox_kv_attend_args& p, uint32_t block) {
     typedef Few<T, C, DP> F;
     typedef typename Frag<T>::V FV;
     constexpr bool QUANT = F::QUANT;
@@ -702,10 +702,10 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, col = lane & 15;
     const sox_kv_view& b = p.b;
-    const int kvh = blockIdx.x % b.heads, rest = blockIdx.x / b.heads, split = rest % p.splits;
-    const RowTile r = row_tile<16, false>(p, rest / p.splits, lane);
+    const int kvh = block % b.heads, rest = block / b.heads, splits = p.splits_few, split = rest % splits;
+    const RowTile r = row_tile<16, false>(p, rest / splits, lane);
     if (!r.some) return;
-    const Span s = span_of<16, TT>(p, r, split, p.splits);
+    const Span s = span_of<16, TT>(p, r, split, splits);
     const int32_t* const table = b.tables + r.sequence * b.ldt;
     const int mask = (1 << b.shift) - 1;
     unsigned char* const lv = lds + wave * F::BUF;
@@ -956,7 +956,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
             if (l != 0.0f) v += by * *(const float4v*)((const float*)(lds + w * F::BUF) + pair * F::OP + ch);
         }
         const RowOut<T> o = row_out<T>(p, r, kvh, r.m0 + pair, split);
-        if (p.splits > 1) {
+        if (splits > 1) {
             if (ch == 0) o.ml[0] = ref, o.ml[1] = s.begin < s.end ? sum : -1.0f;
             if (s.begin < s.end) *(float4v*)(o.part + ch) = v;
         } else {
@@ -968,12 +968,12 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 // =====================================================================================================================
 // the splits' results joined
 // =====================================================================================================================
-// 64 threads for each (row, query head), 256 where there are many splits (p.tiles: (row, head)s of a workgroup). A row of
+// 64 threads for each (row, query head), 256 where there are many splits (p.each: (row, head)s of a workgroup). A row of
 // partial results takes dim / 4 lanes, so 64 / (dim / 4) of them are in flight for each wave's load, four loads at a time. A split
 // that had no tokens left a sum of -1 and nothing else; such splits are the last.
 template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_attend_args& p) {
     const sox_kv_view& b = p.b;
-    const int each = p.tiles, threads = AT_THREADS / each, tid = threadIdx.x, lane = tid & 63;
+    const int each = p.each, threads = AT_THREADS / each, tid = threadIdx.x, lane = tid & 63;
     const int64_t which = (int64_t)blockIdx.x * each + tid / threads;
     const int row = __builtin_amdgcn_readfirstlane((int)(which / p.q_heads)), head = __builtin_amdgcn_readfirstlane((int)(which % p.q_heads));
     const int s = row < b.rows ? kv_sequence(b, row, lane) : -1;
@@ -1031,7 +1031,15 @@ template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_
     store4((T*)p.y + (int64_t)row * p.ldy + (int64_t)head * b.dim + ch, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
 }
 
+// A batch of both kinds in one launch: the many rows' workgroups, bound by the matrix cores, first, and the single tokens', bound
+// by memory, beside them
 #define KV_ATTEND(NAME, T, C, DP)                                                                                              \
-    extern "C" __global__ void __launch_bounds__(256, (Many<T, C, DP>::WAVES)) sox_kv_many_##NAME##_d##DP(sox_kv_attend_args p) { attend_many<T, C, DP>(p); } \
-    extern "C" __global__ void __launch_bounds__(256, (Few<T, C, DP>::WAVES)) sox_kv_few_##NAME##_d##DP(sox_kv_attend_args p) { attend_few<T, C, DP>(p); }
+    extern "C" __global__ void __launch_bounds__(256, (Many<T, C, DP>::WAVES)) sox_kv_many_##NAME##_d##DP(sox_kv_attend_args p) { attend_many<T, C, DP>(p, blockIdx.x); } \
+    extern "C" __global__ void __launch_bounds__(256, (Few<T, C, DP>::WAVES)) sox_kv_few_##NAME##_d##DP(sox_kv_attend_args p) { attend_few<T, C, DP>(p, blockIdx.x); } \
+    extern "C" __global__ void __launch_bounds__(256, (Many<T, C, DP>::WAVES)) sox_kv_both_##NAME##_d##DP(sox_kv_attend_args p) {                                        \
+        if (blockIdx.x < (uint32_t)p.many)                                                                                     \
+            attend_many<T, C, DP>(p, blockIdx.x);                                                                              \
+        else                                                                                                                   \
+            attend_few<T, C, DP>(p, blockIdx.x - p.many);                                                                      \
+    }
 #define KV_ATTEND_DIMS(NAME, T, C) KV_ATTEND(NAME, T, C, 64) KV_ATTEND(NAME, T, C, 128) KV_ATTEND(NAME, T, C, 256)
