@@ -48,6 +48,16 @@ template <typename T> SOX_DEV float4v mma16(typename Frag<T>::V a, typename Frag
     return c;
 }
 
+// A byte of a word as a number, in the one instruction that the compiler makes two of. Its result goes into a conversion: a
+// matrix instruction may not read it at once, and the compiler, which keeps that distance elsewhere, does not see into an asm.
+template <int I> SOX_DEV float signed_byte(int w) {
+    float f;
+    if constexpr (I == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(w));
+    if constexpr (I == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
+    if constexpr (I == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
+    if constexpr (I == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
+    return f;
+}
 // 16 bytes of the cache as they go to LDS: values of T
 template <typename T, typename C> struct Wide {
     static constexpr int N = sizeof(T) / sizeof(C);  // 16-byte chunks of them
@@ -58,11 +68,25 @@ template <typename T, typename C> struct Wide {
             w.v[0] = __builtin_bit_cast(typename Frag<T>::V, raw);
         } else {
             constexpr int E = Frag<T>::E;
-            asm("" : "+v"(raw));  // (here, not where it was loaded: the compiler takes shifts there, and waits)
+            asm("" : "+v"(raw));  // (here, not where it was loaded: the compiler takes its first steps there, and waits)
 #pragma unroll
-            for (int n = 0; n < N; n++)
+            for (int i = 0; i < 4; i++) {
+                auto& to = w.v[4 * i / E];
+                const int e = 4 * i % E;
+                if constexpr (std::is_same<T, half_t>::value) {  // 0x6400 + u is the number 1024 + u, u = q + 128
+                    const uint32_t u = (uint32_t)raw[i] ^ 0x80808080u;
+                    const half2v by = {(half_t)1152.0f, (half_t)1152.0f};
+                    const half2v a = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - by;
+                    const half2v b = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - by;
+                    to[e] = a[0], to[e + 1] = a[1], to[e + 2] = b[0], to[e + 3] = b[1];
+                } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                for (int e = 0; e < E; e++) w.v[n][e] = (T)(float)(int8_t)(raw[(n * E + e) / 4] >> (n * E + e) % 4 * 8);
+                    for (int n = 0; n < 4; n++) to[e + n] = (float)(int8_t)(raw[i] >> 8 * n);
+                } else {
+                    to[e] = (T)signed_byte<0>(raw[i]), to[e + 1] = (T)signed_byte<1>(raw[i]);
+                    to[e + 2] = (T)signed_byte<2>(raw[i]), to[e + 3] = (T)signed_byte<3>(raw[i]);
+                }
+            }
         }
         return w;
     }
