@@ -343,7 +343,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     constexpr int TT = M::TT, TB = M::TB, DB = M::DB, E = M::E;
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     float(*const scales)[3][TT] = (float(*)[3][TT])(lds + 2 * M::BUF);
-    int* const flags = (int*)(lds + 2 * M::BUF + 2 * 3 * TT * 4);  // a wave found V not finite in a tile that is cut
+    int* const flags = (int*)(lds + 2 * M::BUF + 2 * 3 * TT * 4);  // a wave found what is not finite in a cut tile's V
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     const sox_kv_view& b = p.b;
     const int kvh = block % b.heads, rest = block / b.heads, splits = p.splits_many, split = rest % splits;
@@ -418,7 +418,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                 raw_s = *(const float*)(head_rows(b, head_s, page, ((t0 + (tid & (TT - 1))) & mask) * 4) + scale_at);
         }
     };
-    bool found = false;  // a value of V that is not finite, in a tile that is cut
+    bool found = false;  // a value of V that is not finite (of an 8-bit cache its scale), in a tile that is cut
     // cut: a tile that some rows see less of than others, whose V goes without such values
     auto store = [&](int buf, bool cut, int from = 0, int to = M::SU) {
         const int tid = thread();
@@ -447,6 +447,11 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
             if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (QUANT) {
+            if (cut) {
+                const bool bad = tid >= TT && abs_bits(raw_s) >= 0x7f800000u;
+                raw_s = bad ? 0.0f : raw_s;
+                found |= __any(bad);
+            }
             if (tid < TT) {
                 scales[buf][0][tid] = raw_s * p.scale_log2;
             } else if (tid < 2 * TT) {
@@ -520,21 +525,31 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
             const int t = 32 * tb + 8 * (i >> 2) + (i & 3);
             return (t <= until) & (t > after) & (int)((t < 32 ? (uint32_t)there : (uint32_t)(there >> 32)) >> t % 32 & 1);
         };
+        // (scales a group of four tokens ahead of their use)
+        auto scales4 = [&](int which, int g) { return *(const float4v*)&scales[buf][which][token(g / 4, 4 * (g % 4))]; };
+        constexpr int VS = FORM == SCALE_EXPONENT ? 2 : 1;
         float x[TB][16];
+        {
+            float4v ks[2], lv[2];
+            if constexpr (QUANT) ks[0] = scales4(0, 0);
+            if constexpr (FORM == SCALE_EXPONENT) lv[0] = scales4(1, 0);
 #pragma unroll
-        for (int tb = 0; tb < TB; tb++)
-#pragma unroll
-            for (int i4 = 0; i4 < 4; i4++) {
-                float4v ks4, lv4;
-                if constexpr (QUANT) ks4 = *(const float4v*)&scales[buf][0][token(tb, 4 * i4)];
-                if constexpr (FORM == SCALE_EXPONENT) lv4 = *(const float4v*)&scales[buf][1][token(tb, 4 * i4)];
+            for (int g = 0; g < 4 * TB; g++) {
+                if constexpr (QUANT) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (g + 1 < 4 * TB) {
+                        ks[(g + 1) & 1] = scales4(0, g + 1);
+                        if constexpr (FORM == SCALE_EXPONENT) lv[(g + 1) & 1] = scales4(1, g + 1);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float a = acc[tb][4 * i4 + e];
-                    x[tb][4 * i4 + e] = FORM == SCALE_EXPONENT ? __builtin_fmaf(a, ks4[e], lv4[e]) : QUANT ? a * ks4[e] : a;
+                    const float a = acc[g / 4][4 * (g % 4) + e];
+                    x[g / 4][4 * (g % 4) + e] = FORM == SCALE_EXPONENT ? __builtin_fmaf(a, ks[g & 1][e], lv[g & 1][e]) : QUANT ? a * ks[g & 1][e] : a;
                 }
-                if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
             }
+        }
         if (part) {
 #pragma unroll
             for (int tb = 0; tb < TB; tb++)
@@ -560,25 +575,25 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         for (int tb = 0; tb < TB; tb++)
 #pragma unroll
             for (int i = 0; i < 16; i++) x[tb][i] = __builtin_amdgcn_exp2f(QUANT ? x[tb][i] - ref : __builtin_fmaf(x[tb][i], p.scale_log2, -ref));
-        // the sum, and p as it meets v (a hidden token's scale may be a NaN)
+        // the sum, and p as it meets v
+        if constexpr (!(sizeof(T) == 2 && !QUANT)) {
+            float4v vs[2];
+            if constexpr (QUANT) vs[0] = scales4(VS, 0);
 #pragma unroll
-        for (int tb = 0; tb < TB; tb++)
-#pragma unroll
-            for (int i4 = 0; i4 < 4; i4++) {
-                float4v v4;
-                if constexpr (QUANT) v4 = *(const float4v*)&scales[buf][FORM == SCALE_EXPONENT ? 2 : 1][token(tb, 4 * i4)];
-                if (QUANT && part) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v4[e] = seen(tb, 4 * i4 + e) ? v4[e] : 0.0f;
+            for (int g = 0; g < 4 * TB; g++) {
+                if constexpr (QUANT) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (g + 1 < 4 * TB) vs[(g + 1) & 1] = scales4(VS, g + 1);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    float& a = x[tb][4 * i4 + e];
-                    if constexpr (QUANT || sizeof(T) == 4) soft.sum = FORM == SCALE_EXPONENT ? __builtin_fmaf(a, v4[e], soft.sum) : soft.sum + a;
-                    if constexpr (FORM == SCALE_FACTOR) a *= v4[e];
+                    float& a = x[g / 4][4 * (g % 4) + e];
+                    soft.sum = FORM == SCALE_EXPONENT ? __builtin_fmaf(a, vs[g & 1][e], soft.sum) : soft.sum + a;
+                    if constexpr (FORM == SCALE_FACTOR) a *= vs[g & 1][e];
                 }
-                if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);
             }
+        }
         FV pf[2 * TB];
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -656,12 +671,9 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 
     // ---- out ----  (the pair from the lane number anew: held through the loop, it would cost the widest instances a spill)
     soft.sum = over_32(soft.sum, added);
-    bool special = false;
-    if constexpr (!QUANT) {
-        if (lane == 0) flags[wave] = found;
-        __syncthreads();
-        special = flags[0] | flags[1] | flags[2] | flags[3];
-    }
+    if (lane == 0) flags[wave] = found;
+    __syncthreads();
+    const bool special = flags[0] | flags[1] | flags[2] | flags[3];
     const int me = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), to = r.m0 + 32 * wave + (me & 31), upper = me >> 5;
     const int64_t at = r.length - r.rows + to / p.group;
     if (to >= r.pairs || at < 0) return;
@@ -680,7 +692,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = out[d][4 * i4 + e] * inv;
             if (ch >= b.dim) continue;
-            if (!QUANT && special) {  // what the row sees of the values left out
+            if (special) {  // what the row sees of the values left out
 #pragma unroll 1
                 for (int t = s.begin; t < s.end; t++) {
                     if (!is_cut((t - s.begin) / TT * TT + s.begin)) {
@@ -688,8 +700,13 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                         continue;
                     }
                     const int page = t >= s.lo ? kv_page(b, table, t) : -1;
-                    if (page >= 0 && t <= at && (p.window <= 0 || t > at - p.window))
+                    if (page < 0 || t > at || (p.window > 0 && t <= at - p.window)) continue;
+                    if constexpr (QUANT) {
+                        const float f = *(const float*)(head_rows(b, head_s, page, (t & mask) * 4) + b.vs_at);
+                        v += abs_bits(f) < 0x7f800000u ? 0.0f : f;
+                    } else {
                         v += special4((const T*)(head_rows(b, head, page, (t & mask) * row_bytes) + b.v_at) + ch);
+                    }
                 }
             }
             if (splits > 1)
