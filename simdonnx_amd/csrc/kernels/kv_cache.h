@@ -60,13 +60,18 @@ template <typename F> struct CosSin {
 };
 constexpr int TURN_HALF = 128;  // pairs of a head at most
 
-// The table of a row's cosines and sines, by the threads of a workgroup
-template <typename F>
-SOX_DEV void turn_table(const sox_turn_args& t, int64_t position, CosSin<F>* table, int thread, int threads) {
-    for (int j = thread; j < t.half; j += threads) {
+// Rows' tables of cosines and sines. Pair j stands at turn_at<V>(j), V channels a lane: side by side what lanes of a head read
+// at once (in order, they would read a bank's words 8 deep, and that took longer than the memory).
+template <int V> SOX_DEV int turn_at(int j) { return j % V * (TURN_HALF / V) + j / V; }
+template <int V, typename F, class P>
+SOX_DEV void turn_tables(const sox_turn_args& t, P position, CosSin<F> (*table)[TURN_HALF], int rows, int thread, int threads) {
+    int r = 0, j = thread;
+    for (;; j += threads) {
+        while (j >= t.half && r < rows) j -= t.half, r++;
+        if (r >= rows) break;
         double c, s;
-        turn_cos_sin((uint64_t)position * t.turns[j], c, s);
-        table[j] = {(F)(c * t.amplitude), (F)(s * t.amplitude)};
+        turn_cos_sin((uint64_t)position(r) * t.turns[j], c, s);
+        table[r][turn_at<V>(j)] = {(F)(c * t.amplitude), (F)(s * t.amplitude)};
     }
 }
 
@@ -76,24 +81,16 @@ SOX_DEV void turn_table(const sox_turn_args& t, int64_t position, CosSin<F>* tab
 // wave that reads it: all of its lanes' loads come before their stores.
 template <typename T, typename F> struct TurnedChunk {
     static constexpr int V = 16 / sizeof(T);
+    typedef typename Chunk16<T>::V TV;
+    typedef typename Chunk16<T>::At At;
+    TV own, other;
     float v[V];
-    __device__ __forceinline__ void load(const T* head, int ch, const sox_turn_args& t, const CosSin<F>* table) {
-        typedef typename Chunk16<T>::V TV;
-        typedef typename Chunk16<T>::At At;
-        const TV own = *(const At*)(head + ch);
-        const int half = t.half, end = 2 * half;
-        if (half == 0) {
-#pragma unroll
-            for (int e = 0; e < V; e++) v[e] = (float)own[e];
-            return;
-        }
-        TV other = own;
-        if (t.interleaved) {
-#pragma unroll
-            for (int e = 0; e < V; e++) other[e] = own[e ^ 1];
-        } else if (half % V == 0) {
-            const int at = ch >= end ? ch : ch < half ? ch + half : ch - half;
-            other = *(const At*)(head + at);
+    __device__ __forceinline__ void load(const T* head, int ch, const sox_turn_args& t, int half) {
+        own = *(const At*)(head + ch);
+        const int end = 2 * half;
+        if (half == 0 || ch >= end || t.interleaved) return;
+        if (half % V == 0) {
+            other = *(const At*)(head + (ch < half ? ch + half : ch - half));
         } else {
 #pragma unroll
             for (int e = 0; e < V; e++) {
@@ -101,19 +98,46 @@ template <typename T, typename F> struct TurnedChunk {
                 other[e] = head[at];
             }
         }
+    }
+    __device__ __forceinline__ void turn(int ch, const sox_turn_args& t, int half, const CosSin<F>* table) {
+        const int end = 2 * half;
+        if (ch >= end) {
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            const int c = ch + e, j = t.interleaved ? c >> 1 : c < half ? c : c - half;
-            const bool first = t.interleaved ? !(e & 1) : c < half;
-            const CosSin<F> cs = table[min(j, half - 1)];
-            const F s = first ? -cs.s : cs.s;
-            const float y = (float)(sizeof(F) == 8 ? (F)__builtin_fma((double)(float)other[e], (double)s, (double)(float)own[e] * (double)cs.c)
-                                                   : (F)__builtin_fmaf((float)other[e], (float)s, (float)own[e] * (float)cs.c));
-            v[e] = c < end ? y : (float)own[e];
+            for (int e = 0; e < V; e++) v[e] = (float)own[e];
+            return;
+        }
+        constexpr int NEXT = TURN_HALF / V;
+        if (!t.interleaved && half % V == 0) {  // (the usual heads: one place in the table, and what follows it at constant steps)
+            const bool first = ch < half;
+            const CosSin<F>* const at = table + (first ? ch : ch - half) / V;
+#pragma unroll
+            for (int e = 0; e < V; e++) v[e] = turned(own[e], first ? -other[e] : other[e], at[e * NEXT]);
+        } else if (t.interleaved && end % V == 0) {
+            const int j = ch >> 1;
+            const CosSin<F>* const at = table + turn_at<V>(j);
+#pragma unroll
+            for (int e = 0; e < V; e++) v[e] = turned(own[e], e & 1 ? own[e ^ 1] : -own[e ^ 1], at[(e >> 1) * NEXT]);
+        } else {
+            if (t.interleaved) {
+#pragma unroll
+                for (int e = 0; e < V; e++) other[e] = own[e ^ 1];
+            }
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const int c = ch + e, j = t.interleaved ? c >> 1 : c < half ? c : c - half;
+                const bool first = t.interleaved ? !(e & 1) : c < half;
+                const float y = turned(own[e], first ? -other[e] : other[e], table[turn_at<V>(min(j, half - 1))]);
+                v[e] = c < end ? y : (float)own[e];
+            }
         }
     }
+    SOX_DEV float turned(T x, T other, CosSin<F> by) {
+        if constexpr (sizeof(F) == 8)
+            return (float)__builtin_fma((double)(float)other, by.s, (double)(float)x * by.c);
+        else
+            return __builtin_fmaf((float)other, by.s, (float)x * by.c);
+    }
     __device__ __forceinline__ void store(T* head, int ch) const {
-        typedef typename Chunk16<T>::V TV;
         TV o;
 #pragma unroll
         for (int e = 0; e < V; e++) o[e] = (T)v[e];

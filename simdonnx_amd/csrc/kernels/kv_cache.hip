@@ -5,23 +5,43 @@
 // its row's in 8 bits, so a row goes from memory to its page in one pass.
 #include "kv_cache.h"
 
+// A thread's (row, head)s, one after the other
+struct Walk {
+    int r, h, step, heads, rows;
+    SOX_DEV Walk of(int first, int step, int heads, int rows) {
+        Walk w{0, first - step, step, heads, rows};
+        w.next();
+        return w;
+    }
+    __device__ __forceinline__ void next() {
+        h += step;
+        while (h >= heads && r < rows) h -= heads, r++;
+    }
+    __device__ __forceinline__ bool some() const { return r < rows; }
+};
+
 template <typename T> __device__ __forceinline__ void rotary_body(const sox_rotary_args& p) {
     typedef typename std::conditional<sizeof(T) == 4, double, float>::type F;
     constexpr int V = 16 / sizeof(T);
     __shared__ CosSin<F> table[4][TURN_HALF];
     const int tid = threadIdx.x, rpb = p.rows_per_block, row0 = blockIdx.x * rpb, rows = min(rpb, p.rows - row0);
-    for (int r = 0; r < rows; r++) turn_table(p.turn, p.positions[row0 + r], table[r], tid, 256);
+    const int ch = (tid & ((1 << p.lanes) - 1)) * V, half = p.turn.half;
+    Walk w = Walk::of(tid >> p.lanes, 256 >> p.lanes, p.heads, rows);
+    TurnedChunk<T, F> next;
+    auto load = [&] {
+        if (w.some() && ch < p.dim) next.load((const T*)p.x + (int64_t)(row0 + w.r) * p.ldx + (int64_t)w.h * p.dim, ch, p.turn, half);
+    };
+    load();
+    turn_tables<V>(p.turn, [&](int r) { return p.positions[row0 + r]; }, table, rows, tid, 256);
     __syncthreads();
-    const int ch = (tid & ((1 << p.lanes) - 1)) * V, step = 256 >> p.lanes;
-    int r = 0, h = tid >> p.lanes;
-    for (;; h += step) {
-        while (h >= p.heads && r < rows) h -= p.heads, r++;
-        if (r >= rows) break;
+    while (w.some()) {
+        TurnedChunk<T, F> c = next;
+        const int r = w.r, h = w.h;
+        w.next();
+        load();
         if (ch >= p.dim) continue;
-        const int64_t at = (int64_t)h * p.dim, row = row0 + r;
-        TurnedChunk<T, F> c;
-        c.load((const T*)p.x + row * p.ldx + at, ch, p.turn, table[r]);
-        c.store((T*)p.y + row * p.ldy + at, ch);
+        c.turn(ch, p.turn, half, table[r]);
+        c.store((T*)p.y + (int64_t)(row0 + r) * p.ldy + (int64_t)h * p.dim, ch);
     }
 }
 
@@ -48,39 +68,42 @@ template <typename T, typename C> __device__ __forceinline__ void kv_write_body(
     __shared__ RowAt where[KV_ROWS];
     const sox_kv_view& b = p.b;
     const int tid = threadIdx.x, lane = tid & 63, rpb = p.rows_per_block, row0 = blockIdx.x * rpb, rows = min(rpb, b.rows - row0);
+    const int sub = tid & ((1 << p.lanes) - 1), ch = sub * V;
+    Walk w = Walk::of(tid >> p.lanes, 256 >> p.lanes, p.q_heads + 2 * b.heads, rows);
+    TurnedChunk<T, F> next;  // on its way while the one before is worked on, the first while the rows' pages are looked for
+    auto load = [&] {
+        if (!w.some() || ch >= b.dim) return;
+        const bool q = w.h < p.q_heads, k = w.h < p.q_heads + b.heads;
+        const int64_t row = row0 + w.r;
+        const T* const from = q ? (const T*)p.q + row * p.ldq : k ? (const T*)p.k + row * p.ldk : (const T*)p.v + row * p.ldv;
+        next.load(from + (int64_t)(q ? w.h : w.h - p.q_heads - (k ? 0 : b.heads)) * b.dim, ch, p.turn, k ? p.turn.half : 0);
+    };
+    load();
     for (int r = tid >> 6; r < rows; r += 4) {
         const RowAt at = row_at(b, row0 + r, lane);
         if (lane == 0) where[r] = at;
     }
     __syncthreads();
-    if (p.turn.half)
-        for (int r = 0; r < rows; r++) turn_table(p.turn, where[r].position, table[r], tid, 256);
+    if (p.turn.half) turn_tables<V>(p.turn, [&](int r) { return where[r].position; }, table, rows, tid, 256);
     __syncthreads();
-    const int sub = tid & ((1 << p.lanes) - 1), ch = sub * V, step = 256 >> p.lanes, heads = p.q_heads + 2 * b.heads;
-    const sox_turn_args straight{nullptr, 1.0, 0, 0};
-    int r = 0, h = tid >> p.lanes;
-    for (;; h += step) {
-        while (h >= heads && r < rows) h -= heads, r++;
-        if (r >= rows) break;
-        const int64_t row = row0 + r;
+    while (w.some()) {
+        TurnedChunk<T, F> c = next;
+        const int r = w.r, h = w.h;
+        w.next();
+        load();
+        const bool is_q = h < p.q_heads, is_k = h < p.q_heads + b.heads;
+        const int head = is_q ? h : h - p.q_heads - (is_k ? 0 : b.heads);
         const RowAt at = where[r];
-        if (at.position < 0) continue;
-        TurnedChunk<T, F> c;
-        if (h < p.q_heads) {
-            if (ch >= b.dim) continue;
-            c.load((const T*)p.q + row * p.ldq + (int64_t)h * b.dim, ch, p.turn, table[r]);
-            c.store((T*)p.y + row * p.ldy + (int64_t)h * b.dim, ch);
+        if (at.position < 0 || (at.page < 0 && !is_q)) continue;
+        const bool turned = is_k && p.turn.half;
+        if (ch < b.dim) c.turn(ch, p.turn, turned ? p.turn.half : 0, table[r]);
+        if (is_q) {
+            if (ch < b.dim) c.store((T*)p.y + (int64_t)(row0 + r) * p.ldy + (int64_t)head * b.dim, ch);
             continue;
         }
-        if (at.page < 0) continue;
-        const bool is_k = h < p.q_heads + b.heads;
-        const int kh = h - p.q_heads - (is_k ? 0 : b.heads);
-        const T* from = is_k ? (const T*)p.k + row * p.ldk : (const T*)p.v + row * p.ldv;
-        from += (int64_t)kh * b.dim;
-        const int64_t token = ((int64_t)kh << b.shift) + (at.position & ((1 << b.shift) - 1));
+        const int64_t token = ((int64_t)head << b.shift) + (at.position & ((1 << b.shift) - 1));
         uint8_t* const page = b.pool + at.page * b.page_bytes;
         C* const to = (C*)(page + (is_k ? 0 : b.v_at)) + token * b.dim;
-        if (ch < b.dim) c.load(from, ch, is_k ? p.turn : straight, table[r]);
         if constexpr (!QUANT) {
             if (ch < b.dim) c.store((T*)to, ch);
         } else {
@@ -89,13 +112,47 @@ template <typename T, typename C> __device__ __forceinline__ void kv_write_body(
 #pragma unroll
                 for (int e = 0; e < V; e++) top = max(top, abs_bits(c.v[e]));
             for (int o = 1; o < 1 << p.lanes; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-            const RowQuant<float> q = RowQuant<float>::make(top);
+            float scale;
+            uint32_t q[V / 4];
+            bool sure = false;
+            if (turned) {  // (of full precision, whatever T is)
+                // In fp32 first: 127 / amax and its product with x are off by less than 2^-15 for a result up to 127, so one
+                // that is at least 2^-14 from the middle between two integers rounds as the exact one does. About one wave's
+                // chunk in 30 has a value that is nearer and takes the steps in 64 bits, as rows at fp32's ends do.
+                const float a = __uint_as_float(top), by = 127.0f / a;
+                float far = 0.0f;
+                uint32_t low[V];
+                if (ch < b.dim) {
+#pragma unroll
+                    for (int e = 0; e < V; e++) {
+                        const float x = c.v[e] * by, up = x + 12582912.0f;
+                        low[e] = __float_as_uint(up);
+                        far = fmaxf(far, fabsf(x - (up - 12582912.0f)));
+                    }
+                }
+                sure = !__any(!(far < 0.5f - 0x1p-14f) || !(a > 0x1p-60f && a < 0x1p60f));
+                if (sure) {
+                    scale = a / 127.0f;
+#pragma unroll
+                    for (int e = 0; e < V; e += 4)
+                        q[e / 4] = __builtin_amdgcn_perm(low[e + 1], low[e], 0x0c0c0400) | __builtin_amdgcn_perm(low[e + 3], low[e + 2], 0x04000c0c);
+                }
+            }
+            auto exact = [&](const auto& by) {
+                typedef typename std::decay<decltype(by)>::type Q;
+#pragma unroll
+                for (int e = 0; e < V; e += 4) q[e / 4] = Q::q4(c.v[e], c.v[e + 1], c.v[e + 2], c.v[e + 3], by);
+                scale = by.scale;
+            };
+            if (!turned)
+                exact(RowQuant<T>::make(top));
+            else if (!sure)
+                exact(RowQuant<float>::make(top));
             if (ch < b.dim) {
 #pragma unroll
-                for (int e = 0; e < V; e += 4)
-                    *(uint32_t*)(to + ch + e) = RowQuant<float>::q4(c.v[e], c.v[e + 1], c.v[e + 2], c.v[e + 3], q);
+                for (int e = 0; e < V / 4; e++) *(uint32_t*)(to + ch + 4 * e) = q[e];
             }
-            if (sub == 0) ((float*)(page + (is_k ? b.ks_at : b.vs_at)))[token] = q.scale;
+            if (sub == 0) ((float*)(page + (is_k ? b.ks_at : b.vs_at)))[token] = scale;
         }
     }
 }
@@ -110,36 +167,49 @@ template <typename T, typename C> __device__ __forceinline__ void kv_read_body(c
         if (lane == 0) where[r] = at;
     }
     __syncthreads();
-    const int ch = (tid & ((1 << p.lanes) - 1)) * V, step = 256 >> p.lanes, heads = 2 * b.heads;
-    int r = 0, h = tid >> p.lanes;
-    for (;; h += step) {
-        while (h >= heads && r < rows) h -= heads, r++;
-        if (r >= rows) break;
-        if (ch >= b.dim) continue;
-        const int64_t row = row0 + r;
-        const RowAt at = where[r];
-        if (at.position < 0) continue;
-        const bool is_k = h < b.heads;
-        const int kh = is_k ? h : h - b.heads;
-        T* const to = (is_k ? (T*)p.k + row * p.ldk : (T*)p.v + row * p.ldv) + (int64_t)kh * b.dim + ch;
-        typedef typename Chunk16<T>::V TV;
-        TV o = {};
-        if (at.page >= 0) {
-            const int64_t token = ((int64_t)kh << b.shift) + (at.position & ((1 << b.shift) - 1));
-            const uint8_t* const page = b.pool + at.page * b.page_bytes;
-            const C* const from = (const C*)(page + (is_k ? 0 : b.v_at)) + token * b.dim + ch;
-            if constexpr (sizeof(C) == 1) {
-                const float scale = ((const float*)(page + (is_k ? b.ks_at : b.vs_at)))[token];
-                typedef int8_t Bytes __attribute__((ext_vector_type(V)));
-                typedef Bytes BytesAt __attribute__((aligned(4)));
-                const Bytes q = *(const BytesAt*)from;
-#pragma unroll
-                for (int e = 0; e < V; e++) o[e] = (T)((float)q[e] * scale);
-            } else {
-                o = *(const typename Chunk16<T>::At*)from;
-            }
+    const int ch = (tid & ((1 << p.lanes) - 1)) * V;
+    if (ch >= b.dim) return;
+    typedef typename Chunk16<T>::V TV;
+    typedef int8_t Bytes __attribute__((ext_vector_type(V)));
+    typedef Bytes BytesAt __attribute__((aligned(4)));
+    Walk w = Walk::of(tid >> p.lanes, 256 >> p.lanes, 2 * b.heads, rows);
+    struct Chunk {
+        TV v;
+        Bytes q;
+        float scale;
+    };
+    auto load = [&](Chunk& c) {
+        c.v = TV{};
+        c.q = Bytes{};
+        c.scale = 0.0f;
+        if (!w.some()) return;
+        const RowAt at = where[w.r];
+        if (at.page < 0) return;
+        const bool is_k = w.h < b.heads;
+        const int64_t token = ((int64_t)(is_k ? w.h : w.h - b.heads) << b.shift) + (at.position & ((1 << b.shift) - 1));
+        const uint8_t* const page = b.pool + at.page * b.page_bytes;
+        const C* const from = (const C*)(page + (is_k ? 0 : b.v_at)) + token * b.dim + ch;
+        if constexpr (sizeof(C) == 1) {
+            c.scale = ((const float*)(page + (is_k ? b.ks_at : b.vs_at)))[token];
+            c.q = *(const BytesAt*)from;
+        } else {
+            c.v = *(const typename Chunk16<T>::At*)from;
         }
-        *(typename Chunk16<T>::At*)to = o;
+    };
+    Chunk next;
+    load(next);
+    while (w.some()) {  // (a chunk's loads on their way while the one before is stored)
+        Chunk c = next;
+        const int r = w.r, h = w.h;
+        w.next();
+        load(next);
+        if (where[r].position < 0) continue;
+        if constexpr (sizeof(C) == 1) {
+#pragma unroll
+            for (int e = 0; e < V; e++) c.v[e] = (T)((float)c.q[e] * c.scale);
+        }
+        T* const to = (h < b.heads ? (T*)p.k + (int64_t)(row0 + r) * p.ldk + (int64_t)h * b.dim : (T*)p.v + (int64_t)(row0 + r) * p.ldv + (int64_t)(h - b.heads) * b.dim) + ch;
+        *(typename Chunk16<T>::At*)to = c.v;
     }
 }
 
