@@ -677,7 +677,8 @@ typedef struct sox_kv_attend_args {
     int64_t ldq, ldy;
     int32_t q_heads, group, window, only;
     int32_t splits_few, splits_many;  /* of a tile's tokens; the merge takes them by a sequence's pairs */
-    int32_t stride, min_tokens;       /* of the partial results of a (row, query head); of a split */
+    int32_t min_few, min_many;        /* tokens of a split at least */
+    int32_t stride;                   /* of the partial results of a (row, query head) */
     int32_t many, each;               /* both kernels in one: the many rows' workgroups; the merge: (row, head)s of a workgroup */
     float scale_log2;                 /* scale * log2(e) */
 } sox_kv_attend_args;

@@ -5726,9 +5726,12 @@ struct KvCall : LayerCall {
 };
 
 // Which kernels attend, with how many row tiles and splits each.
-//   few   tiles of 16 pairs (row, query head of a kv head's group): where single tokens are all there is
+//   few   tiles of 16 pairs (row, query head of a kv head's group): where single tokens are all there is, and where its
+//         workgroups all run at once over few tokens: a tile of 128 pairs would have as many tokens to walk on fewer CUs. 1024
+//         tokens on each CU is about where the two meet (45 new tokens of 3 sequences of up to 333, 16 query heads: 13 us
+//         against 18; 200 of 200: 10 against 17; 16 behind 4096: 19 against 21; but 32 behind 4096: 29 against 22)
 //   many  tiles of 128
-//   both, each for its sequences, where a batch may hold single tokens and longer pieces
+//   both, each for its sequences, in one launch: where a batch may hold single tokens and longer pieces
 // The host knows the rows of the whole batch alone; each kernel is right for every sequence.
 // Splits: so many that the workgroups fill the CUs about `fill` times, while a row's partial results stay within PARTIALS.
 struct AttendPlan {
@@ -5739,7 +5742,8 @@ struct AttendPlan {
 
     AttendPlan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t tokens, int cus) {
         const int64_t pairs = rows * (q_heads / kv_heads);
-        if (pairs <= 16 || (pairs <= 16 * sequences && rows <= 4 * sequences))
+        const int64_t fine = (pairs / 16 + sequences) * kv_heads;
+        if (pairs <= 16 || (pairs <= 16 * sequences && rows <= 4 * sequences) || (fine <= 2 * cus && fine * tokens <= 1024 * (int64_t)cus))
             use_few = true;
         else if (sequences == 1)
             use_many = true;
@@ -5747,11 +5751,11 @@ struct AttendPlan {
             use_few = use_many = true;
         few_tiles = use_many ? sequences : pairs / 16 + sequences;
         many_tiles = pairs / 128 + (use_few ? std::min(sequences, pairs / 17) : sequences);
-        if (use_few) few_splits = splits(few_tiles * kv_heads, rows * q_heads, tokens / MIN_TOKENS, 4 * cus);
+        if (use_few) few_splits = splits(few_tiles * kv_heads, rows * q_heads, tokens / MIN_FEW, 4 * cus);
         // (beside single tokens the many rows are most often one sequence's: the tiles that there are, not those that there may be)
-        if (use_many) many_splits = splits((use_few ? pairs / 128 + 1 : many_tiles) * kv_heads, rows * q_heads, tokens / MIN_TOKENS, 2 * cus);
+        if (use_many) many_splits = splits((use_few ? pairs / 128 + 1 : many_tiles) * kv_heads, rows * q_heads, tokens / MIN_MANY, 2 * cus);
     }
-    static constexpr int MIN_TOKENS = 256;  // of a split, at least
+    static constexpr int MIN_FEW = 256, MIN_MANY = 256;  // tokens of a split at least
     static int splits(int64_t workgroups, int64_t heads, int64_t most, int64_t fill) {
         const int64_t n = std::min({(fill + workgroups - 1) / workgroups, most, MAX_SPLITS, PARTIALS / heads});
         return (int)std::max<int64_t>(n, 1);
@@ -5963,7 +5967,7 @@ int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch
         const Rows Q = c.heads("q", q, ldq, q_heads), Y = c.heads("y", y, ldy, q_heads);
         const int64_t heads = c.rows * q_heads;
         int64_t tokens = (int64_t)batch->table_pages << K->shift;
-        if (window) tokens = std::min(tokens, (int64_t)window + c.rows);
+        if (window) tokens = std::min(tokens, (int64_t)window + std::min<int64_t>(c.rows, 128 / (q_heads / kv) + 1));  // (what a tile's rows see)
         const AttendPlan plan(c.rows, batch->sequences, q_heads, kv, tokens, c.be->info.compute_units);
         Rows W{"workspace"};
         if (const uint64_t need = plan.need(heads, dim)) {
@@ -5990,7 +5994,8 @@ int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch
         a.scale_log2 = (float)((scale == 0 ? 1.0 / std::sqrt((double)dim) : (double)scale) * 1.4426950408889634);
         a.splits_few = plan.use_few ? plan.few_splits : plan.many_splits;  // (the merge asks by a sequence's pairs)
         a.splits_many = plan.use_many ? plan.many_splits : plan.few_splits;
-        a.min_tokens = AttendPlan::MIN_TOKENS;
+        a.min_few = AttendPlan::MIN_FEW;
+        a.min_many = AttendPlan::MIN_MANY;
         const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256, es = (int)c.es;
         const uint32_t few = c.grid(plan.few_tiles * kv * plan.few_splits), many = c.grid(plan.many_tiles * kv * plan.many_splits);
         if (a.only) {

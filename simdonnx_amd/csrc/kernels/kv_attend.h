@@ -246,7 +246,7 @@ struct Span {
     int begin, end;          // of this split, begin a multiple of TT
     int pos_first, pos_last; // positions of the tile's first and last row
 };
-template <int PAIRS, int TT> SOX_DEV Span span_of(const sox_kv_attend_args& p, const RowTile& r, int split, int splits) {
+template <int PAIRS, int TT> SOX_DEV Span span_of(const sox_kv_attend_args& p, const RowTile& r, int split, int splits, int min_tokens) {
     Span s;
     const int64_t base = r.length - r.rows;
     const int last = min(r.m0 + PAIRS, r.pairs) - 1;
@@ -255,7 +255,7 @@ template <int PAIRS, int TT> SOX_DEV Span span_of(const sox_kv_attend_args& p, c
     s.lo = p.window > 0 ? max(s.pos_first - p.window + 1, 0) : 0;
     s.hi = (int)min((int64_t)s.pos_last + 1, (int64_t)p.b.table_pages << p.b.shift);
     const int from = s.lo / TT * TT, tiles = max((s.hi - from + TT - 1) / TT, 0);
-    const int per = max((tiles + splits - 1) / splits, (p.min_tokens + TT - 1) / TT);
+    const int per = max((tiles + splits - 1) / splits, (min_tokens + TT - 1) / TT);
     s.begin = min(from + (int)min((int64_t)split * per * TT, (int64_t)1 << 30), max(s.hi, from));
     s.end = min(s.begin + per * TT, s.hi);
     return s;
@@ -349,7 +349,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     const int kvh = block % b.heads, rest = block / b.heads, splits = p.splits_many, split = rest % splits;
     const RowTile r = row_tile<128, true>(p, rest / splits, lane);
     if (!r.some) return;
-    const Span s = span_of<128, TT>(p, r, split, splits);
+    const Span s = span_of<128, TT>(p, r, split, splits, p.min_many);
     const int32_t* const table = b.tables + r.sequence * b.ldt;
     const int mask = (1 << b.shift) - 1;
     const int64_t scale_at = tid < TT ? b.ks_at : b.vs_at;  // of what this thread stages of the scales
@@ -746,7 +746,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     const int kvh = block % b.heads, rest = block / b.heads, splits = p.splits_few, split = rest % splits;
     const RowTile r = row_tile<16, false>(p, rest / splits, lane);
     if (!r.some) return;
-    const Span s = span_of<16, TT>(p, r, split, splits);
+    const Span s = span_of<16, TT>(p, r, split, splits, p.min_few);
     const int32_t* const table = b.tables + r.sequence * b.ldt;
     const int mask = (1 << b.shift) - 1;
     unsigned char* const lv = lds + wave * F::BUF;

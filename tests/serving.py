@@ -5,6 +5,7 @@ from layers import SMALL, UNIT, Matrix, quantize, to_bits
 from simdonnx_amd.backend import HipKvBatch, HipKvCache
 
 U32 = 2.0 ** -24
+TABLE_TOKENS = 0  # tokens that a Serving's tables have room for at least, beyond what its sequences hold
 
 
 class Ints(Matrix):
@@ -44,7 +45,7 @@ class Serving:
         counts = [-(-length // page) for length, _ in sequences]
         self.pages = sum(counts) + spare
         order = rng.permutation(self.pages)
-        self.tables = np.full((len(sequences), max(counts + [1]) + 1), -1, np.int32)
+        self.tables = np.full((len(sequences), max(max(counts + [1]) + 1, TABLE_TOKENS // page)), -1, np.int32)
         at = 0
         for s, n in enumerate(counts):
             self.tables[s, :n] = order[at:at + n]
