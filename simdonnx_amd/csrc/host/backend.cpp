@@ -5925,7 +5925,7 @@ int sox_kv_cache_write(sox_kv_cache* K, void* stream, const sox_kv_batch* batch,
         a.ldq = ldq;
         a.ldy = ldy;
         a.q_heads = q ? q_heads : 0;
-        a.lanes = head_lanes(K->p.head_dim, c.es);
+        a.lanes = head_lanes(((K->p.head_dim / 2 * (int)c.es + 15) / 16) * 16, 1);  // (of the head's first half)
         a.rows_per_block = rows_per_block(c.rows, c.be->info.compute_units);
         if (rotary) a.turn = rotary->turn();
         c.launch(K->write[storage], (uint32_t)((c.rows + a.rows_per_block - 1) / a.rows_per_block), 1, 256, stream, a);

@@ -131,6 +131,16 @@ template <typename T, typename F> struct TurnedChunk {
             }
         }
     }
+    // Two chunks of a head that are each other's pairs, a the first ones
+    SOX_DEV void turn_pairs(TurnedChunk& a, TurnedChunk& b, int ch, const CosSin<F>* table) {
+        const CosSin<F>* const at = table + ch / V;
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const CosSin<F> by = at[e * (TURN_HALF / V)];
+            a.v[e] = turned(a.own[e], -b.own[e], by);
+            b.v[e] = turned(b.own[e], a.own[e], by);
+        }
+    }
     SOX_DEV float turned(T x, T other, CosSin<F> by) {
         if constexpr (sizeof(F) == 8)
             return (float)__builtin_fma((double)(float)other, by.s, (double)(float)x * by.c);

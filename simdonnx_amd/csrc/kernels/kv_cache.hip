@@ -60,6 +60,10 @@ SOX_DEV RowAt row_at(const sox_kv_view& b, int row, int lane) {
 
 constexpr int KV_ROWS = 4;  // of a workgroup at most
 
+// A lane takes two chunks of a head, `wide` channels apart, about half of the head. In a head that turns whole they are each
+// other's pairs: nothing is loaded or converted twice, and what a chunk costs beside its values is paid once for two (this
+// kernel is bound by its instructions: with one chunk a lane, 16384 rows of 8 heads of 128 from bf16 to 8 bits took 42 us,
+// and the memory's share of that is 20).
 template <typename T, typename C> __device__ __forceinline__ void kv_write_body(const sox_kv_rows_args& p) {
     constexpr bool QUANT = sizeof(C) == 1;
     typedef typename std::conditional<QUANT || sizeof(T) == 4, double, float>::type F;
@@ -68,15 +72,22 @@ template <typename T, typename C> __device__ __forceinline__ void kv_write_body(
     __shared__ RowAt where[KV_ROWS];
     const sox_kv_view& b = p.b;
     const int tid = threadIdx.x, lane = tid & 63, rpb = p.rows_per_block, row0 = blockIdx.x * rpb, rows = min(rpb, b.rows - row0);
-    const int sub = tid & ((1 << p.lanes) - 1), ch = sub * V;
+    const int wide = (b.dim / 2 + V - 1) / V * V, sub = tid & ((1 << p.lanes) - 1), half = p.turn.half;
+    const int ch0 = sub * V, ch1 = ch0 + wide;
+    const bool some0 = ch0 < wide, some1 = some0 && ch1 < b.dim;
+    const bool pairs = half == wide && b.dim == 2 * wide && !p.turn.interleaved;
     Walk w = Walk::of(tid >> p.lanes, 256 >> p.lanes, p.q_heads + 2 * b.heads, rows);
-    TurnedChunk<T, F> next;  // on its way while the one before is worked on, the first while the rows' pages are looked for
+    struct Two {
+        TurnedChunk<T, F> a, b;
+    } next;  // on its way while the one before is worked on, the first while the rows' pages are looked for
     auto load = [&] {
-        if (!w.some() || ch >= b.dim) return;
+        if (!w.some() || !some0) return;
         const bool q = w.h < p.q_heads, k = w.h < p.q_heads + b.heads;
-        const int64_t row = row0 + w.r;
-        const T* const from = q ? (const T*)p.q + row * p.ldq : k ? (const T*)p.k + row * p.ldk : (const T*)p.v + row * p.ldv;
-        next.load(from + (int64_t)(q ? w.h : w.h - p.q_heads - (k ? 0 : b.heads)) * b.dim, ch, p.turn, k ? p.turn.half : 0);
+        const int64_t ld = q ? p.ldq : k ? p.ldk : p.ldv;
+        const T* const from = (const T*)(q ? p.q : k ? p.k : p.v) + (row0 + w.r) * ld + (q ? w.h : w.h - p.q_heads - (k ? 0 : b.heads)) * b.dim;
+        const int turns = k && !pairs ? half : 0;
+        next.a.load(from, ch0, p.turn, turns);
+        if (some1) next.b.load(from, ch1, p.turn, turns);
     };
     load();
     for (int r = tid >> 6; r < rows; r += 4) {
@@ -84,10 +95,10 @@ template <typename T, typename C> __device__ __forceinline__ void kv_write_body(
         if (lane == 0) where[r] = at;
     }
     __syncthreads();
-    if (p.turn.half) turn_tables<V>(p.turn, [&](int r) { return where[r].position; }, table, rows, tid, 256);
+    if (half) turn_tables<V>(p.turn, [&](int r) { return where[r].position; }, table, rows, tid, 256);
     __syncthreads();
     while (w.some()) {
-        TurnedChunk<T, F> c = next;
+        Two c = next;
         const int r = w.r, h = w.h;
         w.next();
         load();
@@ -95,63 +106,76 @@ template <typename T, typename C> __device__ __forceinline__ void kv_write_body(
         const int head = is_q ? h : h - p.q_heads - (is_k ? 0 : b.heads);
         const RowAt at = where[r];
         if (at.position < 0 || (at.page < 0 && !is_q)) continue;
-        const bool turned = is_k && p.turn.half;
-        if (ch < b.dim) c.turn(ch, p.turn, turned ? p.turn.half : 0, table[r]);
+        const bool turned = is_k && half;
+        if (some0) {
+            if (turned && pairs) {
+                TurnedChunk<T, F>::turn_pairs(c.a, c.b, ch0, table[r]);
+            } else {
+                c.a.turn(ch0, p.turn, turned ? half : 0, table[r]);
+                if (some1) c.b.turn(ch1, p.turn, turned ? half : 0, table[r]);
+            }
+        }
         if (is_q) {
-            if (ch < b.dim) c.store((T*)p.y + (int64_t)(row0 + r) * p.ldy + (int64_t)head * b.dim, ch);
+            T* const to = (T*)p.y + (row0 + r) * p.ldy + head * b.dim;
+            if (some0) c.a.store(to, ch0);
+            if (some1) c.b.store(to, ch1);
             continue;
         }
         const int64_t token = ((int64_t)head << b.shift) + (at.position & ((1 << b.shift) - 1));
         uint8_t* const page = b.pool + at.page * b.page_bytes;
         C* const to = (C*)(page + (is_k ? 0 : b.v_at)) + token * b.dim;
         if constexpr (!QUANT) {
-            if (ch < b.dim) c.store((T*)to, ch);
+            if (some0) c.a.store((T*)to, ch0);
+            if (some1) c.b.store((T*)to, ch1);
         } else {
-            uint32_t top = 0;
-            if (ch < b.dim)
+            float v[2 * V];
 #pragma unroll
-                for (int e = 0; e < V; e++) top = max(top, abs_bits(c.v[e]));
+            for (int e = 0; e < V; e++) v[e] = some0 ? c.a.v[e] : 0.0f, v[V + e] = some1 ? c.b.v[e] : 0.0f;
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 2 * V; e++) top = max(top, abs_bits(v[e]));
             for (int o = 1; o < 1 << p.lanes; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
             float scale;
-            uint32_t q[V / 4];
+            uint32_t q[V / 2];
             bool sure = false;
             if (turned) {  // (of full precision, whatever T is)
                 // In fp32 first: 127 / amax and its product with x are off by less than 2^-15 for a result up to 127, so one
                 // that is at least 2^-14 from the middle between two integers rounds as the exact one does. About one wave's
-                // chunk in 30 has a value that is nearer and takes the steps in 64 bits, as rows at fp32's ends do.
+                // chunks in 15 have a value that is nearer and take the steps in 64 bits, as rows at fp32's ends do.
                 const float a = __uint_as_float(top), by = 127.0f / a;
                 float far = 0.0f;
-                uint32_t low[V];
-                if (ch < b.dim) {
+                uint32_t low[2 * V];
 #pragma unroll
-                    for (int e = 0; e < V; e++) {
-                        const float x = c.v[e] * by, up = x + 12582912.0f;
-                        low[e] = __float_as_uint(up);
-                        far = fmaxf(far, fabsf(x - (up - 12582912.0f)));
-                    }
+                for (int e = 0; e < 2 * V; e++) {
+                    const float x = v[e] * by, up = x + 12582912.0f;
+                    low[e] = __float_as_uint(up);
+                    far = fmaxf(far, fabsf(x - (up - 12582912.0f)));
                 }
                 sure = !__any(!(far < 0.5f - 0x1p-14f) || !(a > 0x1p-60f && a < 0x1p60f));
                 if (sure) {
                     scale = a / 127.0f;
 #pragma unroll
-                    for (int e = 0; e < V; e += 4)
+                    for (int e = 0; e < 2 * V; e += 4)
                         q[e / 4] = __builtin_amdgcn_perm(low[e + 1], low[e], 0x0c0c0400) | __builtin_amdgcn_perm(low[e + 3], low[e + 2], 0x04000c0c);
                 }
             }
             auto exact = [&](const auto& by) {
                 typedef typename std::decay<decltype(by)>::type Q;
 #pragma unroll
-                for (int e = 0; e < V; e += 4) q[e / 4] = Q::q4(c.v[e], c.v[e + 1], c.v[e + 2], c.v[e + 3], by);
+                for (int e = 0; e < 2 * V; e += 4) q[e / 4] = Q::q4(v[e], v[e + 1], v[e + 2], v[e + 3], by);
                 scale = by.scale;
             };
             if (!turned)
                 exact(RowQuant<T>::make(top));
             else if (!sure)
                 exact(RowQuant<float>::make(top));
-            if (ch < b.dim) {
+            typedef uint32_t Q4 __attribute__((ext_vector_type(V / 4)));
+            typedef Q4 At __attribute__((aligned(4)));
+            Q4 q0, q1;
 #pragma unroll
-                for (int e = 0; e < V / 4; e++) *(uint32_t*)(to + ch + 4 * e) = q[e];
-            }
+            for (int e = 0; e < V / 4; e++) q0[e] = q[e], q1[e] = q[V / 4 + e];
+            if (some0) *(At*)(to + ch0) = q0;
+            if (some1) *(At*)(to + ch1) = q1;
             if (sub == 0) ((float*)(page + (is_k ? b.ks_at : b.vs_at)))[token] = scale;
         }
     }
