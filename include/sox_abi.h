@@ -679,7 +679,7 @@ typedef struct sox_kv_attend_args {
     int32_t splits_few, splits_many;  /* of a tile's tokens; the merge takes them by a sequence's pairs */
     int32_t min_few, min_many;        /* tokens of a split at least */
     int32_t stride;                   /* of the partial results of a (row, query head) */
-    int32_t many, few, each;                        /* both kernels in one: workgroups; the merge: (row, head)s of a workgroup */
+    int32_t many, few;                /* both kernels in one: workgroups */
     float scale_log2;                 /* scale * log2(e) */
 } sox_kv_attend_args;
 

@@ -6010,8 +6010,9 @@ int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch
             c.launch(K->few[storage], few, 1, 256, stream, a, attend_lds(false, dp, es));
         }
         if (a.stride > 1) {
-            a.each = a.stride > 8 ? 1 : 4;  // (row, head)s of a workgroup that joins
-            c.launch(K->merge[storage], c.grid((heads + a.each - 1) / a.each), 1, 256, stream, a);
+            // up to 8 splits: a wave for as many of a row's heads as it has lanes for; more: a workgroup for a head
+            const int64_t together = dim <= 64 ? 4 : dim <= 128 ? 2 : 1, waves = c.rows * ((q_heads + together - 1) / together);
+            c.launch(K->merge[storage], c.grid(a.stride <= 8 ? (waves + 3) / 4 : heads), 1, 256, stream, a);
         }
     });
 }

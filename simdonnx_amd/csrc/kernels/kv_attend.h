@@ -1009,21 +1009,66 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 // =====================================================================================================================
 // the splits' results joined
 // =====================================================================================================================
-// 64 threads for each (row, query head), 256 where there are many splits (p.each: (row, head)s of a workgroup). A row of
-// partial results takes dim / 4 lanes, so 64 / (dim / 4) of them are in flight for each wave's load, four loads at a time. A split
-// that had no tokens left a sum of -1 and nothing else; such splits are the last.
-template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_attend_args& p) {
+// A row's splits: none where it is no sequence's, or has one and its result already, or a negative position (left alone)
+SOX_DEV int merge_splits(const sox_kv_attend_args& p, int row, int lane) {
     const sox_kv_view& b = p.b;
-    const int each = p.each, threads = AT_THREADS / each, tid = threadIdx.x, lane = tid & 63;
-    const int64_t which = (int64_t)blockIdx.x * each + tid / threads;
-    const int row = __builtin_amdgcn_readfirstlane((int)(which / p.q_heads)), head = __builtin_amdgcn_readfirstlane((int)(which % p.q_heads));
-    const int s = row < b.rows ? kv_sequence(b, row, lane) : -1;
-    int splits = 0;
-    if (s >= 0) {
-        const int first = min(max(b.starts[s], 0), b.rows), rows = max(min(b.starts[s + 1], b.rows) - first, 0);
-        splits = (int64_t)rows * p.group > 16 ? p.splits_many : p.splits_few;
-        if (splits < 2 || (int64_t)max(b.lengths[s], 0) - rows + (row - first) < 0) splits = 0;
+    const int s = kv_sequence(b, row, lane);
+    if (s < 0) return 0;
+    const int first = min(max(b.starts[s], 0), b.rows), rows = max(min(b.starts[s + 1], b.rows) - first, 0);
+    const int splits = (int64_t)rows * p.group > 16 ? p.splits_many : p.splits_few;
+    return splits < 2 || (int64_t)max(b.lengths[s], 0) - rows + (row - first) < 0 ? 0 : splits;
+}
+// What a partial result counts, from its reference and sum (the sum of one without a token is 0)
+SOX_DEV float merge_weight(float from, float l, float ref) { return l == 0.0f ? 0.0f : from == ref ? 1.0f : __builtin_amdgcn_exp2f(from - ref); }
+constexpr int MERGE_WAVE = 8;  // splits that one lane joins
+
+// A partial result takes dim / 4 lanes. Up to MERGE_WAVE of them: a wave for a row's 1, 2 or 4 heads, each lane its channels of all
+// splits, and everything, whether the row turns out to need it or not, on its way at once (512 rows and 31 tokens of 32 heads, three
+// splits: 9 us against 12 with a wave for each head that looked for its row first).
+template <typename T> __device__ __forceinline__ void merge_wave(const sox_kv_attend_args& p) {
+    const sox_kv_view& b = p.b;
+    const int lane = threadIdx.x & 63, lanes = b.dim <= 64 ? 16 : b.dim <= 128 ? 32 : 64, heads = 64 / lanes, units = (p.q_heads + heads - 1) / heads;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * (AT_THREADS / 64) + threadIdx.x / 64);
+    const int row = (int)(w / (uint32_t)units), head = (int)(w % (uint32_t)units) * heads + lane / lanes, ch = lane % lanes * 4;
+    if (row >= b.rows) return;
+    const bool mine = head < p.q_heads && ch < b.dim;
+    const int64_t at = ((int64_t)row * p.q_heads + min(head, p.q_heads - 1)) * p.stride;
+    const float* const part = p.part + at * b.dim + min(ch, b.dim - 4);
+    float4v o[MERGE_WAVE];
+    float from[MERGE_WAVE], l[MERGE_WAVE];
+#pragma unroll
+    for (int i = 0; i < MERGE_WAVE; i++)
+        if (i < p.stride) {
+            from[i] = p.ml[(at + i) * 2], l[i] = p.ml[(at + i) * 2 + 1];
+            o[i] = *(const float4v*)(part + (int64_t)i * b.dim);
+        }
+    const int splits = merge_splits(p, row, lane);
+    if (splits == 0) return;
+    float ref = -__builtin_inff(), sum = 0.0f;
+    float4v v = {};
+#pragma unroll
+    for (int i = 0; i < MERGE_WAVE; i++)
+        if (i < splits && l[i] != -1.0f) ref = fmaxf(ref, from[i]);
+#pragma unroll
+    for (int i = 0; i < MERGE_WAVE; i++)
+        if (i < splits && l[i] != -1.0f) {
+            const float by = merge_weight(from[i], l[i], ref);
+            sum += by * l[i];
+            v += by * o[i];
+        }
+    if (mine) store4((T*)p.y + (int64_t)row * p.ldy + (int64_t)head * b.dim + ch, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
+}
+
+// More: 256 threads for a (row, head), 256 / (dim / 4) results in flight for each load, four loads at a time. A split that had no
+// tokens left a sum of -1 and nothing else; such splits are the last.
+template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_attend_args& p) {
+    if (p.stride <= MERGE_WAVE) {
+        merge_wave<T>(p);
+        return;
     }
+    const sox_kv_view& b = p.b;
+    const int tid = threadIdx.x, lane = tid & 63, row = (int)(blockIdx.x / (uint32_t)p.q_heads), head = (int)(blockIdx.x % (uint32_t)p.q_heads);
+    const int splits = merge_splits(p, row, lane);
     const int64_t at = ((int64_t)row * p.q_heads + head) * p.stride;
     const float* const ml = p.ml + at * 2;
     float ref = -__builtin_inff();
@@ -1034,8 +1079,8 @@ template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_
         n += __popcll(__ballot(some));
     }
     for (int o = 1; o < 64; o <<= 1) ref = fmaxf(ref, __shfl_xor(ref, o));
-    const int lanes = b.dim <= 64 ? 16 : b.dim <= 128 ? 32 : 64, groups = threads / lanes;
-    const int mine = tid % threads, group = mine / lanes, ch = mine % lanes * 4;
+    const int lanes = b.dim <= 64 ? 16 : b.dim <= 128 ? 32 : 64, groups = AT_THREADS / lanes;
+    const int group = tid / lanes, ch = tid % lanes * 4;
     const float* const part = p.part + at * b.dim + ch;
     float sum = 0.0f;
     float4v v = {};
@@ -1054,7 +1099,7 @@ template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_
         }
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const float by = l[k] == 0.0f ? 0.0f : from[k] == ref ? 1.0f : __builtin_amdgcn_exp2f(from[k] - ref);
+            const float by = merge_weight(from[k], l[k], ref);
             sum += by * l[k];
             v += by * o[k];
         }
