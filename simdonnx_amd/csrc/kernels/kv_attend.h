@@ -1020,7 +1020,7 @@ SOX_DEV int merge_splits(const sox_kv_attend_args& p, int row, int lane) {
 }
 // What a partial result counts, from its reference and sum (the sum of one without a token is 0)
 SOX_DEV float merge_weight(float from, float l, float ref) { return l == 0.0f ? 0.0f : from == ref ? 1.0f : __builtin_amdgcn_exp2f(from - ref); }
-constexpr int MERGE_WAVE = 8;  // splits that one lane joins
+constexpr int MERGE_WAVE = 8;  // results that a lane has on their way; splits that one lane joins alone
 
 // A partial result takes dim / 4 lanes. Up to MERGE_WAVE of them: a wave for a row's 1, 2 or 4 heads, each lane its channels of all
 // splits, and everything, whether the row turns out to need it or not, on its way at once (512 rows and 31 tokens of 32 heads, three
@@ -1059,7 +1059,7 @@ template <typename T> __device__ __forceinline__ void merge_wave(const sox_kv_at
     if (mine) store4((T*)p.y + (int64_t)row * p.ldy + (int64_t)head * b.dim + ch, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
 }
 
-// More: 256 threads for a (row, head), 256 / (dim / 4) results in flight for each load, four loads at a time. A split that had no
+// More: 256 threads for a (row, head), 256 / (dim / 4) results in flight for each load, eight loads at a time. A split that had no
 // tokens left a sum of -1 and nothing else; such splits are the last.
 template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_attend_args& p) {
     if (p.stride <= MERGE_WAVE) {
@@ -1084,11 +1084,11 @@ template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_
     const float* const part = p.part + at * b.dim + ch;
     float sum = 0.0f;
     float4v v = {};
-    for (int i0 = group; i0 < n; i0 += 4 * groups) {
-        float4v o[4];
-        float from[4], l[4];
+    for (int i0 = group; i0 < n; i0 += MERGE_WAVE * groups) {
+        float4v o[MERGE_WAVE];
+        float from[MERGE_WAVE], l[MERGE_WAVE];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < MERGE_WAVE; k++) {
             const int i = i0 + k * groups;
             o[k] = float4v{};
             from[k] = ref, l[k] = 0.0f;
@@ -1098,7 +1098,7 @@ template <typename T> __device__ __forceinline__ void attend_merge(const sox_kv_
             }
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < MERGE_WAVE; k++) {
             const float by = merge_weight(from[k], l[k], ref);
             sum += by * l[k];
             v += by * o[k];
