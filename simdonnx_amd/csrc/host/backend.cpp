@@ -5720,7 +5720,7 @@ struct KvCall : LayerCall {
         return v;
     }
     uint32_t grid(int64_t workgroups) const {
-        if (workgroups > 0x7fffffff) fail(SOX_E_UNSUPPORTED, std::string(name) + ": too many rows");
+        if (workgroups > 0xffffff) fail(SOX_E_UNSUPPORTED, std::string(name) + ": too many rows");  // (a launch has less than 2^32 threads)
         return (uint32_t)workgroups;
     }
 };
@@ -5970,9 +5970,12 @@ int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch
         if (c.idle()) return;
         const Rows Q = c.heads("q", q, ldq, q_heads), Y = c.heads("y", y, ldy, q_heads);
         const int64_t heads = c.rows * q_heads;
+        if (heads > 1 << 30) fail(SOX_E_UNSUPPORTED, "KvCache.Attend: more than 2^30 rows times q_heads");  // (the kernels count them in 32 bits)
         int64_t tokens = (int64_t)batch->table_pages << K->shift;
         if (window) tokens = std::min(tokens, (int64_t)window + std::min<int64_t>(c.rows, 128 / (q_heads / kv) + 1));  // (what a tile's rows see)
         const AttendPlan plan(c.rows, batch->sequences, q_heads, kv, tokens, c.be->info.compute_units);
+        const uint32_t few = c.grid(plan.few_tiles * kv * plan.few_splits), many = c.grid(plan.many_tiles * kv * plan.many_splits);
+        if (plan.use_few && plan.use_many) c.grid((int64_t)few + many);
         Rows W{"workspace"};
         if (const uint64_t need = plan.need(heads, dim)) {
             if (!workspace || workspace_bytes < need)
@@ -6001,11 +6004,10 @@ int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch
         a.min_few = AttendPlan::MIN_FEW;
         a.min_many = AttendPlan::MIN_MANY;
         const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256, es = (int)c.es;
-        const uint32_t few = c.grid(plan.few_tiles * kv * plan.few_splits), many = c.grid(plan.many_tiles * kv * plan.many_splits);
         if (a.only) {
             a.many = (int32_t)std::min<int64_t>(many, plan.usual_tiles * kv * plan.many_splits);
             a.few = (int32_t)few;
-            c.launch(K->both[storage], c.grid((int64_t)many + few), 1, 256, stream, a, std::max(attend_lds(true, dp, es), attend_lds(false, dp, es)));
+            c.launch(K->both[storage], many + few, 1, 256, stream, a, std::max(attend_lds(true, dp, es), attend_lds(false, dp, es)));
         } else if (plan.use_many) {
             c.launch(K->many[storage], many, 1, 256, stream, a, attend_lds(true, dp, es));
         } else {

@@ -105,7 +105,8 @@ def attend64(q, k, v, first, scale, window, storage, absent=None):
 
     A score: dim products summed in fp32, each partial sum off by a unit of the sum of magnitudes, and four more for the scales
     and the exponential's argument; e is the largest of a row. p is off by that twice over (its own and the reference's,
-    which the sum divides out) and by half a step of the storage type where 16 bits hold it for its product; p too
+    which the sum divides out) and by half a step of the storage type where 16 bits hold it for its product; the sum may take p as
+    it is or as rounded, and then is off by at most that half step of itself, y by that half step of |y|; p too
     small for fp16's normal numbers by half of 2^-24 of the largest value for each token, and p below fp32's normal numbers by
     itself, 2^-126 at most (the reference is no larger than the largest score, so the sum that divides is 1 or more). The
     sums of n terms: n units, twice."""
@@ -133,7 +134,7 @@ def attend64(q, k, v, first, scale, window, storage, absent=None):
             n = int(sees.sum())
             half = 0.0 if storage == "f32" else UNIT[storage]
             tiny = n * (2.0 ** -25 if storage == "f16" else 2.0 ** -126) * np.abs(vv).max(axis=0)
-            tol[i, mine] = (half + 4 * e + (2 * n + 16) * U32) * size + tiny + UNIT[storage] * np.abs(y[i, mine]) + SMALL[storage]
+            tol[i, mine] = (half + 4 * e + (2 * n + 16) * U32) * size + tiny + (half + UNIT[storage]) * np.abs(y[i, mine]) + SMALL[storage]
     return y, tol
 
 

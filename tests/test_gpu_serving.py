@@ -92,6 +92,30 @@ def test_halves_of_turned_keys(hip, storage):
     s.free()
 
 
+# ---- weights that are small each and count together ----
+@pytest.mark.parametrize("room", [0, 1 << 19])
+@pytest.mark.parametrize("storage,fmt", FORMATS)
+@pytest.mark.parametrize("new", [1, 64])
+def test_many_small_weights(hip, monkeypatch, storage, fmt, room, new):
+    """One token of weight 1 and 4095 of 2^-16, below fp16's normal numbers, with the opposite value."""
+    monkeypatch.setattr(serving, "TABLE_TOKENS", room)
+    n, dim = 4096, 64
+    s = Serving(hip, [(n, new)], 1, dim, 16, fmt)
+    k, v, q = np.zeros((n, 1, dim), np.float32), -np.ones((n, 1, dim), np.float32), np.zeros((new, 2, dim), np.float32)
+    k[100, 0, 0], v[100] = rounded(np.array([[16 * np.log(2.0)]], np.float32), storage)[0, 0], 1
+    q[..., 0] = 8  # (scale 1 / 8: the score is k's first value)
+    K, V, Q, Y = Matrix(k.reshape(n, -1), storage), Matrix(v.reshape(n, -1), storage), Matrix(q.reshape(new, -1), storage), Matrix(None, storage, new, 2 * dim)
+    W = Matrix(None, "i8", 1, s.cache.workspace(new, 1, 2))
+    s.cache.write(s.every, K.ptr, V.ptr, storage)
+    s.cache.attend(s.batch, Q.ptr, 2, Y.ptr, storage, workspace=W.ptr, workspace_bytes=W.cols)
+    want, tol = attend64(q.astype(np.float64), held64(k, storage, fmt), held64(v, storage, fmt), n - new, dim ** -0.5, 0, storage)
+    assert 0.87 < want.min() and want.max() < 0.9  # (without the small weights it would be 1)
+    close(Y.read().reshape(want.shape), want, tol, "y")
+    for m in (K, V, Q, Y, W):
+        m.free()
+    s.free()
+
+
 # ---- captured ----
 class Side:
     """A batch, its workspace and its stream, with room for its sequences to grow."""

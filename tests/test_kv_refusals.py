@@ -238,3 +238,15 @@ def test_a_backend_of_its_own(offline, cache):  # noqa: F811
     refused("another head_dim or backend", cache.write, batch(), at(0), at(1), rotary=r)
     r.close()
     b.close()
+
+
+def test_attend_too_large(offline):  # noqa: F811
+    """More (row, query head)s than 32 bits count with their tiles, more workgroups than a launch holds."""
+    c, q, y = HipKvCache(offline, 128, 8, 16, "f16"), at(0) + (1 << 40), at(0) + (1 << 41)
+    far = dict(tables=at(0) + (1 << 42), starts=at(0) + (1 << 43), lengths=at(0) + (1 << 44))
+    with pytest.raises(NotSupportedError, match="2\\^30 rows times q_heads"):
+        c.attend(batch(rows=1 << 23), q, 256, y)
+    in_order(c.attend, batch(sequences=1 << 16, rows=1 << 16, ldt=12, **far), q, 128, y)
+    with pytest.raises(NotSupportedError, match="too many rows"):
+        c.attend(batch(sequences=1 << 20, rows=1 << 20, ldt=12, **far), q, 128, y)
+    c.close()
