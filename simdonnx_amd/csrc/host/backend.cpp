@@ -5753,13 +5753,17 @@ struct AttendPlan {
             use_few = use_many = true;
         few_tiles = use_many ? sequences : pairs / 16 + sequences;
         many_tiles = pairs / 128 + (use_few ? std::min(sequences, pairs / 17) : sequences);
-        if (use_few) few_splits = splits(few_tiles * kv_heads, rows * q_heads, tokens / MIN_FEW, 2 * cus);
+        if (few_tiles * kv_heads * 4 <= cus) few_min = 128;
+        if (use_few) few_splits = splits(few_tiles * kv_heads, rows * q_heads, tokens / few_min, 2 * cus);
         // Beside single tokens the many rows are most often one sequence's: the tiles that there are, not those that there may be,
         // and one workgroup a CU, with the single tokens' for neighbours (512 rows and 31 tokens: 144 us against 156 with two)
         usual_tiles = use_few ? pairs / 128 + 1 : many_tiles;
         if (use_many) many_splits = splits(usual_tiles * kv_heads, rows * q_heads, tokens / MIN_MANY, (use_few ? 1 : 2) * cus);
     }
-    static constexpr int MIN_FEW = 256, MIN_MANY = 256;  // tokens of a split at least
+    // Tokens of a split at least. Where few workgroups leave most CUs idle, one tile for each of a workgroup's waves is worth its
+    // join (6 fp32 heads, pieces of 333 tokens, 57 workgroups: 17 us against 21); where they do not, it is not (288: 22 against 13).
+    static constexpr int MIN_MANY = 256;
+    int few_min = 256;
     static int splits(int64_t workgroups, int64_t heads, int64_t most, int64_t fill) {
         const int64_t n = std::min({(fill + workgroups - 1) / workgroups, most, MAX_SPLITS, PARTIALS / heads});
         return (int)std::max<int64_t>(n, 1);
@@ -6001,7 +6005,7 @@ int sox_kv_cache_attend(sox_kv_cache* K, void* stream, const sox_kv_batch* batch
         a.scale_log2 = (float)((scale == 0 ? 1.0 / std::sqrt((double)dim) : (double)scale) * 1.4426950408889634);
         a.splits_few = plan.use_few ? plan.few_splits : plan.many_splits;  // (the merge asks by a sequence's pairs)
         a.splits_many = plan.use_many ? plan.many_splits : plan.few_splits;
-        a.min_few = AttendPlan::MIN_FEW;
+        a.min_few = plan.few_min;
         a.min_many = AttendPlan::MIN_MANY;
         const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256, es = (int)c.es;
         if (a.only) {
