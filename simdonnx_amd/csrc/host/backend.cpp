@@ -5670,6 +5670,8 @@ int head_lanes(int dim, int64_t es) {
     while ((16 << lanes) < dim * es) lanes++;
     return lanes;
 }
+// and of its first half, in whole lanes
+int half_lanes(int dim, int64_t es) { return head_lanes((dim / 2 * (int)es + 15) / 16 * 16, 1); }
 // Rows of a workgroup: one where there are few, so that they spread over the CUs; four otherwise, which share the table's work
 int rows_per_block(int64_t rows, int cus) { return rows > 8 * cus ? 4 : 1; }
 
@@ -5857,7 +5859,7 @@ int sox_rotary_run(sox_rotary* R, void* stream, int32_t storage, const int32_t* 
         a.rows = rows;
         a.heads = heads;
         a.dim = R->p.head_dim;
-        a.lanes = head_lanes(a.dim, c.es);
+        a.lanes = half_lanes(a.dim, c.es);
         a.rows_per_block = rows_per_block(rows, c.be->info.compute_units);
         a.turn = R->turn();
         c.launch(R->fns[storage], (uint32_t)((rows + a.rows_per_block - 1) / a.rows_per_block), 1, 256, stream, a);
@@ -5931,7 +5933,7 @@ int sox_kv_cache_write(sox_kv_cache* K, void* stream, const sox_kv_batch* batch,
         a.ldq = ldq;
         a.ldy = ldy;
         a.q_heads = q ? q_heads : 0;
-        a.lanes = head_lanes(((K->p.head_dim / 2 * (int)c.es + 15) / 16) * 16, 1);  // (of the head's first half)
+        a.lanes = half_lanes(K->p.head_dim, c.es);
         a.rows_per_block = rows_per_block(c.rows, c.be->info.compute_units);
         if (rotary) a.turn = rotary->turn();
         c.launch(K->write[storage], (uint32_t)((c.rows + a.rows_per_block - 1) / a.rows_per_block), 1, 256, stream, a);

@@ -20,28 +20,66 @@ struct Walk {
     __device__ __forceinline__ bool some() const { return r < rows; }
 };
 
+// A lane takes two chunks of a head, `wide` channels apart, about half of the head. In a head that turns whole they are each
+// other's pairs: nothing is loaded or converted twice, and what a chunk costs beside its values is paid once for two.
+template <typename T, typename F> struct Halves {
+    static constexpr int V = 16 / sizeof(T);
+    int wide, ch0, ch1;
+    bool some0, some1, pairs;
+    SOX_DEV Halves of(int dim, const sox_turn_args& t, int sub) {
+        Halves l;
+        l.wide = (dim / 2 + V - 1) / V * V;
+        l.ch0 = sub * V;
+        l.ch1 = l.ch0 + l.wide;
+        l.some0 = l.ch0 < l.wide;
+        l.some1 = l.some0 && l.ch1 < dim;
+        l.pairs = t.half == l.wide && dim == 2 * l.wide && !t.interleaved;
+        return l;
+    }
+};
+template <typename T, typename F> struct Two {
+    TurnedChunk<T, F> a, b;
+    __device__ __forceinline__ void load(const Halves<T, F>& l, const T* head, const sox_turn_args& t, bool turned) {
+        if (!l.some0) return;
+        const int half = turned && !l.pairs ? t.half : 0;
+        a.load(head, l.ch0, t, half);
+        if (l.some1) b.load(head, l.ch1, t, half);
+    }
+    __device__ __forceinline__ void turn(const Halves<T, F>& l, const sox_turn_args& t, bool turned, const CosSin<F>* table) {
+        if (!l.some0) return;
+        if (turned && l.pairs) {
+            TurnedChunk<T, F>::turn_pairs(a, b, l.ch0, table);
+        } else {
+            a.turn(l.ch0, t, turned ? t.half : 0, table);
+            if (l.some1) b.turn(l.ch1, t, turned ? t.half : 0, table);
+        }
+    }
+    __device__ __forceinline__ void store(const Halves<T, F>& l, T* head) const {
+        if (l.some0) a.store(head, l.ch0);
+        if (l.some1) b.store(head, l.ch1);
+    }
+};
+
 template <typename T> __device__ __forceinline__ void rotary_body(const sox_rotary_args& p) {
     typedef typename std::conditional<sizeof(T) == 4, double, float>::type F;
-    constexpr int V = 16 / sizeof(T);
     __shared__ CosSin<F> table[4][TURN_HALF];
     const int tid = threadIdx.x, rpb = p.rows_per_block, row0 = blockIdx.x * rpb, rows = min(rpb, p.rows - row0);
-    const int ch = (tid & ((1 << p.lanes) - 1)) * V, half = p.turn.half;
+    const Halves<T, F> l = Halves<T, F>::of(p.dim, p.turn, tid & ((1 << p.lanes) - 1));
     Walk w = Walk::of(tid >> p.lanes, 256 >> p.lanes, p.heads, rows);
-    TurnedChunk<T, F> next;
+    Two<T, F> next;
     auto load = [&] {
-        if (w.some() && ch < p.dim) next.load((const T*)p.x + (int64_t)(row0 + w.r) * p.ldx + (int64_t)w.h * p.dim, ch, p.turn, half);
+        if (w.some()) next.load(l, (const T*)p.x + (row0 + w.r) * p.ldx + (int64_t)w.h * p.dim, p.turn, true);
     };
     load();
-    turn_tables<V>(p.turn, [&](int r) { return p.positions[row0 + r]; }, table, rows, tid, 256);
+    turn_tables<16 / sizeof(T)>(p.turn, [&](int r) { return p.positions[row0 + r]; }, table, rows, tid, 256);
     __syncthreads();
     while (w.some()) {
-        TurnedChunk<T, F> c = next;
+        Two<T, F> c = next;
         const int r = w.r, h = w.h;
         w.next();
         load();
-        if (ch >= p.dim) continue;
-        c.turn(ch, p.turn, half, table[r]);
-        c.store((T*)p.y + (int64_t)(row0 + r) * p.ldy + (int64_t)h * p.dim, ch);
+        c.turn(l, p.turn, true, table[r]);
+        c.store(l, (T*)p.y + (row0 + r) * p.ldy + (int64_t)h * p.dim);
     }
 }
 
@@ -60,10 +98,8 @@ SOX_DEV RowAt row_at(const sox_kv_view& b, int row, int lane) {
 
 constexpr int KV_ROWS = 4;  // of a workgroup at most
 
-// A lane takes two chunks of a head, `wide` channels apart, about half of the head. In a head that turns whole they are each
-// other's pairs: nothing is loaded or converted twice, and what a chunk costs beside its values is paid once for two (this
-// kernel is bound by its instructions: with one chunk a lane, 16384 rows of 8 heads of 128 from bf16 to 8 bits took 42 us,
-// and the memory's share of that is 20).
+// Bound by its instructions in 8 bits: 16384 rows of 8 heads of 128 from bf16 take 37 us (42 with one chunk a lane), and the memory's
+// share of that is 20.
 template <typename T, typename C> __device__ __forceinline__ void kv_write_body(const sox_kv_rows_args& p) {
     constexpr bool QUANT = sizeof(C) == 1;
     typedef typename std::conditional<QUANT || sizeof(T) == 4, double, float>::type F;
@@ -72,22 +108,16 @@ template <typename T, typename C> __device__ __forceinline__ void kv_write_body(
     __shared__ RowAt where[KV_ROWS];
     const sox_kv_view& b = p.b;
     const int tid = threadIdx.x, lane = tid & 63, rpb = p.rows_per_block, row0 = blockIdx.x * rpb, rows = min(rpb, b.rows - row0);
-    const int wide = (b.dim / 2 + V - 1) / V * V, sub = tid & ((1 << p.lanes) - 1), half = p.turn.half;
-    const int ch0 = sub * V, ch1 = ch0 + wide;
-    const bool some0 = ch0 < wide, some1 = some0 && ch1 < b.dim;
-    const bool pairs = half == wide && b.dim == 2 * wide && !p.turn.interleaved;
+    const int sub = tid & ((1 << p.lanes) - 1), half = p.turn.half;
+    const Halves<T, F> l = Halves<T, F>::of(b.dim, p.turn, sub);
     Walk w = Walk::of(tid >> p.lanes, 256 >> p.lanes, p.q_heads + 2 * b.heads, rows);
-    struct Two {
-        TurnedChunk<T, F> a, b;
-    } next;  // on its way while the one before is worked on, the first while the rows' pages are looked for
+    Two<T, F> next;  // on its way while the one before is worked on, the first while the rows' pages are looked for
     auto load = [&] {
-        if (!w.some() || !some0) return;
+        if (!w.some()) return;
         const bool q = w.h < p.q_heads, k = w.h < p.q_heads + b.heads;
         const int64_t ld = q ? p.ldq : k ? p.ldk : p.ldv;
         const T* const from = (const T*)(q ? p.q : k ? p.k : p.v) + (row0 + w.r) * ld + (q ? w.h : w.h - p.q_heads - (k ? 0 : b.heads)) * b.dim;
-        const int turns = k && !pairs ? half : 0;
-        next.a.load(from, ch0, p.turn, turns);
-        if (some1) next.b.load(from, ch1, p.turn, turns);
+        next.load(l, from, p.turn, k);
     };
     load();
     for (int r = tid >> 6; r < rows; r += 4) {
@@ -98,7 +128,7 @@ template <typename T, typename C> __device__ __forceinline__ void kv_write_body(
     if (half) turn_tables<V>(p.turn, [&](int r) { return where[r].position; }, table, rows, tid, 256);
     __syncthreads();
     while (w.some()) {
-        Two c = next;
+        Two<T, F> c = next;
         const int r = w.r, h = w.h;
         w.next();
         load();
@@ -107,30 +137,20 @@ template <typename T, typename C> __device__ __forceinline__ void kv_write_body(
         const RowAt at = where[r];
         if (at.position < 0 || (at.page < 0 && !is_q)) continue;
         const bool turned = is_k && half;
-        if (some0) {
-            if (turned && pairs) {
-                TurnedChunk<T, F>::turn_pairs(c.a, c.b, ch0, table[r]);
-            } else {
-                c.a.turn(ch0, p.turn, turned ? half : 0, table[r]);
-                if (some1) c.b.turn(ch1, p.turn, turned ? half : 0, table[r]);
-            }
-        }
+        c.turn(l, p.turn, turned, table[r]);
         if (is_q) {
-            T* const to = (T*)p.y + (row0 + r) * p.ldy + head * b.dim;
-            if (some0) c.a.store(to, ch0);
-            if (some1) c.b.store(to, ch1);
+            c.store(l, (T*)p.y + (row0 + r) * p.ldy + head * b.dim);
             continue;
         }
         const int64_t token = ((int64_t)head << b.shift) + (at.position & ((1 << b.shift) - 1));
         uint8_t* const page = b.pool + at.page * b.page_bytes;
         C* const to = (C*)(page + (is_k ? 0 : b.v_at)) + token * b.dim;
         if constexpr (!QUANT) {
-            if (some0) c.a.store((T*)to, ch0);
-            if (some1) c.b.store((T*)to, ch1);
+            c.store(l, (T*)to);
         } else {
             float v[2 * V];
 #pragma unroll
-            for (int e = 0; e < V; e++) v[e] = some0 ? c.a.v[e] : 0.0f, v[V + e] = some1 ? c.b.v[e] : 0.0f;
+            for (int e = 0; e < V; e++) v[e] = l.some0 ? c.a.v[e] : 0.0f, v[V + e] = l.some1 ? c.b.v[e] : 0.0f;
             uint32_t top = 0;
 #pragma unroll
             for (int e = 0; e < 2 * V; e++) top = max(top, abs_bits(v[e]));
@@ -174,8 +194,8 @@ template <typename T, typename C> __device__ __forceinline__ void kv_write_body(
             Q4 q0, q1;
 #pragma unroll
             for (int e = 0; e < V / 4; e++) q0[e] = q[e], q1[e] = q[V / 4 + e];
-            if (some0) *(At*)(to + ch0) = q0;
-            if (some1) *(At*)(to + ch1) = q1;
+            if (l.some0) *(At*)(to + l.ch0) = q0;
+            if (l.some1) *(At*)(to + l.ch1) = q1;
             if (sub == 0) ((float*)(page + (is_k ? b.ks_at : b.vs_at)))[token] = scale;
         }
     }
