@@ -248,14 +248,20 @@ struct Span {
     int lo, hi;              // tokens that any row sees
     int begin, end;          // of this split, begin a multiple of TT
     int pos_first, pos_last; // positions of the tile's first and last row
+    int low_last;            // the last token that the last row's window leaves out, or -1
 };
+// The last token that a window leaves out for a row at `pos`, or -1
+SOX_DEV int window_low(const sox_kv_attend_args& p, int pos) {
+    return p.window > 0 ? (int)max((int64_t)pos - p.window, (int64_t)-1) : -1;
+}
 template <int PAIRS, int TT> SOX_DEV Span span_of(const sox_kv_attend_args& p, const RowTile& r, int split, int splits, int min_tokens) {
     Span s;
     const int64_t base = r.length - r.rows;
     const int last = min(r.m0 + PAIRS, r.pairs) - 1;
     s.pos_first = (int)(base + r.m0 / p.group);
     s.pos_last = (int)(base + last / p.group);
-    s.lo = p.window > 0 ? max(s.pos_first - p.window + 1, 0) : 0;
+    s.lo = window_low(p, s.pos_first) + 1;
+    s.low_last = window_low(p, s.pos_last);
     s.hi = (int)min((int64_t)s.pos_last + 1, (int64_t)p.b.table_pages << p.b.shift);
     const int from = s.lo / TT * TT, tiles = max((s.hi - from + TT - 1) / TT, 0);
     const int per = max((tiles + splits - 1) / splits, (min_tokens + TT - 1) / TT);
@@ -361,7 +367,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     const int m = r.m0 + 32 * wave + col;
     const bool mine = m < r.pairs;
     // (a lane without a pair sees all: nothing, and its wave would look for a reference in every tile)
-    const int pos = mine ? (int)(r.length - r.rows + m / p.group) : 0x7fffffff, low = mine && p.window > 0 ? pos - p.window : -1;
+    const int pos = mine ? (int)(r.length - r.rows + m / p.group) : 0x7fffffff, low = mine ? window_low(p, pos) : -1;
     const int wave_last = r.m0 + 32 * wave < r.pairs ? (int)(r.length - r.rows + (min(r.m0 + 32 * wave + 32, r.pairs) - 1) / p.group) : -1;
     FV qf[M::KS];
     {
@@ -468,7 +474,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
             }
         }
     };
-    auto is_cut = [&](int t0) { return t0 + TT - 1 > s.pos_first || (p.window > 0 && t0 <= s.pos_last - p.window); };
+    auto is_cut = [&](int t0) { return t0 + TT - 1 > s.pos_first || t0 <= s.low_last; };
     auto in_part = [&](int t0, uint64_t valid) { return is_cut(t0) || ~valid << (64 - TT) != 0; };  // (or without some of its tokens)
 
     // ---- a tile ----
@@ -758,7 +764,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 
     const int m = r.m0 + col;
     const bool mine = m < r.pairs;
-    const int pos = mine ? (int)(r.length - r.rows + m / p.group) : -1, low = p.window > 0 ? pos - p.window : -1;
+    const int pos = mine ? (int)(r.length - r.rows + m / p.group) : -1, low = window_low(p, pos);
     FV qf[F::KU][F::NCH];
     {
         const T* const q = row_q<T>(p, r, kvh, mine ? m : r.m0);
@@ -781,7 +787,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     auto entry = [&](int t0) { return tile_entry(b, table, t0 + min(lane, TT - 1)); };
     auto page_of = [&](int t0, int entry) { return lane < TT ? tile_page(b, entry, t0 + lane, s.lo, s.end) : -1; };
     auto row_at = [&](int t0, int page, int row) { return head_rows(b, head, page, ((t0 + row) & mask) * row_bytes); };
-    const int scale_at = lane < TT ? b.ks_at : b.vs_at;
+    const int64_t scale_at = lane < TT ? b.ks_at : b.vs_at;
     const uint32_t lane_k = (uint32_t)(col * DP * (int)sizeof(C) + quad * 16);
     const bool wide_pages = b.shift >= 4 && b.dim == DP;  // 16 tokens of a tile seen whole stand in one page
     auto load = [&](int t0, int pages, bool part) {
@@ -828,7 +834,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     int t0 = s.begin + wave * TT;
     int pages = page_of(t0, entry(t0)), next = entry(t0 + stride);
     auto in_part = [&](int t0, uint64_t valid) {  // a tile that not every row sees whole
-        return t0 + TT - 1 > s.pos_first || (p.window > 0 && t0 <= s.pos_last - p.window) || ~valid << (64 - TT) != 0;
+        return t0 + TT - 1 > s.pos_first || t0 <= s.low_last || ~valid << (64 - TT) != 0;
     };
     uint64_t next_valid = __ballot(pages >= 0);
     bool next_part = in_part(t0, next_valid);

@@ -92,6 +92,65 @@ def test_halves_of_turned_keys(hip, storage):
     s.free()
 
 
+# ---- the ends of what is allowed ----
+@pytest.mark.parametrize("room", [0, 1 << 19])
+@pytest.mark.parametrize("fmt", ["f16", "i8"])
+def test_widest_window(hip, monkeypatch, fmt, room):
+    """A window of 2^31 - 1 tokens is none, also where a sequence has more rows than tokens."""
+    monkeypatch.setattr(serving, "TABLE_TOKENS", room)
+    case = ([(300, 150), (40, 40), (70, 1)], 2, 2, 64, 16, 0)
+    s, k, v, q, K, V, Q, Y, W = kv_cache.attend_case(hip, case, "f16", fmt)
+    s.d_lengths.write([300, 25, 70])
+    for window in (0, 2 ** 31 - 1, 2 ** 30):
+        Y.refill()
+        s.cache.attend(s.batch, Q.ptr, 4, Y.ptr, "f16", window=window, workspace=W.ptr, workspace_bytes=W.cols)
+        y = Y.read()
+        if window == 0:
+            first = y
+            hk, hv = held64(k, "f16", fmt), held64(v, "f16", fmt)
+            rows = slice(s.starts[1] + 15, s.starts[2])  # (25 tokens: rows 15 .. 39 hold them)
+            want, tol = attend64(q[rows].astype(np.float64), hk[300:325], hv[300:325], 0, 0.125, 0, "f16")
+            close(y[rows].reshape(want.shape), want, tol, "y")
+        own = s.positions() >= 0
+        own[s.starts[1]:s.starts[1] + 15] = False
+        assert np.array_equal(y[own], first[own]) and kv_cache.untouched(Y, ~own)
+    for m in (K, V, Q, Y, W):
+        m.free()
+    s.free()
+
+
+def test_page_past_2_gib(hip):
+    """A page whose scales stand behind 2^31 bytes."""
+    kv, dim, n = 1024, 256, 9
+    cache = HipKvCache(hip, kv, dim, page=4096, format="i8")
+    assert 2 ** 31 < cache.page_bytes < 2 ** 32
+    p = ctypes.c_void_p()
+    N.check(N.thin().sox_malloc(ctypes.byref(p), cache.page_bytes), "page")
+    T, S, L, S1 = Ints([0]), Ints([0, n]), Ints([n]), Ints([0, 1])
+    k, v, q = normal(1, "f16", n, kv, dim), normal(2, "f16", n, kv, dim), normal(3, "f16", n, kv, dim)
+    K, V, Q = (Matrix(x.reshape(n, -1), "f16") for x in (k, v, q))
+    Y, K2, V2 = (Matrix(None, "f16", n, kv * dim) for _ in range(3))
+    W = Matrix(None, "i8", 1, cache.workspace(n, 1, kv))
+    whole = HipKvBatch(p.value, 1, T.ptr, 1, S.ptr, L.ptr, 1, n)
+    print("[gpu] page past 2 GiB", flush=True)
+    cache.write(whole, K.ptr, V.ptr, "f16")
+    cache.read(whole, K2.ptr, V2.ptr, "f16")
+    hk, hv = held64(k, "f16", "i8"), held64(v, "f16", "i8")
+    for m, want in ((K2, hk), (V2, hv)):
+        close(m.read().reshape(want.shape), want, (2.0 ** -11 + 2.0 ** -24) * np.abs(want) + 2.0 ** -25, "read")
+    want, tol = attend64(q.astype(np.float64), hk, hv, 0, 1 / 16, 0, "f16")
+    cache.attend(whole, Q.ptr, kv, Y.ptr, "f16", workspace=W.ptr, workspace_bytes=W.cols)
+    close(Y.read().reshape(want.shape), want, tol, "rows")
+    one = HipKvBatch(p.value, 1, T.ptr, 1, S1.ptr, L.ptr, 1, 1)  # (row 0 as the last token)
+    want, tol = attend64(q[:1].astype(np.float64), hk, hv, n - 1, 1 / 16, 0, "f16")
+    cache.attend(one, Q.ptr, kv, Y.ptr, "f16", workspace=W.ptr, workspace_bytes=W.cols)
+    close(Y.read().reshape(q.shape)[:1], want, tol, "one row")
+    for m in (T, S, L, S1, K, V, Q, Y, K2, V2, W):
+        m.free()
+    N.thin().sox_free(p)
+    cache.close()
+
+
 # ---- weights that are small each and count together ----
 @pytest.mark.parametrize("room", [0, 1 << 19])
 @pytest.mark.parametrize("storage,fmt", FORMATS)
