@@ -245,7 +245,7 @@ template <int PAIRS, bool LARGE> SOX_DEV RowTile row_tile(const sox_kv_attend_ar
 
 // The tokens of a tile of rows, and a split's share of them in steps of TT
 struct Span {
-    int lo, hi;              // tokens that any row sees
+    int lo, hi;              // tokens that any row sees, within the table: at most 2^30, so that no sum of them leaves 32 bits
     int begin, end;          // of this split, begin a multiple of TT
     int pos_first, pos_last; // positions of the tile's first and last row
     int low_last;            // the last token that the last row's window leaves out, or -1
@@ -260,9 +260,9 @@ template <int PAIRS, int TT> SOX_DEV Span span_of(const sox_kv_attend_args& p, c
     const int last = min(r.m0 + PAIRS, r.pairs) - 1;
     s.pos_first = (int)(base + r.m0 / p.group);
     s.pos_last = (int)(base + last / p.group);
-    s.lo = window_low(p, s.pos_first) + 1;
     s.low_last = window_low(p, s.pos_last);
     s.hi = (int)min((int64_t)s.pos_last + 1, (int64_t)p.b.table_pages << p.b.shift);
+    s.lo = min(window_low(p, s.pos_first) + 1, max(s.hi, 0));
     const int from = s.lo / TT * TT, tiles = max((s.hi - from + TT - 1) / TT, 0);
     const int per = max((tiles + splits - 1) / splits, (min_tokens + TT - 1) / TT);
     s.begin = min(from + (int)min((int64_t)split * per * TT, (int64_t)1 << 30), max(s.hi, from));

@@ -1,0 +1,75 @@
+"""The paged cache and its attention at the ends of what a call may hold: positions next to 2^31, scores of 2^30, weights and scales far
+apart, rows by the thousand, on the GPU against the operators in 64 bits."""
+import numpy as np
+import pytest
+
+import serving
+import test_gpu_kv_cache as kv_cache
+from layers import SMALL, UNIT, Matrix, rounded
+from serving import U32, Ints, Serving, attend64, close, held64, turned64
+from simdonnx_amd.backend import HipRotary
+from test_gpu_kv_cache import normal, untouched
+
+pytestmark = pytest.mark.gpu
+FORMATS = [("f16", "f16"), ("bf16", "bf16"), ("f32", "f32"), ("f16", "i8"), ("bf16", "i8"), ("f32", "i8")]
+ROOM = 1 << 19  # tokens that tables have room for where every piece is to go to the kernel over 128 pairs
+
+
+def attended(s, k, v, q, storage, scale=0.0, window=0, written=None):
+    """The attention of q [rows, heads, dim] over k and v [tokens, kv, dim], written from another storage type where one is named."""
+    written = written or storage
+    K, V = Matrix(k.reshape(k.shape[0], -1), written), Matrix(v.reshape(v.shape[0], -1), written)
+    Q, Y = Matrix(q.reshape(q.shape[0], -1), storage), Matrix(None, storage, q.shape[0], q.shape[1] * q.shape[2])
+    W = Matrix(None, "i8", 1, s.cache.workspace(s.rows, len(s.sequences), q.shape[1]))
+    s.cache.write(s.every, K.ptr, V.ptr, written)
+    s.cache.attend(s.batch, Q.ptr, q.shape[1], Y.ptr, storage, scale=scale, window=window, workspace=W.ptr, workspace_bytes=W.cols)
+    y = Y.read().reshape(q.shape)
+    for m in (K, V, Q, Y, W):
+        m.free()
+    return y
+
+
+# ---- the longest sequences ----
+@pytest.mark.parametrize("storage,fmt", FORMATS)
+def test_window_behind_the_table(hip, monkeypatch, storage, fmt):
+    """Sequences of 2^31 - 1 tokens whose window lies behind what their tables hold, split nine ways (the last split's first
+    token would be 2^31): zeros, whatever the workspace held; the other sequences as ever. Then a piece of 50 rows likewise."""
+    monkeypatch.setattr(serving, "TABLE_TOKENS", 4096)
+    dim, window = 64, 1023
+    lengths = [(10, 1)] + [(20, 4)] * 39
+    s = Serving(hip, lengths, 1, dim, 16, fmt)
+    s.d_lengths.write([2 ** 31 - 1] + [20] * 39)
+    total = int(s.whole[-1])
+    k, v, q = normal(1, storage, total, 1, dim), normal(2, storage, total, 1, dim), normal(3, storage, s.rows, 1, dim)
+    K, V, Q = (Matrix(x.reshape(x.shape[0], -1), storage) for x in (k, v, q))
+    size = s.cache.workspace(s.rows, len(lengths), 1)
+    Y, W = Matrix(None, storage, s.rows, dim), Matrix(np.full((1, size // 4), 7.0, np.float32), "f32")
+    s.d_lengths.write([10] + [20] * 39)
+    s.cache.write(s.every, K.ptr, V.ptr, storage)
+    s.d_lengths.write([2 ** 31 - 1] + [20] * 39)
+    print(f"[gpu] window behind the table {storage} {fmt}", flush=True)
+    s.cache.attend(s.batch, Q.ptr, 1, Y.ptr, storage, window=window, workspace=W.ptr, workspace_bytes=size)
+    y = Y.read().reshape(q.shape)
+    assert (y[0] == 0).all()
+    hk, hv = held64(k, storage, fmt), held64(v, storage, fmt)
+    for i in range(1, 40):
+        a, r = s.whole[i], slice(s.starts[i], s.starts[i + 1])
+        want, tol = attend64(q[r].astype(np.float64), hk[a:a + 20], hv[a:a + 20], 16, dim ** -0.5, window, storage)
+        close(y[r], want, tol, f"sequence {i}")
+    W.read()
+    for m in (K, V, Q, Y, W):
+        m.free()
+    s.free()
+    for window in (255, 1023, 4095, 2 ** 31 - 1):  # (the last: all that the table holds, and nothing is in a page there)
+        s = Serving(hip, [(60, 50)], 1, dim, 16, fmt)
+        s.d_lengths.write([2 ** 31 - 1])
+        s.d_tables.write(np.full_like(s.tables, -1))
+        Q, Y = Matrix(normal(4, storage, 50, 4 * dim), storage), Matrix(None, storage, 50, 4 * dim)
+        size = s.cache.workspace(50, 1, 4)
+        W = Matrix(np.full((1, size // 4), 7.0, np.float32), "f32")
+        s.cache.attend(s.batch, Q.ptr, 4, Y.ptr, storage, window=window, workspace=W.ptr, workspace_bytes=size)
+        assert (Y.read() == 0).all()
+        W.read()
+        for m in (Q, Y, W):
+            m.free()
+        s.free()
