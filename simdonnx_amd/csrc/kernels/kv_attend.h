@@ -314,13 +314,18 @@ template <typename T> SOX_DEV typename Frag<T>::V load_q(const T* q, int ch, int
 
 // The running reference and sum of a lane's pair. Scores in powers of two.
 struct Soft {
-    float ref = -__builtin_inff(), sum = 0.0f;
+    float ref = -__builtin_inff(), limit = -__builtin_inff(), sum = 0.0f;
     SOX_DEV float of(float ref) { return ref == -__builtin_inff() ? 0.0f : ref; }  // (nothing seen yet: any reference will do)
-    // moves the reference to `top` where it passes it by AT_SLACK; what the sum and the outputs are to be multiplied by
+    // whether `top` passes the reference by AT_SLACK (a limit held from the last move on: the sum with a reference whose steps are 16
+    // would be off by 8, and p of 2^16 is too much for fp16)
+    __device__ __forceinline__ bool passed(float top) const { return top > limit; }
+    // moves the reference to `top`; what the sum and the outputs are to be multiplied by
     __device__ __forceinline__ float move(float top) {
         const float now = fmaxf(ref, top);
         const float by = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - now);
         ref = now;
+        limit = ref + AT_SLACK;
+        if (limit - ref > AT_SLACK) limit = ref;
         sum *= by;
         return by;
     }
@@ -379,6 +384,10 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 #pragma unroll
     for (int d = 0; d < DB; d++) out[d] = float16v{};
     Soft soft;
+    // Scores without scales of their own meet the score's in the subtraction, one instruction for both. The reference is a product
+    // rounded, the fma's is not: up to half a step of the reference apart, which past 2^24 are powers of two in p. So behind a
+    // reference past 2^20, of any of the wave's pairs, products are rounded first.
+    bool large = false;
 
     // ---- staging ----
     int4v raw_k[M::SU], raw_v[M::SU];
@@ -559,31 +568,44 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                 }
             }
         }
-        if (part) {
+        auto scaled = [&] {
 #pragma unroll
             for (int tb = 0; tb < TB; tb++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) x[tb][i] = seen(tb, i) ? x[tb][i] : -__builtin_inff();
+                for (int i = 0; i < 16; i++) x[tb][i] *= p.scale_log2;
+        };
+        if (part | large) {
+            if (!QUANT && large) scaled();
+            if (part) {
+#pragma unroll
+                for (int tb = 0; tb < TB; tb++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x[tb][i] = seen(tb, i) ? x[tb][i] : -__builtin_inff();
+            }
         }
         float top = x[0][0];
 #pragma unroll
         for (int tb = 0; tb < TB; tb++)
 #pragma unroll
             for (int i = 0; i < 16; i++) top = fmaxf(top, x[tb][i]);
-        if constexpr (!QUANT) top *= p.scale_log2;
-        if (__any(top > soft.ref + AT_SLACK)) {
+        if constexpr (!QUANT) top *= large ? 1.0f : p.scale_log2;
+        if (__any(soft.passed(top))) {
             const float by = soft.move(over_32(top, larger));
+            if (!QUANT && !large && __any(__builtin_fabsf(Soft::of(soft.ref)) > 0x1p20f)) {
+                large = true;
+                scaled();
+            }
 #pragma unroll
             for (int d = 0; d < DB; d++) {
                 out[d] *= by;
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        const float ref = Soft::of(soft.ref);
+        const float ref = Soft::of(soft.ref), scale = large ? 1.0f : p.scale_log2;
 #pragma unroll
         for (int tb = 0; tb < TB; tb++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[tb][i] = __builtin_amdgcn_exp2f(QUANT ? x[tb][i] - ref : __builtin_fmaf(x[tb][i], p.scale_log2, -ref));
+            for (int i = 0; i < 16; i++) x[tb][i] = __builtin_amdgcn_exp2f(QUANT ? x[tb][i] - ref : __builtin_fmaf(x[tb][i], scale, -ref));
         // the sum, and p as it meets v
         if constexpr (!(sizeof(T) == 2 && !QUANT)) {
             float4v vs[2];
@@ -925,7 +947,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         next_valid = __ballot(pages >= 0);
         next_part = in_part(t0 + stride, next_valid);
         if (more) load(t0 + stride, pages, next_part);
-        if (__any(top > soft.ref + AT_SLACK)) {
+        if (__any(soft.passed(top))) {
             const float by = soft.move(over_32(over_16(top, larger), larger));
 #pragma unroll
             for (int d = 0; d < DB; d++) {

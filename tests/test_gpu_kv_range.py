@@ -73,3 +73,31 @@ def test_window_behind_the_table(hip, monkeypatch, storage, fmt):
         for m in (Q, Y, W):
             m.free()
         s.free()
+
+
+# ---- scores ----
+@pytest.mark.parametrize("storage,fmt", FORMATS)
+@pytest.mark.parametrize("new,room", [(1, 0), (40, 0), (40, ROOM)])
+@pytest.mark.parametrize("power", [10, 16, 24])
+def test_large_scores(hip, monkeypatch, storage, fmt, new, room, power):
+    """Scores so large that a step of fp32 is more than the softmax's range (2^30 with power 16): each row is the value of the token
+    with the largest. Half a step of the storage type for its weight's product with v, half for the output, and a unit of fp32
+    each for the product, the sum, the quotient and the last product."""
+    power = min(power, 17) if storage == "f16" else power
+    monkeypatch.setattr(serving, "TABLE_TOKENS", room)
+    n, dim, heads = 300, 64, 6
+    rng = np.random.default_rng(power)
+    s = Serving(hip, [(n, new)], 2, dim, 16, fmt)
+    k, q, by = np.zeros((n, 2, dim), np.float32), np.zeros((new, heads, dim), np.float32), 2.0 ** (power - 8)
+    # (whole numbers of 7 bits, so that every form of the cache holds them as they are; token 0's leads by a sixth)
+    k[:, :, 5] = np.stack([rng.permutation(n) % 100 for _ in range(2)], 1) * by
+    k[0, :, 5] = rng.integers(120, 127, 2) * by
+    k[:, :, 9] = 127 * by  # every head's amax in 8 bits, where q holds zeros
+    q[..., 5] = rng.integers(100, 127, (new, heads)) * by
+    assert np.array_equal(rounded(k, storage), k) and np.array_equal(rounded(q, storage), q)
+    v = normal(3, storage, n, 2, dim)
+    print(f"[gpu] large scores {storage} {fmt} {new} {room} {power}", flush=True)
+    y = attended(s, k, v, q, storage, scale=0.7)
+    want = np.repeat(held64(v, storage, fmt)[0], heads // 2, axis=0)
+    close(y, np.broadcast_to(want, y.shape), (2 * UNIT[storage] + 4 * U32) * np.abs(want) + SMALL[storage], "y")
+    s.free()
