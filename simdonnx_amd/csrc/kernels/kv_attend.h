@@ -13,7 +13,9 @@
 // step is that of the score registers; V's rows are read to match it (transposing LDS reads for 16 bits).
 // The reference moves only when a score passes it by 2^8: what it leaves in p is divided out by the sum, and the outputs are
 // rescaled a few times, not once a tile. Sums and outputs in fp32; p is rounded to the storage type for its product (half a
-// step each, unbiased, on terms that the sum averages).
+// step each, unbiased, on terms that the sum averages). In fp16 the reference stands 2^7 below the score that moved it, which with
+// the 2^8 is what its numbers have room for: small weights, of which a long context has many, are then normal numbers down
+// to 2^-21 of the largest.
 // An 8-bit cache: k and v go into the products as whole numbers (exact in every storage type); k's scale multiplies the score,
 // v's p, before its rounding. In fp16, whose exponents end soon, v's scale goes into the exponent instead (2^(s + log2
 // scale), the reference bounds p times scale) and the sum divides it out again: exact while the scales span less than
@@ -25,7 +27,7 @@
 #include "kv_cache.h"
 
 constexpr int AT_THREADS = 256;
-constexpr float AT_SLACK = 8.0f;  // powers of two that p may stand above the reference
+constexpr float AT_SLACK = 8.0f;  // powers of two that p may rise before the reference moves
 
 // ---- storage types' steps ----
 template <typename T> struct Frag {  // 16 bytes of a row
@@ -313,19 +315,20 @@ template <typename T> SOX_DEV typename Frag<T>::V load_q(const T* q, int ch, int
 }
 
 // The running reference and sum of a lane's pair. Scores in powers of two.
-struct Soft {
+template <typename T> struct Soft {
+    static constexpr float LIFT = std::is_same<T, half_t>::value ? 7.0f : 0.0f;  // of the score that moves the reference above it
     float ref = -__builtin_inff(), limit = -__builtin_inff(), sum = 0.0f;
     SOX_DEV float of(float ref) { return ref == -__builtin_inff() ? 0.0f : ref; }  // (nothing seen yet: any reference will do)
-    // whether `top` passes the reference by AT_SLACK (a limit held from the last move on: the sum with a reference whose steps are 16
-    // would be off by 8, and p of 2^16 is too much for fp16)
+    // whether `top` passes the reference by AT_SLACK more (a limit held from the last move on: the sum with a reference whose steps are
+    // 2 to 16 may be off by half of that, and p of 2^16 is too much for fp16)
     __device__ __forceinline__ bool passed(float top) const { return top > limit; }
-    // moves the reference to `top`; what the sum and the outputs are to be multiplied by
+    // moves the reference up to `top`; what the sum and the outputs are to be multiplied by
     __device__ __forceinline__ float move(float top) {
-        const float now = fmaxf(ref, top);
+        const float now = fmaxf(ref, top - LIFT);
         const float by = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - now);
         ref = now;
-        limit = ref + AT_SLACK;
-        if (limit - ref > AT_SLACK) limit = ref;
+        limit = ref + (LIFT + AT_SLACK);
+        if (limit - ref > LIFT + AT_SLACK) limit = ref;
         sum *= by;
         return by;
     }
@@ -383,7 +386,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     float16v out[DB];
 #pragma unroll
     for (int d = 0; d < DB; d++) out[d] = float16v{};
-    Soft soft;
+    Soft<T> soft;
     // Scores without scales of their own meet the score's in the subtraction, one instruction for both. The reference is a product
     // rounded, the fma's is not: up to half a step of the reference apart, which past 2^24 are powers of two in p. So behind a
     // reference past 2^20, of any of the wave's pairs, products are rounded first.
@@ -591,7 +594,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         if constexpr (!QUANT) top *= large ? 1.0f : p.scale_log2;
         if (__any(soft.passed(top))) {
             const float by = soft.move(over_32(top, larger));
-            if (!QUANT && !large && __any(__builtin_fabsf(Soft::of(soft.ref)) > 0x1p20f)) {
+            if (!QUANT && !large && __any(__builtin_fabsf(Soft<T>::of(soft.ref)) > 0x1p20f)) {
                 large = true;
                 scaled();
             }
@@ -601,7 +604,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        const float ref = Soft::of(soft.ref), scale = large ? 1.0f : p.scale_log2;
+        const float ref = Soft<T>::of(soft.ref), scale = large ? 1.0f : p.scale_log2;
 #pragma unroll
         for (int tb = 0; tb < TB; tb++)
 #pragma unroll
@@ -798,7 +801,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     float4v out[DB];
 #pragma unroll
     for (int d = 0; d < DB; d++) out[d] = float4v{};
-    Soft soft;
+    Soft<T> soft;
 
     int4v raw_k[NB][F::KU], raw_v[F::SU];
     float raw_s = 0.0f;  // lanes 0 .. TT - 1: K's scale of their token, TT .. 2 TT - 1: V's
@@ -955,7 +958,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        const float ref = Soft::of(soft.ref);
+        const float ref = Soft<T>::of(soft.ref);
 #pragma unroll
         for (int n = 0; n < NB; n++)
 #pragma unroll

@@ -101,3 +101,32 @@ def test_large_scores(hip, monkeypatch, storage, fmt, new, room, power):
     want = np.repeat(held64(v, storage, fmt)[0], heads // 2, axis=0)
     close(y, np.broadcast_to(want, y.shape), (2 * UNIT[storage] + 4 * U32) * np.abs(want) + SMALL[storage], "y")
     s.free()
+
+
+# ---- weights and scales far apart in fp16 ----
+@pytest.mark.parametrize("fmt", ["f16", "i8"])
+@pytest.mark.parametrize("new,room", [(1, 0), (40, 0), (40, ROOM)])
+@pytest.mark.parametrize("power", [20.7, 26.3])
+def test_small_weights_in_fp16(hip, monkeypatch, fmt, new, room, power):
+    """One token in 32 of weight 1, the others' 2^-20.7 or 2^-26.3, which fp16 alone would hold in 3 bits or not at all: their
+    values stand in the channels where the first ones hold zeros. The tolerance is attend64's, but for the part of weights below
+    fp16's normal numbers: the largest weights stand at 2^7 there (half of it at least where v's scale takes its part), so
+    a token is off by half of 2^-24 of 2^-6 of its value at most, and the sum is their number at least."""
+    monkeypatch.setattr(serving, "TABLE_TOKENS", room)
+    n, dim = 4096, 64
+    s = Serving(hip, [(n, new)], 1, dim, 16, fmt)
+    k, v, q = np.zeros((n, 1, dim), np.float32), np.zeros((n, 1, dim), np.float32), np.zeros((new, 2, dim), np.float32)
+    v[..., 1:] = np.random.default_rng(5).uniform(30000, 60000, (n, 1, dim - 1))
+    k[::32, 0, 0], v[::32] = power * np.log(2.0), 0
+    v[::32, 0, 0] = 1
+    q[..., 0] = 8  # (scale 1 / 8: the score is k's first value)
+    k, v = rounded(k, "f16"), rounded(v, "f16")
+    print(f"[gpu] small weights {fmt} {new} {room} {power}", flush=True)
+    y = attended(s, k, v, q, "f16")
+    hk, hv = held64(k, "f16", fmt), held64(v, "f16", fmt)
+    want, tol = attend64(q.astype(np.float64), hk, hv, n - new, dim ** -0.5, 0, "f16")
+    seen = np.arange(n - new + 1, n + 1)[:, None, None]
+    tol -= seen * 2.0 ** -25 * np.abs(hv).max(axis=0) * (1 - 2.0 ** -6 / (seen // 32))
+    assert (tol[..., 1:] < 0.07 * want[..., 1:]).all()  # (2^-31 / 2^-26.3 / 0.75, and the rest)
+    close(y, want, tol, "y")
+    s.free()
