@@ -17,9 +17,9 @@
 // the 2^8 is what its numbers have room for: small weights, of which a long context has many, are then normal numbers down
 // to 2^-21 of the largest.
 // An 8-bit cache: k and v go into the products as whole numbers (exact in every storage type); k's scale multiplies the score,
-// v's p, before its rounding. In fp16, whose exponents end soon, v's scale goes into the exponent instead (2^(s + log2
-// scale), the reference bounds p times scale) and the sum divides it out again: exact while the scales span less than
-// 2^110, as fp16 rows' do (2^-31 to 2^9; scales below 2^-100 count as that).
+// v's p, before its rounding. In fp16, whose exponents end soon, p times scale would lose its bits beside a token of far larger
+// scale, in the channels where that one holds zeros too. There V takes the scale's power of two and p the rest of it, in its
+// exponent (scale_power, scale_rest; the reference bounds p times the rest, the sum divides it out again).
 // Tokens that a row does not see add nothing, whatever their K and V hold: tokens that no row of the tile sees are not read,
 // masked scores are replaced, and a V that is not finite within a tile that is masked in part goes through without its values
 // that are not finite (special4).
@@ -67,7 +67,8 @@ template <int I> SOX_DEV float signed_byte(int w) {
 template <typename T, typename C> struct Wide {
     static constexpr int N = sizeof(T) / sizeof(C);  // 16-byte chunks of them
     typename Frag<T>::V v[N];
-    SOX_DEV Wide of(int4v raw) {
+    // (POWER: times a power of two, scale_power's, in fp16)
+    template <bool POWER = false> SOX_DEV Wide of(int4v raw, half2v power = {}) {
         Wide w;
         if constexpr (N == 1) {
             w.v[0] = __builtin_bit_cast(typename Frag<T>::V, raw);
@@ -81,8 +82,13 @@ template <typename T, typename C> struct Wide {
                 if constexpr (std::is_same<T, half_t>::value) {  // 0x6400 + u is the number 1024 + u, u = q + 128
                     const uint32_t u = (uint32_t)raw[i] ^ 0x80808080u;
                     const half2v by = {(half_t)1152.0f, (half_t)1152.0f};
-                    const half2v a = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - by;
-                    const half2v b = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - by;
+                    half2v a = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+                    half2v b = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+                    if constexpr (POWER) {
+                        a = __builtin_elementwise_fma(a, power, -by * power), b = __builtin_elementwise_fma(b, power, -by * power);
+                    } else {
+                        a -= by, b -= by;
+                    }
                     to[e] = a[0], to[e + 1] = a[1], to[e + 2] = b[0], to[e + 3] = b[1];
                 } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -169,12 +175,23 @@ template <int I, int N, class F> SOX_DEV void static_for(F&& f) {
     }
 }
 
-// How v's scale in 8 bits takes part: not at all, as a factor of p, or in its exponent
+// How v's scale in 8 bits takes part: not at all, as a factor of p, or in V's and p's exponents
 enum { SCALE_NONE, SCALE_FACTOR, SCALE_EXPONENT };
 template <typename T, typename C> constexpr int scale_form() {
     return sizeof(C) == 1 ? std::is_same<T, half_t>::value ? SCALE_EXPONENT : SCALE_FACTOR : SCALE_NONE;
 }
-SOX_DEV float exponent_scale(float scale) { return __builtin_elementwise_maximum(scale, 0x1p-100f); }  // (a NaN stays one)
+// A scale's power of two, as V takes it: from 2^-24 (V's whole numbers times that are fp16's smallest steps) to 2^5 (times 1152, as
+// the bytes become numbers, it is in fp16's range)
+SOX_DEV float scale_power(float scale) {
+    return __uint_as_float(min(max(__float_as_uint(scale) & 0x7f800000u, 103u << 23), 132u << 23));
+}
+SOX_DEV half2v scale_power2(float scale) { return half2v{(half_t)scale_power(scale), (half_t)scale_power(scale)}; }
+// and the rest, 1 to 2 for scales of 2^-24 to 2^6: it moves p by that much, a scale of 2^9, the last of fp16 rows, by 16. Below,
+// where V is less than half of fp16's smallest step, it ends at 2^-20; a row of zeros has 1; a NaN stays one.
+SOX_DEV float scale_rest(float scale) {
+    const float rest = scale * __uint_as_float(0x7f000000u - __float_as_uint(scale_power(scale)));
+    return scale == 0.0f ? 1.0f : __builtin_elementwise_maximum(rest, 0x1p-20f);
+}
 
 // c + the sum of eight values
 SOX_DEV float sum8(half8 v, float c) {
@@ -395,6 +412,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     // ---- staging ----
     int4v raw_k[M::SU], raw_v[M::SU];
     float raw_s = 0.0f;  // threads 0 .. TT - 1: K's scale of their token, TT .. 2 TT - 1: V's
+    float raw_e[FORM == SCALE_EXPONENT ? M::SU : 1];  // V's scales of raw_v's tokens
     const uint32_t row_bytes = (uint32_t)b.dim * sizeof(C);
     const uint8_t* const head = b.pool + ((int64_t)kvh << b.shift) * row_bytes;
     const uint8_t* const head_s = b.pool + ((int64_t)kvh << b.shift) * 4;
@@ -415,6 +433,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                 const uint8_t* const at = head_rows(b, head, page, ((t0 + row) & mask) * (DP * (int)sizeof(C)));
                 raw_k[j] = *(const At*)(at + lane * 16);
                 raw_v[j] = *(const At*)(at + b.v_at + lane * 16);
+                if constexpr (FORM == SCALE_EXPONENT) raw_e[j] = *(const float*)(head_rows(b, head_s, page, ((t0 + row) & mask) * 4) + b.vs_at + lane / M::UR * 4);
             }
         } else {
             const int tid = thread();
@@ -425,6 +444,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
             for (int j = from; j < to; j++) {
                 const int u = j * AT_THREADS + tid, row = u / M::UR, c = u % M::UR, page = of[j];
                 raw_k[j] = raw_v[j] = int4v{};
+                if constexpr (FORM == SCALE_EXPONENT) raw_e[j] = page >= 0 ? *(const float*)(head_rows(b, head_s, page, ((t0 + row) & mask) * 4) + b.vs_at) : 0.0f;
                 if (page >= 0 && c * M::EC < b.dim) {
                     const uint8_t* const at = head_rows(b, head, page, ((t0 + row) & mask) * row_bytes + c * 16);
                     raw_k[j] = *(const At*)at;
@@ -459,7 +479,12 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 #pragma unroll
         for (int j = from; j < to; j++) {
             const int u = j * AT_THREADS + tid, row = u / M::UR, c = (u % M::UR) * M::NCH;
-            const Wide<T, C> k = Wide<T, C>::of(raw_k[j]), v = Wide<T, C>::of(raw_v[j]);
+            const Wide<T, C> k = Wide<T, C>::of(raw_k[j]);
+            Wide<T, C> v;
+            if constexpr (FORM == SCALE_EXPONENT)
+                v = Wide<T, C>::template of<true>(raw_v[j], scale_power2(raw_e[j]));
+            else
+                v = Wide<T, C>::of(raw_v[j]);
 #pragma unroll
             for (int n = 0; n < M::NCH; n++) {
                 *(FV*)(lk + row * M::PITCH + (((c + n) ^ at_k<M::CH>(row)) << 4)) = k.v[n];
@@ -477,7 +502,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
                 scales[buf][0][tid] = raw_s * p.scale_log2;
             } else if (tid < 2 * TT) {
                 if constexpr (FORM == SCALE_EXPONENT) {
-                    const float v = exponent_scale(raw_s);
+                    const float v = scale_rest(raw_s);
                     scales[buf][1][tid - TT] = __builtin_amdgcn_logf(v);
                     scales[buf][2][tid - TT] = 1.0f / v;
                 } else {
@@ -785,7 +810,7 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
     const int mask = (1 << b.shift) - 1;
     unsigned char* const lv = lds + wave * F::BUF;
     float* const ends = (float*)(lds + 4 * F::BUF);  // [wave][pair][reference, sum]
-    float* const scales = ends + 4 * 16 * 2 + wave * 3 * TT;  // k's times the score's, log2 of v's, what v's are to p or the sum
+    float* const scales = ends + 4 * 16 * 2 + wave * 3 * TT;  // k's times the score's, log2 of v's rest, what v's are to p or the sum
 
     const int m = r.m0 + col;
     const bool mine = m < r.pairs;
@@ -868,12 +893,20 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
         const uint64_t valid = next_valid;
         const bool part = next_part;
         const bool more = t0 + stride < s.end;
+        // V's scales' powers of two, for what this lane stages: from the lanes that have the scales (TT .. 2 TT - 1), long before they are
+        // used (64 single tokens with heads of 128: 165 us, 172 where they are)
+        int power[F::SU];
+        if constexpr (FORM == SCALE_EXPONENT) {
+            const int mine = __builtin_bit_cast(int, scale_power2(raw_s));
+#pragma unroll
+            for (int j = 0; j < F::SU; j++) power[j] = __shfl(mine, TT + (j * 64 + lane) / F::UR);
+        }
         if constexpr (QUANT) {
             if (lane < TT) {
                 scales[lane] = raw_s * p.scale_log2;
             } else if (lane < 2 * TT) {
                 if constexpr (FORM == SCALE_EXPONENT) {
-                    const float v = exponent_scale(raw_s);
+                    const float v = scale_rest(raw_s);
                     scales[lane] = __builtin_amdgcn_logf(v);
                     scales[TT + lane] = __builtin_amdgcn_rcpf(v);
                 } else {
@@ -940,7 +973,11 @@ template <typename T, typename C, int DP> __device__ __forceinline__ void attend
 #pragma unroll
         for (int j = 0; j < F::SU; j++) {
             const int u = j * 64 + lane, row = u / F::UR, c = (u % F::UR) * F::NCH;
-            const Wide<T, C> v = Wide<T, C>::of(raw_v[j]);
+            Wide<T, C> v;
+            if constexpr (FORM == SCALE_EXPONENT)
+                v = Wide<T, C>::template of<true>(raw_v[j], __builtin_bit_cast(half2v, power[j]));
+            else
+                v = Wide<T, C>::of(raw_v[j]);
 #pragma unroll
             for (int n = 0; n < F::NCH; n++) *(FV*)(lv + row * F::PITCH + (((c + n) ^ at_v<F::CH, sizeof(T), true>(row)) << 4)) = v.v[n];
             if constexpr (QUANT) __builtin_amdgcn_sched_barrier(0);

@@ -130,3 +130,44 @@ def test_small_weights_in_fp16(hip, monkeypatch, fmt, new, room, power):
     assert (tol[..., 1:] < 0.07 * want[..., 1:]).all()  # (2^-31 / 2^-26.3 / 0.75, and the rest)
     close(y, want, tol, "y")
     s.free()
+
+
+@pytest.mark.parametrize("written,large,small", [("f16", 1000, 1e-3), ("f16", 60000, 1e-2), ("f16", 60000, 1e-3), ("f16", 1, 3e-5), ("f16", 2e-6, 6e-8),
+                                                 ("f32", 1.5e5, 0.1), ("f32", 1.0, 1e-12), ("bf16", 1e-20, 1e-30)])
+@pytest.mark.parametrize("new,room", [(1, 0), (40, 0), (40, ROOM)])
+@pytest.mark.parametrize("by", [0.0, 1.5])
+def test_scales_far_apart_in_fp16(hip, monkeypatch, written, large, small, new, room, by):
+    """fp16 rows over 8 bits, where some tokens' values of v are far larger than the others' in one channel and zero in the rest:
+    there the others count, to their last bits."""
+    monkeypatch.setattr(serving, "TABLE_TOKENS", room)
+    n, kv, dim, heads = 200, 2, 72, 4
+    s = Serving(hip, [(n, new)], kv, dim, 8, "i8")
+    k, v, q = normal(1, written, n, kv, dim), normal(2, written, n, kv, dim, by=small), normal(3, "f16", new, heads, dim, by=by)
+    for token in (0, 90, 159):
+        v[token], v[token, :, 3] = 0, large
+    v = rounded(v, written)
+    print(f"[gpu] scales far apart {written} {large} {small} {new} {room} {by}", flush=True)
+    y = attended(s, k, v, q, "f16", written=written)
+    want, tol = attend64(q.astype(np.float64), held64(k, written, "i8"), held64(v, written, "i8"), n - new, dim ** -0.5, 0, "f16")
+    close(y, want, tol, "y")
+    s.free()
+
+
+@pytest.mark.parametrize("new,room", [(1, 0), (40, 0), (40, ROOM)])
+def test_rows_of_zeros_in_fp16(hip, monkeypatch, new, room):
+    """One token of large values and 4095 of zeros, in 8 bits: their weights of 2^-18 take the sum up by 2^-6."""
+    monkeypatch.setattr(serving, "TABLE_TOKENS", room)
+    n, dim = 4096, 64
+    s = Serving(hip, [(n, new)], 1, dim, 16, "i8")
+    k, v, q = np.zeros((n, 1, dim), np.float32), np.zeros((n, 1, dim), np.float32), np.zeros((new, 2, dim), np.float32)
+    k[0, 0, 0], v[0] = 18 * np.log(2.0), 30000 * (1 + np.arange(dim) / dim)
+    q[..., 0] = 8
+    k, v = rounded(k, "f16"), rounded(v, "f16")
+    print(f"[gpu] rows of zeros {new} {room}", flush=True)
+    y = attended(s, k, v, q, "f16")
+    hk, hv = held64(k, "f16", "i8"), held64(v, "f16", "i8")
+    want, tol = attend64(q.astype(np.float64), hk, hv, n - new, dim ** -0.5, 0, "f16")
+    tol -= np.arange(n - new + 1, n + 1)[:, None, None] * 2.0 ** -25 * np.abs(hv).max(axis=0) * (1 - 2.0 ** -6)  # (as above)
+    assert (want < 0.99 * hv[0]).all() and (tol < 0.004 * want).all()
+    close(y, want, tol, "y")
+    s.free()
