@@ -395,7 +395,7 @@ typedef struct sox_block_norm_node_p {
  * frequency[j] = f (keep + (1 - keep) / factor), f = base^(-2 j / rotary_dim), and with original > 0, keep = (original * f /
  * (2 pi) - low) / (high - low) held to 0 .. 1: frequencies that turn less than `low` times within `original` positions
  * are divided by the factor, those of more than `high` turns kept; without (original = 0), keep = 0. Or frequencies given
- * one by one. Angles are exact to 2^-33 of a turn at any position. */
+ * one by one. Angles are exact to 2^-33 of a turn at any position for frequencies up to 2^42 (to |frequency| 2^-75 beyond). */
 typedef struct sox_rotary_p {
     int32_t head_dim, rotary_dim; /* rotary_dim: even, 2 .. head_dim */
     int32_t interleaved;

@@ -5675,6 +5675,19 @@ int half_lanes(int dim, int64_t es) { return head_lanes((dim / 2 * (int)es + 15)
 // Rows of a workgroup: one where there are few, so that they spread over the CUs; four otherwise, which share the table's work
 int rows_per_block(int64_t rows, int cus) { return rows > 8 * cus ? 4 : 1; }
 
+// A frequency as a fraction of a turn, in units of 2^-64 (whole turns do not matter, as positions are whole numbers): f / (2 pi) as the
+// sum of two doubles, whose rounding an fma finds. Off by half a unit and |f| 2^-107.
+uint64_t turn_of(double f) {
+    constexpr double INVERSE = 0x1.45f306dc9c883p-3, INVERSE_LOW = -0x1.6b01ec5417056p-57;  // 1 / (2 pi)
+    const double a = std::fabs(f), high = a * INVERSE;
+    double low = std::fma(a, INVERSE, -high) + a * INVERSE_LOW;
+    low -= std::rint(low);
+    const double units = (high - std::floor(high)) * 0x1p64, whole = std::floor(units), rest = low * 0x1p64 + (units - whole);
+    uint64_t t = (uint64_t)whole;
+    t += rest < 0 ? 0 - (uint64_t)std::rint(-rest) : (uint64_t)std::rint(rest);
+    return f < 0 ? 0 - t : t;
+}
+
 // What a batch's calls check alike.
 struct KvCall : LayerCall {
     const sox_kv_cache* cache;
@@ -5820,9 +5833,7 @@ int sox_rotary_create(sox_backend* be, const sox_rotary_p* p, const double* freq
             }
             if (!std::isfinite(f)) fail(SOX_E_INVALID, "Rotary: frequencies have to be finite");
             R->frequencies.push_back(f);
-            // whole turns do not matter, as positions are whole numbers
-            const long double turn = (long double)f / 6.283185307179586476925286766559L, part = turn - std::floor(turn);
-            turns.push_back(part >= 1.0L ? 0 : (uint64_t)(part * 18446744073709551616.0L));
+            turns.push_back(turn_of(f));
         }
         R->mem.upload(be, turns.data(), turns.size() * 8, "Rotary frequencies");
         for (int s = 0; s < 3; s++) R->fns[s] = be->fn(std::string("sox_rotary_") + STORAGE_NAME[s]);

@@ -27,8 +27,8 @@ SOX_DEV int kv_page(const sox_kv_view& b, const int32_t* table, int64_t token) {
 
 // cos and sin of t / 2^64 of a turn: t less its nearest quarter turn, as an angle of [-pi / 4, pi / 4], in their Taylor series
 // (the first terms left out are below 2e-14), and the quarter's signs. The product position * turns[j] in whole numbers keeps
-// the fraction of a turn exactly, however far the position (its error is the position times 2^-65 of a turn), and 64 bits
-// leave nothing next to the borders of a value's 8-bit form.
+// the fraction of a turn exactly, however far the position (its error is the position times turns[j]'s, half of 2^-64 of a turn
+// and the frequency times 2^-107), and 64 bits leave nothing next to the borders of a value's 8-bit form.
 SOX_DEV void turn_cos_sin(uint64_t t, double& c, double& s) {
     const uint64_t quarter = (t + (1ull << 61)) >> 62;
     const int64_t r = (int64_t)(t - (quarter << 62));

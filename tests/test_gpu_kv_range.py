@@ -171,3 +171,51 @@ def test_rows_of_zeros_in_fp16(hip, monkeypatch, new, room):
     assert (want < 0.99 * hv[0]).all() and (tol < 0.004 * want).all()
     close(y, want, tol, "y")
     s.free()
+
+
+# ---- far positions ----
+def turns_of(positions, frequencies):
+    """[positions, frequencies]: position * frequency as a fraction of a turn, from whole numbers: pi to 1400 bits by Machin's
+    formula, 16 arctan(1 / 5) - 4 arctan(1 / 239)."""
+    bits = 1400
+
+    def arctan_inverse(n):
+        total, term, i = 0, (1 << bits) // n, 0
+        while term:
+            total += (-term if i & 1 else term) // (2 * i + 1)
+            term //= n * n
+            i += 1
+        return total
+
+    turn = 2 * (16 * arctan_inverse(5) - 4 * arctan_inverse(239))
+    out = np.empty((len(positions), len(frequencies)))
+    for i, p in enumerate(positions):
+        for j, f in enumerate(frequencies):
+            a, b = float(f).as_integer_ratio()
+            out[i, j] = ((int(p) * a << bits) // b) % turn / turn
+    return out
+
+
+@pytest.mark.parametrize("scale", [1e-6, 1.0, 3e3, 1e6, 1e9, 1e12])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_far_and_fast(hip, scale, interleaved):
+    """Positions up to both ends of 32 bits with frequencies of many turns a position: angles are off by 2^-33 of a turn at most."""
+    rows, heads, dim = 64, 3, 32
+    rng = np.random.default_rng(int(np.log10(scale)) + 50)
+    f = scale * rng.uniform(0.5, 2.0, dim // 2) * rng.choice([-1, 1], dim // 2)
+    pos = np.concatenate([[0, 1, -1, 2 ** 31 - 1, -2 ** 31, 2 ** 30], rng.integers(-2 ** 31, 2 ** 31, rows - 6)])
+    x = normal(8, "f32", rows, heads, dim)
+    r = HipRotary(hip, dim, interleaved=interleaved, frequencies=f)
+    X, P = Matrix(x.reshape(rows, -1), "f32"), Ints(pos)
+    print(f"[gpu] rotary far {scale} {interleaved}", flush=True)
+    r.run(X.ptr, P.ptr, rows, heads, X.ptr, "f32")
+    angle = 2 * np.pi * turns_of(pos, f)[:, None]
+    i, j = (slice(0, dim, 2), slice(1, dim, 2)) if interleaved else (slice(0, dim // 2), slice(dim // 2, dim))
+    a, b, want = x[..., i].astype(np.float64), x[..., j].astype(np.float64), np.empty(x.shape)
+    want[..., i], want[..., j] = a * np.cos(angle) - b * np.sin(angle), b * np.cos(angle) + a * np.sin(angle)
+    # (cos, sin, products and sums in 64 bits here and there: a hundred units are plenty)
+    tol = U32 * np.abs(want) + (2 * np.pi * 2.0 ** -33 + 100 * 2.0 ** -53) * 2 * np.abs(x).max()
+    close(X.read().reshape(x.shape), want, tol, "turned")
+    for m in (X, P):
+        m.free()
+    r.close()
