@@ -800,6 +800,8 @@ class HipKvCache:
               rotary: Optional[HipRotary] = None, q: Optional[int] = None, ldq: Optional[int] = None, q_heads: int = 0,
               y: Optional[int] = None, ldy: Optional[int] = None, stream: Optional[int] = None):
         """The rows' k (turned by `rotary`, if any) and v into their pages; with q, y = q turned in the same launch."""
+        if rotary is not None and not rotary.h:
+            raise ValueError("the rotary is closed")  # (its handle would say that there is none, and k would go in as it is)
         n, m = self.kv_heads * self.head_dim, q_heads * self.head_dim
         rc = self._write(self.h, stream, batch.ref, STORAGE[storage], None if rotary is None else rotary.h, k, n if ldk is None else ldk,
                          v, n if ldv is None else ldv, q, m if ldq is None else ldq, _count(q_heads), y, m if ldy is None else ldy)
