@@ -219,3 +219,41 @@ def test_rotary_far_and_fast(hip, scale, interleaved):
     for m in (X, P):
         m.free()
     r.close()
+
+
+# ---- rows by the thousand: four to a workgroup ----
+@pytest.mark.parametrize("storage,fmt", FORMATS)
+@pytest.mark.parametrize("kv,dim,page", [(3, 40, 8), (2, 128, 64), (1, 8, 1)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_write_and_read_many(hip, monkeypatch, kv, dim, page, storage, fmt, interleaved):
+    """2062 rows with two ahead of the sequences and three behind, borders between sequences within a workgroup's rows."""
+    monkeypatch.setattr(kv_cache, "CACHES", [([(1500, 1301), (5, 5), (0, 0), (900, 751)], kv, dim, page)])
+    kv_cache.test_write_and_read(hip, 0, storage, fmt, interleaved)
+
+
+@pytest.mark.parametrize("room", [0, ROOM])
+@pytest.mark.parametrize("storage", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("case", [([(90, 40)], 1, 2, 256, 16, 0), ([(170, 150)], 1, 1, 200, 8, 20)])
+def test_wide_heads_that_are_not_finite(hip, monkeypatch, case, storage, room):
+    monkeypatch.setattr(serving, "TABLE_TOKENS", room)
+    kv_cache.test_values_that_are_not_finite(hip, case, storage)
+
+
+@pytest.mark.parametrize("room", [0, ROOM])
+@pytest.mark.parametrize("storage", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("dim", [72, 128, 256])
+def test_heads_that_are_not_finite_in_8_bits(hip, monkeypatch, dim, storage, room):
+    """Heads of k and v with an infinity or a NaN, in tiles that some rows see in part: NaN for the rows that see their token."""
+    monkeypatch.setattr(serving, "TABLE_TOKENS", room)
+    n, new = 140, 90
+    s = Serving(hip, [(n, new)], 1, dim, 16, "i8")
+    k, v, q = normal(1, storage, n, 1, dim), normal(2, storage, n, 1, dim), normal(3, storage, new, 2, dim)
+    clean = held64(k, storage, "i8"), held64(v, storage, "i8")
+    k[131, 0, 5], v[118, 0, 7], v[130, 0, 0] = np.nan, np.inf, -np.inf
+    print(f"[gpu] not finite in 8 bits {storage} {dim} {room}", flush=True)
+    y = attended(s, k, v, q, storage)
+    first = 118 - (n - new)
+    assert np.isnan(y[first:]).all()
+    want, tol = attend64(q[:first].astype(np.float64), *clean, n - new, dim ** -0.5, 0, storage)
+    close(y[:first], want, tol, "y")
+    s.free()
