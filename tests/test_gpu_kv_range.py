@@ -257,3 +257,54 @@ def test_heads_that_are_not_finite_in_8_bits(hip, monkeypatch, dim, storage, roo
     want, tol = attend64(q[:first].astype(np.float64), *clean, n - new, dim ** -0.5, 0, storage)
     close(y[:first], want, tol, "y")
     s.free()
+
+
+# ---- weights of few rows over 8 bits ----
+@pytest.mark.parametrize("storage", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("sequences,kv,group,dim", [([(5, 1)], 2, 4, 128), ([(300, 1), (40, 2)], 1, 5, 72), ([(3000, 1)], 2, 2, 64), ([(77, 3)], 1, 4, 256)])
+def test_weights_of_few_rows(hip, sequences, kv, group, dim, storage):
+    """Up to 16 pairs a sequence: weights with their scales meet v in two parts, so what 16 bits leave of them is the square of their
+    half step, and an output is off by little more than its own rounding. (The rest of the tolerance is attend64's; fp16's as in
+    test_small_weights_in_fp16.)"""
+    s = Serving(hip, sequences, kv, dim, 16, "i8")
+    total, heads = int(s.whole[-1]), kv * group
+    k, v, q = normal(1, storage, total, kv, dim), normal(2, storage, total, kv, dim), normal(3, storage, s.rows, heads, dim, by=1.5)
+    print(f"[gpu] weights of few rows {sequences} {dim} {storage}", flush=True)
+    y = attended(s, k, v, q, storage)
+    hk, hv, half = held64(k, storage, "i8"), held64(v, storage, "i8"), UNIT[storage]
+    for i, (length, new) in enumerate(sequences):
+        a, r = s.whole[i], slice(s.starts[i], s.starts[i + 1])
+        kk, vv, qq = hk[a:a + length], hv[a:a + length], q[r].astype(np.float64)
+        want, _ = attend64(qq, kk, vv, length - new, dim ** -0.5, 0, storage)
+        tol = np.empty(want.shape)
+        for j in range(new):
+            for h in range(heads):
+                g, n = h // group, length - new + j + 1
+                p = np.exp(dim ** -0.5 * (kk[:n, g] @ qq[j, h]))
+                size = p @ np.abs(vv[:n, g]) / p.sum()
+                e = (dim + 6) * U32 * dim ** -0.5 * (np.abs(kk[:n, g]) @ np.abs(qq[j, h])).max()
+                tiny = n * (2.0 ** -31 if storage == "f16" else 2.0 ** -126) * np.abs(vv[:n, g]).max(axis=0)
+                left = 0.0 if storage == "f32" else half * half
+                tol[j, h] = (left + 4 * e + (2 * n + 16) * U32) * size + tiny + half * np.abs(want[j, h]) * 1.001 + SMALL[storage]
+        close(y[r], want, tol, f"sequence {i}")
+    s.free()
+
+
+@pytest.mark.parametrize("storage,fmt", FORMATS)
+@pytest.mark.parametrize("new,room", [(1, 0), (3, 0), (40, ROOM)])
+def test_infinite_values_seen_whole(hip, monkeypatch, storage, fmt, new, room):
+    """Infinities and NaN of v in tiles that every row sees whole: they reach their channels and no other (in 8 bits, which hold
+    such a head as NaN, all of its head's)."""
+    monkeypatch.setattr(serving, "TABLE_TOKENS", room)
+    n, kv, dim = 600, 2, 72
+    s = Serving(hip, [(n, new)], kv, dim, 16, fmt)
+    k, v, q = normal(1, storage, n, kv, dim), normal(2, storage, n, kv, dim), normal(3, storage, new, 2 * kv, dim)
+    want, tol = attend64(q.astype(np.float64), held64(k, storage, fmt), held64(v, storage, fmt), n - new, dim ** -0.5, 0, storage)
+    v[5, 0, 3], v[37, 0, 4], v[38, 0, 5], v[70, 0, 5], v[200, 0, 71] = np.inf, -np.inf, np.inf, -np.inf, np.nan
+    want[:, :2, 3], want[:, :2, 4], want[:, :2, 5], want[:, :2, 71] = np.inf, -np.inf, np.nan, np.nan
+    if fmt == "i8":
+        want[:, :2] = np.nan
+    print(f"[gpu] infinite values seen whole {storage} {fmt} {new} {room}", flush=True)
+    y = attended(s, k, v, q, storage)
+    close(y, want, tol, "y")
+    s.free()
