@@ -455,7 +455,8 @@ uint64_t sox_kv_cache_workspace(sox_kv_cache* cache, int32_t rows, int32_t seque
  *   y = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j)  over the tokens j <= its own position,
  * and with window > 0 over the last `window` of them. scale > 0; 0: 1 / sqrt(head_dim). Sums in fp32. A row without such a
  * token (or with none but scores of minus infinity) gives zeros; tokens that a row does not see do not reach it, whatever they
- * hold. The tokens' k and v have to be in the cache (the rows' own too). workspace: 16-byte aligned, held until the work has run. */
+ * hold. (fp16 rows over 8 bits: beside values of v beyond 2^33, which only rows of another storage can have written, the other tokens'
+ * weights lose bits.) The tokens' k and v have to be in the cache (the rows' own too). workspace: 16-byte aligned, held until the work has run. */
 int sox_kv_cache_attend(sox_kv_cache* cache, void* stream, const sox_kv_batch* batch, int32_t storage, const void* q, int64_t ldq,
                         int32_t q_heads, void* y, int64_t ldy, float scale, int32_t window, void* workspace,
                         uint64_t workspace_bytes);

@@ -3,8 +3,8 @@
 // in one pass over the sequence's tokens with the running reference of a softmax. Two kernels:
 //   many  a workgroup takes 128 pairs (new row, query head of one kv head's group), 32 a wave, and walks the tokens tile by
 //         tile through LDS, which all of its waves read; bound by the softmax's instructions beside the matrix cores. Two prompts of
-//         8192, 32 query heads over 8: heads of 128 1.27 ms in bf16 (865 TFLOP/s), 1.38 in 8 bits; of 64 0.69; of 256 (one
-//         wave a SIMD, for its registers) 1.88 with 16 over 4
+//         8192, 32 query heads over 8: heads of 128 1.25 ms in bf16 (880 TFLOP/s), 1.39 in 8 bits; of 64 0.69; of 256 (one
+//         wave a SIMD, for its registers) 1.91 with 16 over 4
 //   few   16 pairs (a single new token's group): its waves walk different tokens, K straight to registers; bound by reading the
 //         cache. One token over 131072: 93 us in bf16 (5.8 TB/s), 64 over 4096 to 8192 in 8 bits 161 (5.2 TB/s)
 // (both: the two in one launch)
@@ -190,7 +190,8 @@ SOX_DEV float scale_power(float scale) {
 }
 SOX_DEV half2v scale_power2(float scale) { return half2v{(half_t)scale_power(scale), (half_t)scale_power(scale)}; }
 // and the rest, 1 to 2 for scales of 2^-24 to 2^6: it moves p by that much, a scale of 2^9, the last of fp16 rows, by 16. Below,
-// where V is less than half of fp16's smallest step, it ends at 2^-20; a row of zeros has 1; a NaN stays one.
+// where V is less than half of fp16's smallest step, it ends at 2^-20; a row of zeros has 1; a NaN stays one. (Scales past 2^26, of
+// values that fp16 rows cannot have, take p of other tokens below its normal numbers.)
 SOX_DEV float scale_rest(float scale) {
     const float rest = scale * __uint_as_float(0x7f000000u - __float_as_uint(scale_power(scale)));
     return scale == 0.0f ? 1.0f : __builtin_elementwise_maximum(rest, 0x1p-20f);
